@@ -25,6 +25,11 @@ BNR_QUANTIZATION_ERROR = 5
 BNR_MIRROR_INCREMENTAL = 0
 BNR_MIRROR_FULL = 1
 
+BNR_KV_F32 = 0
+BNR_KV_BF16 = 1
+BNR_KV_FP8 = 2
+BNR_KV_INT8 = 3
+
 BNR_GLUE_PLAIN = 0
 BNR_GLUE_RESIDUAL = 1
 BNR_GLUE_SQRELU = 2
@@ -101,6 +106,16 @@ _sz = _c.c_size_t
 _vp = _c.c_void_p
 _i32p = _c.POINTER(_c.c_int32)
 
+
+class PagedKVDesc(ctypes.Structure):
+    """bnr_paged_kv"""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scales", _vp), ("v_scales", _vp), ("n_pages", _sz),
+                ("page_size", _sz), ("n_kv_heads", _sz), ("head_dim", _sz), ("format", _c.c_int)]
+
+
+_pkv = _c.POINTER(PagedKVDesc)
+
 # name -> (restype, argtypes); one entry per function in include/bitnet_hip.h
 SIGNATURES = {
     "bnr_last_error": (_c.c_char_p, []),
@@ -170,6 +185,13 @@ SIGNATURES = {
                                      _vp]),
     "bnr_kv_dev_prefill": (_c.c_int, [_vp, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _c.c_float,
                                       _vp, _vp]),
+    "bnr_dev_rope_table": (_c.c_int, [_vp, _sz, _sz, _c.c_float, _vp, _vp, _vp]),
+    "bnr_dev_paged_append": (_c.c_int, [_vp, _pkv, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp,
+                                        _sz, _sz, _vp, _vp, _sz, _vp]),
+    "bnr_dev_paged_read": (_c.c_int, [_vp, _pkv, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "bnr_paged_decode_workspace": (_c.c_int, [_vp, _pkv, _sz, _sz, _c.POINTER(_sz)]),
+    "bnr_dev_paged_decode_attention": (_c.c_int, [_vp, _pkv, _vp, _sz, _vp, _sz, _sz, _vp, _vp,
+                                                  _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -21,7 +21,7 @@ from . import _lib
 from ._lib import (BNR_MIRROR_FULL, BNR_MIRROR_INCREMENTAL, BackendError, BitNetError,
                    InvalidConfig, InvalidShape, QuantizationError, UnsupportedDevice)
 
-__all__ = ["HipBackend", "DeviceKVCache", "NativeKVCache", "BitNetError", "InvalidShape", "InvalidConfig",
+__all__ = ["HipBackend", "DeviceKVCache", "NativeKVCache", "PagedKV", "BitNetError", "InvalidShape", "InvalidConfig",
            "BackendError", "UnsupportedDevice", "QuantizationError", "BNR_MIRROR_FULL",
            "BNR_MIRROR_INCREMENTAL"]
 
@@ -315,6 +315,101 @@ class HipBackend:
             _dev(h_out, "h_out", True), _dev(q_out, "q_out", dtype=torch.int8),
             _dev(act_absmax, "act_absmax"), _stream(stream)))
 
+    # paged KV cache -----------------------------------------------------------
+    def _on(self, t, name: str, shape, dtype="float32"):
+        """The address of a contiguous tensor of that shape and type on this backend's device."""
+        ok = t.is_cuda and t.is_contiguous() and str(t.dtype)[6:] == dtype and t.device.index == self.device_id
+        if not ok:
+            raise TypeError(f"{name} must be a contiguous {dtype} tensor on cuda:{self.device_id}")
+        if t.shape != shape:
+            raise InvalidShape(f"{name} {list(shape)}", f"{list(t.shape)}")
+        return t.data_ptr()
+
+    def _paged_stream(self, stream):
+        if stream is None:
+            import torch
+
+            return torch.cuda.current_stream(self.device_id).cuda_stream
+        return _stream(stream)
+
+    def rope_table(self, n_positions: int, head_dim: int, theta: float):
+        """The rotation tables (cos, sin) [n_positions, head_dim/2] that rope_embed
+        uses, as tensors for dev_paged_append."""
+        import torch
+
+        cos, sin = (torch.empty(n_positions, head_dim // 2, device=f"cuda:{self.device_id}")
+                    for _ in range(2))
+        _lib.check(self._L.bnr_dev_rope_table(self._h, n_positions, head_dim, theta, cos.data_ptr(),
+                                              sin.data_ptr(), self._paged_stream(None)))
+        return cos, sin
+
+    def dev_paged_append(self, kv: "PagedKV", q, k, v, q_out, positions, block_table, cos=None,
+                         sin=None, seqs=None, stream=None) -> None:
+        """Rotate q [n, n_heads, d] into q_out and k at each token's position, and
+        write k and v [n, n_kv_heads, d] to kv in its format.  Token i is at
+        positions[i] of sequence seqs[i] (None: sequence i) of block_table
+        [n_seqs, pages] (int32, as positions and seqs).  cos / sin: the
+        rotation's tables (rope_table), None for rows that are rotated; q and
+        q_out may both be None."""
+        n = positions.shape[0]
+        rows = (n, kv.n_kv_heads, kv.head_dim)
+        n_seqs, stride = block_table.shape
+        n_heads = 0 if q is None else q.shape[1]
+        if (q is None) != (q_out is None) or (cos is None) != (sin is None):
+            raise TypeError("q and q_out, and cos and sin, go together")
+        qs = (n, n_heads, kv.head_dim)
+        tab = None if cos is None else (cos.shape[0], kv.head_dim // 2)
+        _lib.check(self._L.bnr_dev_paged_append(
+            self._h, kv.desc(self.device_id), None if q is None else self._on(q, "q", qs),
+            self._on(k, "k", rows), self._on(v, "v", rows),
+            None if q is None else self._on(q_out, "q_out", qs), n, n_heads,
+            self._on(positions, "positions", (n,), "int32"),
+            None if seqs is None else self._on(seqs, "seqs", (n,), "int32"),
+            self._on(block_table, "block_table", (n_seqs, stride), "int32"), n_seqs, stride,
+            None if cos is None else self._on(cos, "cos", tab),
+            None if cos is None else self._on(sin, "sin", tab), 0 if cos is None else tab[0],
+            self._paged_stream(stream)))
+
+    def dev_paged_read(self, kv: "PagedKV", block_table, lens, k_out, v_out, starts=None,
+                       stream=None) -> None:
+        """Rows starts[s] (None: 0) .. lens[s]-1 of each sequence of block_table
+        [batch, pages] as fp32 into k_out and v_out [batch, n_kv_heads, cap, d],
+        from row 0 on; what lies behind them stays."""
+        batch, stride = block_table.shape
+        cap = k_out.shape[2]
+        out = (batch, kv.n_kv_heads, cap, kv.head_dim)
+        _lib.check(self._L.bnr_dev_paged_read(
+            self._h, kv.desc(self.device_id),
+            self._on(block_table, "block_table", (batch, stride), "int32"), batch, stride,
+            None if starts is None else self._on(starts, "starts", (batch,), "int32"),
+            self._on(lens, "lens", (batch,), "int32"), self._on(k_out, "k_out", out),
+            self._on(v_out, "v_out", out), cap, self._paged_stream(stream)))
+
+    def paged_workspace(self, kv: "PagedKV", batch: int, n_heads: int):
+        """A zero-filled workspace for dev_paged_decode_attention over kv with up
+        to `batch` sequences of n_heads query heads."""
+        import torch
+
+        n = ctypes.c_size_t()
+        _lib.check(self._L.bnr_paged_decode_workspace(self._h, kv.desc(self.device_id), batch,
+                                                      n_heads, ctypes.byref(n)))
+        return torch.zeros(n.value, dtype=torch.uint8, device=f"cuda:{self.device_id}")
+
+    def dev_paged_decode_attention(self, kv: "PagedKV", q, block_table, lens, out, workspace,
+                                   stream=None) -> None:
+        """Attention of one token of each sequence, q [batch, n_heads, d] (rotated),
+        over rows 0..lens[s]-1 of its own, into out (as q).  `workspace` from
+        paged_workspace; calls that share one must be ordered."""
+        batch, stride = block_table.shape
+        n_heads = q.shape[1]
+        qs = (batch, n_heads, kv.head_dim)
+        _lib.check(self._L.bnr_dev_paged_decode_attention(
+            self._h, kv.desc(self.device_id), self._on(q, "q", qs), n_heads,
+            self._on(block_table, "block_table", (batch, stride), "int32"), batch, stride,
+            self._on(lens, "lens", (batch,), "int32"), self._on(out, "out", qs),
+            self._on(workspace, "workspace", workspace.shape, "uint8"), workspace.numel(),
+            self._paged_stream(stream)))
+
     def dev_synchronize(self, stream=None) -> None:
         _lib.check(self._L.bnr_dev_synchronize(self._h, _stream(stream)))
 
@@ -362,6 +457,70 @@ class DeviceKVCache:
 
     def __len__(self) -> int:
         return self.filled_positions
+
+
+class PagedKV:
+    """One layer's pool of a paged KV cache: codes ``k`` and ``v`` ``[n_pages,
+    n_kv_heads, page_size, head_dim]`` and, for the 8-bit formats, one fp32
+    scale a row (``k_scales``, ``v_scales`` ``[n_pages, n_kv_heads,
+    page_size]``).  ``fmt``: "f32", "bf16", "fp8" (e4m3) or "int8".  Which page
+    holds which rows is the caller's block table."""
+
+    FORMATS = {"f32": (_lib.BNR_KV_F32, "float32"), "bf16": (_lib.BNR_KV_BF16, "bfloat16"),
+               "fp8": (_lib.BNR_KV_FP8, "float8_e4m3fn"), "int8": (_lib.BNR_KV_INT8, "int8")}
+
+    def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+                 fmt: str = "bf16", device: str = "cuda"):
+        import torch
+
+        if fmt not in self.FORMATS:
+            raise InvalidConfig(f"unknown paged KV format {fmt!r}")
+        dtype = getattr(torch, self.FORMATS[fmt][1])
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        ks = vs = None
+        if fmt in ("fp8", "int8"):
+            ks, vs = (torch.zeros(shape[:3], device=device) for _ in range(2))
+        self._take(k, v, ks, vs)
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scales=None, v_scales=None) -> "PagedKV":
+        """A pool in tensors that the caller has, the format by their type."""
+        kv = cls.__new__(cls)
+        kv._take(k, v, k_scales, v_scales)
+        return kv
+
+    def _take(self, k, v, k_scales, v_scales) -> None:
+        kinds = {name: fmt for fmt, (_, name) in self.FORMATS.items()}
+        fmt = kinds.get(str(k.dtype)[6:])
+        if fmt is None or v.dtype != k.dtype:
+            raise InvalidConfig(f"no paged KV format of {k.dtype} keys and {v.dtype} values")
+        if k.dim() != 4 or v.shape != k.shape:
+            raise InvalidShape("k and v [n_pages, n_kv_heads, page_size, head_dim]",
+                               f"{list(k.shape)} and {list(v.shape)}")
+        tensors = [k, v]
+        if fmt in ("fp8", "int8"):
+            for s in (k_scales, v_scales):
+                if s is None or s.shape != k.shape[:3] or str(s.dtype) != "torch.float32":
+                    raise InvalidShape(f"float32 scales {list(k.shape[:3])}",
+                                       "none" if s is None else f"{s.dtype} {list(s.shape)}")
+            tensors += [k_scales, v_scales]
+        elif k_scales is not None or v_scales is not None:
+            raise InvalidConfig(f"the {fmt} format has no scales")
+        for t in tensors:
+            if not t.is_contiguous() or t.device != k.device:
+                raise TypeError("a pool's tensors must be contiguous and on one device")
+        self.fmt, self.k, self.v, self.k_scales, self.v_scales = fmt, k, v, k_scales, v_scales
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        at = [t.data_ptr() for t in tensors] + [None] * (4 - len(tensors))
+        self._desc = _lib.PagedKVDesc(*at, self.n_pages, self.page_size, self.n_kv_heads,
+                                      self.head_dim, self.FORMATS[fmt][0])
+
+    def desc(self, device_id: int):
+        """The pool as the library takes it."""
+        if self.k.device.type != "cuda" or self.k.device.index != device_id:
+            raise TypeError(f"the pool must be on cuda:{device_id}, it is on {self.k.device}")
+        return ctypes.byref(self._desc)
 
 
 class NativeKVCache:

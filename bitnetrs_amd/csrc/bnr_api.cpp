@@ -869,7 +869,7 @@ extern "C" int bnr_last_error_parts(const char **first, const char **second) {
   return g_err.kind;
 }
 
-extern "C" uint32_t bnr_abi_version(void) { return (1u << 16) | 2u; }
+extern "C" uint32_t bnr_abi_version(void) { return (1u << 16) | 3u; }
 
 extern "C" int bnr_create(int device_id, bnr_ctx **out) {
   if (!out) return err_backend("bnr_create: out is NULL");
@@ -2674,5 +2674,219 @@ extern "C" int bnr_kv_dev_prefill(bnr_ctx *c, bnr_kv_cache *kc, size_t layer, fl
                        kc->k(layer), kc->v(layer), kc->max_seq, out, stream);
   if (st) return st;
   kv_mark_stored(kc, layer, start_pos, n_tokens);
+  return set_ok();
+}
+
+// ---------------------------------------------------------------------------
+// Paged KV cache
+// ---------------------------------------------------------------------------
+namespace {
+
+// A sequence has at most this many rows, so that a row's number and a
+// length rounded up to any tile are ints.
+constexpr size_t kPagedMaxRows = (size_t)1 << 30;
+constexpr size_t kPagedMaxCount = (size_t)1 << 31;  // pages; sequences x heads
+
+// Checks the pool and the table, and fills the kernels' view of them.
+int paged_pool(const bnr_paged_kv *kv, const int32_t *table, size_t table_stride, PagedPool &p) {
+  if (!kv) return err_backend("paged: kv is NULL");
+  if (kv->format < BNR_KV_F32 || kv->format > BNR_KV_INT8)
+    return err_config(fmt("unknown paged KV format %d", kv->format));
+  if (kv->n_kv_heads == 0) return err_config("n_kv_heads must be > 0");
+  if (kv->head_dim == 0) return err_shape("head_dim > 0", "head_dim = 0");
+  if (kv->head_dim % 2 != 0 || kv->head_dim > (size_t)kPagedMaxDim)
+    return err_config(fmt("paged KV head_dim must be even and at most %d, got %zu", kPagedMaxDim,
+                          kv->head_dim));
+  if (kv->n_pages == 0 || kv->n_pages >= kPagedMaxCount)
+    return err_shape(fmt("0 < n_pages < %zu", kPagedMaxCount), fmt("n_pages = %zu", kv->n_pages));
+  if (kv->page_size == 0 || kv->page_size > kPagedMaxRows)
+    return err_shape(fmt("0 < page_size <= %zu", kPagedMaxRows),
+                     fmt("page_size = %zu", kv->page_size));
+  if (kv->n_kv_heads > 65536) return err_config(fmt("n_kv_heads must be at most 65536, got %zu", kv->n_kv_heads));
+  // 2^31 * 2^16 * 2^9 leaves 2^7 rows a page; the product is checked in steps
+  const size_t most = (size_t)1 << 60, per_row = kv->n_kv_heads * kv->head_dim;
+  if (kv->page_size > most / per_row || kv->n_pages > most / (per_row * kv->page_size))
+    return err_shape("a pool of at most 2^60 elements",
+                     fmt("n_pages = %zu, page_size = %zu", kv->n_pages, kv->page_size));
+  if (table_stride == 0 || table_stride > kPagedMaxRows / kv->page_size)
+    return err_shape(fmt("0 < table_stride * page_size <= %zu", kPagedMaxRows),
+                     fmt("table_stride = %zu, page_size = %zu", table_stride, kv->page_size));
+  const bool scaled = kv->format == BNR_KV_FP8 || kv->format == BNR_KV_INT8;
+  if (!kv->k || !kv->v || (scaled && (!kv->k_scales || !kv->v_scales)))
+    return err_backend("paged: NULL pool pointer");
+  const uintptr_t unit = kv->format == BNR_KV_F32 ? 4 : kv->format == BNR_KV_BF16 ? 2 : 1;
+  if (((uintptr_t)kv->k | (uintptr_t)kv->v) % unit != 0)
+    return err_shape(fmt("%zu-byte aligned pool pointers", (size_t)unit), "an unaligned pointer");
+  p.k = kv->k;
+  p.v = kv->v;
+  p.k_scales = scaled ? kv->k_scales : nullptr;
+  p.v_scales = scaled ? kv->v_scales : nullptr;
+  p.table = table;
+  p.table_stride = (long long)table_stride;
+  p.n_pages = (int)kv->n_pages;
+  p.page = (int)kv->page_size;
+  p.n_kv = (int)kv->n_kv_heads;
+  p.d = (int)kv->head_dim;
+  return BNR_OK;
+}
+
+int check_paged_count(size_t n, const char *what) {
+  if (n >= kPagedMaxCount) return err_shape(fmt("%s < %zu", what, kPagedMaxCount), fmt("%zu", n));
+  return BNR_OK;
+}
+
+// Workspace: a ticket for each sequence and query head, then the pieces.
+size_t paged_ticket_bytes(size_t batch, size_t n_heads) {
+  return (batch * n_heads * sizeof(unsigned) + 255) / 256 * 256;
+}
+
+size_t paged_workspace_bytes(size_t batch, size_t n_heads, size_t group, size_t head_dim) {
+  return paged_ticket_bytes(batch, n_heads) + (size_t)2 * kPagedMaxWgs *
+             paged_part_floats((int)group, (int)head_dim) * sizeof(float);
+}
+
+int check_paged_heads(const bnr_paged_kv *kv, size_t batch, size_t n_heads) {
+  int st = check_heads(n_heads, kv->n_kv_heads, kv->head_dim);
+  if (st) return st;
+  if (n_heads > 65536) return err_config(fmt("n_heads must be at most 65536, got %zu", n_heads));
+  if (batch >= kPagedMaxCount / n_heads)
+    return err_shape(fmt("batch * n_heads < %zu", kPagedMaxCount),
+                     fmt("batch = %zu, n_heads = %zu", batch, n_heads));
+  return BNR_OK;
+}
+
+}  // namespace
+
+extern "C" int bnr_dev_rope_table(bnr_ctx *c, size_t n_positions, size_t head_dim, float theta,
+                                  float *cos_out, float *sin_out, void *stream) {
+  if (!c) return err_backend("context is NULL");
+  int st = check_rope(head_dim, theta);
+  if (st) return st;
+  if (n_positions == 0) return set_ok();
+  if (n_positions > kPagedMaxRows)
+    return err_shape(fmt("n_positions <= %zu", kPagedMaxRows), fmt("n_positions = %zu", n_positions));
+  if (!cos_out || !sin_out) return err_backend("rope_table: NULL pointer");
+  std::lock_guard<std::mutex> lk(c->mu);
+  DeviceGuard dg(c->device);
+  st = ensure_table(c, n_positions - 1, head_dim, theta);
+  if (st) return st;
+  const size_t bytes = n_positions * (head_dim / 2) * sizeof(float);
+  hipStream_t s = (hipStream_t)stream;
+  HIP_TRY(hipMemcpyAsync(cos_out, c->d_cos, bytes, hipMemcpyDeviceToDevice, s), "rope table copy");
+  HIP_TRY(hipMemcpyAsync(sin_out, c->d_sin, bytes, hipMemcpyDeviceToDevice, s), "rope table copy");
+  // the context may replace its own table once the lock is released
+  HIP_TRY(hipStreamSynchronize(s), "rope table copy");
+  return set_ok();
+}
+
+extern "C" int bnr_dev_paged_append(bnr_ctx *c, const bnr_paged_kv *kv, const float *q,
+                                    const float *k, const float *v, float *q_out, size_t n_tokens,
+                                    size_t n_heads, const int32_t *positions, const int32_t *seqs,
+                                    const int32_t *block_table, size_t n_seqs, size_t table_stride,
+                                    const float *cos_tab, const float *sin_tab, size_t n_positions,
+                                    void *stream) {
+  if (!c) return err_backend("context is NULL");
+  PagedAppendArgs a{};
+  int st = paged_pool(kv, block_table, table_stride, a.pool);
+  if (!st && (q || q_out)) st = check_heads(n_heads, kv->n_kv_heads, kv->head_dim);
+  if (!st && (q || q_out) && n_heads > 65536)
+    st = err_config(fmt("n_heads must be at most 65536, got %zu", n_heads));
+  if (!st) st = check_paged_count(n_tokens, "n_tokens");
+  if (!st) st = check_paged_count(n_seqs, "n_seqs");
+  if (st) return st;
+  if (n_tokens == 0) return set_ok();
+  if (!k || !v || !positions || !block_table || !q != !q_out || !cos_tab != !sin_tab)
+    return err_backend("paged_append: NULL pointer");
+  a.q = q;
+  a.q_out = q_out;
+  a.k = k;
+  a.v = v;
+  a.positions = positions;
+  a.seqs = seqs;
+  a.cos_tab = cos_tab;
+  a.sin_tab = sin_tab;
+  a.n_positions = (long long)std::min(n_positions, kPagedMaxRows);
+  a.n_tokens = (long long)n_tokens;
+  a.n_seqs = (long long)n_seqs;
+  a.n_heads = (int)n_heads;
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_paged_append(a, kv->format, (hipStream_t)stream), "paged append launch");
+  return set_ok();
+}
+
+extern "C" int bnr_dev_paged_read(bnr_ctx *c, const bnr_paged_kv *kv, const int32_t *block_table,
+                                  size_t batch, size_t table_stride, const int32_t *starts,
+                                  const int32_t *lens, float *k_out, float *v_out, size_t cap,
+                                  void *stream) {
+  if (!c) return err_backend("context is NULL");
+  PagedReadArgs a{};
+  int st = paged_pool(kv, block_table, table_stride, a.pool);
+  if (!st) st = check_paged_count(batch, "batch");
+  if (st) return st;
+  if (cap > kPagedMaxRows)
+    return err_shape(fmt("cap <= %zu", kPagedMaxRows), fmt("cap = %zu", cap));
+  if (batch == 0 || cap == 0) return set_ok();
+  const size_t most = (size_t)1 << 60, per = kv->n_kv_heads * kv->head_dim;
+  if (batch > most / (per * cap))
+    return err_shape("outputs of at most 2^60 elements", fmt("batch = %zu, cap = %zu", batch, cap));
+  if (!block_table || !lens || !k_out || !v_out) return err_backend("paged_read: NULL pointer");
+  a.starts = starts;
+  a.lens = lens;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.batch = (long long)batch;
+  a.cap = (long long)cap;
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_paged_read(a, kv->format, (hipStream_t)stream), "paged read launch");
+  return set_ok();
+}
+
+extern "C" int bnr_paged_decode_workspace(bnr_ctx *c, const bnr_paged_kv *kv, size_t batch,
+                                          size_t n_heads, size_t *bytes) {
+  if (!c) return err_backend("context is NULL");
+  if (!kv || !bytes) return err_backend("paged_decode_workspace: NULL pointer");
+  PagedPool p{};
+  int st = paged_pool(kv, nullptr, 1, p);
+  if (!st) st = check_paged_heads(kv, batch, n_heads);
+  if (st) return st;
+  *bytes = paged_workspace_bytes(batch, n_heads, n_heads / kv->n_kv_heads, kv->head_dim);
+  return set_ok();
+}
+
+extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv, const float *q,
+                                              size_t n_heads, const int32_t *block_table,
+                                              size_t batch, size_t table_stride,
+                                              const int32_t *lens, float *out, void *workspace,
+                                              size_t workspace_bytes, void *stream) {
+  if (!c) return err_backend("context is NULL");
+  PagedDecodeArgs a{};
+  int st = paged_pool(kv, block_table, table_stride, a.pool);
+  if (!st) st = check_paged_heads(kv, batch, n_heads);
+  if (st) return st;
+  if (batch == 0) return set_ok();
+  if (!q || !block_table || !lens || !out || !workspace)
+    return err_backend("paged_decode_attention: NULL pointer");
+  const size_t group = n_heads / kv->n_kv_heads;
+  const size_t need = paged_workspace_bytes(batch, n_heads, group, kv->head_dim);
+  if (workspace_bytes < need)
+    return err_shape(fmt("workspace of %zu bytes", need), fmt("%zu bytes", workspace_bytes));
+  if (!aligned16(workspace))
+    return err_shape("16-byte aligned workspace", "an unaligned pointer");
+  a.q = q;
+  a.out = out;
+  a.lens = lens;
+  a.tickets = (unsigned *)workspace;
+  a.parts = (float *)((char *)workspace + paged_ticket_bytes(batch, n_heads));
+  a.batch = (int)batch;
+  a.n_heads = (int)n_heads;
+  a.group = (int)group;
+  a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)kv->head_dim));
+  // no more workgroups than units that the table has room for
+  const size_t units = (table_stride * kv->page_size + kPagedGenericTile - 1) / kPagedGenericTile;
+  a.wgs = units >= kPagedMaxWgs ? kPagedMaxWgs
+                                : (int)std::min<size_t>(kPagedMaxWgs, units * batch * n_heads);
+  a.part_floats = paged_part_floats(1, (int)kv->head_dim);
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_paged_decode_generic(a, kv->format, (hipStream_t)stream), "paged decode launch");
   return set_ok();
 }

@@ -679,4 +679,69 @@ inline long long sqrelu_blocks(long long n) {
 }
 hipError_t launch_residual(float *h, const float *delta, long long n, hipStream_t s);
 
+
+// ---------------------------------------------------------------------------
+// Paged KV cache (bnr_paged.hip).  One pool holds the rows of many sequences:
+// codes [n_pages][n_kv][page][d] in one of four formats, scales [n_pages]
+// [n_kv][page] for the 8-bit ones.  table[seq * table_stride + i] names the
+// page of rows i * page .. of a sequence; an entry outside 0 .. n_pages - 1 is
+// a page that is not there.
+// ---------------------------------------------------------------------------
+constexpr int kPagedF32 = 0, kPagedBf16 = 1, kPagedFp8 = 2, kPagedInt8 = 3;
+constexpr int kPagedMaxDim = 512;
+// The least row maximum a scale is made from: 448 / 2^-100 and 2^-100 / 448
+// are both normal floats, so a row of zeros needs no case of its own.
+constexpr float kPagedTiny = 7.888609052210118e-31f;
+
+struct PagedPool {
+  void *k, *v;
+  float *k_scales, *v_scales;
+  const int *table;
+  long long table_stride;
+  int n_pages, page, n_kv, d;
+};
+
+struct PagedAppendArgs {
+  PagedPool pool;
+  const float *q;  // [n_tokens][n_heads][d], or null with q_out null
+  float *q_out;    // may be q
+  const float *k, *v;  // [n_tokens][n_kv][d]
+  const int *positions, *seqs;  // [n_tokens]; seqs null: token i is of sequence i
+  const float *cos_tab, *sin_tab;  // [n_positions][d / 2], or null: nothing is rotated
+  long long n_positions;
+  long long n_tokens, n_seqs;
+  int n_heads;
+};
+hipError_t launch_paged_append(const PagedAppendArgs &a, int format, hipStream_t s);
+
+struct PagedReadArgs {
+  PagedPool pool;
+  const int *starts, *lens;  // [batch]; starts null: 0
+  float *k_out, *v_out;      // [batch][n_kv][cap][d]
+  long long batch, cap;
+};
+hipError_t launch_paged_read(const PagedReadArgs &a, int format, hipStream_t s);
+
+// Decode attention.  The work is one line of units, sequence by sequence and
+// head by head, a unit being `tile` rows; workgroup w of `wgs` takes a
+// contiguous, equal share of it, found on the device from lens.
+struct PagedDecodeArgs {
+  PagedPool pool;
+  const float *q;   // [batch][n_heads][d]
+  float *out;       // [batch][n_heads][d]
+  const int *lens;  // [batch]
+  float *parts;     // [2 * wgs][part_floats]: unfinished pieces of the line
+  unsigned *tickets;  // [batch][items of a sequence], zero between launches
+  int batch, n_heads, group;
+  int wgs, part_floats;
+  float scale_log2;  // log2(e) / sqrt(d)
+};
+// Floats of a piece of `heads` query heads: outputs, then (max, sum) of each.
+constexpr int paged_part_floats(int heads, int d) { return (heads * (d + 2) + 3) / 4 * 4; }
+// Workgroups of a launch over at most `rows` rows of `items` (sequence, head)
+// pairs each.
+constexpr int kPagedMaxWgs = 1024;
+hipError_t launch_paged_decode_generic(const PagedDecodeArgs &a, int format, hipStream_t s);
+constexpr int kPagedGenericTile = 64;
+
 }  // namespace bnr

@@ -2,7 +2,8 @@
  * bitnet_hip.h -- C ABI of the MI355X (gfx950) GQA attention hot path of
  * bitnetrs: RoPE (half-split, any theta) on Q/K, KV-cache append into an
  * HBM-resident head-major cache, split-K decode attention and causal
- * flash prefill; and the W2A8 ternary GEMV of the layer projections.
+ * flash prefill; the same over a paged cache that may hold its rows in 16 or
+ * 8 bits; and the W2A8 ternary GEMV of the layer projections.
  *
  * Conventions
  *  - Every entry point returns an int status (BNR_OK == 0) and never aborts.
@@ -396,6 +397,91 @@ int bnr_kv_dev_decode(bnr_ctx *ctx, bnr_kv_cache *cache, size_t layer, const flo
 int bnr_kv_dev_prefill(bnr_ctx *ctx, bnr_kv_cache *cache, size_t layer, float *q, float *k,
                        const float *v, size_t n_tokens, size_t start_pos, size_t n_heads,
                        float theta, float *out, void *stream);
+
+/* ---- Paged KV cache --------------------------------------------------------
+ * No counterpart in the reference, whose KVCache holds one sequence in fp32.
+ * One pool per layer holds the rows of many sequences in pages of page_size
+ * rows, and a block table on the device says which page holds which rows:
+ * rows i*page_size .. (i+1)*page_size-1 of sequence s lie in page
+ * block_table[s*table_stride + i].  Lengths, positions and tables are device
+ * arrays that the kernels read, so a captured launch serves every later
+ * step; a kernel checks each entry it follows:
+ *   - a page outside 0..n_pages-1 is not there: what would be written to it
+ *     is dropped, it reads back as zeros, attention leaves its rows out;
+ *   - a length below 0 counts as 0, one past table_stride*page_size as that.
+ * The pool is the caller's memory; these calls allocate nothing and keep
+ * nothing, so calls on different workspaces may run side by side.
+ *
+ * Formats of a pool's rows, a row being head_dim values of one token and one
+ * kv head.  x is the value in fp32 (for K: after the rotation):
+ *   F32   x
+ *   BF16  x rounded to nearest even
+ *   FP8   e4m3(x * (448 / m)), scale m / 448     m = max(max|x|, 2^-100) of
+ *   INT8  round(x * (127 / m)), scale m / 127    the row, ties to even
+ * A row of FP8 or INT8 that holds an infinity or a NaN gets the scale NaN and
+ * reads back as NaN. */
+#define BNR_KV_F32 0
+#define BNR_KV_BF16 1
+#define BNR_KV_FP8 2
+#define BNR_KV_INT8 3
+typedef struct bnr_paged_kv {
+  void *k, *v;                /* [n_pages][n_kv_heads][page_size][head_dim] */
+  float *k_scales, *v_scales; /* [n_pages][n_kv_heads][page_size]; FP8 and INT8 only */
+  size_t n_pages, page_size, n_kv_heads;
+  size_t head_dim; /* even, at most 512 */
+  int format;      /* BNR_KV_* */
+} bnr_paged_kv;
+
+/* The rotation tables of bnr_rope_embed (the same values) for positions
+ * 0..n_positions-1, into cos_out and sin_out [n_positions x head_dim/2] in
+ * device memory: a caller of bnr_dev_paged_append keeps them.  Builds them on
+ * the host and waits for the copy: not for use under graph capture. */
+int bnr_dev_rope_table(bnr_ctx *ctx, size_t n_positions, size_t head_dim, float theta,
+                       float *cos_out, float *sin_out, void *stream);
+
+/* Rotate and append n_tokens tokens of any sequences: token i has position
+ * positions[i] of sequence seqs[i] (seqs NULL: of sequence i).  q [n_tokens x
+ * n_heads x d] rotated goes to q_out (which may be q); k and v [n_tokens x
+ * n_kv_heads x d] go to the pool, k rotated, both in its format.  q and q_out
+ * may both be NULL.  cos_tab / sin_tab [n_positions x d/2] are the rotation
+ * (half-split pairs, as bnr_rope_embed, bit-identical to it with
+ * bnr_dev_rope_table's tables); both NULL: q and k are taken as rotated.
+ * A token whose position is negative, at or past table_stride*page_size or
+ * n_positions, or whose sequence is outside 0..n_seqs-1 is left out: its
+ * q_out row is not written either.  A row may be named once per call. */
+int bnr_dev_paged_append(bnr_ctx *ctx, const bnr_paged_kv *kv, const float *q, const float *k,
+                         const float *v, float *q_out, size_t n_tokens, size_t n_heads,
+                         const int32_t *positions, const int32_t *seqs,
+                         const int32_t *block_table, size_t n_seqs, size_t table_stride,
+                         const float *cos_tab, const float *sin_tab, size_t n_positions,
+                         void *stream);
+
+/* Read rows back as fp32 in the contiguous layout of the other entry points:
+ * rows starts[s] .. lens[s]-1 of sequence s (starts NULL: from row 0), at most
+ * cap of them, go to k_out and v_out [batch x n_kv_heads x cap x d] from row 0
+ * on; FP8 and INT8 rows as code * scale.  Rows behind them are left as they
+ * were; a sequence with a negative start is left out. */
+int bnr_dev_paged_read(bnr_ctx *ctx, const bnr_paged_kv *kv, const int32_t *block_table,
+                       size_t batch, size_t table_stride, const int32_t *starts,
+                       const int32_t *lens, float *k_out, float *v_out, size_t cap, void *stream);
+
+/* Bytes of workspace that bnr_dev_paged_decode_attention needs for up to
+ * `batch` sequences of n_heads query heads over kv. */
+int bnr_paged_decode_workspace(bnr_ctx *ctx, const bnr_paged_kv *kv, size_t batch,
+                               size_t n_heads, size_t *bytes);
+
+/* Attention of one new token of each sequence over rows 0..lens[s]-1 of its
+ * own (which hold the new token's k and v already; q rotated): out[s][h] =
+ * softmax(q_h . K[h/G] / sqrt(d)) V[h/G], q and out [batch x n_heads x d].  A
+ * sequence without a row gives zeros.  A row with a non-finite value makes
+ * the outputs that weigh it non-finite.  `workspace` (device memory,
+ * 16-byte aligned) must be zero-filled before its first use; each call leaves
+ * it ready for the next.  Calls that share a workspace must be ordered, as on
+ * one stream.  The same inputs give the same bits on every run. */
+int bnr_dev_paged_decode_attention(bnr_ctx *ctx, const bnr_paged_kv *kv, const float *q,
+                                   size_t n_heads, const int32_t *block_table, size_t batch,
+                                   size_t table_stride, const int32_t *lens, float *out,
+                                   void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- Measurement ---------------------------------------------------------
  * A plain streaming read of two device ranges (a_bytes at a, b_bytes at b;
