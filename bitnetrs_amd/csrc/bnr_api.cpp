@@ -2881,12 +2881,20 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
   a.n_heads = (int)n_heads;
   a.group = (int)group;
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)kv->head_dim));
+  const bool fast = kv->head_dim % 16 == 0 && kv->head_dim <= 256 && group <= 16 &&
+                    kv->page_size >= 16 && (kv->page_size & (kv->page_size - 1)) == 0 &&
+                    aligned16(q) && aligned16(out) && aligned16(kv->k) && aligned16(kv->v) &&
+                    aligned16(a.pool.k_scales) && aligned16(a.pool.v_scales);
+  const size_t tile = fast ? kPagedTile : kPagedGenericTile;
+  const size_t items = fast ? kv->n_kv_heads : n_heads;
   // no more workgroups than units that the table has room for
-  const size_t units = (table_stride * kv->page_size + kPagedGenericTile - 1) / kPagedGenericTile;
+  const size_t units = (table_stride * kv->page_size + tile - 1) / tile;
   a.wgs = units >= kPagedMaxWgs ? kPagedMaxWgs
-                                : (int)std::min<size_t>(kPagedMaxWgs, units * batch * n_heads);
-  a.part_floats = paged_part_floats(1, (int)kv->head_dim);
+                                : (int)std::min<size_t>(kPagedMaxWgs, units * batch * items);
+  a.part_floats = paged_part_floats(fast ? (int)group : 1, (int)kv->head_dim);
   DeviceGuard dg(c->device);
-  HIP_TRY(launch_paged_decode_generic(a, kv->format, (hipStream_t)stream), "paged decode launch");
+  HIP_TRY(fast ? launch_paged_decode(a, kv->format, (hipStream_t)stream)
+               : launch_paged_decode_generic(a, kv->format, (hipStream_t)stream),
+          "paged decode launch");
   return set_ok();
 }

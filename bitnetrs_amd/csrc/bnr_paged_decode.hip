@@ -1,0 +1,418 @@
+// bnr_paged_decode.hip -- gfx950 decode attention over a paged KV cache on the
+// matrix cores.
+//
+// An item is one (sequence, kv head): its G <= 16 query heads share one read
+// of each row.  A wave takes 32 rows at a time and keeps everything in
+// registers: no operand passes through LDS.
+//
+//   S  = K q^T   A = 16 rows of K, B = the query heads as 16 columns
+//   O += V^T P   A = 16 dims of V, B = the weights of 32 rows
+//
+// K's rows are operand A as they lie in memory (a lane holds 16 bytes of one
+// row).  D of the first product has a lane hold 4 rows of each 16-row tile
+// for one head, which is how the second product wants its B, for the row
+// order (tile, lane group, 4 rows) within the step.  V's A operand then needs
+// one element of 8 rows from each lane: a lane reads E neighbouring elements
+// of its 8 rows, and output dim E * i + m belongs to row i of product m, so
+// the transposition is inside the lane (byte permutes, or the conversion that
+// the 8-bit formats need anyway).
+//
+// Precision.  f32 rows multiply on the f32 matrix cores.  bf16, e4m3 and
+// int8 codes are exact in bf16; q and the weights are cut into three bf16
+// parts of 8 bits each, which together hold all 24 bits of an fp32 value, and
+// every part has fp32's exponent range: the products are those of fp32, at a
+// third of the bf16 rate, which is far above what the rows' bytes need.  A
+// row's scale multiplies its score and its weight in fp32.
+#include "bnr_paged.h"
+
+namespace bnr {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kW = 4;  // waves of a workgroup
+constexpr int kStep = 32;  // rows of a wave's step
+
+template <int F>
+constexpr int kBytes = F == kPagedF32 ? 4 : F == kPagedBf16 ? 2 : 1;
+
+// `n` bytes (a multiple of 4, at most 64) at p, read once.
+template <int N>
+__device__ __forceinline__ void load_bytes(const char *p, unsigned (&r)[N]) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 4 * i));
+      r[i] = v.x;
+      r[i + 1] = v.y;
+      r[i + 2] = v.z;
+      r[i + 3] = v.w;
+    }
+  } else if constexpr (N == 2) {
+    const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p));
+    r[0] = v.x;
+    r[1] = v.y;
+  } else {
+    r[0] = __builtin_nontemporal_load(reinterpret_cast<const unsigned *>(p));
+  }
+}
+
+// The upper halves of two floats: a's below b's.
+__device__ __forceinline__ unsigned pack_hi(float a, float b) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a),
+                               0x07060302u);
+}
+
+// Three bf16 parts of 8 floats: truncation leaves 8 bits a part, so the parts
+// sum to the value exactly.
+struct Parts {
+  u32x4 p[3];
+};
+__device__ __forceinline__ Parts split8(const float (&x)[8]) {
+  Parts s;
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.p[k][i] = pack_hi(r[2 * i], r[2 * i + 1]);
+    if (k < 2)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        r[i] -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, r[i]) & 0xffff0000u);
+  }
+  return s;
+}
+
+__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Code i (0..3) of a dword of 8-bit codes, as a float.
+template <int F, int I>
+__device__ __forceinline__ float code8(unsigned w) {
+  if constexpr (F == kPagedInt8) return (float)(signed char)(w >> (8 * I));
+  return __builtin_amdgcn_cvt_f32_fp8((int)w, I);
+}
+
+// 8 codes (two dwords) as bf16.
+template <int F>
+__device__ __forceinline__ u32x4 widen8(unsigned a, unsigned b) {
+  u32x4 r;
+  r[0] = pack_hi(code8<F, 0>(a), code8<F, 1>(a));
+  r[1] = pack_hi(code8<F, 2>(a), code8<F, 3>(a));
+  r[2] = pack_hi(code8<F, 0>(b), code8<F, 1>(b));
+  r[3] = pack_hi(code8<F, 2>(b), code8<F, 3>(b));
+  return r;
+}
+
+// Scores of 16 rows x 16 heads, before the scales: the rows' dwords as loaded,
+// the heads' operands from q_operands.
+template <int F, int KW>
+struct QOperands {
+  static constexpr int kN = F == kPagedF32 ? KW * 4 : KW * (F == kPagedBf16 ? 1 : 2);
+  Parts p[F == kPagedF32 ? 1 : kN];
+  float f[F == kPagedF32 ? kN : 1];
+};
+
+// One workgroup's share of the line; waves take steps of kStep rows in turn.
+// DP: head dim, rounded up to 64, 128 or 256; FULL: head dim is DP.
+template <int F, int DP, bool FULL>
+__global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeArgs a) {
+  constexpr int B = kBytes<F>;
+  constexpr int E = DP / 16;        // dims of a lane and V row
+  constexpr int KW = DP * B / 64;   // 16-byte loads of a lane and K tile
+  constexpr int VW = E * B / 4;     // dwords of a lane and V row
+  constexpr int KE = 16 / B;        // elements of a 16-byte load
+  extern __shared__ float s_o[];    // [kW][group][DP]
+  __shared__ float s_m[kW * kJoinHeads], s_l[kW * kJoinHeads];
+  __shared__ JoinShared s_join;
+  const int lane = threadIdx.x & 63, d = a.pool.d, G = a.group;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int row = lane & 15, g = lane >> 4;
+  const int page_shift = __builtin_ctz(a.pool.page);
+  const unsigned row_bytes = (unsigned)d * B;
+  const unsigned k_off = row * row_bytes + 16 * g;
+  const unsigned v_off = 4 * g * row_bytes + row * (E * B);
+  const bool v_in = FULL || row * E < d;
+  paged_empty(a);
+  PagedShare sh = paged_share(a.lens, a.batch, a.pool.n_kv, a.pool, kPagedTile, blockIdx.x, a.wgs);
+
+  for (PagedPiece p; sh.next(p);) {
+    const int row1 = __builtin_amdgcn_readfirstlane(p.row1);
+    const int hk = __builtin_amdgcn_readfirstlane(p.h);
+    const int *table = a.pool.table +
+                       (long long)__builtin_amdgcn_readfirstlane(p.b) * a.pool.table_stride;
+
+    // The page of the 16-row tile at row t, or -1: past the piece, or not there.
+    auto tile_page = [&](int t) {
+      int pg = t < row1 ? table[t >> page_shift] : -1;
+      return __builtin_amdgcn_readfirstlane(pg < 0 || pg >= a.pool.n_pages ? -1 : pg);
+    };
+    // First row of that tile in the pool, in rows; page 0's where there is none.
+    auto tile_row = [&](int pg, int t) {
+      return ((long long)(pg < 0 ? 0 : pg) * a.pool.n_kv + hk) * a.pool.page +
+             (pg < 0 ? 0 : t & (a.pool.page - 1));
+    };
+
+    // The query heads as operands: column `row` is head row of the group.
+    QOperands<F, KW> qo;
+    {
+      const float *q = a.q + ((long long)p.b * a.n_heads + (long long)p.h * G + row) * d;
+#pragma unroll
+      for (int c = 0; c < KW; ++c) {
+        const int e0 = (64 * c + 16 * g) / B;
+        const bool in = row < G && (FULL || e0 < d);
+        if constexpr (F == kPagedF32) {
+          const float4 x = in ? ld4(q + e0) : make_float4(0.f, 0.f, 0.f, 0.f);
+          qo.f[4 * c] = x.x;
+          qo.f[4 * c + 1] = x.y;
+          qo.f[4 * c + 2] = x.z;
+          qo.f[4 * c + 3] = x.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < KE / 8; ++e) {
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (in) {
+              const float4 lo = ld4(q + e0 + 8 * e), hi = ld4(q + e0 + 8 * e + 4);
+              x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
+              x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+            }
+            qo.p[c * (KE / 8) + e] = split8(x);
+          }
+        }
+      }
+    }
+
+    float m = -INFINITY, l = 0.f;  // of head `row`; l over this lane's rows only
+    f32x4 o[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    unsigned kr[2][KW * 4], vr[2][4][VW];
+    f32x4 ks[2], vs[2];
+    auto load_k = [&](int t, const int (&pg)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long at = tile_row(pg[h], t + 16 * h);
+        const char *src = static_cast<const char *>(a.pool.k) + at * row_bytes;
+#pragma unroll
+        for (int c = 0; c < KW; ++c) {
+          unsigned w[4] = {0u, 0u, 0u, 0u};
+          if (FULL || (64 * c + 16 * g) / B < d) load_bytes(src + k_off + 64 * c, w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) kr[h][4 * c + i] = w[i];
+        }
+        if (kPagedScaled<F>) ks[h] = *reinterpret_cast<const f32x4 *>(a.pool.k_scales + at + 4 * g);
+      }
+    };
+    auto load_v = [&](int t, const int (&pg)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long at = tile_row(pg[h], t + 16 * h);
+        const char *src = static_cast<const char *>(a.pool.v) + at * row_bytes;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          unsigned w[VW];
+#pragma unroll
+          for (int i = 0; i < VW; ++i) w[i] = 0u;
+          if (v_in) load_bytes(src + v_off + r * row_bytes, w);
+#pragma unroll
+          for (int i = 0; i < VW; ++i) vr[h][r][i] = w[i];
+        }
+        if (kPagedScaled<F>) vs[h] = *reinterpret_cast<const f32x4 *>(a.pool.v_scales + at + 4 * g);
+      }
+    };
+
+    int t = __builtin_amdgcn_readfirstlane(p.row0) + kStep * wave;
+    int pg[2], pn[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) pg[h] = tile_page(t + 16 * h);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) pn[h] = tile_page(t + kW * kStep + 16 * h);
+    if (t < row1) {
+      load_k(t, pg);
+      load_v(t, pg);
+    }
+    for (; t < row1; t += kW * kStep) {
+      // scores: lane has head `row`, rows 4 g + r of both tiles
+      f32x4 s[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KW; ++c) {
+          if constexpr (F == kPagedF32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  __builtin_bit_cast(float, kr[h][4 * c + i]), qo.f[4 * c + i], s[h], 0, 0, 0);
+          } else if constexpr (F == kPagedBf16) {
+            const u32x4 w = {kr[h][4 * c], kr[h][4 * c + 1], kr[h][4 * c + 2], kr[h][4 * c + 3]};
+#pragma unroll
+            for (int k = 0; k < 3; ++k) s[h] = mfma_bf16(w, qo.p[c].p[k], s[h]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const u32x4 w = widen8<F>(kr[h][4 * c + 2 * e], kr[h][4 * c + 2 * e + 1]);
+#pragma unroll
+              for (int k = 0; k < 3; ++k) s[h] = mfma_bf16(w, qo.p[2 * c + e].p[k], s[h]);
+            }
+          }
+        }
+      }
+      float x[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[4 * h + r] = kPagedScaled<F> ? s[h][r] * a.scale_log2 * ks[h][r] : s[h][r] * a.scale_log2;
+      const bool all = pg[0] >= 0 && pg[1] >= 0 && t + kStep <= row1;
+      if (!all)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (pg[h] < 0 || t + 16 * h + 4 * g + r >= row1) x[4 * h + r] = -INFINITY;
+      // the next step's K goes out while this one's weights are made
+      const int tn = t + kW * kStep;
+      int p2[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) p2[h] = tile_page(tn + kW * kStep + 16 * h);
+      if (tn < row1) load_k(tn, pn);
+
+      float mx = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
+      if (__any(mx > m)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float keep = join_weight(m, mx);
+        m = mx;
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] *= keep;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = fast_exp2(x[i] - mu);
+        l += w[i];
+        if (kPagedScaled<F>) w[i] *= vs[i >> 2][i & 3];
+      }
+      if (!all)  // rows that are not there: no weight, whatever lies in their place
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (pg[h] < 0 || t + 16 * h + 4 * g + r >= row1) {
+              w[4 * h + r] = 0.f;
+#pragma unroll
+              for (int i = 0; i < VW; ++i) vr[h][r][i] = 0u;
+            }
+
+      if constexpr (F == kPagedF32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+              o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[h][r][i]),
+                                                          w[4 * h + r], o[i], 0, 0, 0);
+      } else {
+        const Parts wp = split8(w);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          u32x4 c;  // dim i of the lane's 8 rows
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const unsigned lo = vr[k >> 1][2 * (k & 1)][i * B / 4];
+            const unsigned hi = vr[k >> 1][2 * (k & 1) + 1][i * B / 4];
+            if constexpr (F == kPagedBf16)
+              c[k] = __builtin_amdgcn_perm(hi, lo, i & 1 ? 0x07060302u : 0x05040100u);
+            else
+              c[k] = i % 4 == 0   ? pack_hi(code8<F, 0>(lo), code8<F, 0>(hi))
+                     : i % 4 == 1 ? pack_hi(code8<F, 1>(lo), code8<F, 1>(hi))
+                     : i % 4 == 2 ? pack_hi(code8<F, 2>(lo), code8<F, 2>(hi))
+                                  : pack_hi(code8<F, 3>(lo), code8<F, 3>(hi));
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k) o[i] = mfma_bf16(c, wp.p[k], o[i]);
+        }
+      }
+      if (tn < row1) load_v(tn, pn);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        pg[h] = pn[h];
+        pn[h] = p2[h];
+      }
+    }
+
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    __syncthreads();  // the piece before this one has been read
+    if (row < G) {
+      if (g == 0) {
+        s_m[wave * G + row] = m;
+        s_l[wave * G + row] = l;
+      }
+      float *so = s_o + (wave * G + row) * DP + 4 * g * E;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < E; ++i) so[r * E + i] = o[i][r];
+    }
+    __syncthreads();
+    paged_finish<kW>(a, p, sh, s_o, DP, s_m, s_l, G, s_join);
+  }
+}
+
+template <int F>
+hipError_t launch_format(const PagedDecodeArgs &a, hipStream_t s) {
+  const int d = a.pool.d;
+  const int dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  const size_t lds = (size_t)kW * a.group * dp * sizeof(float);
+  const dim3 grid((unsigned)a.wgs), block(64 * kW);
+  // more than the 64 KB a workgroup gets unasked: 16 heads of 256
+  constexpr size_t kUnasked = 60 * 1024;
+#define BNR_LAUNCH(DP)                                          \
+  {                                                             \
+    const auto kernel = d == DP ? paged_decode_kernel<F, DP, true> : paged_decode_kernel<F, DP, false>; \
+    if (lds > kUnasked) {                                       \
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), \
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); \
+      if (e != hipSuccess) return e;                            \
+    }                                                           \
+    kernel<<<grid, block, lds, s>>>(a);                         \
+  }
+  if (dp == 64) {
+    BNR_LAUNCH(64)
+  } else if (dp == 128) {
+    BNR_LAUNCH(128)
+  } else {
+    BNR_LAUNCH(256)
+  }
+#undef BNR_LAUNCH
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_decode(const PagedDecodeArgs &a, int format, hipStream_t s) {
+  switch (format) {
+    case kPagedF32: return launch_format<kPagedF32>(a, s);
+    case kPagedBf16: return launch_format<kPagedBf16>(a, s);
+    case kPagedFp8: return launch_format<kPagedFp8>(a, s);
+    case kPagedInt8: return launch_format<kPagedInt8>(a, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace bnr
