@@ -2885,12 +2885,13 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
                     kv->page_size >= 16 && (kv->page_size & (kv->page_size - 1)) == 0 &&
                     aligned16(q) && aligned16(out) && aligned16(kv->k) && aligned16(kv->v) &&
                     aligned16(a.pool.k_scales) && aligned16(a.pool.v_scales);
-  const size_t tile = fast ? kPagedTile : kPagedGenericTile;
-  const size_t items = fast ? kv->n_kv_heads : n_heads;
-  // no more workgroups than units that the table has room for
-  const size_t units = (table_stride * kv->page_size + tile - 1) / tile;
-  a.wgs = units >= kPagedMaxWgs ? kPagedMaxWgs
-                                : (int)std::min<size_t>(kPagedMaxWgs, units * batch * items);
+  size_t tile = fast ? kPagedTile : kPagedGenericTile;
+  const size_t items = batch * (fast ? kv->n_kv_heads : n_heads);
+  const size_t rows = table_stride * kv->page_size;
+  // units that the table has room for: under 2^31, and no fewer than workgroups
+  while ((rows + tile - 1) / tile * items >= kPagedMaxCount) tile *= 2;
+  a.tile = (int)tile;
+  a.wgs = (int)std::min<size_t>(kPagedMaxWgs, (rows + tile - 1) / tile * items);
   a.part_floats = paged_part_floats(fast ? (int)group : 1, (int)kv->head_dim);
   DeviceGuard dg(c->device);
   HIP_TRY(fast ? launch_paged_decode(a, kv->format, (hipStream_t)stream)

@@ -733,14 +733,14 @@ struct PagedDecodeArgs {
   float *parts;     // [2 * wgs][part_floats]: unfinished pieces of the line
   unsigned *tickets;  // [batch][items of a sequence], zero between launches
   int batch, n_heads, group;
-  int wgs, part_floats;
+  int wgs, part_floats, tile;
   float scale_log2;  // log2(e) / sqrt(d)
 };
 // Floats of a piece of `heads` query heads: outputs, then (max, sum) of each.
 constexpr int paged_part_floats(int heads, int d) { return (heads * (d + 2) + 3) / 4 * 4; }
 // Workgroups of a launch over at most `rows` rows of `items` (sequence, head)
 // pairs each.
-constexpr int kPagedMaxWgs = 1024;
+constexpr int kPagedMaxWgs = 512;
 hipError_t launch_paged_decode_generic(const PagedDecodeArgs &a, int format, hipStream_t s);
 constexpr int kPagedGenericTile = 64;
 // On the matrix cores: 16-byte aligned pools, q and out, head_dim a multiple

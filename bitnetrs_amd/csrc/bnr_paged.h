@@ -75,19 +75,19 @@ __device__ __forceinline__ float load_code(const void *codes, long long i) {
 // Rows.
 // ---------------------------------------------------------------------------
 // A sequence's length as the table can hold it.
-__device__ __forceinline__ int paged_len(int len, const PagedPool &p) {
+__host__ __device__ __forceinline__ int paged_len(int len, const PagedPool &p) {
   const long long most = p.table_stride * p.page;  // at most INT_MAX, checked by the host
   return len < 0 ? 0 : len > most ? (int)most : len;
 }
 
 // The page of row t of a sequence, or -1 where there is none.  0 <= t < stride * page.
-__device__ __forceinline__ int paged_page(const PagedPool &p, long long seq, int t) {
+__host__ __device__ __forceinline__ int paged_page(const PagedPool &p, long long seq, int t) {
   const int page = p.table[seq * p.table_stride + t / p.page];
   return page < 0 || page >= p.n_pages ? -1 : page;
 }
 
 // Row t of kv head h, counted in rows of the pool; -1 where its page is not there.
-__device__ __forceinline__ long long paged_row(const PagedPool &p, long long seq, int h, int t) {
+__host__ __device__ __forceinline__ long long paged_row(const PagedPool &p, long long seq, int h, int t) {
   const int page = paged_page(p, seq, t);
   if (page < 0) return -1;
   return ((long long)page * p.n_kv + h) * p.page + t % p.page;
@@ -109,7 +109,7 @@ struct AppendRow {
 };
 // False: nothing to do (a token whose position or sequence is outside the
 // table, or outside the rotation's tables; a page that is not there).
-__device__ __forceinline__ bool append_row(const PagedAppendArgs &a, long long row, AppendRow &r) {
+__host__ __device__ __forceinline__ bool append_row(const PagedAppendArgs &a, long long row, AppendRow &r) {
   const PagedPool &p = a.pool;
   const int nq = a.q ? a.n_heads : 0, per = nq + 2 * p.n_kv;
   const long long i = row / per;
@@ -147,113 +147,110 @@ __device__ __forceinline__ bool append_row(const PagedAppendArgs &a, long long r
 // workgroup's share is a run of pieces, each of one item: at most its first
 // and its last piece belong to items that other workgroups share.  Nothing
 // about the lengths is known on the host, so a captured launch serves every
-// later step, and ragged batches are balanced to one unit.
+// later step, and ragged batches are balanced to one unit.  The host picks
+// `tile` so that all units that the table has room for fit 31 bits.
 // ---------------------------------------------------------------------------
 struct PagedPiece {
-  int b, h;         // sequence, item
-  int row0, row1;   // rows of it
-  long long item0, item1;  // the whole item's units on the line
-  long long unit;   // the piece's first unit
+  int b, h;        // sequence, item
+  int row0, row1;  // rows of it
+  unsigned w0, w1;  // the workgroups that share the item: the first, the last
 };
 
 struct PagedShare {
-  const int *lens;
-  const PagedPool *pool;
-  long long at, end;   // units left to this workgroup
-  long long base;      // first unit of sequence b
-  unsigned long long per, rest;
-  int b, items, tile, len, n;  // n: units of an item of sequence b
-  unsigned wg;
+  unsigned at, end;     // units left to this workgroup
+  unsigned item0;       // first unit of the item at `at`
+  unsigned per, rest, wg;
+  int b, h, items, tile, len;
+  unsigned n;           // units of an item of sequence b
 
   // The workgroup that has unit t.
-  __device__ unsigned wg_of(unsigned long long t) const {
-    const unsigned long long big = rest * (per + 1);
-    if (t < big) return (unsigned)div(t, per + 1);
-    return (unsigned)(rest + div(t - big, per));
+  __host__ __device__ unsigned wg_of(unsigned t) const {
+    const unsigned big = rest * (per + 1);
+    return t < big ? t / (per + 1) : rest + (t - big) / per;
   }
-  __device__ static unsigned long long div(unsigned long long x, unsigned long long y) {
-    return (x | y) >> 32 ? x / y : (unsigned)x / (unsigned)y;
-  }
-  __device__ bool next(PagedPiece &p) {
+  // The next piece; lens as the launch has them.
+  __host__ __device__ bool next(const int *lens, const PagedPool &pool, PagedPiece &p) {
     if (at >= end) return false;
-    while (at >= base + (long long)items * n) {
-      base += (long long)items * n;
-      ++b;
-      len = paged_len(lens[b], *pool);
-      n = (len + tile - 1) / tile;  // len + tile is in range: the host bounds len
+    if (at == item0 + n) {  // past the item before
+      item0 = at;
+      if (++h == items) {
+        h = 0;
+        do {
+          len = paged_len(lens[++b], pool);
+        } while (len == 0);
+        n = (unsigned)(len + tile - 1) / (unsigned)tile;
+      }
     }
     p.b = b;
-    p.h = (int)div((unsigned long long)(at - base), (unsigned)n);
-    p.item0 = base + (long long)p.h * n;
-    p.item1 = p.item0 + n;
-    p.unit = at;
-    const long long to = p.item1 < end ? p.item1 : end;
-    p.row0 = (int)(at - p.item0) * tile;
-    const long long r1 = (to - p.item0) * tile;
-    p.row1 = r1 < len ? (int)r1 : len;
+    p.h = h;
+    const unsigned item1 = item0 + n, to = item1 < end ? item1 : end;
+    p.w0 = at == item0 ? wg : wg_of(item0);
+    p.w1 = item1 <= end ? wg : wg_of(item1 - 1);
+    p.row0 = (int)((at - item0) * (unsigned)tile);
+    const unsigned r1 = (to - item0) * (unsigned)tile;
+    p.row1 = r1 < (unsigned)len ? (int)r1 : len;
     at = to;
     return true;
   }
 };
 
-// Sum over the wave's lanes; inclusive sums of its lanes.
+// Inclusive sums over the wave's lanes.
 __device__ __forceinline__ unsigned wave_scan(unsigned v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
+#define BNR_SCAN(CTRL, ROWS) \
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false)
+  BNR_SCAN(0x111, 0xF);  // row_shr:1, 2, 4, 8: sums within each row of 16 lanes
+  BNR_SCAN(0x112, 0xF);
+  BNR_SCAN(0x114, 0xF);
+  BNR_SCAN(0x118, 0xF);
+  BNR_SCAN(0x142, 0xA);  // row_bcast:15 into rows 1 and 3
+  BNR_SCAN(0x143, 0xC);  // row_bcast:31 into rows 2 and 3
+#undef BNR_SCAN
   return v;
 }
 
-__device__ __forceinline__ PagedShare paged_share(const int *lens, int batch, int items,
-                                                  const PagedPool &pool, int tile, unsigned wg,
-                                                  unsigned wgs) {
+__device__ __forceinline__ unsigned lane_of(unsigned v, int lane) {
+  return (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+__device__ __forceinline__ PagedShare paged_share(const PagedDecodeArgs &a, int items) {
   const int lane = threadIdx.x & 63;
-  // Units of an item of each sequence, 64 sequences at a time.  A wave's sum
-  // of them fits 32 bits: a sequence has under 2^31 rows, a tile 64 or more.
+  const unsigned tile = (unsigned)a.tile, wgs = (unsigned)a.wgs;
+  // Units of an item of each sequence, 64 sequences at a time.
   auto units = [&](int b) -> unsigned {
-    return b < batch ? ((unsigned)paged_len(lens[b], pool) + tile - 1) / tile : 0u;
+    return b < a.batch ? ((unsigned)paged_len(a.lens[b], a.pool) + tile - 1) / tile : 0u;
   };
   const unsigned first = wave_scan(units(lane));
-  unsigned long long total = (unsigned)__builtin_amdgcn_readlane((int)first, 63);
-  for (int b0 = 64; b0 < batch; b0 += 64)
-    total += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(units(b0 + lane)), 63);
+  unsigned total = lane_of(first, 63);
+  for (int b0 = 64; b0 < a.batch; b0 += 64) total += lane_of(wave_scan(units(b0 + lane)), 63);
   total *= (unsigned)items;
   PagedShare s;
-  s.lens = lens;
-  s.pool = &pool;
-  s.per = PagedShare::div(total, wgs);
+  s.wg = blockIdx.x;
+  s.per = total / wgs;
   s.rest = total - s.per * wgs;
-  s.wg = wg;
   s.items = items;
-  s.tile = tile;
-  s.at = (long long)(wg * s.per + (wg < s.rest ? wg : s.rest));
-  s.end = s.at + (long long)(s.per + (wg < s.rest ? 1 : 0));
-  s.base = 0;
-  s.b = 0;
-  s.n = 0;
-  s.len = 0;
+  s.tile = a.tile;
+  s.at = s.wg * s.per + (s.wg < s.rest ? s.wg : s.rest);
+  s.end = s.at + s.per + (s.wg < s.rest ? 1 : 0);
   if (s.at >= s.end) return s;
-  // The sequence that has unit `at`.
-  const unsigned long long want = PagedShare::div((unsigned long long)s.at, (unsigned)items);
-  unsigned long long before = 0;
-  unsigned incl = first;
+  // The sequence that has unit `at`, and the item of it.
+  const unsigned want = s.at / (unsigned)items;
+  unsigned before = 0, incl = first;
   for (int b0 = 0;; b0 += 64) {
     if (b0) incl = wave_scan(units(b0 + lane));
-    const unsigned sum = (unsigned)__builtin_amdgcn_readlane((int)incl, 63);
+    const unsigned sum = lane_of(incl, 63);
     if (want < before + sum) {
       const int k = __builtin_ctzll(__ballot(before + incl > want));
+      const unsigned lo = k ? lane_of(incl, k - 1) : 0u;
       s.b = b0 + k;
-      before += k ? (unsigned)__builtin_amdgcn_readlane((int)incl, k - 1) : 0u;
+      s.n = lane_of(incl, k) - lo;
+      before += lo;
       break;
     }
     before += sum;
   }
-  s.base = (long long)(before * (unsigned)items);
-  s.len = paged_len(lens[s.b], pool);
-  s.n = (s.len + tile - 1) / tile;
+  s.len = paged_len(a.lens[s.b], a.pool);
+  s.h = (int)((s.at - before * (unsigned)items) / s.n);
+  s.item0 = before * (unsigned)items + (unsigned)s.h * s.n;
   return s;
 }
 
@@ -273,12 +270,16 @@ __device__ __forceinline__ void paged_empty(const PagedDecodeArgs &a) {
 // item is normalised and written.  Otherwise it goes to the launch's
 // workspace; the last workgroup to bring a piece of the item joins all of
 // them, in the line's order, so the same inputs give the same bits.
+//
+// What a join costs is latency: a store, a ticket and a load, each to the
+// device's coherence point and back.  So the loads of kJoin pieces are all in
+// flight before the first is used, and nothing else waits for memory.
 // ---------------------------------------------------------------------------
-constexpr int kJoin = 32;      // pieces joined at a time
+constexpr int kJoin = 8;        // pieces in flight in a thread
 constexpr int kJoinHeads = 16;  // heads of an item at most
+template <int W, int V>
 struct JoinShared {
-  float m[kJoinHeads], l[kJoinHeads];
-  float w[kJoin][kJoinHeads];
+  float o[W * 64][V], m[W * 64], l[W * 64];
   int last;
 };
 
@@ -287,89 +288,118 @@ __device__ __forceinline__ float join_weight(float m, float top) {
   return m == -INFINITY ? 0.f : fast_exp2(m - top);
 }
 
-template <int W>
-__device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, const PagedShare &sh,
-                             const float *o, int o_stride, const float *wm, const float *wl,
-                             int heads, JoinShared &js) {
-  const int tid = threadIdx.x, nt = W * 64, d = a.pool.d;
-  const unsigned w0 = sh.wg_of((unsigned long long)p.item0);
-  const unsigned w1 = sh.wg_of((unsigned long long)(p.item1 - 1));
-  const bool whole = w0 == w1;
-  float *part = a.parts + (size_t)(2 * sh.wg + (sh.wg == w0 ? 1 : 0)) * a.part_floats;
-  float *out = a.out + ((long long)p.b * a.n_heads + (long long)p.h * heads) * d;
-  if (tid < heads) {
-    float m = -INFINITY, l = 0.f;
-    for (int w = 0; w < W; ++w) m = fmaxf(m, wm[w * heads + tid]);
-    for (int w = 0; w < W; ++w) {
-      const float f = join_weight(wm[w * heads + tid], m);
-      js.w[w][tid] = f;
-      l = fmaf(f, wl[w * heads + tid], l);
-    }
-    js.m[tid] = m;
-    js.l[tid] = l;
-    if (!whole) {
-      st_agent(part + heads * d + 2 * tid, m);
-      st_agent(part + heads * d + 2 * tid + 1, l);
-    }
+// A state of one head and V outputs, and another put to it.
+template <int V>
+struct JoinState {
+  float m, l, o[V];
+  __device__ __forceinline__ void add(float m2, float l2, const float (&o2)[V]) {
+    const float top = fmaxf(m, m2), f = join_weight(m, top), f2 = join_weight(m2, top);
+    m = top;
+    l = l * f + l2 * f2;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = o[i] * f + o2[i] * f2;
   }
-  __syncthreads();
-  for (int e = tid; e < heads * d; e += nt) {
-    const int g = e / d, x = e - g * d;
-    float s = 0.f;
-    for (int w = 0; w < W; ++w) s = fmaf(js.w[w][g], o[(w * heads + g) * o_stride + x], s);
-    if (whole)
-      out[e] = js.l[g] == 0.f ? 0.f : s / js.l[g];
-    else
-      st_agent(part + e, s);
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = 0.f;
+  }
+  __device__ __forceinline__ void write(float *out) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = l == 0.f ? 0.f : o[i] / l;
+  }
+};
+
+// V: outputs of a thread, 4 where d is a multiple of 4 and out is 16-byte
+// aligned, or 1.
+template <int W, int V>
+__device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsigned wg, const float *o,
+                             int o_stride, const float *wm, const float *wl, int heads,
+                             JoinShared<W, V> &js) {
+  constexpr int nt = W * 64;
+  const int tid = threadIdx.x, d = a.pool.d, work = heads * d / V;
+  const bool whole = p.w0 == p.w1;
+  float *out = a.out + ((long long)p.b * a.n_heads + (long long)p.h * heads) * d;
+  const __amdgpu_buffer_rsrc_t parts = agent_buf(a.parts);
+  const int stride = a.part_floats * 4;
+  const int mine = (int)(2 * wg + (wg == p.w0 ? 1 : 0)) * stride;
+  for (int e = tid; e < work; e += nt) {
+    const int g = e * V / d, x = e * V - g * d;
+    JoinState<V> s;
+    s.clear();
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      float ow[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) ow[i] = o[(w * heads + g) * o_stride + x + i];
+      s.add(wm[w * heads + g], wl[w * heads + g], ow);
+    }
+    if (whole) {
+      s.write(out + e * V);
+    } else {
+      if constexpr (V == 4)
+        st4_agent(parts, mine + e * 16, make_float4(s.o[0], s.o[1], s.o[2], s.o[3]));
+      else
+        st_agent(a.parts + mine / 4 + e, s.o[0]);
+      if (x == 0) st2_agent(parts, mine + (heads * d + 2 * g) * 4, s.m, s.l);
+    }
   }
   if (whole) return;
   // every store of the workgroup is at the device's coherence point before its ticket
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   unsigned *ticket = a.tickets + (size_t)p.b * (a.n_heads / heads) + p.h;
-  const unsigned n = w1 - w0 + 1;
+  const int n = (int)(p.w1 - p.w0) + 1;
   if (tid == 0)
-    js.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+    js.last = (int)__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
   __syncthreads();
   if (!js.last) return;
   if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // piece i of the item: the first is its workgroup's last piece, the others their workgroups' first
-  auto piece = [&](unsigned i) {
-    return a.parts + (size_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * a.part_floats;
-  };
-  const int wave = tid >> 6, lane = tid & 63;
-  for (int g = wave; g < heads; g += W) {
-    float m = -INFINITY;
-    for (unsigned i = lane; i < n; i += 64) m = fmaxf(m, ld_agent(piece(i) + heads * d + 2 * g));
-    m = wave_max(m);
-    float l = 0.f;
-    for (unsigned i = lane; i < n; i += 64)
-      l = fmaf(join_weight(ld_agent(piece(i) + heads * d + 2 * g), m),
-               ld_agent(piece(i) + heads * d + 2 * g + 1), l);
-    l = wave_sum(l);
-    if (lane == 0) {
-      js.m[g] = m;
-      js.l[g] = l;
-    }
-  }
-  for (int e0 = 0; e0 < heads * d; e0 += nt) {
-    const int e = e0 + tid, g = e / d;
-    float s = 0.f;
-    for (unsigned i0 = 0; i0 < n; i0 += kJoin) {
-      const int c = (int)(n - i0 < kJoin ? n - i0 : kJoin);
-      __syncthreads();
-      for (int k = tid; k < c * heads; k += nt) {
-        const int i = k / heads, hg = k - i * heads;
-        js.w[i][hg] = join_weight(ld_agent(piece(i0 + i) + heads * d + 2 * hg), js.m[hg]);
+  // Piece i of the item is in slot 2 (w0 + i), the first in slot 2 w0 + 1.
+  // `ways` threads share the pieces of one output; thread k of them takes
+  // pieces k, k + ways, ...
+  const int ways = work >= nt ? 1 : nt / work;
+  for (int e0 = 0; e0 < work; e0 += nt) {
+    const int way = work >= nt ? 0 : tid / work, e = work >= nt ? e0 + tid : tid - way * work;
+    JoinState<V> s;
+    s.clear();
+    if (way < ways && e < work) {
+      const int g = e * V / d;
+      for (int i0 = way; i0 < n; i0 += kJoin * ways) {
+        float2 ml[kJoin];
+        float po[kJoin][V];
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) {
+          const int i = i0 + k * ways;
+          ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int j = 0; j < V; ++j) po[k][j] = 0.f;
+          if (i >= n) continue;
+          const int at = (int)(2 * (p.w0 + (unsigned)i) + (i == 0 ? 1 : 0)) * stride;
+          ml[k] = ld2_agent(parts, at + (heads * d + 2 * g) * 4);
+          if constexpr (V == 4) {
+            const float4 v = ld4_agent(parts, at + e * 16);
+            po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
+          } else {
+            po[k][0] = ld_agent(a.parts + at / 4 + e);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) s.add(ml[k].x, ml[k].y, po[k]);
       }
-      __syncthreads();
-      if (e < heads * d)
-#pragma unroll 4
-        for (int i = 0; i < c; ++i) s = fmaf(js.w[i][g], ld_agent(piece(i0 + i) + e), s);
     }
-    if (e < heads * d) out[e] = js.l[g] == 0.f ? 0.f : s / js.l[g];
+    if (ways > 1) {  // work < nt: one round
+      js.m[tid] = s.m;
+      js.l[tid] = s.l;
+#pragma unroll
+      for (int i = 0; i < V; ++i) js.o[tid][i] = s.o[i];
+      __syncthreads();
+      if (way == 0)
+        for (int k = 1; k < ways; ++k) s.add(js.m[tid + k * work], js.l[tid + k * work], js.o[tid + k * work]);
+    }
+    if (way == 0 && e < work) s.write(out + e * V);
   }
-  __syncthreads();
 }
 
 }  // namespace bnr

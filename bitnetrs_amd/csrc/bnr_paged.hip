@@ -116,11 +116,11 @@ template <int F>
 __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(PagedDecodeArgs a) {
   __shared__ float s_o[kWaves][kPagedMaxDim];
   __shared__ float s_m[kWaves], s_l[kWaves];
-  __shared__ JoinShared s_join;
+  __shared__ JoinShared<kWaves, 1> s_join;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = a.pool.d;
   paged_empty(a);
-  PagedShare sh = paged_share(a.lens, a.batch, a.n_heads, a.pool, kPagedGenericTile, blockIdx.x, a.wgs);
-  for (PagedPiece p; sh.next(p);) {
+  PagedShare sh = paged_share(a, a.n_heads);
+  for (PagedPiece p; sh.next(a.lens, a.pool, p);) {
     const int h = p.h / a.group;
     const float *q = a.q + ((long long)p.b * a.n_heads + p.h) * d;
     float qr[kElems], o[kElems];
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
       s_l[wave] = l;
     }
     __syncthreads();
-    paged_finish<kWaves>(a, p, sh, &s_o[0][0], kPagedMaxDim, s_m, s_l, 1, s_join);
+    paged_finish<kWaves, 1>(a, p, sh.wg, &s_o[0][0], kPagedMaxDim, s_m, s_l, 1, s_join);
   }
 }
 

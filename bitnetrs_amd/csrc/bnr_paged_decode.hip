@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
   constexpr int KE = 16 / B;        // elements of a 16-byte load
   extern __shared__ float s_o[];    // [kW][group][DP]
   __shared__ float s_m[kW * kJoinHeads], s_l[kW * kJoinHeads];
-  __shared__ JoinShared s_join;
+  __shared__ JoinShared<kW, 4> s_join;
   const int lane = threadIdx.x & 63, d = a.pool.d, G = a.group;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int row = lane & 15, g = lane >> 4;
@@ -141,9 +141,9 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
   const unsigned v_off = 4 * g * row_bytes + row * (E * B);
   const bool v_in = FULL || row * E < d;
   paged_empty(a);
-  PagedShare sh = paged_share(a.lens, a.batch, a.pool.n_kv, a.pool, kPagedTile, blockIdx.x, a.wgs);
+  PagedShare sh = paged_share(a, a.pool.n_kv);
 
-  for (PagedPiece p; sh.next(p);) {
+  for (PagedPiece p; sh.next(a.lens, a.pool, p);) {
     const int row1 = __builtin_amdgcn_readfirstlane(p.row1);
     const int hk = __builtin_amdgcn_readfirstlane(p.h);
     const int *table = a.pool.table +
@@ -159,35 +159,6 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
       return ((long long)(pg < 0 ? 0 : pg) * a.pool.n_kv + hk) * a.pool.page +
              (pg < 0 ? 0 : t & (a.pool.page - 1));
     };
-
-    // The query heads as operands: column `row` is head row of the group.
-    QOperands<F, KW> qo;
-    {
-      const float *q = a.q + ((long long)p.b * a.n_heads + (long long)p.h * G + row) * d;
-#pragma unroll
-      for (int c = 0; c < KW; ++c) {
-        const int e0 = (64 * c + 16 * g) / B;
-        const bool in = row < G && (FULL || e0 < d);
-        if constexpr (F == kPagedF32) {
-          const float4 x = in ? ld4(q + e0) : make_float4(0.f, 0.f, 0.f, 0.f);
-          qo.f[4 * c] = x.x;
-          qo.f[4 * c + 1] = x.y;
-          qo.f[4 * c + 2] = x.z;
-          qo.f[4 * c + 3] = x.w;
-        } else {
-#pragma unroll
-          for (int e = 0; e < KE / 8; ++e) {
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (in) {
-              const float4 lo = ld4(q + e0 + 8 * e), hi = ld4(q + e0 + 8 * e + 4);
-              x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
-              x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-            }
-            qo.p[c * (KE / 8) + e] = split8(x);
-          }
-        }
-      }
-    }
 
     float m = -INFINITY, l = 0.f;  // of head `row`; l over this lane's rows only
     f32x4 o[E];
@@ -235,9 +206,39 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
     for (int h = 0; h < 2; ++h) pg[h] = tile_page(t + 16 * h);
 #pragma unroll
     for (int h = 0; h < 2; ++h) pn[h] = tile_page(t + kW * kStep + 16 * h);
+    // The query heads: column `row` is head row of the group.
+    float4 qx[KW * KE / 4];
+    {
+      const float *q = a.q + ((long long)p.b * a.n_heads + (long long)p.h * G + row) * d;
+#pragma unroll
+      for (int c = 0; c < KW; ++c) {
+        const int e0 = (64 * c + 16 * g) / B;
+        const bool in = row < G && (FULL || e0 < d);
+#pragma unroll
+        for (int i = 0; i < KE / 4; ++i)
+          qx[c * (KE / 4) + i] = in ? ld4(q + e0 + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
     if (t < row1) {
       load_k(t, pg);
       load_v(t, pg);
+    }
+    QOperands<F, KW> qo;
+    if constexpr (F == kPagedF32) {
+#pragma unroll
+      for (int c = 0; c < KW; ++c) {
+        qo.f[4 * c] = qx[c].x;
+        qo.f[4 * c + 1] = qx[c].y;
+        qo.f[4 * c + 2] = qx[c].z;
+        qo.f[4 * c + 3] = qx[c].w;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < KW * KE / 8; ++c) {
+        const float4 lo = qx[2 * c], hi = qx[2 * c + 1];
+        const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        qo.p[c] = split8(x);
+      }
     }
     for (; t < row1; t += kW * kStep) {
       // scores: lane has head `row`, rows 4 g + r of both tiles
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
         for (int i = 0; i < E; ++i) so[r * E + i] = o[i][r];
     }
     __syncthreads();
-    paged_finish<kW>(a, p, sh, s_o, DP, s_m, s_l, G, s_join);
+    paged_finish<kW, 4>(a, p, sh.wg, s_o, DP, s_m, s_l, G, s_join);
   }
 }
 
