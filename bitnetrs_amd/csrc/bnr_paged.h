@@ -153,7 +153,7 @@ __host__ __device__ __forceinline__ bool append_row(const PagedAppendArgs &a, lo
 struct PagedPiece {
   int b, h;        // sequence, item
   int row0, row1;  // rows of it
-  unsigned w0, w1;  // the workgroups that share the item: the first, the last
+  unsigned item0, item1;  // the item's units
 };
 
 struct PagedShare {
@@ -183,9 +183,9 @@ struct PagedShare {
     }
     p.b = b;
     p.h = h;
-    const unsigned item1 = item0 + n, to = item1 < end ? item1 : end;
-    p.w0 = at == item0 ? wg : wg_of(item0);
-    p.w1 = item1 <= end ? wg : wg_of(item1 - 1);
+    p.item0 = item0;
+    p.item1 = item0 + n;
+    const unsigned to = p.item1 < end ? p.item1 : end;
     p.row0 = (int)((at - item0) * (unsigned)tile);
     const unsigned r1 = (to - item0) * (unsigned)tile;
     p.row1 = r1 < (unsigned)len ? (int)r1 : len;
@@ -283,21 +283,32 @@ struct JoinShared {
   int last;
 };
 
-// exp2(m - top), 0 for a state without a row (whose m is -inf).
-__device__ __forceinline__ float join_weight(float m, float top) {
-  return m == -INFINITY ? 0.f : fast_exp2(m - top);
-}
+// A running maximum as something to subtract: 0 while there is no row, so that
+// exp2 of what it is subtracted from (-inf) is 0.
+__device__ __forceinline__ float above(float m) { return m == -INFINITY ? 0.f : m; }
 
-// A state of one head and V outputs, and another put to it.
+// A state of one head and V outputs.
 template <int V>
 struct JoinState {
   float m, l, o[V];
-  __device__ __forceinline__ void add(float m2, float l2, const float (&o2)[V]) {
-    const float top = fmaxf(m, m2), f = join_weight(m, top), f2 = join_weight(m2, top);
-    m = top;
-    l = l * f + l2 * f2;
+  // N more states.
+  template <int N>
+  __device__ __forceinline__ void add(const float (&m2)[N], const float (&l2)[N], const float (&o2)[N][V]) {
+    float top = m;
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = o[i] * f + o2[i] * f2;
+    for (int k = 0; k < N; ++k) top = fmaxf(top, m2[k]);
+    const float mu = above(top), f = fast_exp2(m - mu);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] *= f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float w = fast_exp2(m2[k] - mu);
+      l = fmaf(l2[k], w, l);
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = fmaf(o2[k][i], w, o[i]);
+    }
   }
   __device__ __forceinline__ void clear() {
     m = -INFINITY;
@@ -305,43 +316,51 @@ struct JoinState {
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.f;
   }
+  // l is at least 1 wherever there is a row
   __device__ __forceinline__ void write(float *out) const {
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = l == 0.f ? 0.f : o[i] / l;
+    const float r = l == 0.f ? 0.f : 1.0f / l;
+    if constexpr (V == 4)
+      st4(out, make_float4(o[0] * r, o[1] * r, o[2] * r, o[3] * r));
+    else
+      out[0] = o[0] * r;
   }
 };
 
 // V: outputs of a thread, 4 where d is a multiple of 4 and out is 16-byte
-// aligned, or 1.
-template <int W, int V>
-__device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsigned wg, const float *o,
-                             int o_stride, const float *wm, const float *wl, int heads,
+// aligned, or 1.  D: stride of the heads in LDS, a power of two; w0, w1: the
+// first and the last workgroup of the item.
+template <int W, int V, int D>
+__device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsigned wg, unsigned w0,
+                             unsigned w1, const float *o, const float *wm, const float *wl, int heads,
                              JoinShared<W, V> &js) {
-  constexpr int nt = W * 64;
-  const int tid = threadIdx.x, d = a.pool.d, work = heads * d / V;
-  const bool whole = p.w0 == p.w1;
+  constexpr int nt = W * 64, per = D / V;
+  const int tid = threadIdx.x, d = a.pool.d, work = heads * per;
+  const bool whole = w0 == w1;
   float *out = a.out + ((long long)p.b * a.n_heads + (long long)p.h * heads) * d;
   const __amdgpu_buffer_rsrc_t parts = agent_buf(a.parts);
   const int stride = a.part_floats * 4;
-  const int mine = (int)(2 * wg + (wg == p.w0 ? 1 : 0)) * stride;
+  const int mine = (int)(2 * wg + (wg == w0 ? 1 : 0)) * stride;
   for (int e = tid; e < work; e += nt) {
-    const int g = e * V / d, x = e * V - g * d;
+    const int g = e / per, x = e % per * V;
+    if (x >= d) continue;
     JoinState<V> s;
     s.clear();
+    float m[W], l[W], ow[W][V];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      float ow[V];
+      m[w] = wm[w * heads + g];
+      l[w] = wl[w * heads + g];
 #pragma unroll
-      for (int i = 0; i < V; ++i) ow[i] = o[(w * heads + g) * o_stride + x + i];
-      s.add(wm[w * heads + g], wl[w * heads + g], ow);
+      for (int i = 0; i < V; ++i) ow[w][i] = o[(w * heads + g) * D + x + i];
     }
+    s.add(m, l, ow);
     if (whole) {
-      s.write(out + e * V);
+      s.write(out + g * d + x);
     } else {
       if constexpr (V == 4)
-        st4_agent(parts, mine + e * 16, make_float4(s.o[0], s.o[1], s.o[2], s.o[3]));
+        st4_agent(parts, mine + (g * d + x) * 4, make_float4(s.o[0], s.o[1], s.o[2], s.o[3]));
       else
-        st_agent(a.parts + mine / 4 + e, s.o[0]);
+        st_agent(a.parts + mine / 4 + g * d + x, s.o[0]);
       if (x == 0) st2_agent(parts, mine + (heads * d + 2 * g) * 4, s.m, s.l);
     }
   }
@@ -350,7 +369,7 @@ __device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsi
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   unsigned *ticket = a.tickets + (size_t)p.b * (a.n_heads / heads) + p.h;
-  const int n = (int)(p.w1 - p.w0) + 1;
+  const int n = (int)(w1 - w0) + 1;
   if (tid == 0)
     js.last = (int)__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
   __syncthreads();
@@ -362,32 +381,32 @@ __device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsi
   const int ways = work >= nt ? 1 : nt / work;
   for (int e0 = 0; e0 < work; e0 += nt) {
     const int way = work >= nt ? 0 : tid / work, e = work >= nt ? e0 + tid : tid - way * work;
+    const int g = e / per, x = e % per * V;
+    const bool in = way < ways && e < work && x < d;
     JoinState<V> s;
     s.clear();
-    if (way < ways && e < work) {
-      const int g = e * V / d;
-      for (int i0 = way; i0 < n; i0 += kJoin * ways) {
-        float2 ml[kJoin];
-        float po[kJoin][V];
+    for (int i0 = way; in && i0 < n; i0 += kJoin * ways) {
+      float m[kJoin], l[kJoin], po[kJoin][V];
 #pragma unroll
-        for (int k = 0; k < kJoin; ++k) {
-          const int i = i0 + k * ways;
-          ml[k] = make_float2(-INFINITY, 0.f);
+      for (int k = 0; k < kJoin; ++k) {
+        const int i = i0 + k * ways;
+        m[k] = -INFINITY;
+        l[k] = 0.f;
 #pragma unroll
-          for (int j = 0; j < V; ++j) po[k][j] = 0.f;
-          if (i >= n) continue;
-          const int at = (int)(2 * (p.w0 + (unsigned)i) + (i == 0 ? 1 : 0)) * stride;
-          ml[k] = ld2_agent(parts, at + (heads * d + 2 * g) * 4);
-          if constexpr (V == 4) {
-            const float4 v = ld4_agent(parts, at + e * 16);
-            po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
-          } else {
-            po[k][0] = ld_agent(a.parts + at / 4 + e);
-          }
+        for (int j = 0; j < V; ++j) po[k][j] = 0.f;
+        if (i >= n) continue;
+        const int at = (int)(2 * (w0 + (unsigned)i) + (i == 0 ? 1 : 0)) * stride;
+        const float2 ml = ld2_agent(parts, at + (heads * d + 2 * g) * 4);
+        m[k] = ml.x;
+        l[k] = ml.y;
+        if constexpr (V == 4) {
+          const float4 v = ld4_agent(parts, at + (g * d + x) * 4);
+          po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
+        } else {
+          po[k][0] = ld_agent(a.parts + at / 4 + g * d + x);
         }
-#pragma unroll
-        for (int k = 0; k < kJoin; ++k) s.add(ml[k].x, ml[k].y, po[k]);
       }
+      s.add(m, l, po);
     }
     if (ways > 1) {  // work < nt: one round
       js.m[tid] = s.m;
@@ -396,9 +415,16 @@ __device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsi
       for (int i = 0; i < V; ++i) js.o[tid][i] = s.o[i];
       __syncthreads();
       if (way == 0)
-        for (int k = 1; k < ways; ++k) s.add(js.m[tid + k * work], js.l[tid + k * work], js.o[tid + k * work]);
+        for (int k = 1; k < ways; ++k) {
+          const int at = tid + k * work;
+          const float m[1] = {js.m[at]}, l[1] = {js.l[at]};
+          float po[1][V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) po[0][i] = js.o[at][i];
+          s.add(m, l, po);
+        }
     }
-    if (way == 0 && e < work) s.write(out + e * V);
+    if (way == 0 && in) s.write(out + g * d + x);
   }
 }
 

@@ -39,6 +39,10 @@ constexpr int kStep = 32;  // rows of a wave's step
 template <int F>
 constexpr int kBytes = F == kPagedF32 ? 4 : F == kPagedBf16 ? 2 : 1;
 
+// Waves of a SIMD that the registers are shared out for.
+template <int F, int DP>
+constexpr int kWavesOf = DP == 256 ? (F == kPagedInt8 || F == kPagedFp8 ? 2 : 1) : F == kPagedF32 ? 2 : 3;
+
 // `n` bytes (a multiple of 4, at most 64) at p, read once.
 template <int N>
 __device__ __forceinline__ void load_bytes(const char *p, unsigned (&r)[N]) {
@@ -111,25 +115,23 @@ __device__ __forceinline__ u32x4 widen8(unsigned a, unsigned b) {
   return r;
 }
 
-// Scores of 16 rows x 16 heads, before the scales: the rows' dwords as loaded,
-// the heads' operands from q_operands.
-template <int F, int KW>
-struct QOperands {
-  static constexpr int kN = F == kPagedF32 ? KW * 4 : KW * (F == kPagedBf16 ? 1 : 2);
-  Parts p[F == kPagedF32 ? 1 : kN];
-  float f[F == kPagedF32 ? kN : 1];
-};
+// The query heads as operands of the first product, in LDS for the whole
+// workgroup: chunk c of a lane's operand is at q[c * 64 + lane].
+// f32: four of the lane's floats; else eight dims as bf16, chunk (c, part).
+template <int F, int DP>
+constexpr int kQChunks = F == kPagedF32 ? DP / 16 : DP / 32 * 3;
 
 // One workgroup's share of the line; waves take steps of kStep rows in turn.
 // DP: head dim, rounded up to 64, 128 or 256; FULL: head dim is DP.
 template <int F, int DP, bool FULL>
-__global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeArgs a) {
+__global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kernel(PagedDecodeArgs a) {
   constexpr int B = kBytes<F>;
   constexpr int E = DP / 16;        // dims of a lane and V row
   constexpr int KW = DP * B / 64;   // 16-byte loads of a lane and K tile
   constexpr int VW = E * B / 4;     // dwords of a lane and V row
-  constexpr int KE = 16 / B;        // elements of a 16-byte load
+  constexpr int QN = kQChunks<F, DP>;
   extern __shared__ float s_o[];    // [kW][group][DP]
+  __shared__ u32x4 s_q[QN * 64];
   __shared__ float s_m[kW * kJoinHeads], s_l[kW * kJoinHeads];
   __shared__ JoinShared<kW, 4> s_join;
   const int lane = threadIdx.x & 63, d = a.pool.d, G = a.group;
@@ -146,19 +148,39 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
   for (PagedPiece p; sh.next(a.lens, a.pool, p);) {
     const int row1 = __builtin_amdgcn_readfirstlane(p.row1);
     const int hk = __builtin_amdgcn_readfirstlane(p.h);
-    const int *table = a.pool.table +
-                       (long long)__builtin_amdgcn_readfirstlane(p.b) * a.pool.table_stride;
+    const int bs = __builtin_amdgcn_readfirstlane(p.b);
+    const int *table = a.pool.table + (long long)bs * a.pool.table_stride;
+    int t = __builtin_amdgcn_readfirstlane(p.row0) + kStep * wave;
 
-    // The page of the 16-row tile at row t, or -1: past the piece, or not there.
-    auto tile_page = [&](int t) {
-      int pg = t < row1 ? table[t >> page_shift] : -1;
-      return __builtin_amdgcn_readfirstlane(pg < 0 || pg >= a.pool.n_pages ? -1 : pg);
+    // Pages of the wave's next 32 steps, lane 2 i + h that of tile h of step
+    // i: one load for all of them.  -1: past the piece, or not there.
+    auto load_pages = [&](int t0) {
+      const int at = t0 + (lane >> 1) * (kW * kStep) + (lane & 1) * 16;
+      const int pg = at < row1 ? table[at >> page_shift] : -1;
+      return (unsigned)pg < (unsigned)a.pool.n_pages ? pg : -1;
     };
-    // First row of that tile in the pool, in rows; page 0's where there is none.
-    auto tile_row = [&](int pg, int t) {
-      return ((long long)(pg < 0 ? 0 : pg) * a.pool.n_kv + hk) * a.pool.page +
-             (pg < 0 ? 0 : t & (a.pool.page - 1));
-    };
+    int pages = load_pages(t), step = 0;
+
+    // This workgroup's part of the operands in LDS.
+    __syncthreads();  // the piece before this one has been read
+    for (int c = wave; c < (F == kPagedF32 ? QN : QN / 3); c += kW) {
+      const float *q = a.q + ((long long)bs * a.n_heads + (long long)hk * G + row) * d;
+      // the dims that a lane's K bytes hold: 16 bytes at 64 c' + 16 g of the row
+      const int e0 = F == kPagedF32    ? 16 * c + 4 * g
+                     : F == kPagedBf16 ? 32 * c + 8 * g
+                                       : 64 * (c >> 1) + 16 * g + 8 * (c & 1);
+      const bool in = row < G && (FULL || e0 < d);
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), lo = in ? ld4(q + e0) : zero;
+      if constexpr (F == kPagedF32) {
+        s_q[c * 64 + lane] = __builtin_bit_cast(u32x4, lo);
+      } else {
+        const float4 hi = in ? ld4(q + e0 + 4) : zero;
+        const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        const Parts s = split8(x);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) s_q[(c * 3 + k) * 64 + lane] = s.p[k];
+      }
+    }
 
     float m = -INFINITY, l = 0.f;  // of head `row`; l over this lane's rows only
     f32x4 o[E];
@@ -167,6 +189,11 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
 
     unsigned kr[2][KW * 4], vr[2][4][VW];
     f32x4 ks[2], vs[2];
+    // First row, in rows of the pool, of the 16-row tile at row t; page 0's where there is none.
+    auto tile_row = [&](int pg, int t) {
+      return ((long long)(pg < 0 ? 0 : pg) * a.pool.n_kv + hk) * a.pool.page +
+             (pg < 0 ? 0 : t & (a.pool.page - 1));
+    };
     auto load_k = [&](int t, const int (&pg)[2]) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -200,69 +227,55 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
       }
     };
 
-    int t = __builtin_amdgcn_readfirstlane(p.row0) + kStep * wave;
     int pg[2], pn[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) pg[h] = tile_page(t + 16 * h);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) pn[h] = tile_page(t + kW * kStep + 16 * h);
-    // The query heads: column `row` is head row of the group.
-    float4 qx[KW * KE / 4];
-    {
-      const float *q = a.q + ((long long)p.b * a.n_heads + (long long)p.h * G + row) * d;
-#pragma unroll
-      for (int c = 0; c < KW; ++c) {
-        const int e0 = (64 * c + 16 * g) / B;
-        const bool in = row < G && (FULL || e0 < d);
-#pragma unroll
-        for (int i = 0; i < KE / 4; ++i)
-          qx[c * (KE / 4) + i] = in ? ld4(q + e0 + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+    for (int h = 0; h < 2; ++h) {
+      pg[h] = __builtin_amdgcn_readlane(pages, h);
+      pn[h] = __builtin_amdgcn_readlane(pages, 2 + h);
     }
     if (t < row1) {
       load_k(t, pg);
       load_v(t, pg);
     }
-    QOperands<F, KW> qo;
-    if constexpr (F == kPagedF32) {
-#pragma unroll
-      for (int c = 0; c < KW; ++c) {
-        qo.f[4 * c] = qx[c].x;
-        qo.f[4 * c + 1] = qx[c].y;
-        qo.f[4 * c + 2] = qx[c].z;
-        qo.f[4 * c + 3] = qx[c].w;
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < KW * KE / 8; ++c) {
-        const float4 lo = qx[2 * c], hi = qx[2 * c + 1];
-        const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        qo.p[c] = split8(x);
-      }
-    }
+    // while they are on their way
+    const unsigned w0 = sh.wg_of(p.item0), w1 = sh.wg_of(p.item1 - 1);
+    __syncthreads();  // the operands
     for (; t < row1; t += kW * kStep) {
       // scores: lane has head `row`, rows 4 g + r of both tiles
-      f32x4 s[2];
+      f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      // read again in each step: kept in registers the operands would cost a wave of a SIMD
+      int ql = lane;
+      asm volatile("" : "+v"(ql));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < KW; ++c) {
+        if constexpr (F == kPagedF32) {
+          const f32x4 qc = __builtin_bit_cast(f32x4, s_q[c * 64 + ql]);
 #pragma unroll
-        for (int c = 0; c < KW; ++c) {
-          if constexpr (F == kPagedF32) {
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int h = 0; h < 2; ++h)
               s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                  __builtin_bit_cast(float, kr[h][4 * c + i]), qo.f[4 * c + i], s[h], 0, 0, 0);
-          } else if constexpr (F == kPagedBf16) {
-            const u32x4 w = {kr[h][4 * c], kr[h][4 * c + 1], kr[h][4 * c + 2], kr[h][4 * c + 3]};
+                  __builtin_bit_cast(float, kr[h][4 * c + i]), qc[i], s[h], 0, 0, 0);
+        } else if constexpr (F == kPagedBf16) {
 #pragma unroll
-            for (int k = 0; k < 3; ++k) s[h] = mfma_bf16(w, qo.p[c].p[k], s[h]);
-          } else {
+          for (int k = 0; k < 3; ++k) {
+            const u32x4 qc = s_q[(c * 3 + k) * 64 + ql];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const u32x4 w = widen8<F>(kr[h][4 * c + 2 * e], kr[h][4 * c + 2 * e + 1]);
+            for (int h = 0; h < 2; ++h)
+              s[h] = mfma_bf16(u32x4{kr[h][4 * c], kr[h][4 * c + 1], kr[h][4 * c + 2], kr[h][4 * c + 3]},
+                               qc, s[h]);
+          }
+        } else {
 #pragma unroll
-              for (int k = 0; k < 3; ++k) s[h] = mfma_bf16(w, qo.p[2 * c + e].p[k], s[h]);
+          for (int e = 0; e < 2; ++e) {
+            u32x4 w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[h] = widen8<F>(kr[h][4 * c + 2 * e], kr[h][4 * c + 2 * e + 1]);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              const u32x4 qc = s_q[((2 * c + e) * 3 + k) * 64 + ql];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) s[h] = mfma_bf16(w[h], qc, s[h]);
             }
           }
         }
@@ -282,9 +295,6 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
             if (pg[h] < 0 || t + 16 * h + 4 * g + r >= row1) x[4 * h + r] = -INFINITY;
       // the next step's K goes out while this one's weights are made
       const int tn = t + kW * kStep;
-      int p2[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) p2[h] = tile_page(tn + kW * kStep + 16 * h);
       if (tn < row1) load_k(tn, pn);
 
       float mx = m;
@@ -293,13 +303,13 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
       if (__any(mx > m)) {
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float keep = join_weight(m, mx);
+        const float keep = fast_exp2(m - above(mx));
         m = mx;
         l *= keep;
 #pragma unroll
         for (int i = 0; i < E; ++i) o[i] *= keep;
       }
-      const float mu = m == -INFINITY ? 0.f : m;
+      const float mu = above(m);
       float w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -349,16 +359,20 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
         }
       }
       if (tn < row1) load_v(tn, pn);
+      // pages of the step after the next
+      if (++step == 31) {
+        pages = load_pages(tn + kW * kStep);
+        step = -1;
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         pg[h] = pn[h];
-        pn[h] = p2[h];
+        pn[h] = __builtin_amdgcn_readlane(pages, 2 * (step + 1) + h);
       }
     }
 
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    __syncthreads();  // the piece before this one has been read
     if (row < G) {
       if (g == 0) {
         s_m[wave * G + row] = m;
@@ -371,7 +385,7 @@ __global__ __launch_bounds__(64 * kW, DP == 256 ? 1 : 2) void paged_decode_kerne
         for (int i = 0; i < E; ++i) so[r * E + i] = o[i][r];
     }
     __syncthreads();
-    paged_finish<kW, 4>(a, p, sh.wg, s_o, DP, s_m, s_l, G, s_join);
+    paged_finish<kW, 4, DP>(a, p, sh.wg, w0, w1, s_o, s_m, s_l, G, s_join);
   }
 }
 
@@ -381,8 +395,8 @@ hipError_t launch_format(const PagedDecodeArgs &a, hipStream_t s) {
   const int dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
   const size_t lds = (size_t)kW * a.group * dp * sizeof(float);
   const dim3 grid((unsigned)a.wgs), block(64 * kW);
-  // more than the 64 KB a workgroup gets unasked: 16 heads of 256
-  constexpr size_t kUnasked = 60 * 1024;
+  // what a workgroup gets unasked is 64 KB, of which up to 32 are static
+  constexpr size_t kUnasked = 32 * 1024;
 #define BNR_LAUNCH(DP)                                          \
   {                                                             \
     const auto kernel = d == DP ? paged_decode_kernel<F, DP, true> : paged_decode_kernel<F, DP, false>; \
