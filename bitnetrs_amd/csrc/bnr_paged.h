@@ -215,13 +215,13 @@ __device__ __forceinline__ unsigned lane_of(unsigned v, int lane) {
 __device__ __forceinline__ PagedShare paged_share(const PagedDecodeArgs &a, int items) {
   const int lane = threadIdx.x & 63;
   const unsigned tile = (unsigned)a.tile, wgs = (unsigned)a.wgs;
-  // Units of an item of each sequence, 64 sequences at a time.
-  auto units = [&](int b) -> unsigned {
-    return b < a.batch ? ((unsigned)paged_len(a.lens[b], a.pool) + tile - 1) / tile : 0u;
-  };
-  const unsigned first = wave_scan(units(lane));
+  // Lengths, and units of an item, of each sequence, 64 sequences at a time.
+  auto length = [&](int b) { return b < a.batch ? paged_len(a.lens[b], a.pool) : 0; };
+  auto units = [&](int len) { return ((unsigned)len + tile - 1) / tile; };
+  const int first_len = length(lane);
+  const unsigned first = wave_scan(units(first_len));
   unsigned total = lane_of(first, 63);
-  for (int b0 = 64; b0 < a.batch; b0 += 64) total += lane_of(wave_scan(units(b0 + lane)), 63);
+  for (int b0 = 64; b0 < a.batch; b0 += 64) total += lane_of(wave_scan(units(length(b0 + lane))), 63);
   total *= (unsigned)items;
   PagedShare s;
   s.wg = blockIdx.x;
@@ -235,29 +235,38 @@ __device__ __forceinline__ PagedShare paged_share(const PagedDecodeArgs &a, int 
   // The sequence that has unit `at`, and the item of it.
   const unsigned want = s.at / (unsigned)items;
   unsigned before = 0, incl = first;
+  int len = first_len;
   for (int b0 = 0;; b0 += 64) {
-    if (b0) incl = wave_scan(units(b0 + lane));
+    if (b0) {
+      len = length(b0 + lane);
+      incl = wave_scan(units(len));
+    }
     const unsigned sum = lane_of(incl, 63);
     if (want < before + sum) {
       const int k = __builtin_ctzll(__ballot(before + incl > want));
       const unsigned lo = k ? lane_of(incl, k - 1) : 0u;
       s.b = b0 + k;
       s.n = lane_of(incl, k) - lo;
+      s.len = (int)lane_of((unsigned)len, k);
       before += lo;
       break;
     }
     before += sum;
   }
-  s.len = paged_len(a.lens[s.b], a.pool);
   s.h = (int)((s.at - before * (unsigned)items) / s.n);
   s.item0 = before * (unsigned)items + (unsigned)s.h * s.n;
   return s;
 }
 
 // A sequence without a row has no unit on the line; its outputs are zeros.
-__device__ __forceinline__ void paged_empty(const PagedDecodeArgs &a) {
+// Workgroup w sees to sequences w, w + wgs, ...; first_len: lens[w], loaded at
+// the kernel's start so that its end does not wait for it (1 past the batch).
+__device__ __forceinline__ int paged_first_len(const PagedDecodeArgs &a) {
+  return (int)blockIdx.x < a.batch ? a.lens[blockIdx.x] : 1;
+}
+__device__ __forceinline__ void paged_empty(const PagedDecodeArgs &a, int first_len) {
   for (int b = (int)blockIdx.x; b < a.batch; b += a.wgs) {
-    if (a.lens[b] > 0) continue;
+    if ((b == (int)blockIdx.x ? first_len : a.lens[b]) > 0) continue;
     float *out = a.out + (long long)b * a.n_heads * a.pool.d;
     for (int e = (int)threadIdx.x; e < a.n_heads * a.pool.d; e += (int)blockDim.x) out[e] = 0.f;
   }

@@ -118,7 +118,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
   __shared__ float s_m[kWaves], s_l[kWaves];
   __shared__ JoinShared<kWaves, 1> s_join;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = a.pool.d;
-  paged_empty(a);
+  const int first_len = paged_first_len(a);
   PagedShare sh = paged_share(a, a.n_heads);
   for (PagedPiece p; sh.next(a.lens, a.pool, p);) {
     const int h = p.h / a.group;
@@ -164,6 +164,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
     paged_finish<kWaves, 1, kPagedMaxDim>(a, p, sh.wg, sh.wg_of(p.item0), sh.wg_of(p.item1 - 1),
                                           &s_o[0][0], s_m, s_l, 1, s_join);
   }
+  paged_empty(a, first_len);
 }
 
 }  // namespace

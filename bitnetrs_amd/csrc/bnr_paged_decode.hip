@@ -101,13 +101,20 @@ __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
 template <int F, int I>
 __device__ __forceinline__ float code8(unsigned w) {
   if constexpr (F == kPagedInt8) return (float)(signed char)(w >> (8 * I));
-  return __builtin_amdgcn_cvt_f32_fp8((int)w, I);
+  return __builtin_amdgcn_cvt_pk_f32_fp8((int)w, I >= 2)[I & 1];
 }
 
 // 8 codes (two dwords) as bf16.
 template <int F>
 __device__ __forceinline__ u32x4 widen8(unsigned a, unsigned b) {
   u32x4 r;
+  if constexpr (F == kPagedFp8) {  // two codes an instruction
+    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false));
+    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true));
+    r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false));
+    r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true));
+    return r;
+  }
   r[0] = pack_hi(code8<F, 0>(a), code8<F, 1>(a));
   r[1] = pack_hi(code8<F, 2>(a), code8<F, 3>(a));
   r[2] = pack_hi(code8<F, 0>(b), code8<F, 1>(b));
@@ -142,7 +149,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
   const unsigned k_off = row * row_bytes + 16 * g;
   const unsigned v_off = 4 * g * row_bytes + row * (E * B);
   const bool v_in = FULL || row * E < d;
-  paged_empty(a);
+  const int first_len = paged_first_len(a);
   PagedShare sh = paged_share(a, a.pool.n_kv);
 
   for (PagedPiece p; sh.next(a.lens, a.pool, p);) {
@@ -161,25 +168,21 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
     };
     int pages = load_pages(t), step = 0;
 
-    // This workgroup's part of the operands in LDS.
-    __syncthreads();  // the piece before this one has been read
-    for (int c = wave; c < (F == kPagedF32 ? QN : QN / 3); c += kW) {
+    // The wave's chunks of the query heads: the dims that a lane's K bytes
+    // hold, 16 bytes at 64 c + 16 g of the row.
+    constexpr int QL = F == kPagedF32 ? QN : QN / 3, QC = (QL + kW - 1) / kW;
+    float4 qx[QC][F == kPagedF32 ? 1 : 2];
+#pragma unroll
+    for (int i = 0; i < QC; ++i) {
+      const int c = wave + i * kW;
       const float *q = a.q + ((long long)bs * a.n_heads + (long long)hk * G + row) * d;
-      // the dims that a lane's K bytes hold: 16 bytes at 64 c' + 16 g of the row
       const int e0 = F == kPagedF32    ? 16 * c + 4 * g
                      : F == kPagedBf16 ? 32 * c + 8 * g
                                        : 64 * (c >> 1) + 16 * g + 8 * (c & 1);
-      const bool in = row < G && (FULL || e0 < d);
-      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), lo = in ? ld4(q + e0) : zero;
-      if constexpr (F == kPagedF32) {
-        s_q[c * 64 + lane] = __builtin_bit_cast(u32x4, lo);
-      } else {
-        const float4 hi = in ? ld4(q + e0 + 4) : zero;
-        const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        const Parts s = split8(x);
+      const bool in = c < QL && row < G && (FULL || e0 < d);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) s_q[(c * 3 + k) * 64 + lane] = s.p[k];
-      }
+      for (int k = 0; k < (F == kPagedF32 ? 1 : 2); ++k)
+        qx[i][k] = in ? ld4(q + e0 + 4 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 
     float m = -INFINITY, l = 0.f;  // of head `row`; l over this lane's rows only
@@ -238,6 +241,21 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
       load_v(t, pg);
     }
     // while they are on their way
+    __syncthreads();  // the piece before this one has been read
+#pragma unroll
+    for (int i = 0; i < QC; ++i) {
+      const int c = wave + i * kW;
+      if (c >= QL) break;
+      if constexpr (F == kPagedF32) {
+        s_q[c * 64 + lane] = __builtin_bit_cast(u32x4, qx[i][0]);
+      } else {
+        const float4 lo = qx[i][0], hi = qx[i][1];
+        const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        const Parts s = split8(x);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) s_q[(c * 3 + k) * 64 + lane] = s.p[k];
+      }
+    }
     const unsigned w0 = sh.wg_of(p.item0), w1 = sh.wg_of(p.item1 - 1);
     __syncthreads();  // the operands
     for (; t < row1; t += kW * kStep) {
@@ -387,6 +405,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
     __syncthreads();
     paged_finish<kW, 4, DP>(a, p, sh.wg, w0, w1, s_o, s_m, s_l, G, s_join);
   }
+  paged_empty(a, first_len);
 }
 
 template <int F>
