@@ -274,8 +274,8 @@ __device__ __forceinline__ void paged_empty(const PagedDecodeArgs &a, int first_
 
 // ---------------------------------------------------------------------------
 // The end of a piece.  The workgroup's waves have left their states in LDS:
-// for each of `heads` query heads a maximum, a sum and d unnormalised outputs
-// (wave w, head g at o[(w * heads + g) * o_stride]).  A piece that is a whole
+// for each of `heads` query heads a maximum, a sum (wm, wl: [wave][head]) and
+// d unnormalised outputs (get(w, g, x, o): V of them from x on).  A piece that is a whole
 // item is normalised and written.  Otherwise it goes to the launch's
 // workspace; the last workgroup to bring a piece of the item joins all of
 // them, in the line's order, so the same inputs give the same bits.
@@ -336,12 +336,12 @@ struct JoinState {
 };
 
 // V: outputs of a thread, 4 where d is a multiple of 4 and out is 16-byte
-// aligned, or 1.  D: stride of the heads in LDS, a power of two; w0, w1: the
-// first and the last workgroup of the item.
-template <int W, int V, int D>
-__device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsigned wg, unsigned w0,
-                             unsigned w1, const float *o, const float *wm, const float *wl, int heads,
-                             JoinShared<W, V> &js) {
+// aligned, or 1.  D: d rounded up to a power of two; w0, w1: the first and the
+// last workgroup of the item.
+template <int W, int V, int D, class Get>
+__device__ __forceinline__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsigned wg,
+                                             unsigned w0, unsigned w1, Get get, const float *wm,
+                                             const float *wl, int heads, JoinShared<W, V> &js) {
   constexpr int nt = W * 64, per = D / V;
   const int tid = threadIdx.x, d = a.pool.d, work = heads * per;
   const bool whole = w0 == w1;
@@ -359,8 +359,7 @@ __device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsi
     for (int w = 0; w < W; ++w) {
       m[w] = wm[w * heads + g];
       l[w] = wl[w * heads + g];
-#pragma unroll
-      for (int i = 0; i < V; ++i) ow[w][i] = o[(w * heads + g) * D + x + i];
+      get(w, g, x, ow[w]);
     }
     s.add(m, l, ow);
     if (whole) {
@@ -398,12 +397,8 @@ __device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsi
       float m[kJoin], l[kJoin], po[kJoin][V];
 #pragma unroll
       for (int k = 0; k < kJoin; ++k) {
-        const int i = i0 + k * ways;
-        m[k] = -INFINITY;
-        l[k] = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) po[k][j] = 0.f;
-        if (i >= n) continue;
+        // past the last piece: the last again, without a weight (a branch would part the loads)
+        const int i = i0 + k * ways < n ? i0 + k * ways : n - 1;
         const int at = (int)(2 * (w0 + (unsigned)i) + (i == 0 ? 1 : 0)) * stride;
         const float2 ml = ld2_agent(parts, at + (heads * d + 2 * g) * 4);
         m[k] = ml.x;
@@ -414,6 +409,14 @@ __device__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsi
         } else {
           po[k][0] = ld_agent(a.parts + at / 4 + g * d + x);
         }
+      }
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k) {
+        const bool there = i0 + k * ways < n;
+        m[k] = there ? m[k] : -INFINITY;
+        l[k] = there ? l[k] : 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) po[k][j] = there ? po[k][j] : 0.f;
       }
       s.add(m, l, po);
     }

@@ -15,7 +15,9 @@
 // one element of 8 rows from each lane: a lane reads E neighbouring elements
 // of its 8 rows, and output dim E * i + m belongs to row i of product m, so
 // the transposition is inside the lane (byte permutes, or the conversion that
-// the 8-bit formats need anyway).
+// the 8-bit formats need anyway).  More than 16 bytes of a row (E = u * U) are
+// u units of 16, each over the 16 lanes' neighbouring bytes: dim 16 U unit +
+// U i + m.
 //
 // Precision.  f32 rows multiply on the f32 matrix cores.  bf16, e4m3 and
 // int8 codes are exact in bf16; q and the weights are cut into three bf16
@@ -136,8 +138,11 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
   constexpr int E = DP / 16;        // dims of a lane and V row
   constexpr int KW = DP * B / 64;   // 16-byte loads of a lane and K tile
   constexpr int VW = E * B / 4;     // dwords of a lane and V row
+  constexpr int U = E * B > 16 ? 16 / B : E, VU = E / U;  // dims of a unit, units
   constexpr int QN = kQChunks<F, DP>;
-  extern __shared__ float s_o[];    // [kW][group][DP]
+  // outputs of the waves, four dims at a time: [kW][E][4 group + 1], lane (g, row) of quad q at
+  // q * (4 group + 1) + g * group + row, which is free of bank conflicts both ways
+  extern __shared__ f32x4 s_o[];
   __shared__ u32x4 s_q[QN * 64];
   __shared__ float s_m[kW * kJoinHeads], s_l[kW * kJoinHeads];
   __shared__ JoinShared<kW, 4> s_join;
@@ -147,8 +152,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
   const int page_shift = __builtin_ctz(a.pool.page);
   const unsigned row_bytes = (unsigned)d * B;
   const unsigned k_off = row * row_bytes + 16 * g;
-  const unsigned v_off = 4 * g * row_bytes + row * (E * B);
-  const bool v_in = FULL || row * E < d;
+  const unsigned v_off = 4 * g * row_bytes + row * (U * B);
   const int first_len = paged_first_len(a);
   PagedShare sh = paged_share(a, a.pool.n_kv);
 
@@ -219,12 +223,15 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
         const char *src = static_cast<const char *>(a.pool.v) + at * row_bytes;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          unsigned w[VW];
 #pragma unroll
-          for (int i = 0; i < VW; ++i) w[i] = 0u;
-          if (v_in) load_bytes(src + v_off + r * row_bytes, w);
+          for (int u = 0; u < VU; ++u) {
+            unsigned w[VW / VU];
 #pragma unroll
-          for (int i = 0; i < VW; ++i) vr[h][r][i] = w[i];
+            for (int i = 0; i < VW / VU; ++i) w[i] = 0u;
+            if (FULL || 16 * U * u + U * row < d) load_bytes(src + v_off + r * row_bytes + 16 * U * B * u, w);
+#pragma unroll
+            for (int i = 0; i < VW / VU; ++i) vr[h][r][u * (VW / VU) + i] = w[i];
+          }
         }
         if (kPagedScaled<F>) vs[h] = *reinterpret_cast<const f32x4 *>(a.pool.v_scales + at + 4 * g);
       }
@@ -396,14 +403,21 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
         s_m[wave * G + row] = m;
         s_l[wave * G + row] = l;
       }
-      float *so = s_o + (wave * G + row) * DP + 4 * g * E;
+      f32x4 *so = s_o + wave * E * (4 * G + 1) + g * G + row;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < E; ++i) so[r * E + i] = o[i][r];
+        for (int i = 0; i < E; i += 4)
+          so[(r * (E / 4) + i / 4) * (4 * G + 1)] = f32x4{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]};
     }
     __syncthreads();
-    paged_finish<kW, 4, DP>(a, p, sh.wg, w0, w1, s_o, s_m, s_l, G, s_join);
+    const auto get = [&](int w, int hd, int x, float(&to)[4]) {
+      const int i = x / (16 * U) * U + x % U, rg = x % (16 * U) / U;  // element of the lane; 4 g + r
+      const f32x4 v = s_o[(w * E + (rg & 3) * (E / 4) + i / 4) * (4 * G + 1) + (rg >> 2) * G + hd];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) to[k] = v[k];
+    };
+    paged_finish<kW, 4, DP>(a, p, sh.wg, w0, w1, get, s_m, s_l, G, s_join);
   }
   paged_empty(a, first_len);
 }
@@ -412,7 +426,7 @@ template <int F>
 hipError_t launch_format(const PagedDecodeArgs &a, hipStream_t s) {
   const int d = a.pool.d;
   const int dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
-  const size_t lds = (size_t)kW * a.group * dp * sizeof(float);
+  const size_t lds = (size_t)kW * (dp / 16) * (4 * a.group + 1) * sizeof(f32x4);
   const dim3 grid((unsigned)a.wgs), block(64 * kW);
   // what a workgroup gets unasked is 64 KB, of which up to 32 are static
   constexpr size_t kUnasked = 32 * 1024;
