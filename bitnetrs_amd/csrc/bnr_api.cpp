@@ -2810,7 +2810,10 @@ extern "C" int bnr_dev_paged_append(bnr_ctx *c, const bnr_paged_kv *kv, const fl
   a.n_seqs = (long long)n_seqs;
   a.n_heads = (int)n_heads;
   DeviceGuard dg(c->device);
-  HIP_TRY(launch_paged_append(a, kv->format, (hipStream_t)stream), "paged append launch");
+  const bool vec = kv->head_dim % 8 == 0 && aligned16(q) && aligned16(q_out) && aligned16(k) &&
+                   aligned16(v) && aligned16(cos_tab) && aligned16(sin_tab) && aligned16(kv->k) &&
+                   aligned16(kv->v);
+  HIP_TRY(launch_paged_append(a, kv->format, vec, (hipStream_t)stream), "paged append launch");
   return set_ok();
 }
 
@@ -2837,7 +2840,9 @@ extern "C" int bnr_dev_paged_read(bnr_ctx *c, const bnr_paged_kv *kv, const int3
   a.batch = (long long)batch;
   a.cap = (long long)cap;
   DeviceGuard dg(c->device);
-  HIP_TRY(launch_paged_read(a, kv->format, (hipStream_t)stream), "paged read launch");
+  const bool vec = kv->head_dim % 4 == 0 && aligned16(kv->k) && aligned16(kv->v) &&
+                   aligned16(k_out) && aligned16(v_out);
+  HIP_TRY(launch_paged_read(a, kv->format, vec, (hipStream_t)stream), "paged read launch");
   return set_ok();
 }
 

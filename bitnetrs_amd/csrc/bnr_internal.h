@@ -712,7 +712,8 @@ struct PagedAppendArgs {
   long long n_tokens, n_seqs;
   int n_heads;
 };
-hipError_t launch_paged_append(const PagedAppendArgs &a, int format, hipStream_t s);
+// vec: d a multiple of 8; q, q_out, k, v, the tables and the pool 16-byte aligned.
+hipError_t launch_paged_append(const PagedAppendArgs &a, int format, bool vec, hipStream_t s);
 
 struct PagedReadArgs {
   PagedPool pool;
@@ -720,7 +721,8 @@ struct PagedReadArgs {
   float *k_out, *v_out;      // [batch][n_kv][cap][d]
   long long batch, cap;
 };
-hipError_t launch_paged_read(const PagedReadArgs &a, int format, hipStream_t s);
+// vec: d a multiple of 4; the pool and the outputs 16-byte aligned.
+hipError_t launch_paged_read(const PagedReadArgs &a, int format, bool vec, hipStream_t s);
 
 // Decode attention.  The work is one line of units, sequence by sequence and
 // head by head, a unit being `tile` rows; workgroup w of `wgs` takes a

@@ -21,25 +21,25 @@ constexpr bool kPagedScaled = F == kPagedFp8 || F == kPagedInt8;
 template <int F>
 constexpr float kPagedTop = F == kPagedInt8 ? 127.0f : 448.0f;
 
-__device__ __forceinline__ bool is_finite(float x) {
-  return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) != 0x7f800000u;
+// |x| as an integer: ordered as the magnitudes are, infinity and NaN on top, so
+// that one maximum finds a row's largest value and whether all are finite.
+__device__ __forceinline__ unsigned magnitude(float x) {
+  return __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
 }
 
 struct RowScale {
   float scale, inv;
 };
 template <int F>
-__device__ __forceinline__ RowScale row_scale(float mx, bool finite) {
-  const float m = fmaxf(mx, kPagedTiny);
-  return finite ? RowScale{m / kPagedTop<F>, kPagedTop<F> / m}
-                : RowScale{__builtin_nanf(""), 0.f};
+__device__ __forceinline__ RowScale row_scale(unsigned largest) {
+  const float m = fmaxf(__builtin_bit_cast(float, largest), kPagedTiny);
+  return largest < 0x7f800000u ? RowScale{m / kPagedTop<F>, kPagedTop<F> / m}
+                               : RowScale{__builtin_nanf(""), 0.f};
 }
 
 // bf16 bits of x, rounded to nearest even; a NaN stays one.
 __device__ __forceinline__ unsigned bf16_bits(float x) {
-  unsigned u = __builtin_bit_cast(unsigned, x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
-  return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+  return __builtin_bit_cast(unsigned short, (__bf16)x);
 }
 
 template <int F>
@@ -93,27 +93,32 @@ __host__ __device__ __forceinline__ long long paged_row(const PagedPool &p, long
   return ((long long)page * p.n_kv + h) * p.page + t % p.page;
 }
 
-// Rows of an append launch.
-__host__ __device__ __forceinline__ long long append_rows(const PagedAppendArgs &a) {
-  return a.n_tokens * ((a.q ? a.n_heads : 0) + 2 * a.pool.n_kv);
+// Rows of a token of an append launch.
+__host__ __device__ __forceinline__ int append_rows(const PagedAppendArgs &a) {
+  return (a.q ? a.n_heads : 0) + 2 * a.pool.n_kv;
 }
 
-// Row `row` of an append launch: the q rows of a token, its k rows, its v rows.
+// Row j of a token of an append launch: its q rows, its k rows, its v rows.
 struct AppendRow {
-  const float *in;
   float *out;           // q rows: where the rotated row goes
   const float *cos, *sin;  // null: not rotated
   void *codes;          // k and v rows: the pool, the row's first element in it,
   long long at;
   float *scale;         // and where its scale goes
 };
+__host__ __device__ __forceinline__ const float *append_in(const PagedAppendArgs &a, long long i, int j) {
+  const int nq = a.q ? a.n_heads : 0, kv = a.pool.n_kv;
+  return j < nq        ? a.q + (i * nq + j) * a.pool.d
+         : j < nq + kv ? a.k + (i * kv + (j - nq)) * a.pool.d
+                       : a.v + (i * kv + (j - nq - kv)) * a.pool.d;
+}
+
 // False: nothing to do (a token whose position or sequence is outside the
 // table, or outside the rotation's tables; a page that is not there).
-__host__ __device__ __forceinline__ bool append_row(const PagedAppendArgs &a, long long row, AppendRow &r) {
+__host__ __device__ __forceinline__ bool append_row(const PagedAppendArgs &a, long long i, int j,
+                                                    AppendRow &r) {
   const PagedPool &p = a.pool;
-  const int nq = a.q ? a.n_heads : 0, per = nq + 2 * p.n_kv;
-  const long long i = row / per;
-  const int j = (int)(row - i * per);
+  const int nq = a.q ? a.n_heads : 0;
   const int pos = a.positions[i];
   const long long seq = a.seqs ? a.seqs[i] : i;
   if (pos < 0 || pos >= p.table_stride * p.page || seq < 0 || seq >= a.n_seqs) return false;
@@ -124,7 +129,6 @@ __host__ __device__ __forceinline__ bool append_row(const PagedAppendArgs &a, lo
     r.sin = a.sin_tab + (long long)pos * (p.d / 2);
   }
   if (j < nq) {
-    r.in = a.q + (i * nq + j) * p.d;
     r.out = a.q_out + (i * nq + j) * p.d;
     return true;
   }
@@ -132,7 +136,6 @@ __host__ __device__ __forceinline__ bool append_row(const PagedAppendArgs &a, lo
   const int h = j - nq - (is_v ? p.n_kv : 0);
   const long long at = paged_row(p, seq, h, pos);
   if (at < 0) return false;
-  r.in = (is_v ? a.v : a.k) + (i * p.n_kv + h) * p.d;
   r.codes = is_v ? p.v : p.k;
   r.at = at * p.d;
   float *sc = is_v ? p.v_scales : p.k_scales;

@@ -4,6 +4,8 @@
 // form that takes any head dimension, group, page size and alignment.
 #include "bnr_paged.h"
 
+#include <algorithm>
+
 namespace bnr {
 namespace {
 
@@ -17,57 +19,148 @@ constexpr long long kMaxRowGrid = 1 << 20;  // workgroups of the row kernels at 
 // ---------------------------------------------------------------------------
 constexpr int kPairs = kPagedMaxDim / 2 / 64;
 
+// Maximum over the N lanes (a power of two) that share a row.
+template <int N>
+__device__ __forceinline__ unsigned row_largest(unsigned v) {
+  auto step = [&](unsigned u) { v = v > u ? v : u; };
+#define BNR_DPP(CTRL) (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false)
+  if (N >= 2) step(BNR_DPP(0xB1));    // quad_perm [1,0,3,2]
+  if (N >= 4) step(BNR_DPP(0x4E));    // quad_perm [2,3,0,1]
+  if (N >= 8) step(BNR_DPP(0x141));   // row_half_mirror
+  if (N >= 16) step(BNR_DPP(0x140));  // row_mirror
+#undef BNR_DPP
+  if (N >= 32) step(__shfl_xor(v, 16));
+  if (N >= 64) step(__shfl_xor(v, 32));
+  return v;
+}
+
 template <int F>
 __global__ __launch_bounds__(64 * kWaves) void paged_append_kernel(PagedAppendArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int half = a.pool.d / 2;
-  for (long long row = (long long)blockIdx.x * kWaves + (threadIdx.x >> 6); row < append_rows(a);
-       row += (long long)gridDim.x * kWaves) {
+  const int lane = threadIdx.x & 63, half = a.pool.d / 2, per = append_rows(a);
+  for (long long n = (long long)blockIdx.x * kWaves + (threadIdx.x >> 6); n < a.n_tokens * per;
+       n += (long long)gridDim.x * kWaves) {
+    const long long token = n / per;
+    const int j = (int)(n - token * per);
     AppendRow r;
-    if (!append_row(a, row, r)) continue;
+    if (!append_row(a, token, j, r)) continue;
+    const float *in = append_in(a, token, j);
     float lo[kPairs], hi[kPairs];
-    float mx = 0.f;
-    bool finite = true;
+    unsigned largest = 0;
 #pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      const int i = lane + 64 * j;
-      lo[j] = hi[j] = 0.f;
+    for (int k = 0; k < kPairs; ++k) {
+      const int i = lane + 64 * k;
+      lo[k] = hi[k] = 0.f;
       if (i < half) {
-        lo[j] = r.in[i];
-        hi[j] = r.in[half + i];
+        lo[k] = in[i];
+        hi[k] = in[half + i];
         if (r.cos) {
           float l, h;
-          rot_pair(lo[j], hi[j], r.cos[i], r.sin[i], l, h);
-          lo[j] = l;
-          hi[j] = h;
+          rot_pair(lo[k], hi[k], r.cos[i], r.sin[i], l, h);
+          lo[k] = l;
+          hi[k] = h;
         }
-        mx = fmaxf(mx, fmaxf(fabsf(lo[j]), fabsf(hi[j])));
-        finite = finite && is_finite(lo[j]) && is_finite(hi[j]);
+        largest = max(largest, max(magnitude(lo[k]), magnitude(hi[k])));
       }
-    }
-    if (r.out) {
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        const int i = lane + 64 * j;
-        if (i < half) {
-          r.out[i] = lo[j];
-          r.out[half + i] = hi[j];
-        }
-      }
-      continue;
     }
     float inv = 1.f;
-    if (kPagedScaled<F>) {
-      const RowScale s = row_scale<F>(wave_max(mx), __all(finite));
+    if (kPagedScaled<F> && !r.out) {
+      const RowScale s = row_scale<F>(row_largest<64>(largest));
       inv = s.inv;
       if (lane == 0) *r.scale = s.scale;
     }
 #pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      const int i = lane + 64 * j;
-      if (i < half) {
-        store_code<F>(r.codes, r.at + i, lo[j], inv);
-        store_code<F>(r.codes, r.at + half + i, hi[j], inv);
+    for (int k = 0; k < kPairs; ++k) {
+      const int i = lane + 64 * k;
+      if (i >= half) continue;
+      if (r.out) {
+        r.out[i] = lo[k];
+        r.out[half + i] = hi[k];
+      } else {
+        store_code<F>(r.codes, r.at + i, lo[k], inv);
+        store_code<F>(r.codes, r.at + half + i, hi[k], inv);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Append, head dimensions that are multiples of 8, 16-byte aligned rows: L
+// lanes (d / 8, rounded up to a power of two) share a row, each with 4 pairs:
+// 16 bytes of either half.  A workgroup takes `tokens` whole tokens, about as
+// many rows as it has lane groups, so a token's position, table entry and
+// rotation are read by one workgroup only, and a thread has the loads of kAt
+// rows in flight.  Bound by the rows' bytes.
+// ---------------------------------------------------------------------------
+constexpr int kAt = 3;
+
+template <int F>
+__device__ __forceinline__ void store_codes4(void *codes, long long at, float4 x, float inv) {
+  if constexpr (F == kPagedF32) {
+    st4(static_cast<float *>(codes) + at, x);
+  } else if constexpr (F == kPagedBf16) {
+    uint2 w;
+    w.x = code_of<F>(x.x, inv) | code_of<F>(x.y, inv) << 16;
+    w.y = code_of<F>(x.z, inv) | code_of<F>(x.w, inv) << 16;
+    *reinterpret_cast<uint2 *>(static_cast<unsigned short *>(codes) + at) = w;
+  } else {
+    *reinterpret_cast<unsigned *>(static_cast<unsigned char *>(codes) + at) =
+        code_of<F>(x.x, inv) | code_of<F>(x.y, inv) << 8 | code_of<F>(x.z, inv) << 16 |
+        code_of<F>(x.w, inv) << 24;
+  }
+}
+
+__device__ __forceinline__ unsigned largest4(float4 x) {
+  return max(max(magnitude(x.x), magnitude(x.y)), max(magnitude(x.z), magnitude(x.w)));
+}
+
+template <int F, int L>
+__global__ __launch_bounds__(64 * kWaves) void paged_append_vec_kernel(PagedAppendArgs a, int tokens) {
+  constexpr int kGroups = 64 * kWaves / L;
+  const int group = threadIdx.x / L, x = 4 * (threadIdx.x % L), half = a.pool.d / 2;
+  const int per = append_rows(a);
+  for (long long first = (long long)blockIdx.x * tokens; first < a.n_tokens;
+       first += (long long)gridDim.x * tokens) {
+    const int rows = (int)(a.n_tokens - first < tokens ? a.n_tokens - first : tokens) * per;
+    for (int n0 = group; n0 < rows; n0 += kAt * kGroups) {
+      float4 lo[kAt], hi[kAt];
+      AppendRow r[kAt];
+      bool in[kAt];
+#pragma unroll
+      for (int k = 0; k < kAt; ++k) {
+        const int n = n0 + k * kGroups, i = n / per, j = n - i * per;
+        lo[k] = hi[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        in[k] = n < rows && x < half;
+        if (in[k]) {
+          const float *src = append_in(a, first + i, j);
+          lo[k] = ld4(src + x);
+          hi[k] = ld4(src + half + x);
+          in[k] = append_row(a, first + i, j, r[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAt; ++k) {
+        if (in[k] && r[k].cos) {
+          const float4 c = ld4(r[k].cos + x), s = ld4(r[k].sin + x);
+          float4 l, h;
+          rot4(lo[k], hi[k], c, s, l, h);
+          lo[k] = l;
+          hi[k] = h;
+        }
+        float inv = 1.f;
+        if (kPagedScaled<F>) {
+          // every lane takes part: a row's lanes are all in or all out but for those past its end
+          const RowScale s = row_scale<F>(row_largest<L>(max(largest4(lo[k]), largest4(hi[k]))));
+          inv = s.inv;
+          if (in[k] && !r[k].out && x == 0) *r[k].scale = s.scale;
+        }
+        if (!in[k]) continue;
+        if (r[k].out) {
+          st4(r[k].out + x, lo[k]);
+          st4(r[k].out + half + x, hi[k]);
+        } else {
+          store_codes4<F>(r[k].codes, r[k].at + x, lo[k], inv);
+          store_codes4<F>(r[k].codes, r[k].at + half + x, hi[k], inv);
+        }
       }
     }
   }
@@ -100,6 +193,84 @@ __global__ __launch_bounds__(64 * kWaves) void paged_read_kernel(PagedReadArgs a
     for (int x = lane; x < d; x += 64) {
       ko[x] = at < 0 ? 0.f : load_code<F>(a.pool.k, at * d + x) * ks;
       vo[x] = at < 0 ? 0.f : load_code<F>(a.pool.v, at * d + x) * vs;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Read, head dimensions that are multiples of 4, rows and outputs aligned to
+// four elements: L lanes (d / 4, rounded up to a power of two) share a row,
+// each with four elements, so that a wave's stores are whole lines; a
+// workgroup takes kReadRows rows of one kv head, k and v, a thread with all
+// its loads in flight.  Bound by the outputs' bytes: 4 of them to one or two
+// of the rows'.
+// ---------------------------------------------------------------------------
+constexpr int kReadPasses = 4;
+template <int L>
+constexpr int kReadRows = kReadPasses * 64 * kWaves / L;
+
+// Four codes as fp32, before the scale.
+template <int F>
+__device__ __forceinline__ float4 load_codes4(const void *codes, long long at) {
+  if constexpr (F == kPagedF32) {
+    return ld4(static_cast<const float *>(codes) + at);
+  } else if constexpr (F == kPagedBf16) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const unsigned short *>(codes) + at);
+    return make_float4(__builtin_bit_cast(float, w.x << 16), __builtin_bit_cast(float, w.x & 0xffff0000u),
+                       __builtin_bit_cast(float, w.y << 16), __builtin_bit_cast(float, w.y & 0xffff0000u));
+  } else {
+    const unsigned w = *reinterpret_cast<const unsigned *>(static_cast<const unsigned char *>(codes) + at);
+    if constexpr (F == kPagedInt8)
+      return make_float4((float)(signed char)w, (float)(signed char)(w >> 8),
+                         (float)(signed char)(w >> 16), (float)(signed char)(w >> 24));
+    return make_float4(__builtin_amdgcn_cvt_f32_fp8((int)w, 0), __builtin_amdgcn_cvt_f32_fp8((int)w, 1),
+                       __builtin_amdgcn_cvt_f32_fp8((int)w, 2), __builtin_amdgcn_cvt_f32_fp8((int)w, 3));
+  }
+}
+
+template <int F, int L>
+__global__ __launch_bounds__(64 * kWaves) void paged_read_vec_kernel(PagedReadArgs a) {
+  constexpr int kPass = 64 * kWaves / L;  // rows of a pass
+  const int x = 4 * (threadIdx.x % L), d = a.pool.d;
+  const long long chunks = (a.cap + kReadRows<L> - 1) / kReadRows<L>;
+  for (long long b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    const int start = a.starts ? a.starts[b] : 0;
+    const int len = paged_len(a.lens[b], a.pool);
+    if (start < 0) continue;
+    const long long rows = len - (long long)start < a.cap ? len - (long long)start : a.cap;
+    for (long long w = blockIdx.x; w < chunks * a.pool.n_kv; w += gridDim.x) {
+      const int h = (int)((w | chunks) >> 32 ? w / chunks : (unsigned)w / (unsigned)chunks);
+      const long long i0 = (w - h * chunks) * kReadRows<L> + threadIdx.x / L;
+      if (i0 >= rows || x >= d) continue;
+      long long at[kReadPasses];
+      float4 k[kReadPasses], v[kReadPasses];
+      float ks[kReadPasses], vs[kReadPasses];
+#pragma unroll
+      for (int p = 0; p < kReadPasses; ++p) {
+        const long long i = i0 + p * kPass;
+        // past the last row: the first again, not written (a branch would part the loads)
+        at[p] = paged_row(a.pool, b, h, start + (int)(i < rows ? i : i0));
+      }
+#pragma unroll
+      for (int p = 0; p < kReadPasses; ++p) {
+        const long long from = at[p] < 0 ? 0 : at[p];
+        k[p] = load_codes4<F>(a.pool.k, from * d + x);
+        v[p] = load_codes4<F>(a.pool.v, from * d + x);
+        ks[p] = vs[p] = 1.f;
+        if (kPagedScaled<F>) {
+          ks[p] = a.pool.k_scales[from];
+          vs[p] = a.pool.v_scales[from];
+        }
+      }
+      float *ko = a.k_out + ((b * a.pool.n_kv + h) * a.cap + i0) * d + x;
+      float *vo = a.v_out + ((b * a.pool.n_kv + h) * a.cap + i0) * d + x;
+#pragma unroll
+      for (int p = 0; p < kReadPasses; ++p) {
+        if (i0 + p * kPass >= rows) break;
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        st4(ko + (long long)p * kPass * d, at[p] < 0 ? zero : kPagedScaled<F> ? scale4(ks[p], k[p]) : k[p]);
+        st4(vo + (long long)p * kPass * d, at[p] < 0 ? zero : kPagedScaled<F> ? scale4(vs[p], v[p]) : v[p]);
+      }
     }
   }
 }
@@ -179,23 +350,61 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
     default: return hipErrorInvalidValue;              \
   }
 
-// Workgroups for `rows` rows, one a wave; past the limit a wave takes several.
-static dim3 row_grid(long long rows) {
-  const long long wgs = (rows + kWaves - 1) / kWaves;
-  return dim3((unsigned)(wgs < kMaxRowGrid ? wgs : kMaxRowGrid));
+// Workgroups for n of them; past the limit a workgroup takes several turns.
+static unsigned row_grid(long long n) { return (unsigned)(n < kMaxRowGrid ? n : kMaxRowGrid); }
+
+template <int F, int L>
+static void append_vec(const PagedAppendArgs &a, hipStream_t s) {
+  const int tokens = std::max(1, 64 * kWaves / L / append_rows(a));
+  paged_append_vec_kernel<F, L><<<row_grid((a.n_tokens + tokens - 1) / tokens), 64 * kWaves, 0, s>>>(a, tokens);
 }
 
-hipError_t launch_paged_append(const PagedAppendArgs &a, int format, hipStream_t s) {
-  const dim3 grid = row_grid(append_rows(a));
-#define CALL(F) paged_append_kernel<F><<<grid, 64 * kWaves, 0, s>>>(a)
+template <int F>
+static void append_format(const PagedAppendArgs &a, bool vec, hipStream_t s) {
+  const int d = a.pool.d;
+  if (!vec)
+    paged_append_kernel<F><<<row_grid((a.n_tokens * append_rows(a) + kWaves - 1) / kWaves), 64 * kWaves, 0, s>>>(a);
+  else if (d <= 64)
+    append_vec<F, 8>(a, s);
+  else if (d <= 128)
+    append_vec<F, 16>(a, s);
+  else if (d <= 256)
+    append_vec<F, 32>(a, s);
+  else
+    append_vec<F, 64>(a, s);
+}
+
+hipError_t launch_paged_append(const PagedAppendArgs &a, int format, bool vec, hipStream_t s) {
+#define CALL(F) append_format<F>(a, vec, s)
   BNR_BY_FORMAT(format, CALL)
 #undef CALL
   return hipGetLastError();
 }
 
-hipError_t launch_paged_read(const PagedReadArgs &a, int format, hipStream_t s) {
-  const dim3 grid = row_grid(a.batch * a.cap * a.pool.n_kv);
-#define CALL(F) paged_read_kernel<F><<<grid, 64 * kWaves, 0, s>>>(a)
+template <int F, int L>
+static void read_vec(const PagedReadArgs &a, hipStream_t s) {
+  const long long chunks = (a.cap + kReadRows<L> - 1) / kReadRows<L>;
+  const dim3 grid(row_grid(chunks * a.pool.n_kv), (unsigned)std::min<long long>(a.batch, 65535));
+  paged_read_vec_kernel<F, L><<<grid, 64 * kWaves, 0, s>>>(a);
+}
+
+template <int F>
+static void read_format(const PagedReadArgs &a, bool vec, hipStream_t s) {
+  const int d = a.pool.d;
+  if (!vec)
+    paged_read_kernel<F><<<row_grid((a.batch * a.cap * a.pool.n_kv + kWaves - 1) / kWaves), 64 * kWaves, 0, s>>>(a);
+  else if (d <= 64)
+    read_vec<F, 16>(a, s);
+  else if (d <= 128)
+    read_vec<F, 32>(a, s);
+  else if (d <= 256)
+    read_vec<F, 64>(a, s);
+  else
+    read_vec<F, 128>(a, s);
+}
+
+hipError_t launch_paged_read(const PagedReadArgs &a, int format, bool vec, hipStream_t s) {
+#define CALL(F) read_format<F>(a, vec, s)
   BNR_BY_FORMAT(format, CALL)
 #undef CALL
   return hipGetLastError();
