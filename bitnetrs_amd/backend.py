@@ -54,6 +54,16 @@ def _dev(t, name: str, allow_none: bool = False, dtype=None):
     return ctypes.c_void_p(t.data_ptr())
 
 
+def _on(t, name: str, dtype, device: int, shape=None):
+    """The address of a contiguous tensor of that type (and shape) on that GPU.
+    A decode step calls this for every operand: each check is one call."""
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} tensor on cuda:{device}")
+    if shape is not None and t.shape != shape:
+        raise InvalidShape(f"{name} {list(shape)}", f"{list(t.shape)}")
+    return t.data_ptr()
+
+
 def _stream(stream):
     if stream is None:
         import torch
@@ -316,21 +326,8 @@ class HipBackend:
             _dev(act_absmax, "act_absmax"), _stream(stream)))
 
     # paged KV cache -----------------------------------------------------------
-    def _on(self, t, name: str, shape, dtype="float32"):
-        """The address of a contiguous tensor of that shape and type on this backend's device."""
-        ok = t.is_cuda and t.is_contiguous() and str(t.dtype)[6:] == dtype and t.device.index == self.device_id
-        if not ok:
-            raise TypeError(f"{name} must be a contiguous {dtype} tensor on cuda:{self.device_id}")
-        if t.shape != shape:
-            raise InvalidShape(f"{name} {list(shape)}", f"{list(t.shape)}")
-        return t.data_ptr()
-
-    def _paged_stream(self, stream):
-        if stream is None:
-            import torch
-
-            return torch.cuda.current_stream(self.device_id).cuda_stream
-        return _stream(stream)
+    def _paged_stream(self, kv, stream):
+        return kv.raw_stream(self.device_id) if stream is None else _stream(stream)
 
     def rope_table(self, n_positions: int, head_dim: int, theta: float):
         """The rotation tables (cos, sin) [n_positions, head_dim/2] that rope_embed
@@ -340,7 +337,8 @@ class HipBackend:
         cos, sin = (torch.empty(n_positions, head_dim // 2, device=f"cuda:{self.device_id}")
                     for _ in range(2))
         _lib.check(self._L.bnr_dev_rope_table(self._h, n_positions, head_dim, theta, cos.data_ptr(),
-                                              sin.data_ptr(), self._paged_stream(None)))
+                                              sin.data_ptr(),
+                                              torch.cuda.current_stream(self.device_id).cuda_stream))
         return cos, sin
 
     def dev_paged_append(self, kv: "PagedKV", q, k, v, q_out, positions, block_table, cos=None,
@@ -351,39 +349,42 @@ class HipBackend:
         [n_seqs, pages] (int32, as positions and seqs).  cos / sin: the
         rotation's tables (rope_table), None for rows that are rotated; q and
         q_out may both be None."""
-        n = positions.shape[0]
-        rows = (n, kv.n_kv_heads, kv.head_dim)
-        n_seqs, stride = block_table.shape
-        n_heads = 0 if q is None else q.shape[1]
-        if (q is None) != (q_out is None) or (cos is None) != (sin is None):
-            raise TypeError("q and q_out, and cos and sin, go together")
-        qs = (n, n_heads, kv.head_dim)
-        tab = None if cos is None else (cos.shape[0], kv.head_dim // 2)
+        dev, f32, i32, d = self.device_id, kv.f32, kv.i32, kv.head_dim
+        n, (n_seqs, stride), n_heads, qp, qop = len(positions), block_table.shape, 0, None, None
+        if q is not None and q_out is not None:
+            n_heads = q.shape[1]
+            qp = _on(q, "q", f32, dev, (n, n_heads, d))
+            qop = qp if q_out is q else _on(q_out, "q_out", f32, dev, (n, n_heads, d))
+        elif q is not q_out:
+            raise TypeError("q and q_out go together")
+        cp = sp = None
+        n_pos = 0
+        if cos is not None and sin is not None:
+            n_pos = len(cos)
+            cp = _on(cos, "cos", f32, dev, (n_pos, d // 2))
+            sp = _on(sin, "sin", f32, dev, (n_pos, d // 2))
+        elif cos is not sin:
+            raise TypeError("cos and sin go together")
+        rows = (n, kv.n_kv_heads, d)
         _lib.check(self._L.bnr_dev_paged_append(
-            self._h, kv.desc(self.device_id), None if q is None else self._on(q, "q", qs),
-            self._on(k, "k", rows), self._on(v, "v", rows),
-            None if q is None else self._on(q_out, "q_out", qs), n, n_heads,
-            self._on(positions, "positions", (n,), "int32"),
-            None if seqs is None else self._on(seqs, "seqs", (n,), "int32"),
-            self._on(block_table, "block_table", (n_seqs, stride), "int32"), n_seqs, stride,
-            None if cos is None else self._on(cos, "cos", tab),
-            None if cos is None else self._on(sin, "sin", tab), 0 if cos is None else tab[0],
-            self._paged_stream(stream)))
+            self._h, kv.desc(dev), qp, _on(k, "k", f32, dev, rows), _on(v, "v", f32, dev, rows), qop, n,
+            n_heads, _on(positions, "positions", i32, dev, (n,)),
+            None if seqs is None else _on(seqs, "seqs", i32, dev, (n,)),
+            _on(block_table, "block_table", i32, dev), n_seqs, stride, cp, sp, n_pos,
+            self._paged_stream(kv, stream)))
 
     def dev_paged_read(self, kv: "PagedKV", block_table, lens, k_out, v_out, starts=None,
                        stream=None) -> None:
         """Rows starts[s] (None: 0) .. lens[s]-1 of each sequence of block_table
         [batch, pages] as fp32 into k_out and v_out [batch, n_kv_heads, cap, d],
         from row 0 on; what lies behind them stays."""
-        batch, stride = block_table.shape
-        cap = k_out.shape[2]
+        dev, i32, (batch, stride), cap = self.device_id, kv.i32, block_table.shape, k_out.shape[2]
         out = (batch, kv.n_kv_heads, cap, kv.head_dim)
         _lib.check(self._L.bnr_dev_paged_read(
-            self._h, kv.desc(self.device_id),
-            self._on(block_table, "block_table", (batch, stride), "int32"), batch, stride,
-            None if starts is None else self._on(starts, "starts", (batch,), "int32"),
-            self._on(lens, "lens", (batch,), "int32"), self._on(k_out, "k_out", out),
-            self._on(v_out, "v_out", out), cap, self._paged_stream(stream)))
+            self._h, kv.desc(dev), _on(block_table, "block_table", i32, dev), batch, stride,
+            None if starts is None else _on(starts, "starts", i32, dev, (batch,)),
+            _on(lens, "lens", i32, dev, (batch,)), _on(k_out, "k_out", kv.f32, dev, out),
+            _on(v_out, "v_out", kv.f32, dev, out), cap, self._paged_stream(kv, stream)))
 
     def paged_workspace(self, kv: "PagedKV", batch: int, n_heads: int):
         """A zero-filled workspace for dev_paged_decode_attention over kv with up
@@ -400,15 +401,13 @@ class HipBackend:
         """Attention of one token of each sequence, q [batch, n_heads, d] (rotated),
         over rows 0..lens[s]-1 of its own, into out (as q).  `workspace` from
         paged_workspace; calls that share one must be ordered."""
-        batch, stride = block_table.shape
-        n_heads = q.shape[1]
+        dev, i32, (batch, stride), n_heads = self.device_id, kv.i32, block_table.shape, q.shape[1]
         qs = (batch, n_heads, kv.head_dim)
         _lib.check(self._L.bnr_dev_paged_decode_attention(
-            self._h, kv.desc(self.device_id), self._on(q, "q", qs), n_heads,
-            self._on(block_table, "block_table", (batch, stride), "int32"), batch, stride,
-            self._on(lens, "lens", (batch,), "int32"), self._on(out, "out", qs),
-            self._on(workspace, "workspace", workspace.shape, "uint8"), workspace.numel(),
-            self._paged_stream(stream)))
+            self._h, kv.desc(dev), _on(q, "q", kv.f32, dev, qs), n_heads,
+            _on(block_table, "block_table", i32, dev), batch, stride, _on(lens, "lens", i32, dev, (batch,)),
+            _on(out, "out", kv.f32, dev, qs), _on(workspace, "workspace", kv.u8, dev), len(workspace),
+            self._paged_stream(kv, stream)))
 
     def dev_synchronize(self, stream=None) -> None:
         _lib.check(self._L.bnr_dev_synchronize(self._h, _stream(stream)))
@@ -515,12 +514,19 @@ class PagedKV:
         at = [t.data_ptr() for t in tensors] + [None] * (4 - len(tensors))
         self._desc = _lib.PagedKVDesc(*at, self.n_pages, self.page_size, self.n_kv_heads,
                                       self.head_dim, self.FORMATS[fmt][0])
+        # what every call needs, looked up once
+        import torch
+
+        self._ref, self._device = ctypes.byref(self._desc), k.get_device()
+        self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
+        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
 
     def desc(self, device_id: int):
         """The pool as the library takes it."""
-        if self.k.device.type != "cuda" or self.k.device.index != device_id:
+        if self._device != device_id:
             raise TypeError(f"the pool must be on cuda:{device_id}, it is on {self.k.device}")
-        return ctypes.byref(self._desc)
+        return self._ref
 
 
 class NativeKVCache:

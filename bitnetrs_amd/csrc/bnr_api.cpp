@@ -2824,7 +2824,9 @@ extern "C" int bnr_dev_paged_read(bnr_ctx *c, const bnr_paged_kv *kv, const int3
   if (!c) return err_backend("context is NULL");
   PagedReadArgs a{};
   int st = paged_pool(kv, block_table, table_stride, a.pool);
-  if (!st) st = check_paged_count(batch, "batch");
+  if (!st && batch >= kPagedMaxCount / kv->n_kv_heads)
+    st = err_shape(fmt("batch * n_kv_heads < %zu", kPagedMaxCount),
+                   fmt("batch = %zu, n_kv_heads = %zu", batch, kv->n_kv_heads));
   if (st) return st;
   if (cap > kPagedMaxRows)
     return err_shape(fmt("cap <= %zu", kPagedMaxRows), fmt("cap = %zu", cap));

@@ -115,6 +115,12 @@ __device__ __forceinline__ void st4(float *p, float4 v) {
   *reinterpret_cast<float4 *>(p) = v;
 }
 
+// ... with the non-temporal hint, for streams of more than the caches hold.
+__device__ __forceinline__ void st4_nt(float *p, float4 v) {
+  typedef float f4v __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(f4v{v.x, v.y, v.z, v.w}, reinterpret_cast<f4v *>(p));
+}
+
 // Agent-coherent scalar store / load: performed at the device-wide coherence
 // point, so another workgroup -- on any XCD, behind its own L2 -- that reads
 // after observing the ticket below sees the value without a cache writeback

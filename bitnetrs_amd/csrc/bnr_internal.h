@@ -720,6 +720,7 @@ struct PagedReadArgs {
   const int *starts, *lens;  // [batch]; starts null: 0
   float *k_out, *v_out;      // [batch][n_kv][cap][d]
   long long batch, cap;
+  int wgs, tile;  // set by the launch
 };
 // vec: d a multiple of 4; the pool and the outputs 16-byte aligned.
 hipError_t launch_paged_read(const PagedReadArgs &a, int format, bool vec, hipStream_t s);

@@ -144,9 +144,9 @@ __host__ __device__ __forceinline__ bool append_row(const PagedAppendArgs &a, lo
 }
 
 // ---------------------------------------------------------------------------
-// Shares of a decode launch.  Sequence b has ceil(lens[b] / tile) units for
-// each of its `items` heads; all units in order are one line, and workgroup w
-// takes units w * per + min(w, rest) .. of it (total = per * wgs + rest).  A
+// Shares of a launch.  Sequence b has ceil(rows(b) / tile) units for each of
+// its `items` heads; all units in order are one line, and workgroup w takes
+// units w * per + min(w, rest) .. of it (total = per * wgs + rest).  A
 // workgroup's share is a run of pieces, each of one item: at most its first
 // and its last piece belong to items that other workgroups share.  Nothing
 // about the lengths is known on the host, so a captured launch serves every
@@ -171,15 +171,16 @@ struct PagedShare {
     const unsigned big = rest * (per + 1);
     return t < big ? t / (per + 1) : rest + (t - big) / per;
   }
-  // The next piece; lens as the launch has them.
-  __host__ __device__ bool next(const int *lens, const PagedPool &pool, PagedPiece &p) {
+  // The next piece.
+  template <class Rows>
+  __host__ __device__ bool next(Rows rows, PagedPiece &p) {
     if (at >= end) return false;
     if (at == item0 + n) {  // past the item before
       item0 = at;
       if (++h == items) {
         h = 0;
         do {
-          len = paged_len(lens[++b], pool);
+          len = rows(++b);
         } while (len == 0);
         n = (unsigned)(len + tile - 1) / (unsigned)tile;
       }
@@ -215,23 +216,24 @@ __device__ __forceinline__ unsigned lane_of(unsigned v, int lane) {
   return (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
 
-__device__ __forceinline__ PagedShare paged_share(const PagedDecodeArgs &a, int items) {
+template <class Rows>
+__device__ __forceinline__ PagedShare paged_share(Rows rows, int batch, int items, unsigned tile,
+                                                  unsigned wgs) {
   const int lane = threadIdx.x & 63;
-  const unsigned tile = (unsigned)a.tile, wgs = (unsigned)a.wgs;
-  // Lengths, and units of an item, of each sequence, 64 sequences at a time.
-  auto length = [&](int b) { return b < a.batch ? paged_len(a.lens[b], a.pool) : 0; };
+  // Rows, and units of an item, of each sequence, 64 sequences at a time.
+  auto length = [&](int b) { return b < batch ? rows(b) : 0; };
   auto units = [&](int len) { return ((unsigned)len + tile - 1) / tile; };
   const int first_len = length(lane);
   const unsigned first = wave_scan(units(first_len));
   unsigned total = lane_of(first, 63);
-  for (int b0 = 64; b0 < a.batch; b0 += 64) total += lane_of(wave_scan(units(length(b0 + lane))), 63);
+  for (int b0 = 64; b0 < batch; b0 += 64) total += lane_of(wave_scan(units(length(b0 + lane))), 63);
   total *= (unsigned)items;
   PagedShare s;
   s.wg = blockIdx.x;
   s.per = total / wgs;
   s.rest = total - s.per * wgs;
   s.items = items;
-  s.tile = a.tile;
+  s.tile = (int)tile;
   s.at = s.wg * s.per + (s.wg < s.rest ? s.wg : s.rest);
   s.end = s.at + s.per + (s.wg < s.rest ? 1 : 0);
   if (s.at >= s.end) return s;

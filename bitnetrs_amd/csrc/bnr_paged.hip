@@ -86,13 +86,12 @@ __global__ __launch_bounds__(64 * kWaves) void paged_append_kernel(PagedAppendAr
 // ---------------------------------------------------------------------------
 // Append, head dimensions that are multiples of 8, 16-byte aligned rows: L
 // lanes (d / 8, rounded up to a power of two) share a row, each with 4 pairs:
-// 16 bytes of either half.  A workgroup takes `tokens` whole tokens, about as
-// many rows as it has lane groups, so a token's position, table entry and
-// rotation are read by one workgroup only, and a thread has the loads of kAt
-// rows in flight.  Bound by the rows' bytes.
+// 16 bytes of either half.  A workgroup takes a run of rows, a token's rows
+// being neighbours, so that most tokens' positions, table entries and
+// rotations are read by one workgroup only.  Bound by the rows' bytes; with the
+// loads of two or four rows in flight in a thread 8000 tokens of 32/8 heads
+// took 3 and 10 us more.
 // ---------------------------------------------------------------------------
-constexpr int kAt = 3;
-
 template <int F>
 __device__ __forceinline__ void store_codes4(void *codes, long long at, float4 x, float inv) {
   if constexpr (F == kPagedF32) {
@@ -114,54 +113,45 @@ __device__ __forceinline__ unsigned largest4(float4 x) {
 }
 
 template <int F, int L>
-__global__ __launch_bounds__(64 * kWaves) void paged_append_vec_kernel(PagedAppendArgs a, int tokens) {
-  constexpr int kGroups = 64 * kWaves / L;
-  const int group = threadIdx.x / L, x = 4 * (threadIdx.x % L), half = a.pool.d / 2;
-  const int per = append_rows(a);
-  for (long long first = (long long)blockIdx.x * tokens; first < a.n_tokens;
-       first += (long long)gridDim.x * tokens) {
-    const int rows = (int)(a.n_tokens - first < tokens ? a.n_tokens - first : tokens) * per;
-    for (int n0 = group; n0 < rows; n0 += kAt * kGroups) {
-      float4 lo[kAt], hi[kAt];
-      AppendRow r[kAt];
-      bool in[kAt];
-#pragma unroll
-      for (int k = 0; k < kAt; ++k) {
-        const int n = n0 + k * kGroups, i = n / per, j = n - i * per;
-        lo[k] = hi[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        in[k] = n < rows && x < half;
-        if (in[k]) {
-          const float *src = append_in(a, first + i, j);
-          lo[k] = ld4(src + x);
-          hi[k] = ld4(src + half + x);
-          in[k] = append_row(a, first + i, j, r[k]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kAt; ++k) {
-        if (in[k] && r[k].cos) {
-          const float4 c = ld4(r[k].cos + x), s = ld4(r[k].sin + x);
-          float4 l, h;
-          rot4(lo[k], hi[k], c, s, l, h);
-          lo[k] = l;
-          hi[k] = h;
-        }
-        float inv = 1.f;
-        if (kPagedScaled<F>) {
-          // every lane takes part: a row's lanes are all in or all out but for those past its end
-          const RowScale s = row_scale<F>(row_largest<L>(max(largest4(lo[k]), largest4(hi[k]))));
-          inv = s.inv;
-          if (in[k] && !r[k].out && x == 0) *r[k].scale = s.scale;
-        }
-        if (!in[k]) continue;
-        if (r[k].out) {
-          st4(r[k].out + x, lo[k]);
-          st4(r[k].out + half + x, hi[k]);
-        } else {
-          store_codes4<F>(r[k].codes, r[k].at + x, lo[k], inv);
-          store_codes4<F>(r[k].codes, r[k].at + half + x, hi[k], inv);
-        }
-      }
+__global__ __launch_bounds__(64 * kWaves) void paged_append_vec_kernel(PagedAppendArgs a) {
+  constexpr int kRows = 64 * kWaves / L;
+  const int x = 4 * (threadIdx.x % L), half = a.pool.d / 2, per = append_rows(a);
+  const unsigned long long total = (unsigned long long)a.n_tokens * per;
+  for (unsigned long long n0 = (unsigned long long)blockIdx.x * kRows; n0 < total;
+       n0 += (unsigned long long)gridDim.x * kRows) {
+    const unsigned long long first = n0 >> 32 ? n0 / per : (unsigned)n0 / (unsigned)per;
+    const int n = (int)(n0 - first * per) + threadIdx.x / L, i = n / per, j = n - i * per;
+    const long long token = (long long)first + i;
+    float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+    AppendRow r;
+    bool in = token < a.n_tokens && x < half;
+    if (in) {
+      const float *src = append_in(a, token, j);
+      lo = ld4(src + x);
+      hi = ld4(src + half + x);
+      in = append_row(a, token, j, r);
+    }
+    if (in && r.cos) {
+      const float4 c = ld4(r.cos + x), s = ld4(r.sin + x);
+      float4 l, h;
+      rot4(lo, hi, c, s, l, h);
+      lo = l;
+      hi = h;
+    }
+    float inv = 1.f;
+    if (kPagedScaled<F>) {
+      // every lane takes part: those past a row's end bring zeros
+      const RowScale s = row_scale<F>(row_largest<L>(max(largest4(lo), largest4(hi))));
+      inv = s.inv;
+      if (in && !r.out && x == 0) *r.scale = s.scale;
+    }
+    if (!in) continue;
+    if (r.out) {
+      st4(r.out + x, lo);
+      st4(r.out + half + x, hi);
+    } else {
+      store_codes4<F>(r.codes, r.at + x, lo, inv);
+      store_codes4<F>(r.codes, r.at + half + x, hi, inv);
     }
   }
 }
@@ -201,11 +191,16 @@ __global__ __launch_bounds__(64 * kWaves) void paged_read_kernel(PagedReadArgs a
 // Read, head dimensions that are multiples of 4, rows and outputs aligned to
 // four elements: L lanes (d / 4, rounded up to a power of two) share a row,
 // each with four elements, so that a wave's stores are whole lines; a
-// workgroup takes kReadRows rows of one kv head, k and v, a thread with all
-// its loads in flight.  Bound by the outputs' bytes: 4 of them to one or two
-// of the rows'.
+// workgroup takes equal shares of all rows that are to be read, kReadRows of
+// one kv head at a time, k and v, a thread with all its loads in flight.
+// Bound by the outputs' bytes: 4 of them to one or two of the rows'.
 // ---------------------------------------------------------------------------
-constexpr int kReadPasses = 4;
+// Workgroups at most: many more than the card holds, so that what is written
+// at one time lies close together.  32 int8 sequences of 100 to 4096 rows: 90
+// us; 95 with 4096, 102 with 2048, 108 with a workgroup for every 32 rows that
+// there is room for (half of them without a row).
+constexpr int kReadWgs = 16384;
+constexpr int kReadPasses = 4;  // 2: 111 us, 8: 116 us, of 107 us then
 template <int L>
 constexpr int kReadRows = kReadPasses * 64 * kWaves / L;
 
@@ -232,44 +227,44 @@ template <int F, int L>
 __global__ __launch_bounds__(64 * kWaves) void paged_read_vec_kernel(PagedReadArgs a) {
   constexpr int kPass = 64 * kWaves / L;  // rows of a pass
   const int x = 4 * (threadIdx.x % L), d = a.pool.d;
-  const long long chunks = (a.cap + kReadRows<L> - 1) / kReadRows<L>;
-  for (long long b = blockIdx.y; b < a.batch; b += gridDim.y) {
-    const int start = a.starts ? a.starts[b] : 0;
-    const int len = paged_len(a.lens[b], a.pool);
-    if (start < 0) continue;
-    const long long rows = len - (long long)start < a.cap ? len - (long long)start : a.cap;
-    for (long long w = blockIdx.x; w < chunks * a.pool.n_kv; w += gridDim.x) {
-      const int h = (int)((w | chunks) >> 32 ? w / chunks : (unsigned)w / (unsigned)chunks);
-      const long long i0 = (w - h * chunks) * kReadRows<L> + threadIdx.x / L;
-      if (i0 >= rows || x >= d) continue;
+  const auto rows = [&](int b) {
+    const int start = a.starts ? a.starts[b] : 0, len = paged_len(a.lens[b], a.pool);
+    if (start < 0 || start >= len) return 0;
+    return len - start < a.cap ? len - start : (int)a.cap;
+  };
+  PagedShare sh = paged_share(rows, (int)a.batch, a.pool.n_kv, a.tile, a.wgs);
+  for (PagedPiece p; sh.next(rows, p);) {
+    const int start = a.starts ? a.starts[p.b] : 0;
+    const long long to = ((long long)p.b * a.pool.n_kv + p.h) * a.cap;
+    for (int i0 = p.row0 + (int)threadIdx.x / L; i0 < p.row1; i0 += kReadRows<L>) {
+      if (x >= d) continue;
       long long at[kReadPasses];
       float4 k[kReadPasses], v[kReadPasses];
       float ks[kReadPasses], vs[kReadPasses];
 #pragma unroll
-      for (int p = 0; p < kReadPasses; ++p) {
-        const long long i = i0 + p * kPass;
+      for (int n = 0; n < kReadPasses; ++n) {
+        const int i = i0 + n * kPass;
         // past the last row: the first again, not written (a branch would part the loads)
-        at[p] = paged_row(a.pool, b, h, start + (int)(i < rows ? i : i0));
+        at[n] = paged_row(a.pool, p.b, p.h, start + (i < p.row1 ? i : i0));
       }
 #pragma unroll
-      for (int p = 0; p < kReadPasses; ++p) {
-        const long long from = at[p] < 0 ? 0 : at[p];
-        k[p] = load_codes4<F>(a.pool.k, from * d + x);
-        v[p] = load_codes4<F>(a.pool.v, from * d + x);
-        ks[p] = vs[p] = 1.f;
+      for (int n = 0; n < kReadPasses; ++n) {
+        const long long from = at[n] < 0 ? 0 : at[n];
+        k[n] = load_codes4<F>(a.pool.k, from * d + x);
+        v[n] = load_codes4<F>(a.pool.v, from * d + x);
+        ks[n] = vs[n] = 1.f;
         if (kPagedScaled<F>) {
-          ks[p] = a.pool.k_scales[from];
-          vs[p] = a.pool.v_scales[from];
+          ks[n] = a.pool.k_scales[from];
+          vs[n] = a.pool.v_scales[from];
         }
       }
-      float *ko = a.k_out + ((b * a.pool.n_kv + h) * a.cap + i0) * d + x;
-      float *vo = a.v_out + ((b * a.pool.n_kv + h) * a.cap + i0) * d + x;
 #pragma unroll
-      for (int p = 0; p < kReadPasses; ++p) {
-        if (i0 + p * kPass >= rows) break;
+      for (int n = 0; n < kReadPasses; ++n) {
+        const int i = i0 + n * kPass;
+        if (i >= p.row1) break;
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        st4(ko + (long long)p * kPass * d, at[p] < 0 ? zero : kPagedScaled<F> ? scale4(ks[p], k[p]) : k[p]);
-        st4(vo + (long long)p * kPass * d, at[p] < 0 ? zero : kPagedScaled<F> ? scale4(vs[p], v[p]) : v[p]);
+        st4_nt(a.k_out + (to + i) * d + x, at[n] < 0 ? zero : kPagedScaled<F> ? scale4(ks[n], k[n]) : k[n]);
+        st4_nt(a.v_out + (to + i) * d + x, at[n] < 0 ? zero : kPagedScaled<F> ? scale4(vs[n], v[n]) : v[n]);
       }
     }
   }
@@ -290,8 +285,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
   __shared__ JoinShared<kWaves, 1> s_join;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = a.pool.d;
   const int first_len = paged_first_len(a);
-  PagedShare sh = paged_share(a, a.n_heads);
-  for (PagedPiece p; sh.next(a.lens, a.pool, p);) {
+  const auto rows = [&](int b) { return paged_len(a.lens[b], a.pool); };
+  PagedShare sh = paged_share(rows, a.batch, a.n_heads, a.tile, a.wgs);
+  for (PagedPiece p; sh.next(rows, p);) {
     const int h = p.h / a.group;
     const float *q = a.q + ((long long)p.b * a.n_heads + p.h) * d;
     float qr[kElems], o[kElems];
@@ -355,8 +351,8 @@ static unsigned row_grid(long long n) { return (unsigned)(n < kMaxRowGrid ? n : 
 
 template <int F, int L>
 static void append_vec(const PagedAppendArgs &a, hipStream_t s) {
-  const int tokens = std::max(1, 64 * kWaves / L / append_rows(a));
-  paged_append_vec_kernel<F, L><<<row_grid((a.n_tokens + tokens - 1) / tokens), 64 * kWaves, 0, s>>>(a, tokens);
+  const long long rows = a.n_tokens * append_rows(a), per = 64 * kWaves / L;
+  paged_append_vec_kernel<F, L><<<row_grid((rows + per - 1) / per), 64 * kWaves, 0, s>>>(a);
 }
 
 template <int F>
@@ -382,10 +378,13 @@ hipError_t launch_paged_append(const PagedAppendArgs &a, int format, bool vec, h
 }
 
 template <int F, int L>
-static void read_vec(const PagedReadArgs &a, hipStream_t s) {
-  const long long chunks = (a.cap + kReadRows<L> - 1) / kReadRows<L>;
-  const dim3 grid(row_grid(chunks * a.pool.n_kv), (unsigned)std::min<long long>(a.batch, 65535));
-  paged_read_vec_kernel<F, L><<<grid, 64 * kWaves, 0, s>>>(a);
+static void read_vec(PagedReadArgs a, hipStream_t s) {
+  // units that there is room for: under 2^31, and no fewer than workgroups
+  const long long items = a.batch * a.pool.n_kv;
+  a.tile = kReadRows<L>;
+  while ((a.cap + a.tile - 1) / a.tile * items >= 1ll << 31) a.tile *= 2;
+  a.wgs = (int)std::min<long long>(kReadWgs, (a.cap + a.tile - 1) / a.tile * items);
+  paged_read_vec_kernel<F, L><<<a.wgs, 64 * kWaves, 0, s>>>(a);
 }
 
 template <int F>

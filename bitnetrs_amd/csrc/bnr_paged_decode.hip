@@ -154,9 +154,10 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
   const unsigned k_off = row * row_bytes + 16 * g;
   const unsigned v_off = 4 * g * row_bytes + row * (U * B);
   const int first_len = paged_first_len(a);
-  PagedShare sh = paged_share(a, a.pool.n_kv);
+  const auto rows = [&](int b) { return paged_len(a.lens[b], a.pool); };
+  PagedShare sh = paged_share(rows, a.batch, a.pool.n_kv, a.tile, a.wgs);
 
-  for (PagedPiece p; sh.next(a.lens, a.pool, p);) {
+  for (PagedPiece p; sh.next(rows, p);) {
     const int row1 = __builtin_amdgcn_readfirstlane(p.row1);
     const int hk = __builtin_amdgcn_readfirstlane(p.h);
     const int bs = __builtin_amdgcn_readfirstlane(p.b);
