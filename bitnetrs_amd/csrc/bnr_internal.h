@@ -741,8 +741,9 @@ struct PagedDecodeArgs {
 };
 // Floats of a piece of `heads` query heads: outputs, then (max, sum) of each.
 constexpr int paged_part_floats(int heads, int d) { return (heads * (d + 2) + 3) / 4 * 4; }
-// Workgroups of a launch over at most `rows` rows of `items` (sequence, head)
-// pairs each.
+// Workgroups of a decode launch: two a CU.  A third, which the registers of
+// most forms allow, changed 64 int8 sequences of up to 32768 rows by less than
+// 1 % and cost one of 131072 e4m3 rows 8 % (each adds a piece to join).
 constexpr int kPagedMaxWgs = 512;
 hipError_t launch_paged_decode_generic(const PagedDecodeArgs &a, int format, hipStream_t s);
 constexpr int kPagedGenericTile = 64;
