@@ -2735,14 +2735,13 @@ int check_paged_count(size_t n, const char *what) {
   return BNR_OK;
 }
 
-// Workspace: a ticket for each sequence and query head, then the pieces.
-size_t paged_ticket_bytes(size_t batch, size_t n_heads) {
-  return (batch * n_heads * sizeof(unsigned) + 255) / 256 * 256;
-}
+// Workspace: a ticket for each workgroup, at the same place whatever the call's
+// shape (they must be zero for the next one), then the pieces.
+constexpr size_t kPagedTicketBytes = (size_t)kPagedMaxWgs * kCounterStride * sizeof(unsigned);
 
-size_t paged_workspace_bytes(size_t batch, size_t n_heads, size_t group, size_t head_dim) {
-  return paged_ticket_bytes(batch, n_heads) + (size_t)2 * kPagedMaxWgs *
-             paged_part_floats((int)group, (int)head_dim) * sizeof(float);
+size_t paged_workspace_bytes(size_t group, size_t head_dim) {
+  return kPagedTicketBytes +
+         (size_t)2 * kPagedMaxWgs * paged_part_floats((int)group, (int)head_dim) * sizeof(float);
 }
 
 int check_paged_heads(const bnr_paged_kv *kv, size_t batch, size_t n_heads) {
@@ -2856,7 +2855,7 @@ extern "C" int bnr_paged_decode_workspace(bnr_ctx *c, const bnr_paged_kv *kv, si
   int st = paged_pool(kv, nullptr, 1, p);
   if (!st) st = check_paged_heads(kv, batch, n_heads);
   if (st) return st;
-  *bytes = paged_workspace_bytes(batch, n_heads, n_heads / kv->n_kv_heads, kv->head_dim);
+  *bytes = paged_workspace_bytes(n_heads / kv->n_kv_heads, kv->head_dim);
   return set_ok();
 }
 
@@ -2874,7 +2873,7 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
   if (!q || !block_table || !lens || !out || !workspace)
     return err_backend("paged_decode_attention: NULL pointer");
   const size_t group = n_heads / kv->n_kv_heads;
-  const size_t need = paged_workspace_bytes(batch, n_heads, group, kv->head_dim);
+  const size_t need = paged_workspace_bytes(group, kv->head_dim);
   if (workspace_bytes < need)
     return err_shape(fmt("workspace of %zu bytes", need), fmt("%zu bytes", workspace_bytes));
   if (!aligned16(workspace))
@@ -2883,7 +2882,7 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
   a.out = out;
   a.lens = lens;
   a.tickets = (unsigned *)workspace;
-  a.parts = (float *)((char *)workspace + paged_ticket_bytes(batch, n_heads));
+  a.parts = (float *)((char *)workspace + kPagedTicketBytes);
   a.batch = (int)batch;
   a.n_heads = (int)n_heads;
   a.group = (int)group;

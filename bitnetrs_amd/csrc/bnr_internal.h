@@ -734,7 +734,7 @@ struct PagedDecodeArgs {
   float *out;       // [batch][n_heads][d]
   const int *lens;  // [batch]
   float *parts;     // [2 * wgs][part_floats]: unfinished pieces of the line
-  unsigned *tickets;  // [batch][items of a sequence], zero between launches
+  unsigned *tickets;  // [kPagedMaxWgs] x kCounterStride, zero between launches
   int batch, n_heads, group;
   int wgs, part_floats, tile;
   float scale_log2;  // log2(e) / sqrt(d)

@@ -283,13 +283,14 @@ __device__ __forceinline__ void paged_empty(const PagedDecodeArgs &a, int first_
 // d unnormalised outputs (get(w, g, x, o): V of them from x on).  A piece that is a whole
 // item is normalised and written.  Otherwise it goes to the launch's
 // workspace; the last workgroup to bring a piece of the item joins all of
-// them, in the line's order, so the same inputs give the same bits.
+// them, in the line's order, so the same inputs give the same bits.  An item's
+// ticket is its first workgroup's: of the items that a workgroup starts, only
+// the last can go on in the next, so a workgroup needs one.
 //
 // What a join costs is latency: a store, a ticket and a load, each to the
-// device's coherence point and back.  So the loads of kJoin pieces are all in
+// device's coherence point and back.  So the loads of N pieces are all in
 // flight before the first is used, and nothing else waits for memory.
 // ---------------------------------------------------------------------------
-constexpr int kJoin = 8;        // pieces in flight in a thread
 constexpr int kJoinHeads = 16;  // heads of an item at most
 template <int W, int V>
 struct JoinShared {
@@ -342,8 +343,8 @@ struct JoinState {
 
 // V: outputs of a thread, 4 where d is a multiple of 4 and out is 16-byte
 // aligned, or 1.  D: d rounded up to a power of two; w0, w1: the first and the
-// last workgroup of the item.
-template <int W, int V, int D, class Get>
+// last workgroup of the item; N: pieces in flight in a thread.
+template <int W, int V, int D, int N, class Get>
 __device__ __forceinline__ void paged_finish(const PagedDecodeArgs &a, const PagedPiece &p, unsigned wg,
                                              unsigned w0, unsigned w1, Get get, const float *wm,
                                              const float *wl, int heads, JoinShared<W, V> &js) {
@@ -381,7 +382,7 @@ __device__ __forceinline__ void paged_finish(const PagedDecodeArgs &a, const Pag
   // every store of the workgroup is at the device's coherence point before its ticket
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  unsigned *ticket = a.tickets + (size_t)p.b * (a.n_heads / heads) + p.h;
+  unsigned *ticket = a.tickets + w0 * kCounterStride;
   const int n = (int)(w1 - w0) + 1;
   if (tid == 0)
     js.last = (int)__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
@@ -398,10 +399,10 @@ __device__ __forceinline__ void paged_finish(const PagedDecodeArgs &a, const Pag
     const bool in = way < ways && e < work && x < d;
     JoinState<V> s;
     s.clear();
-    for (int i0 = way; in && i0 < n; i0 += kJoin * ways) {
-      float m[kJoin], l[kJoin], po[kJoin][V];
+    for (int i0 = way; in && i0 < n; i0 += N * ways) {
+      float m[N], l[N], po[N][V];
 #pragma unroll
-      for (int k = 0; k < kJoin; ++k) {
+      for (int k = 0; k < N; ++k) {
         // past the last piece: the last again, without a weight (a branch would part the loads)
         const int i = i0 + k * ways < n ? i0 + k * ways : n - 1;
         const int at = (int)(2 * (w0 + (unsigned)i) + (i == 0 ? 1 : 0)) * stride;
@@ -416,7 +417,7 @@ __device__ __forceinline__ void paged_finish(const PagedDecodeArgs &a, const Pag
         }
       }
 #pragma unroll
-      for (int k = 0; k < kJoin; ++k) {
+      for (int k = 0; k < N; ++k) {
         const bool there = i0 + k * ways < n;
         m[k] = there ? m[k] : -INFINITY;
         l[k] = there ? l[k] : 0.f;

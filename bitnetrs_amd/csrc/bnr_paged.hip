@@ -329,7 +329,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
     }
     __syncthreads();
     const auto get = [&](int w, int, int x, float(&to)[1]) { to[0] = s_o[w][x]; };
-    paged_finish<kWaves, 1, kPagedMaxDim>(a, p, sh.wg, sh.wg_of(p.item0), sh.wg_of(p.item1 - 1), get, s_m,
+    paged_finish<kWaves, 1, kPagedMaxDim, 16>(a, p, sh.wg, sh.wg_of(p.item0), sh.wg_of(p.item1 - 1), get, s_m,
                                           s_l, 1, s_join);
   }
   paged_empty(a, first_len);

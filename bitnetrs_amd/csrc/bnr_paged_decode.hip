@@ -45,7 +45,7 @@ constexpr int kBytes = F == kPagedF32 ? 4 : F == kPagedBf16 ? 2 : 1;
 
 // Waves of a SIMD that the registers are shared out for.
 template <int F, int DP>
-constexpr int kWavesOf = DP == 256 ? (F == kPagedInt8 || F == kPagedFp8 ? 2 : 1) : F == kPagedF32 ? 2 : 3;
+constexpr int kWavesOf = DP == 256 && (F == kPagedF32 || F == kPagedBf16) ? 1 : 2;
 
 // N dwords at p; NT: with the non-temporal hint.  V's loads take whole lines
 // and have it; K's take half of each line, the other half comes with the next
@@ -435,7 +435,8 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
 #pragma unroll
       for (int k = 0; k < 4; ++k) to[k] = v[k];
     };
-    paged_finish<kW, 4, DP>(a, p, sh.wg, w0, w1, get, s_m, s_l, G, s_join);
+    // (16 in flight would spill the f32 form: its steps hold twice the rows' dwords)
+    paged_finish<kW, 4, DP, F == kPagedF32 ? 8 : 16>(a, p, sh.wg, w0, w1, get, s_m, s_l, G, s_join);
   }
   paged_empty(a, first_len);
 }

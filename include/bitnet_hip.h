@@ -466,7 +466,8 @@ int bnr_dev_paged_read(bnr_ctx *ctx, const bnr_paged_kv *kv, const int32_t *bloc
                        const int32_t *lens, float *k_out, float *v_out, size_t cap, void *stream);
 
 /* Bytes of workspace that bnr_dev_paged_decode_attention needs for up to
- * `batch` sequences of n_heads query heads over kv. */
+ * `batch` sequences of n_heads query heads over kv.  A workspace serves every
+ * shape that needs no more. */
 int bnr_paged_decode_workspace(bnr_ctx *ctx, const bnr_paged_kv *kv, size_t batch,
                                size_t n_heads, size_t *bytes);
 

@@ -367,10 +367,24 @@ def test_decode_same_bits_and_workspace_left_ready(backend, fmt):
     kv, kv2 = pool.device(), small.device()
     ws = backend.paged_workspace(kv, 4, 20)
     first = check_decode(backend, pool, 20, kv=kv, workspace=ws)
-    assert (ws[:4 * 20 * 4] == 0).all()
+    assert (ws[:512 * 256] == 0).all()
     check_decode(backend, small, 20, kv=kv2, workspace=ws)
     again = check_decode(backend, pool, 20, kv=kv, workspace=ws, times=4)
     assert torch.equal(first, again)
+
+
+def test_workspace_of_many_shapes(backend):
+    """One workspace for calls of other batches, heads, groups and kernels in
+    turn, each leaving pieces of its own: none finds another's tickets."""
+    shapes = [([900] * 16, 16, 16, 64, 16), ([5000], 16, 16, 64, 16), ([3000, 10] * 8, 32, 2, 128, 16),
+              ([700] * 9, 4, 4, 26, 5), ([900] * 40, 16, 16, 64, 16), ([2000], 5, 5, 128, 48)]
+    pools = [Pool(rng_of("shapes", i), "bf16", lens, hkv, d, page, spread=0.3)
+             for i, (lens, _, hkv, d, page) in enumerate(shapes)]
+    kvs = [p.device() for p in pools]
+    ws = max((backend.paged_workspace(kv, len(s[0]), s[1]) for kv, s in zip(kvs, shapes)), key=len)
+    for turn in range(2):
+        for p, kv, s in zip(pools, kvs, shapes):
+            check_decode(backend, p, s[1], kv=kv, workspace=ws)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)

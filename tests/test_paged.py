@@ -140,7 +140,8 @@ def test_workspace_bytes():
     assert st == 0 and n > 0 and n % 16 == 0
     # one byte less is refused, for the same sizes
     assert decode(desc(), bytes=n - 1) == _lib.BNR_INVALID_SHAPE
-    assert workspace(desc(), batch=1000, n_heads=64)[1] > n
+    assert workspace(desc(), batch=1000)[1] == n  # batches and kv heads share one
+    assert workspace(desc(), n_heads=64)[1] > n
     assert workspace(desc(), n_heads=3)[0] == _lib.BNR_INVALID_CONFIG
     assert workspace(desc(), out=False)[0] == _lib.BNR_BACKEND_ERROR
     assert workspace(None)[0] == _lib.BNR_BACKEND_ERROR
