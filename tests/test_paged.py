@@ -1,6 +1,8 @@
 """Paged KV cache without a GPU: what the entry points refuse, before they
 touch the device, and what the Python side refuses."""
 import ctypes
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -212,3 +214,14 @@ def test_format_definitions():
         assert (back[0] == 0).all()
         top = np.abs(codes.float().numpy()).max(-1)
         assert (top[2:] == TOP[fmt]).all()
+
+
+def test_index_code_on_the_host():
+    """The kernels' own index code: rows stay inside the pool whatever tables,
+    positions and sequences hold; shares of a launch cover its work once."""
+    native = os.path.join(os.path.dirname(os.path.abspath(__file__)), "native")
+    check = os.path.join(native, "paged_index_check")
+    if not os.path.exists(check):
+        subprocess.run(["make", "-s", "-C", native, check], check=True)
+    out = subprocess.run([check], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout + out.stderr
