@@ -547,8 +547,23 @@ PrefillPlanEntry plan_prefill_cached(bnr_ctx *c, int n_tokens, int start_pos, in
   return e;
 }
 
-// RopeCache::new (bitnet-cpu/src/rope.rs:100-153) on the host: same f32
-// formula, same libm, so the table is bit-identical to the reference's.
+// Rows first .. first + n - 1 of RopeCache::new's table
+// (bitnet-cpu/src/rope.rs:100-153): same f32 formula, same libm, so they are
+// bit-identical to the reference's.
+void rope_rows(size_t first, size_t n, size_t head_dim, float theta, float *hc, float *hs) {
+  const size_t half = head_dim / 2;
+  for (size_t r = 0; r < n; ++r) {
+    for (size_t i = 0; i < half; ++i) {
+      volatile float exponent = -2.0f * (float)i / (float)head_dim;
+      float freq = powf(theta, exponent);
+      volatile float angle = (float)(first + r) * freq;
+      hc[r * half + i] = cosf(angle);
+      hs[r * half + i] = sinf(angle);
+    }
+  }
+}
+
+// The context's table, built on the host.
 int build_table(bnr_ctx *c, size_t max_seq, size_t head_dim, float theta) {
   if (head_dim == 0 || head_dim % 2 != 0)
     return err_config(fmt("head_dim must be even and > 0, got %zu", head_dim));
@@ -556,15 +571,7 @@ int build_table(bnr_ctx *c, size_t max_seq, size_t head_dim, float theta) {
     return err_config("theta must be finite and > 0, got " + rust_f32(theta));
   const size_t half = head_dim / 2, n = max_seq * half;
   std::vector<float> hc(n), hs(n);
-  for (size_t pos = 0; pos < max_seq; ++pos) {
-    for (size_t i = 0; i < half; ++i) {
-      volatile float exponent = -2.0f * (float)i / (float)head_dim;
-      float freq = powf(theta, exponent);
-      volatile float angle = (float)pos * freq;
-      hc[pos * half + i] = cosf(angle);
-      hs[pos * half + i] = sinf(angle);
-    }
-  }
+  rope_rows(0, max_seq, head_dim, theta, hc.data(), hs.data());
   float *dc = nullptr, *ds = nullptr;
   HIP_TRY(hipMalloc((void **)&dc, std::max<size_t>(n, 1) * sizeof(float)), "rope table alloc");
   hipError_t e = hipMalloc((void **)&ds, std::max<size_t>(n, 1) * sizeof(float));
@@ -2685,7 +2692,8 @@ namespace {
 // A sequence has at most this many rows, so that a row's number and a
 // length rounded up to any tile are ints.
 constexpr size_t kPagedMaxRows = (size_t)1 << 30;
-constexpr size_t kPagedMaxCount = (size_t)1 << 31;  // pages; sequences x heads
+constexpr size_t kPagedMaxCount = (size_t)1 << 31;  // pages; tokens; sequences x heads
+constexpr size_t kPagedMaxBatch = (size_t)1 << 20;  // sequences that a kernel adds up the lengths of
 
 // Checks the pool and the table, and fills the kernels' view of them.
 int paged_pool(const bnr_paged_kv *kv, const int32_t *table, size_t table_stride, PagedPool &p) {
@@ -2730,6 +2738,13 @@ int paged_pool(const bnr_paged_kv *kv, const int32_t *table, size_t table_stride
   return BNR_OK;
 }
 
+int check_paged_batch(size_t batch, size_t heads) {
+  if (batch > kPagedMaxBatch || batch >= kPagedMaxCount / heads)
+    return err_shape(fmt("batch <= %zu and batch * heads < %zu", kPagedMaxBatch, kPagedMaxCount),
+                     fmt("batch = %zu, heads = %zu", batch, heads));
+  return BNR_OK;
+}
+
 int check_paged_count(size_t n, const char *what) {
   if (n >= kPagedMaxCount) return err_shape(fmt("%s < %zu", what, kPagedMaxCount), fmt("%zu", n));
   return BNR_OK;
@@ -2748,10 +2763,7 @@ int check_paged_heads(const bnr_paged_kv *kv, size_t batch, size_t n_heads) {
   int st = check_heads(n_heads, kv->n_kv_heads, kv->head_dim);
   if (st) return st;
   if (n_heads > 65536) return err_config(fmt("n_heads must be at most 65536, got %zu", n_heads));
-  if (batch >= kPagedMaxCount / n_heads)
-    return err_shape(fmt("batch * n_heads < %zu", kPagedMaxCount),
-                     fmt("batch = %zu, n_heads = %zu", batch, n_heads));
-  return BNR_OK;
+  return check_paged_batch(batch, n_heads);
 }
 
 }  // namespace
@@ -2762,19 +2774,28 @@ extern "C" int bnr_dev_rope_table(bnr_ctx *c, size_t n_positions, size_t head_di
   int st = check_rope(head_dim, theta);
   if (st) return st;
   if (n_positions == 0) return set_ok();
-  if (n_positions > kPagedMaxRows)
-    return err_shape(fmt("n_positions <= %zu", kPagedMaxRows), fmt("n_positions = %zu", n_positions));
+  if (n_positions > kPagedMaxRows || head_dim > kPagedMaxRows / n_positions * 64)
+    return err_shape(fmt("n_positions * head_dim / 64 <= %zu", kPagedMaxRows),
+                     fmt("n_positions = %zu, head_dim = %zu", n_positions, head_dim));
   if (!cos_out || !sin_out) return err_backend("rope_table: NULL pointer");
-  std::lock_guard<std::mutex> lk(c->mu);
   DeviceGuard dg(c->device);
-  st = ensure_table(c, n_positions - 1, head_dim, theta);
-  if (st) return st;
-  const size_t bytes = n_positions * (head_dim / 2) * sizeof(float);
   hipStream_t s = (hipStream_t)stream;
-  HIP_TRY(hipMemcpyAsync(cos_out, c->d_cos, bytes, hipMemcpyDeviceToDevice, s), "rope table copy");
-  HIP_TRY(hipMemcpyAsync(sin_out, c->d_sin, bytes, hipMemcpyDeviceToDevice, s), "rope table copy");
-  // the context may replace its own table once the lock is released
-  HIP_TRY(hipStreamSynchronize(s), "rope table copy");
+  // A block of rows at a time, and not through the context's own table, which
+  // captured launches may read.
+  constexpr size_t kRows = 4096;
+  const size_t half = head_dim / 2;
+  try {
+    std::vector<float> hc(std::min(kRows, n_positions) * half), hs(hc.size());
+    for (size_t r = 0; r < n_positions; r += kRows) {
+      const size_t n = std::min(kRows, n_positions - r), bytes = n * half * sizeof(float);
+      rope_rows(r, n, head_dim, theta, hc.data(), hs.data());
+      HIP_TRY(hipMemcpyAsync(cos_out + r * half, hc.data(), bytes, hipMemcpyHostToDevice, s), "rope table copy");
+      HIP_TRY(hipMemcpyAsync(sin_out + r * half, hs.data(), bytes, hipMemcpyHostToDevice, s), "rope table copy");
+      HIP_TRY(hipStreamSynchronize(s), "rope table copy");
+    }
+  } catch (const std::bad_alloc &) {
+    return err_backend("rope_table: out of host memory");
+  }
   return set_ok();
 }
 
@@ -2823,9 +2844,7 @@ extern "C" int bnr_dev_paged_read(bnr_ctx *c, const bnr_paged_kv *kv, const int3
   if (!c) return err_backend("context is NULL");
   PagedReadArgs a{};
   int st = paged_pool(kv, block_table, table_stride, a.pool);
-  if (!st && batch >= kPagedMaxCount / kv->n_kv_heads)
-    st = err_shape(fmt("batch * n_kv_heads < %zu", kPagedMaxCount),
-                   fmt("batch = %zu, n_kv_heads = %zu", batch, kv->n_kv_heads));
+  if (!st) st = check_paged_batch(batch, kv->n_kv_heads);
   if (st) return st;
   if (cap > kPagedMaxRows)
     return err_shape(fmt("cap <= %zu", kPagedMaxRows), fmt("cap = %zu", cap));
@@ -2888,7 +2907,7 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
   a.group = (int)group;
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)kv->head_dim));
   const bool fast = kv->head_dim % 16 == 0 && kv->head_dim <= 256 && group <= 16 &&
-                    kv->page_size >= 16 && (kv->page_size & (kv->page_size - 1)) == 0 &&
+                    kv->page_size % 16 == 0 &&
                     aligned16(q) && aligned16(out) && aligned16(kv->k) && aligned16(kv->v) &&
                     aligned16(a.pool.k_scales) && aligned16(a.pool.v_scales);
   size_t tile = fast ? kPagedTile : kPagedGenericTile;

@@ -748,8 +748,8 @@ constexpr int kPagedMaxWgs = 512;
 hipError_t launch_paged_decode_generic(const PagedDecodeArgs &a, int format, hipStream_t s);
 constexpr int kPagedGenericTile = 64;
 // On the matrix cores: 16-byte aligned pools, q and out, head_dim a multiple
-// of 16 up to 256, at most 16 query heads a kv head, pages of a power of two
-// of at least 16 rows.
+// of 16 up to 256, at most 16 query heads a kv head, pages of a multiple of 16
+// rows.
 hipError_t launch_paged_decode(const PagedDecodeArgs &a, int format, hipStream_t s);
 constexpr int kPagedTile = 128;
 

@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
   const int lane = threadIdx.x & 63, d = FULL ? DP : a.pool.d, G = a.group;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int row = lane & 15, g = lane >> 4;
-  const int page_shift = __builtin_ctz(a.pool.page);
+  const int page = a.pool.page, page_shift = page & (page - 1) ? -1 : __builtin_ctz(page);
   const unsigned row_bytes = (unsigned)d * B;
   const unsigned k_off = row * row_bytes + 16 * g;
   const unsigned v_off = 4 * g * row_bytes + row * (U * B);
@@ -170,14 +170,18 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
     const int *table = a.pool.table + (long long)bs * a.pool.table_stride;
     int t = __builtin_amdgcn_readfirstlane(p.row0) + kStep * wave;
 
-    // Pages of the wave's next 32 steps, lane 2 i + h that of tile h of step
-    // i: one load for all of them.  -1: past the piece, or not there.
+    // Where the 16-row tiles of the wave's next 32 steps lie, lane 2 i + h tile
+    // h of step i: one load for all of them.  The page, -1 past the piece or
+    // where it is not there; and the tile's row in it.
+    int pages, rows_in, step = 0;
     auto load_pages = [&](int t0) {
       const int at = t0 + (lane >> 1) * (kW * kStep) + (lane & 1) * 16;
-      const int pg = at < row1 ? table[at >> page_shift] : -1;
-      return (unsigned)pg < (unsigned)a.pool.n_pages ? pg : -1;
+      const int i = page_shift >= 0 ? at >> page_shift : at / page;
+      const int pg = at < row1 ? table[i] : -1;
+      pages = (unsigned)pg < (unsigned)a.pool.n_pages ? pg : -1;
+      rows_in = at - i * page;
     };
-    int pages = load_pages(t), step = 0;
+    load_pages(t);
 
     // The wave's chunks of the query heads: the dims that a lane's K bytes
     // hold, 16 bytes at 64 c + 16 g of the row.
@@ -203,15 +207,14 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
 
     unsigned kr[2][KW * 4], vr[2][4][VW];
     f32x4 ks[2], vs[2];
-    // First row, in rows of the pool, of the 16-row tile at row t; page 0's where there is none.
-    auto tile_row = [&](int pg, int t) {
-      return ((long long)(pg < 0 ? 0 : pg) * a.pool.n_kv + hk) * a.pool.page +
-             (pg < 0 ? 0 : t & (a.pool.page - 1));
+    // First row in the pool of the tile at row `in` of page pg, page 0's first where there is none.
+    auto tile_row = [&](int pg, int in) {
+      return ((long long)(pg < 0 ? 0 : pg) * a.pool.n_kv + hk) * page + (pg < 0 ? 0 : in);
     };
-    auto load_k = [&](int t, const int (&pg)[2]) {
+    auto load_k = [&](const int (&pg)[2], const int (&in)[2]) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const long long at = tile_row(pg[h], t + 16 * h);
+        const long long at = tile_row(pg[h], in[h]);
         const char *src = static_cast<const char *>(a.pool.k) + at * row_bytes;
 #pragma unroll
         for (int c = 0; c < KW; ++c) {
@@ -223,10 +226,10 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
         if (kPagedScaled<F>) ks[h] = *reinterpret_cast<const f32x4 *>(a.pool.k_scales + at + 4 * g);
       }
     };
-    auto load_v = [&](int t, const int (&pg)[2]) {
+    auto load_v = [&](const int (&pg)[2], const int (&in)[2]) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const long long at = tile_row(pg[h], t + 16 * h);
+        const long long at = tile_row(pg[h], in[h]);
         const char *src = static_cast<const char *>(a.pool.v) + at * row_bytes;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -244,16 +247,20 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
       }
     };
 
-    int pg[2], pn[2];
+    // pages of this step's and the next one's tiles, and the latter's rows there
+    int pg[2], pn[2], in[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       pg[h] = __builtin_amdgcn_readlane(pages, h);
+      in[h] = __builtin_amdgcn_readlane(rows_in, h);
       pn[h] = __builtin_amdgcn_readlane(pages, 2 + h);
     }
     if (t < row1) {
-      load_k(t, pg);
-      load_v(t, pg);
+      load_k(pg, in);
+      load_v(pg, in);
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) in[h] = __builtin_amdgcn_readlane(rows_in, 2 + h);
     // while they are on their way
     __syncthreads();  // the piece before this one has been read
 #pragma unroll
@@ -332,7 +339,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
           for (int r = 0; r < 4; ++r)
             if (pg[h] < 0 || t + 16 * h + 4 * g + r >= row1) x[4 * h + r] = -INFINITY;
       // the next step's K goes out while this one's weights are made
-      if constexpr (kMore) load_k(tn, pn);
+      if constexpr (kMore) load_k(pn, in);
 
       float mx = m;
 #pragma unroll
@@ -396,15 +403,16 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
         }
       }
       if constexpr (kMore) {
-        load_v(tn, pn);
+        load_v(pn, in);
         if (++step == 31) {  // pages of the step after the next
-          pages = load_pages(tn + kW * kStep);
+          load_pages(tn + kW * kStep);
           step = -1;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           pg[h] = pn[h];
           pn[h] = __builtin_amdgcn_readlane(pages, 2 * (step + 1) + h);
+          in[h] = __builtin_amdgcn_readlane(rows_in, 2 * (step + 1) + h);
         }
         t = tn;
       }

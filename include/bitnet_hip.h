@@ -412,6 +412,12 @@ int bnr_kv_dev_prefill(bnr_ctx *ctx, bnr_kv_cache *cache, size_t layer, float *q
  * The pool is the caller's memory; these calls allocate nothing and keep
  * nothing, so calls on different workspaces may run side by side.
  *
+ * Sizes: head_dim even and at most 512; a sequence has at most 2^30 rows
+ * (table_stride * page_size), a call at most 2^20 sequences.  Attention runs on
+ * the matrix cores where head_dim is a multiple of 16 up to 256, a kv head has
+ * at most 16 query heads, pages have a multiple of 16 rows and the pool, q and
+ * out are 16-byte aligned; everything else takes a slower kernel.
+ *
  * Formats of a pool's rows, a row being head_dim values of one token and one
  * kv head.  x is the value in fp32 (for K: after the rotation):
  *   F32   x
@@ -435,7 +441,8 @@ typedef struct bnr_paged_kv {
 /* The rotation tables of bnr_rope_embed (the same values) for positions
  * 0..n_positions-1, into cos_out and sin_out [n_positions x head_dim/2] in
  * device memory: a caller of bnr_dev_paged_append keeps them.  Builds them on
- * the host and waits for the copy: not for use under graph capture. */
+ * the host and waits for the copy: not for use under graph capture.  The
+ * context's own table stays as it is. */
 int bnr_dev_rope_table(bnr_ctx *ctx, size_t n_positions, size_t head_dim, float theta,
                        float *cos_out, float *sin_out, void *stream);
 

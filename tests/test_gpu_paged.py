@@ -586,3 +586,32 @@ def test_python_refusals(backend):
                         ((table, lens, ko[:, :1].contiguous(), ko), InvalidShape)):
         with pytest.raises(error):
             backend.dev_paged_read(kv, *args)
+    for call, args in ((backend.dev_paged_append, (q, x, x, out, pos, lens)), (backend.dev_paged_read, (lens, lens, ko, ko)),
+                       (backend.dev_paged_read, (table, lens, ko[0], ko[0])),
+                       (backend.dev_paged_decode_attention, (q[0], table, lens, out, ws)),
+                       (backend.dev_paged_decode_attention, (q, table, lens, out, ws.view(1, -1)))):
+        with pytest.raises(InvalidShape):
+            call(kv, *args)
+
+
+def test_rope_table_leaves_the_contexts_own(backend):
+    """A captured step of the contiguous cache still reads its table after
+    tables of other sizes, head dims and thetas were built for paged caches."""
+    d, hq, hkv, cap = 128, 20, 5, 4096
+    q, k, v = (torch.randn(h * d, device="cuda") for h in (hq, hkv, hkv))
+    kc, vc = (torch.randn(hkv, cap, d, device="cuda") for _ in range(2))
+    out, ref = torch.zeros(hq * d, device="cuda"), torch.zeros(hq * d, device="cuda")
+    args = (q, k, v, 70, hq, hkv, d, THETA, kc, vc, cap)
+    backend.dev_decode_step(*args, ref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        backend.dev_decode_step(*args, out)
+    for n, dim, theta in ((20000, d, THETA), (100, 64, THETA), (5000, d, 1e4)):
+        cos, sin = backend.rope_table(n, dim, theta)
+        assert cos.shape == sin.shape == (n, dim // 2) and (cos[0] == 1).all() and (sin[0] == 0).all()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out - ref).abs().max() <= 1e-5 * ref.abs().max()
+    del graph

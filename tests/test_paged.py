@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import bitnetrs_amd
-from bitnetrs_amd import _lib
+from bitnetrs_amd import _lib, backend
 from bitnetrs_amd._lib import PagedKVDesc
 from common import error_from_parts
 
@@ -106,6 +106,8 @@ def test_null_context_and_pool(call):
     (append, dict(sin=None), _lib.BNR_BACKEND_ERROR),
     (read, dict(stride=0), _lib.BNR_INVALID_SHAPE),
     (read, dict(batch=1 << 31), _lib.BNR_INVALID_SHAPE),
+    (read, dict(batch=(1 << 20) + 1), _lib.BNR_INVALID_SHAPE),
+    (decode, dict(batch=(1 << 20) + 1), _lib.BNR_INVALID_SHAPE),
     (read, dict(cap=(1 << 30) + 1), _lib.BNR_INVALID_SHAPE),
     (read, dict(cap=1 << 30, batch=(1 << 31) - 1), _lib.BNR_INVALID_SHAPE),
     (read, dict(table=None), _lib.BNR_BACKEND_ERROR),
@@ -155,6 +157,7 @@ def test_rope_table_refusals():
     assert f(CTX, 4, 7, 1e4, P, P, None) == _lib.BNR_INVALID_CONFIG
     assert f(CTX, 4, 8, 0.0, P, P, None) == _lib.BNR_INVALID_CONFIG
     assert f(CTX, (1 << 30) + 1, 8, 1e4, P, P, None) == _lib.BNR_INVALID_SHAPE
+    assert f(CTX, 1 << 20, 1 << 20, 1e4, P, P, None) == _lib.BNR_INVALID_SHAPE
     assert f(CTX, 4, 8, 1e4, None, P, None) == _lib.BNR_BACKEND_ERROR
     assert f(CTX, 0, 8, 1e4, None, None, None) == 0
 
@@ -192,6 +195,24 @@ def test_paged_kv_refusals(make, error):
 def test_unknown_format_name():
     with pytest.raises(bitnetrs_amd.InvalidConfig):
         bitnetrs_amd.PagedKV(1, 16, 1, 8, "int4", device="cpu")
+
+
+@pytest.mark.parametrize("t,dtype,shape,error", [
+    (None, torch.float32, (2,), TypeError), (np.zeros(2, np.float32), torch.float32, (2,), TypeError),
+    (torch.zeros(2), torch.float32, (2,), TypeError), ([0.0], torch.float32, (1,), TypeError),
+])
+def test_operand_check(t, dtype, shape, error):
+    # nothing here is a tensor on GPU 0
+    with pytest.raises(error):
+        backend._on(t, "x", dtype, 0, shape)
+
+
+def test_operand_sizes():
+    assert backend._sizes(torch.zeros(2, 3), "x", 2) == (2, 3)
+    with pytest.raises(bitnetrs_amd.InvalidShape):
+        backend._sizes(torch.zeros(2), "x", 2)
+    with pytest.raises(TypeError):
+        backend._sizes(None, "x", 2)
 
 
 def test_format_definitions():
