@@ -68,15 +68,16 @@ def _on(t, name: str, dtype, device: int, shape=None):
     return t.data_ptr()
 
 
-def _sizes(t, name: str, n: int):
-    """The n sizes of a tensor."""
-    try:
-        sizes = t.shape
-    except AttributeError:
-        raise TypeError(f"{name} must be a tensor") from None
-    if len(sizes) != n:
-        raise InvalidShape(f"{name} of {n} dimensions", f"{list(sizes)}")
-    return sizes
+def _check_sizes(*operands) -> None:
+    """Raise for the first of the (tensor, name, dimensions) that has others: what
+    a call says whose operands' sizes did not unpack."""
+    for t, name, n in operands:
+        try:
+            sizes = t.shape
+        except AttributeError:
+            raise TypeError(f"{name} must be a tensor") from None
+        if len(sizes) != n:
+            raise InvalidShape(f"{name} of {n} dimensions", f"{list(sizes)}")
 
 
 def _stream(stream):
@@ -365,18 +366,23 @@ class HipBackend:
         rotation's tables (rope_table), None for rows that are rotated; q and
         q_out may both be None."""
         dev, f32, i32, d = self.device_id, kv.f32, kv.i32, kv.head_dim
-        (n,), (n_seqs, stride) = _sizes(positions, "positions", 1), _sizes(block_table, "block_table", 2)
-        n_heads, qp, qop = 0, None, None
+        n_heads, n_pos, qp, qop, cp, sp = 0, 0, None, None, None, None
+        try:
+            (n,), (n_seqs, stride) = positions.shape, block_table.shape
+            if q is not None:
+                _, n_heads, _ = q.shape
+            if cos is not None:
+                n_pos, _ = cos.shape
+        except (AttributeError, ValueError):
+            _check_sizes((positions, "positions", 1), (block_table, "block_table", 2),
+                         *([] if q is None else [(q, "q", 3)]), *([] if cos is None else [(cos, "cos", 2)]))
+            raise
         if q is not None and q_out is not None:
-            n_heads = _sizes(q, "q", 3)[1]
             qp = _on(q, "q", f32, dev, (n, n_heads, d))
             qop = qp if q_out is q else _on(q_out, "q_out", f32, dev, (n, n_heads, d))
         elif q is not q_out:
             raise TypeError("q and q_out go together")
-        cp = sp = None
-        n_pos = 0
         if cos is not None and sin is not None:
-            n_pos = _sizes(cos, "cos", 2)[0]
             cp = _on(cos, "cos", f32, dev, (n_pos, d // 2))
             sp = _on(sin, "sin", f32, dev, (n_pos, d // 2))
         elif cos is not sin:
@@ -394,8 +400,12 @@ class HipBackend:
         """Rows starts[s] (None: 0) .. lens[s]-1 of each sequence of block_table
         [batch, pages] as fp32 into k_out and v_out [batch, n_kv_heads, cap, d],
         from row 0 on; what lies behind them stays."""
-        dev, i32, cap = self.device_id, kv.i32, _sizes(k_out, "k_out", 4)[2]
-        batch, stride = _sizes(block_table, "block_table", 2)
+        dev, i32 = self.device_id, kv.i32
+        try:
+            (batch, stride), (_, _, cap, _) = block_table.shape, k_out.shape
+        except (AttributeError, ValueError):
+            _check_sizes((block_table, "block_table", 2), (k_out, "k_out", 4))
+            raise
         out = (batch, kv.n_kv_heads, cap, kv.head_dim)
         _lib.check(self._L.bnr_dev_paged_read(
             self._h, kv.desc(dev), _on(block_table, "block_table", i32, dev), batch, stride,
@@ -418,13 +428,17 @@ class HipBackend:
         """Attention of one token of each sequence, q [batch, n_heads, d] (rotated),
         over rows 0..lens[s]-1 of its own, into out (as q).  `workspace` from
         paged_workspace; calls that share one must be ordered."""
-        dev, i32, n_heads = self.device_id, kv.i32, _sizes(q, "q", 3)[1]
-        batch, stride = _sizes(block_table, "block_table", 2)
+        dev, i32 = self.device_id, kv.i32
+        try:
+            (batch, stride), (_, n_heads, _), (n,) = block_table.shape, q.shape, workspace.shape
+        except (AttributeError, ValueError):
+            _check_sizes((block_table, "block_table", 2), (q, "q", 3), (workspace, "workspace", 1))
+            raise
         qs = (batch, n_heads, kv.head_dim)
         _lib.check(self._L.bnr_dev_paged_decode_attention(
             self._h, kv.desc(dev), _on(q, "q", kv.f32, dev, qs), n_heads,
             _on(block_table, "block_table", i32, dev), batch, stride, _on(lens, "lens", i32, dev, (batch,)),
-            _on(out, "out", kv.f32, dev, qs), _on(workspace, "workspace", kv.u8, dev), _sizes(workspace, "workspace", 1)[0],
+            _on(out, "out", kv.f32, dev, qs), _on(workspace, "workspace", kv.u8, dev), n,
             self._paged_stream(kv, stream)))
 
     def dev_synchronize(self, stream=None) -> None:

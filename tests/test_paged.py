@@ -208,11 +208,11 @@ def test_operand_check(t, dtype, shape, error):
 
 
 def test_operand_sizes():
-    assert backend._sizes(torch.zeros(2, 3), "x", 2) == (2, 3)
+    backend._check_sizes((torch.zeros(2, 3), "x", 2), (torch.zeros(1), "y", 1))
     with pytest.raises(bitnetrs_amd.InvalidShape):
-        backend._sizes(torch.zeros(2), "x", 2)
+        backend._check_sizes((torch.zeros(2, 3), "x", 2), (torch.zeros(2), "y", 2))
     with pytest.raises(TypeError):
-        backend._sizes(None, "x", 2)
+        backend._check_sizes((None, "x", 2))
 
 
 def test_format_definitions():
