@@ -6,6 +6,8 @@
 #include "bnr_device.h"
 #include "bnr_paged_index.h"
 
+#include <type_traits>
+
 namespace bnr {
 
 // ---------------------------------------------------------------------------
@@ -273,33 +275,41 @@ __device__ __forceinline__ void paged_finish(const PagedDecodeArgs &a, const Pag
     const bool in = way < ways && e < work && x < d;
     JoinState<V> s;
     s.clear();
-    for (int i0 = way; in && i0 < n; i0 += N * ways) {
-      float m[N], l[N], po[N][V];
+    const auto take = [&](auto at_once) {
+      constexpr int M = decltype(at_once)::value;
+      for (int i0 = way; in && i0 < n; i0 += M * ways) {
+        float m[M], l[M], po[M][V];
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        // past the last piece: the last again, without a weight (a branch would part the loads)
-        const int i = i0 + k * ways < n ? i0 + k * ways : n - 1;
-        const int at = (int)(2 * (w0 + (unsigned)i) + (i == 0 ? 1 : 0)) * stride;
-        const float2 ml = ld2_agent(parts, at + (heads * d + 2 * g) * 4);
-        m[k] = ml.x;
-        l[k] = ml.y;
-        if constexpr (V == 4) {
-          const float4 v = ld4_agent(parts, at + (g * d + x) * 4);
-          po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
-        } else {
-          po[k][0] = ld_agent(a.parts + at / 4 + g * d + x);
+        for (int k = 0; k < M; ++k) {
+          // past the last piece: the last again, without a weight (a branch would part the loads)
+          const int i = i0 + k * ways < n ? i0 + k * ways : n - 1;
+          const int at = (int)(2 * (w0 + (unsigned)i) + (i == 0 ? 1 : 0)) * stride;
+          const float2 ml = ld2_agent(parts, at + (heads * d + 2 * g) * 4);
+          m[k] = ml.x;
+          l[k] = ml.y;
+          if constexpr (V == 4) {
+            const float4 v = ld4_agent(parts, at + (g * d + x) * 4);
+            po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
+          } else {
+            po[k][0] = ld_agent(a.parts + at / 4 + g * d + x);
+          }
         }
-      }
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const bool there = i0 + k * ways < n;
-        m[k] = there ? m[k] : -INFINITY;
-        l[k] = there ? l[k] : 0.f;
+        for (int k = 0; k < M; ++k) {
+          const bool there = i0 + k * ways < n;
+          m[k] = there ? m[k] : -INFINITY;
+          l[k] = there ? l[k] : 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) po[k][j] = there ? po[k][j] : 0.f;
+          for (int j = 0; j < V; ++j) po[k][j] = there ? po[k][j] : 0.f;
+        }
+        s.add(m, l, po);
       }
-      s.add(m, l, po);
-    }
+    };
+    // few pieces: no loads for the places of more (8 sequences of 100 to 900 int8 rows 8.7 -> 7.9 us)
+    if (n <= 4 * ways)
+      take(std::integral_constant<int, 4>{});
+    else
+      take(std::integral_constant<int, N>{});
     if (ways > 1) {  // work < nt: one round
       js.m[tid] = s.m;
       js.l[tid] = s.l;
