@@ -274,6 +274,17 @@ def test_decode_batches(backend, fmt, lens):
     check_decode(backend, pool, 20)
 
 
+@pytest.mark.parametrize("fmt,page", [("int8", 16), ("bf16", 48), ("f32", 64), ("fp8", 128)])
+def test_decode_long_pieces(backend, fmt, page):
+    """Pieces of more than 4096 rows of one workgroup, with pages that are not
+    there among them and a last page that is not full."""
+    say(f"decode long pieces {fmt}")
+    rng = rng_of("long", fmt)
+    pool = Pool(rng, fmt, [150001], 16, 16, page, spread=0.3)
+    pool.table[0, rng.choice(pool.table.shape[1], 40, replace=False)] = -1
+    check_decode(backend, pool, 16)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("d,page", [(128, 16), (128, 64), (80, 32), (10, 3)])
 def test_decode_missing_pages_and_lengths(backend, fmt, d, page):
