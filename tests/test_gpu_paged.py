@@ -254,7 +254,7 @@ RAGGED = [1, 0, 2, 15, 16, 17, 31, 33, 64, 65, 127, 128, 129, 500, 1, 1000]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("hq,hkv,d,page", SHAPES + [(16, 1, 128, 16), (17, 1, 64, 16), (40, 2, 48, 32),
+@pytest.mark.parametrize("hq,hkv,d,page", SHAPES + [(16, 1, 128, 16), (16, 1, 256, 16), (17, 1, 64, 16), (40, 2, 48, 32),
                                                     (2, 2, 16, 16), (6, 2, 192, 16), (1, 1, 128, 64),
                                                     (12, 4, 128, 48), (9, 3, 112, 16)])
 def test_decode(backend, fmt, hq, hkv, d, page):
