@@ -2725,6 +2725,8 @@ int paged_pool(const bnr_paged_kv *kv, const int32_t *table, size_t table_stride
   const uintptr_t unit = kv->format == BNR_KV_F32 ? 4 : kv->format == BNR_KV_BF16 ? 2 : 1;
   if (((uintptr_t)kv->k | (uintptr_t)kv->v) % unit != 0)
     return err_shape(fmt("%zu-byte aligned pool pointers", (size_t)unit), "an unaligned pointer");
+  if (scaled && ((uintptr_t)kv->k_scales | (uintptr_t)kv->v_scales) % 4 != 0)
+    return err_shape("4-byte aligned scales", "an unaligned pointer");
   p.k = kv->k;
   p.v = kv->v;
   p.k_scales = scaled ? kv->k_scales : nullptr;
@@ -2815,6 +2817,8 @@ extern "C" int bnr_dev_paged_append(bnr_ctx *c, const bnr_paged_kv *kv, const fl
   if (!st) st = check_paged_count(n_seqs, "n_seqs");
   if (st) return st;
   if (n_tokens == 0) return set_ok();
+  if (!seqs && n_tokens > n_seqs)
+    return err_shape("a sequence for each token, or seqs", fmt("n_tokens = %zu, n_seqs = %zu", n_tokens, n_seqs));
   if (!k || !v || !positions || !block_table || !q != !q_out || !cos_tab != !sin_tab)
     return err_backend("paged_append: NULL pointer");
   a.q = q;

@@ -447,15 +447,17 @@ int bnr_dev_rope_table(bnr_ctx *ctx, size_t n_positions, size_t head_dim, float 
                        float *cos_out, float *sin_out, void *stream);
 
 /* Rotate and append n_tokens tokens of any sequences: token i has position
- * positions[i] of sequence seqs[i] (seqs NULL: of sequence i).  q [n_tokens x
- * n_heads x d] rotated goes to q_out (which may be q); k and v [n_tokens x
- * n_kv_heads x d] go to the pool, k rotated, both in its format.  q and q_out
- * may both be NULL.  cos_tab / sin_tab [n_positions x d/2] are the rotation
- * (half-split pairs, as bnr_rope_embed, bit-identical to it with
- * bnr_dev_rope_table's tables); both NULL: q and k are taken as rotated.
- * A token whose position is negative, at or past table_stride*page_size or
- * n_positions, or whose sequence is outside 0..n_seqs-1 is left out: its
- * q_out row is not written either.  A row may be named once per call. */
+ * positions[i] of sequence seqs[i] (seqs NULL: of sequence i, n_tokens <=
+ * n_seqs).  q [n_tokens x n_heads x d] rotated goes to q_out (which may be q);
+ * k and v [n_tokens x n_kv_heads x d] go to the pool, k rotated, both in its
+ * format.  q and q_out may both be NULL.  cos_tab / sin_tab [n_positions x
+ * d/2] are the rotation (half-split pairs, as bnr_rope_embed, bit-identical to
+ * it with bnr_dev_rope_table's tables); both NULL: q and k are taken as
+ * rotated.  A token whose position is negative, at or past
+ * table_stride*page_size or n_positions, or whose sequence is outside
+ * 0..n_seqs-1 is left out: its q_out row is not written either.  (Where only
+ * its page is not there, q_out is written and k and v are dropped.)  A row may
+ * be named once per call. */
 int bnr_dev_paged_append(bnr_ctx *ctx, const bnr_paged_kv *kv, const float *q, const float *k,
                          const float *v, float *q_out, size_t n_tokens, size_t n_heads,
                          const int32_t *positions, const int32_t *seqs,

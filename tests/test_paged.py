@@ -71,6 +71,7 @@ BAD_POOLS = [
     (dict(format=_lib.BNR_KV_FP8, v_scales=None), _lib.BNR_BACKEND_ERROR, "NULL"),
     (dict(format=_lib.BNR_KV_BF16, k=P + 1), _lib.BNR_INVALID_SHAPE, "aligned"),
     (dict(format=_lib.BNR_KV_F32, v=P + 2), _lib.BNR_INVALID_SHAPE, "aligned"),
+    (dict(k_scales=P + 2), _lib.BNR_INVALID_SHAPE, "aligned"),
 ]
 
 
@@ -96,6 +97,7 @@ def test_null_context_and_pool(call):
     (append, dict(n_heads=1 << 20), _lib.BNR_INVALID_CONFIG),
     (append, dict(n_tokens=1 << 31), _lib.BNR_INVALID_SHAPE),
     (append, dict(n_seqs=1 << 31), _lib.BNR_INVALID_SHAPE),
+    (append, dict(seqs=None, n_tokens=2), _lib.BNR_INVALID_SHAPE),
     (append, dict(q=None), _lib.BNR_BACKEND_ERROR),
     (append, dict(q_out=None), _lib.BNR_BACKEND_ERROR),
     (append, dict(k=None), _lib.BNR_BACKEND_ERROR),
