@@ -2914,9 +2914,9 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
                     kv->page_size % 16 == 0 &&
                     aligned16(q) && aligned16(out) && aligned16(kv->k) && aligned16(kv->v) &&
                     aligned16(a.pool.k_scales) && aligned16(a.pool.v_scales);
-  size_t tile = fast ? kPagedTile : kPagedGenericTile;
   const size_t items = batch * (fast ? kv->n_kv_heads : n_heads);
   const size_t rows = table_stride * kv->page_size;
+  size_t tile = fast ? paged_tile(kv->format, rows, items) : kPagedGenericTile;
   // units that the table has room for: under 2^31, and no fewer than workgroups
   while ((rows + tile - 1) / tile * items >= kPagedMaxCount) tile *= 2;
   a.tile = (int)tile;

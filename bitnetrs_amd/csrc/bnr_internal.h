@@ -751,6 +751,15 @@ constexpr int kPagedGenericTile = 64;
 // of 16 up to 256, at most 16 query heads a kv head, pages of a multiple of 16
 // rows.
 hipError_t launch_paged_decode(const PagedDecodeArgs &a, int format, hipStream_t s);
-constexpr int kPagedTile = 128;
+// Rows of a unit there, for a table with room for `rows` rows of each of
+// `items` (sequence, kv head) pairs: 128, 32 for each wave.  f32 rows take
+// twice the loads of bf16 ones and their products four times as long, so that
+// two waves a workgroup on twice the workgroups are faster while no workgroup
+// gets two units.  One token over 512 f32 rows of 5 kv heads 10.0 -> 8.7 us, 4
+// over 500 10.4 -> 9.1; but 66 bf16 rows 5.6 -> 7.0 (a piece to join), 4096
+// bf16 rows 8.7 -> 12.0 (64 pieces), 9000 f32 rows 20.5 -> 22.5 (two units).
+constexpr size_t paged_tile(int format, size_t rows, size_t items) {
+  return format == kPagedF32 && rows > 128 && (rows + 63) / 64 * items <= (size_t)kPagedMaxWgs ? 64 : 128;
+}
 
 }  // namespace bnr
