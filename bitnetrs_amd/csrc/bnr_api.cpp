@@ -2920,7 +2920,9 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
   // units that the table has room for: under 2^31, and no fewer than workgroups
   while ((rows + tile - 1) / tile * items >= kPagedMaxCount) tile *= 2;
   a.tile = (int)tile;
-  a.wgs = (int)std::min<size_t>(kPagedMaxWgs, (rows + tile - 1) / tile * items);
+  const size_t room = (rows + tile - 1) / tile;  // units of an item
+  a.wgs = (int)std::min<size_t>(kPagedMaxWgs, room * items);
+  a.join = fast ? paged_join(kv->format, (int)group, (int)kv->head_dim, room) : 0.f;
   a.part_floats = paged_part_floats(fast ? (int)group : 1, (int)kv->head_dim);
   DeviceGuard dg(c->device);
   HIP_TRY(fast ? launch_paged_decode(a, kv->format, (hipStream_t)stream)

@@ -92,9 +92,13 @@ __device__ __forceinline__ unsigned lane_of(unsigned v, int lane) {
   return (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
 
+//
+// With `join`, no share is smaller than joining asks for: an item of n units on
+// workgroups of u each costs u steps and the joining of n / u pieces, least at
+// u = sqrt(n * join), join being the cost of a piece in steps.
 template <class Rows>
 __device__ __forceinline__ PagedShare paged_share(Rows rows, int batch, int items, unsigned tile,
-                                                  unsigned wgs) {
+                                                  unsigned wgs, float join) {
   const int lane = threadIdx.x & 63;
   // Rows, and units of an item, of each sequence, 64 sequences at a time.
   auto length = [&](int b) { return b < batch ? rows(b) : 0; };
@@ -102,16 +106,20 @@ __device__ __forceinline__ PagedShare paged_share(Rows rows, int batch, int item
   const int first_len = length(lane);
   const unsigned first = wave_scan(units(first_len));
   unsigned total = lane_of(first, 63);
-  for (int b0 = 64; b0 < batch; b0 += 64) total += lane_of(wave_scan(units(length(b0 + lane))), 63);
+  int longest = first_len;
+  for (int b0 = 64; b0 < batch; b0 += 64) {
+    const int len = length(b0 + lane);
+    longest = max(longest, len);
+    total += lane_of(wave_scan(units(len)), 63);
+  }
   total *= (unsigned)items;
+  if (join > 0.f) {
+    const float n = wave_max((float)longest) / (float)tile;
+    const unsigned least = (unsigned)(__builtin_amdgcn_sqrtf(n * join) + 0.5f);
+    if (least > 1 && total < least * wgs) wgs = (total + least - 1) / least;
+  }
   PagedShare s;
-  s.wg = blockIdx.x;
-  s.per = total / wgs;
-  s.rest = total - s.per * wgs;
-  s.items = items;
-  s.tile = (int)tile;
-  s.at = s.wg * s.per + (s.wg < s.rest ? s.wg : s.rest);
-  s.end = s.at + s.per + (s.wg < s.rest ? 1 : 0);
+  s.take(total, blockIdx.x, wgs, batch, items, tile);
   if (s.at >= s.end) return s;
   // The sequence that has unit `at`, and the item of it.
   const unsigned want = s.at / (unsigned)items;
@@ -133,6 +141,10 @@ __device__ __forceinline__ PagedShare paged_share(Rows rows, int batch, int item
       break;
     }
     before += sum;
+    if (b0 + 64 >= batch) {  // not reached: `at` is less than the sum of all units
+      s.end = s.at;
+      return s;
+    }
   }
   s.h = (int)((s.at - before * (unsigned)items) / s.n);
   s.item0 = before * (unsigned)items + (unsigned)s.h * s.n;

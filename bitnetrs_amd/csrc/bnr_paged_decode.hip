@@ -170,7 +170,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
   const unsigned v_off = 4 * g * row_bytes + row * (U * B);
   const int first_len = paged_first_len(a);
   const auto rows = [&](int b) { return paged_len(a.lens[b], a.pool); };
-  PagedShare sh = paged_share(rows, a.batch, a.pool.n_kv, a.tile, a.wgs);
+  PagedShare sh = paged_share(rows, a.batch, a.pool.n_kv, a.tile, a.wgs, a.join);
 
   for (PagedPiece p; sh.next(rows, p);) {
     const int row1 = __builtin_amdgcn_readfirstlane(p.row1);
@@ -452,8 +452,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
 #pragma unroll
       for (int k = 0; k < 4; ++k) to[k] = v[k];
     };
-    // (16 in flight would spill the f32 form: its steps hold twice the rows' dwords)
-    paged_finish<kW, 4, DP, F == kPagedF32 ? 8 : 16>(a, p, sh.wg, w0, w1, get, s_m, s_l, G, s_join);
+    paged_finish<kW, 4, DP, paged_in_flight(F)>(a, p, sh.wg, w0, w1, get, s_m, s_l, G, s_join);
   }
   paged_empty(a, first_len);
 }
@@ -461,7 +460,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
 template <int F>
 hipError_t launch_format(const PagedDecodeArgs &a, hipStream_t s) {
   const int d = a.pool.d;
-  const int dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  const int dp = paged_dim(d);
   const size_t lds = (size_t)kW * (dp / 16) * (4 * a.group + 1) * sizeof(f32x4);
   const dim3 grid((unsigned)a.wgs), block(64 * kW);
   // what a workgroup gets unasked is 64 KB, of which up to 32 are static

@@ -99,9 +99,22 @@ struct PagedShare {
   unsigned at, end;     // units left to this workgroup
   unsigned item0;       // first unit of the item at `at`
   unsigned per, rest, wg;
-  int b, h, items, tile, len;
+  int b, h, items, tile, len, batch;
   unsigned n;           // units of an item of sequence b
 
+  // The part of `total` units that workgroup `id` has where `used` of the
+  // launch's workgroups share them; none for the others.
+  __host__ __device__ void take(unsigned total, unsigned id, unsigned used, int batch_, int items_,
+                                unsigned tile_) {
+    wg = id;
+    batch = batch_;
+    per = total / used;
+    rest = total - per * used;
+    items = items_;
+    tile = (int)tile_;
+    at = id < used ? id * per + (id < rest ? id : rest) : total;
+    end = id < used ? at + per + (id < rest ? 1 : 0) : total;
+  }
   // The workgroup that has unit t.
   __host__ __device__ unsigned wg_of(unsigned t) const {
     const unsigned big = rest * (per + 1);
@@ -116,7 +129,8 @@ struct PagedShare {
       if (++h == items) {
         h = 0;
         do {
-          len = rows(++b);
+          if (++b >= batch) return false;  // not reached: `end` lies in the last sequence with a row
+          len = rows(b);
         } while (len == 0);
         n = (unsigned)(len + tile - 1) / (unsigned)tile;
       }

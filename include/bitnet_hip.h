@@ -409,6 +409,7 @@ int bnr_kv_dev_prefill(bnr_ctx *ctx, bnr_kv_cache *cache, size_t layer, float *q
  *   - a page outside 0..n_pages-1 is not there: what would be written to it
  *     is dropped, it reads back as zeros, attention leaves its rows out;
  *   - a length below 0 counts as 0, one past table_stride*page_size as that.
+ * These arrays may not change while a call that reads them runs.
  * The pool is the caller's memory; these calls allocate nothing and keep
  * nothing, so calls on different workspaces may run side by side.
  *

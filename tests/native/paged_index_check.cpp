@@ -29,13 +29,8 @@ static PagedShare share_of(Rows rows, int batch, int items, unsigned tile, unsig
   unsigned total = 0;
   for (int b = 0; b < batch; ++b) total += ((unsigned)rows(b) + tile - 1) / tile * (unsigned)items;
   PagedShare s{};
-  s.wg = wg;
-  s.per = total / wgs;
-  s.rest = total - s.per * wgs;
-  s.items = items;
-  s.tile = (int)tile;
-  s.at = wg * s.per + std::min(wg, s.rest);
-  s.end = s.at + s.per + (wg < s.rest ? 1 : 0);
+  s.take(total, wg, wgs, batch, items, tile);
+  CHECK(s.at <= s.end && s.end <= total);
   if (s.at >= s.end) return s;
   unsigned before = 0;
   for (int b = 0;; ++b) {
@@ -68,9 +63,11 @@ static long long shares(std::mt19937 &rng) {
     unsigned line = 0;              // units given out so far
     std::set<unsigned> first;       // first workgroups of shared items
     std::vector<std::vector<long long>> next((size_t)batch, std::vector<long long>((size_t)items, 0));
-    for (unsigned wg = 0; wg < wgs; ++wg) {
+    // workgroups past the `wgs` that share the line have nothing
+    for (unsigned wg = 0; wg < wgs + 20; ++wg) {
       PagedShare s = share_of(rows, batch, items, tile, wg, wgs);
       CHECK(s.at == line);
+      CHECK(wg < wgs || s.at == s.end);
       const unsigned end = s.end;
       unsigned unfinished = 0;
       for (PagedPiece p; s.next(rows, p); ++pieces) {
