@@ -571,6 +571,80 @@ def test_two_streams_with_their_own_workspaces(backend):
         assert all(torch.equal(o, ref[j]) for o in outs[j])
 
 
+def test_two_graphs(backend):
+    """Two captured calls, replayed in turn on one workspace, and side by side on
+    two streams with a workspace each; eager work between the replays."""
+    pools = [Pool(rng_of("graphs", i), f, lens, 5, 128, 16, spread=0.3)
+             for i, (f, lens) in enumerate((("fp8", [5000, 700]), ("f32", [3000])))]
+    kvs = [p.device() for p in pools]
+    tabs, lens = [i32(p.table) for p in pools], [i32(p.lens) for p in pools]
+    qs = [torch.randn(len(p.lens), 20, 128, device="cuda") for p in pools]
+    refs, outs = ([torch.zeros_like(q) for q in qs] for _ in range(2))
+    for shared in (True, False):
+        ws = [backend.paged_workspace(kv, 2, 20) for kv in kvs]
+        if shared:
+            ws = [max(ws, key=len)] * 2
+        graphs = []
+        for i in range(2):
+            backend.dev_paged_decode_attention(kvs[i], qs[i], tabs[i], lens[i], refs[i], ws[i])
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                backend.dev_paged_decode_attention(kvs[i], qs[i], tabs[i], lens[i], outs[i], ws[i])
+            graphs.append(g)
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for _ in range(4):
+            for o in outs:
+                o.fill_(float("nan"))
+            torch.cuda.synchronize()
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(streams[0] if shared else s):
+                    g.replay()
+            torch.cuda.synchronize()
+            for i in range(2):
+                assert torch.equal(outs[i], refs[i]), (shared, i)
+            check_decode(backend, pools[1], 20, kv=kvs[1], workspace=ws[1])
+        del graphs
+
+
+def test_two_threads(backend):
+    """Calls of two host threads at once, each on its own stream and workspace."""
+    import threading
+
+    pools = [Pool(rng_of("threads", i), f, [4000, 900, 30], 5, 128, 16, spread=0.3)
+             for i, f in enumerate(("bf16", "int8"))]
+    kvs = [p.device() for p in pools]
+    tabs, lens = [i32(p.table) for p in pools], i32([4000, 900, 30])
+    q = torch.randn(3, 20, 128, device="cuda")
+    ws = [backend.paged_workspace(kv, 3, 20) for kv in kvs]
+    outs = [[torch.zeros_like(q) for _ in range(20)] for _ in pools]
+    streams = [torch.cuda.Stream() for _ in pools]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(i):
+        try:
+            for o in outs[i]:
+                backend.dev_paged_decode_attention(kvs[i], q, tabs[i], lens, o, ws[i], stream=streams[i])
+            with pytest.raises(TypeError):  # an error of this thread's own
+                backend.dev_paged_decode_attention(kvs[i], q.cpu(), tabs[i], lens, o, ws[i])
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for i in range(2):
+        ref = torch.zeros_like(q)
+        backend.dev_paged_decode_attention(kvs[i], q, tabs[i], lens, ref, ws[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, ref) for o in outs[i])
+
+
 def test_python_refusals(backend):
     """Wrong shapes, types, layouts and devices are refused before the library."""
     from bitnetrs_amd import InvalidShape, PagedKV
