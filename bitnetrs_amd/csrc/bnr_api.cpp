@@ -2752,13 +2752,13 @@ int check_paged_count(size_t n, const char *what) {
   return BNR_OK;
 }
 
-// Workspace: a ticket for each workgroup, at the same place whatever the call's
-// shape (they must be zero for the next one), then the pieces.
-constexpr size_t kPagedTicketBytes = (size_t)kPagedMaxWgs * kCounterStride * sizeof(unsigned);
+// Workspace: the tickets, at the same place whatever the call's shape (they
+// must be zero for the next one), then the pieces and the groups of them.
+constexpr size_t kPagedTicketBytes = (size_t)kPagedTickets * kCounterStride * sizeof(unsigned);
 
 size_t paged_workspace_bytes(size_t group, size_t head_dim) {
   return kPagedTicketBytes +
-         (size_t)2 * kPagedMaxWgs * paged_part_floats((int)group, (int)head_dim) * sizeof(float);
+         (size_t)4 * kPagedMaxWgs * paged_part_floats((int)group, (int)head_dim) * sizeof(float);
 }
 
 int check_paged_heads(const bnr_paged_kv *kv, size_t batch, size_t n_heads) {
@@ -2916,13 +2916,12 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
                     aligned16(a.pool.k_scales) && aligned16(a.pool.v_scales);
   const size_t items = batch * (fast ? kv->n_kv_heads : n_heads);
   const size_t rows = table_stride * kv->page_size;
-  size_t tile = fast ? paged_tile(kv->format, rows, items) : kPagedGenericTile;
+  const size_t most = fast ? kPagedMaxWgs / 2 * paged_waves(kv->format, (int)kv->head_dim) : kPagedMaxWgs;
+  size_t tile = fast ? paged_tile(kv->format, rows, items, most) : kPagedGenericTile;
   // units that the table has room for: under 2^31, and no fewer than workgroups
   while ((rows + tile - 1) / tile * items >= kPagedMaxCount) tile *= 2;
   a.tile = (int)tile;
-  const size_t room = (rows + tile - 1) / tile;  // units of an item
-  a.wgs = (int)std::min<size_t>(kPagedMaxWgs, room * items);
-  a.join = fast ? paged_join(kv->format, (int)group, (int)kv->head_dim, room) : 0.f;
+  a.wgs = (int)std::min<size_t>(most, (rows + tile - 1) / tile * items);
   a.part_floats = paged_part_floats(fast ? (int)group : 1, (int)kv->head_dim);
   DeviceGuard dg(c->device);
   HIP_TRY(fast ? launch_paged_decode(a, kv->format, (hipStream_t)stream)

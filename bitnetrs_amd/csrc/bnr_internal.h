@@ -733,11 +733,10 @@ struct PagedDecodeArgs {
   const float *q;   // [batch][n_heads][d]
   float *out;       // [batch][n_heads][d]
   const int *lens;  // [batch]
-  float *parts;     // [2 * wgs][part_floats]: unfinished pieces of the line
-  unsigned *tickets;  // [kPagedMaxWgs] x kCounterStride, zero between launches
+  float *parts;     // [2][2 * kPagedMaxWgs][part_floats]: unfinished pieces of the line; groups of them
+  unsigned *tickets;  // [kPagedTickets] x kCounterStride, zero between launches
   int batch, n_heads, group;
   int wgs, part_floats, tile;
-  float join;  // least shares (paged_share), or 0
   float scale_log2;  // log2(e) / sqrt(d)
 };
 // Floats of a piece of `heads` query heads: outputs, then (max, sum) of each.
@@ -746,6 +745,18 @@ constexpr int paged_part_floats(int heads, int d) { return (heads * (d + 2) + 3)
 // most forms allow, changed 64 int8 sequences of up to 32768 rows by less than
 // 1 % and cost one of 131072 e4m3 rows 8 % (each adds a piece to join).
 constexpr int kPagedMaxWgs = 512;
+constexpr int paged_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+// Waves of a SIMD by the registers that a form takes, and so workgroups of a
+// launch: wide rows of 16 or 32 bits leave room for one.  One token over 45908
+// bf16 rows of 14/2 heads of 256: 40.8 us with 512 workgroups, in two rounds.
+constexpr int paged_waves(int format, int d) {
+  return paged_dim(d) == 256 && (format == kPagedF32 || format == kPagedBf16) ? 1 : 2;
+}
+// Pieces that a thread of a join has in flight (16 would spill the f32 form,
+// whose steps hold twice the dwords).
+constexpr int paged_in_flight(int format) { return format == kPagedF32 ? 8 : 16; }
+// A ticket for each workgroup's item, and for each slot of a piece.
+constexpr int kPagedTickets = 3 * kPagedMaxWgs;
 hipError_t launch_paged_decode_generic(const PagedDecodeArgs &a, int format, hipStream_t s);
 constexpr int kPagedGenericTile = 64;
 // On the matrix cores: 16-byte aligned pools, q and out, head_dim a multiple
@@ -753,28 +764,14 @@ constexpr int kPagedGenericTile = 64;
 // rows.
 hipError_t launch_paged_decode(const PagedDecodeArgs &a, int format, hipStream_t s);
 // Rows of a unit there, for a table with room for `rows` rows of each of
-// `items` (sequence, kv head) pairs: 128, 32 for each wave.  f32 rows take
+// `items` (sequence, kv head) pairs on `wgs` workgroups: 128, 32 for each wave.  f32 rows take
 // twice the loads of bf16 ones and their products four times as long, so that
 // two waves a workgroup on twice the workgroups are faster while no workgroup
 // gets two units.  One token over 512 f32 rows of 5 kv heads 10.0 -> 8.7 us, 4
 // over 500 10.4 -> 9.1; but 66 bf16 rows 5.6 -> 7.0 (a piece to join), 4096
 // bf16 rows 8.7 -> 12.0 (64 pieces), 9000 f32 rows 20.5 -> 22.5 (two units).
-constexpr int paged_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-// Pieces that a thread of a join has in flight (16 would spill the f32 form,
-// whose steps hold twice the dwords), and the cost of a piece in steps: a round
-// of them takes 0.8 of a step's time, and `ways` threads share an output.  One
-// token over 30000 bf16 rows of one kv head with 16 query heads 45.6 -> 24.2
-// us, two sequences of 6876 and 17410 f32 rows of 14/2 heads 30.6 -> 25.8; 1 %
-// more where nothing changes (4096 bf16 rows of 5 kv heads 8.71 -> 8.83).  No
-// least shares where the table has no room for sequences that need them.
-constexpr int paged_in_flight(int format) { return format == kPagedF32 ? 8 : 16; }
-inline float paged_join(int format, int group, int d, size_t room) {
-  const int outputs = group * paged_dim(d) / 4, ways = outputs < 256 ? 256 / outputs : 1;
-  const float cost = 0.8f / (float)(paged_in_flight(format) * ways);
-  return (float)room * cost < 1.5f * 1.5f ? 0.f : cost;
-}
-constexpr size_t paged_tile(int format, size_t rows, size_t items) {
-  return format == kPagedF32 && rows > 128 && (rows + 63) / 64 * items <= (size_t)kPagedMaxWgs ? 64 : 128;
+constexpr size_t paged_tile(int format, size_t rows, size_t items, size_t wgs) {
+  return format == kPagedF32 && rows > 128 && (rows + 63) / 64 * items <= wgs ? 64 : 128;
 }
 
 }  // namespace bnr

@@ -92,13 +92,9 @@ __device__ __forceinline__ unsigned lane_of(unsigned v, int lane) {
   return (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
 
-//
-// With `join`, no share is smaller than joining asks for: an item of n units on
-// workgroups of u each costs u steps and the joining of n / u pieces, least at
-// u = sqrt(n * join), join being the cost of a piece in steps.
 template <class Rows>
 __device__ __forceinline__ PagedShare paged_share(Rows rows, int batch, int items, unsigned tile,
-                                                  unsigned wgs, float join) {
+                                                  unsigned wgs) {
   const int lane = threadIdx.x & 63;
   // Rows, and units of an item, of each sequence, 64 sequences at a time.
   auto length = [&](int b) { return b < batch ? rows(b) : 0; };
@@ -106,18 +102,8 @@ __device__ __forceinline__ PagedShare paged_share(Rows rows, int batch, int item
   const int first_len = length(lane);
   const unsigned first = wave_scan(units(first_len));
   unsigned total = lane_of(first, 63);
-  int longest = first_len;
-  for (int b0 = 64; b0 < batch; b0 += 64) {
-    const int len = length(b0 + lane);
-    longest = max(longest, len);
-    total += lane_of(wave_scan(units(len)), 63);
-  }
+  for (int b0 = 64; b0 < batch; b0 += 64) total += lane_of(wave_scan(units(length(b0 + lane))), 63);
   total *= (unsigned)items;
-  if (join > 0.f) {
-    const float n = wave_max((float)longest) / (float)tile;
-    const unsigned least = (unsigned)(__builtin_amdgcn_sqrtf(n * join) + 0.5f);
-    if (least > 1 && total < least * wgs) wgs = (total + least - 1) / least;
-  }
   PagedShare s;
   s.take(total, blockIdx.x, wgs, batch, items, tile);
   if (s.at >= s.end) return s;
@@ -171,9 +157,9 @@ __device__ __forceinline__ void paged_empty(const PagedDecodeArgs &a, int first_
 // d unnormalised outputs (get(w, g, x, o): V of them from x on).  A piece that is a whole
 // item is normalised and written.  Otherwise it goes to the launch's
 // workspace; the last workgroup to bring a piece of the item joins all of
-// them, in the line's order, so the same inputs give the same bits.  An item's
-// ticket is its first workgroup's: of the items that a workgroup starts, only
-// the last can go on in the next, so a workgroup needs one.
+// them, in the line's order, so the same inputs give the same bits.  Many
+// pieces are joined in groups first (JoinStep): the groups by several
+// workgroups at a time, then their states by one.
 //
 // What a join costs is latency: a store, a ticket and a load, each to the
 // device's coherence point and back.  So the loads of N pieces are all in
@@ -267,78 +253,93 @@ __device__ __forceinline__ void paged_finish(const PagedDecodeArgs &a, const Pag
     }
   }
   if (whole) return;
-  // every store of the workgroup is at the device's coherence point before its ticket
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  unsigned *ticket = a.tickets + w0 * kCounterStride;
-  const int n = (int)(w1 - w0) + 1;
-  if (tid == 0)
-    js.last = (int)__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
-  __syncthreads();
-  if (!js.last) return;
-  if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // Piece i of the item is in slot 2 (w0 + i), the first in slot 2 w0 + 1.
   // `ways` threads share the pieces of one output; thread k of them takes
   // pieces k, k + ways, ...
   const int ways = work >= nt ? 1 : nt / work;
-  for (int e0 = 0; e0 < work; e0 += nt) {
-    const int way = work >= nt ? 0 : tid / work, e = work >= nt ? e0 + tid : tid - way * work;
-    const int g = e / per, x = e % per * V;
-    const bool in = way < ways && e < work && x < d;
-    JoinState<V> s;
-    s.clear();
-    const auto take = [&](auto at_once) {
-      constexpr int M = decltype(at_once)::value;
-      for (int i0 = way; in && i0 < n; i0 += M * ways) {
-        float m[M], l[M], po[M][V];
+  const int region = 2 * kPagedMaxWgs * stride;  // bytes of all pieces; the groups' states lie behind them
+  JoinStep c = join_start(w0, w1, wg, N * ways, (work + nt - 1) / nt);
+  for (int from = 0;; from = region) {
+    // every store of the workgroup is at the device's coherence point before its ticket
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    unsigned *ticket = a.tickets + c.ticket(w0) * kCounterStride;
+    if (tid == 0)
+      js.last = (int)__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == c.count - 1;
+    __syncthreads();
+    if (!js.last) return;
+    if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int e0 = 0; e0 < work; e0 += nt) {
+      const int way = work >= nt ? 0 : tid / work, e = work >= nt ? e0 + tid : tid - way * work;
+      const int g = e / per, x = e % per * V;
+      const bool in = way < ways && e < work && x < d;
+      JoinState<V> s;
+      s.clear();
+      const auto take = [&](auto at_once) {
+        constexpr int M = decltype(at_once)::value;
+        for (int i0 = way; in && i0 < c.count; i0 += M * ways) {
+          float m[M], l[M], po[M][V];
 #pragma unroll
-        for (int k = 0; k < M; ++k) {
-          // past the last piece: the last again, without a weight (a branch would part the loads)
-          const int i = i0 + k * ways < n ? i0 + k * ways : n - 1;
-          const int at = (int)(2 * (w0 + (unsigned)i) + (i == 0 ? 1 : 0)) * stride;
-          const float2 ml = ld2_agent(parts, at + (heads * d + 2 * g) * 4);
-          m[k] = ml.x;
-          l[k] = ml.y;
-          if constexpr (V == 4) {
-            const float4 v = ld4_agent(parts, at + (g * d + x) * 4);
-            po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
-          } else {
-            po[k][0] = ld_agent(a.parts + at / 4 + g * d + x);
+          for (int k = 0; k < M; ++k) {
+            // past the last piece: the last again, without a weight (a branch would part the loads)
+            const int i = i0 + k * ways < c.count ? i0 + k * ways : c.count - 1;
+            const int at = c.slot(i, w0) * stride + from;
+            const float2 ml = ld2_agent(parts, at + (heads * d + 2 * g) * 4);
+            m[k] = ml.x;
+            l[k] = ml.y;
+            if constexpr (V == 4) {
+              const float4 v = ld4_agent(parts, at + (g * d + x) * 4);
+              po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
+            } else {
+              po[k][0] = ld_agent(a.parts + at / 4 + g * d + x);
+            }
           }
-        }
 #pragma unroll
-        for (int k = 0; k < M; ++k) {
-          const bool there = i0 + k * ways < n;
-          m[k] = there ? m[k] : -INFINITY;
-          l[k] = there ? l[k] : 0.f;
+          for (int k = 0; k < M; ++k) {
+            const bool there = i0 + k * ways < c.count;
+            m[k] = there ? m[k] : -INFINITY;
+            l[k] = there ? l[k] : 0.f;
 #pragma unroll
-          for (int j = 0; j < V; ++j) po[k][j] = there ? po[k][j] : 0.f;
-        }
-        s.add(m, l, po);
-      }
-    };
-    // few pieces: no loads for the places of more (8 sequences of 100 to 900 int8 rows 8.7 -> 7.9 us)
-    if (n <= 4 * ways)
-      take(std::integral_constant<int, 4>{});
-    else
-      take(std::integral_constant<int, N>{});
-    if (ways > 1) {  // work < nt: one round
-      js.m[tid] = s.m;
-      js.l[tid] = s.l;
-#pragma unroll
-      for (int i = 0; i < V; ++i) js.o[tid][i] = s.o[i];
-      __syncthreads();
-      if (way == 0)
-        for (int k = 1; k < ways; ++k) {
-          const int at = tid + k * work;
-          const float m[1] = {js.m[at]}, l[1] = {js.l[at]};
-          float po[1][V];
-#pragma unroll
-          for (int i = 0; i < V; ++i) po[0][i] = js.o[at][i];
+            for (int j = 0; j < V; ++j) po[k][j] = there ? po[k][j] : 0.f;
+          }
           s.add(m, l, po);
         }
+      };
+      // few pieces: no loads for the places of more (8 sequences of 100 to 900 int8 rows 8.7 -> 7.9 us)
+      if (c.count <= 4 * ways)
+        take(std::integral_constant<int, 4>{});
+      else
+        take(std::integral_constant<int, N>{});
+      if (ways > 1) {  // work < nt: one round
+        js.m[tid] = s.m;
+        js.l[tid] = s.l;
+#pragma unroll
+        for (int i = 0; i < V; ++i) js.o[tid][i] = s.o[i];
+        __syncthreads();
+        if (way == 0)
+          for (int k = 1; k < ways; ++k) {
+            const int at = tid + k * work;
+            const float m[1] = {js.m[at]}, l[1] = {js.l[at]};
+            float po[1][V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) po[0][i] = js.o[at][i];
+            s.add(m, l, po);
+          }
+      }
+      if (way == 0 && in) {
+        if (c.last) {
+          s.write(out + g * d + x);
+        } else {
+          const int to = c.slot(0, w0) * stride + region;
+          if constexpr (V == 4)
+            st4_agent(parts, to + (g * d + x) * 4, make_float4(s.o[0], s.o[1], s.o[2], s.o[3]));
+          else
+            st_agent(a.parts + to / 4 + g * d + x, s.o[0]);
+          if (x == 0) st2_agent(parts, to + (heads * d + 2 * g) * 4, s.m, s.l);
+        }
+      }
     }
-    if (way == 0 && in) s.write(out + g * d + x);
+    if (c.last) return;
+    c = join_groups(w0, w1);
   }
 }
 

@@ -232,7 +232,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_read_vec_kernel(PagedReadAr
     if (start < 0 || start >= len) return 0;
     return len - start < a.cap ? len - start : (int)a.cap;
   };
-  PagedShare sh = paged_share(rows, (int)a.batch, a.pool.n_kv, a.tile, a.wgs, 0.f);
+  PagedShare sh = paged_share(rows, (int)a.batch, a.pool.n_kv, a.tile, a.wgs);
   for (PagedPiece p; sh.next(rows, p);) {
     const int start = a.starts ? a.starts[p.b] : 0;
     const long long to = ((long long)p.b * a.pool.n_kv + p.h) * a.cap;
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = a.pool.d;
   const int first_len = paged_first_len(a);
   const auto rows = [&](int b) { return paged_len(a.lens[b], a.pool); };
-  PagedShare sh = paged_share(rows, a.batch, a.n_heads, a.tile, a.wgs, 0.f);
+  PagedShare sh = paged_share(rows, a.batch, a.n_heads, a.tile, a.wgs);
   for (PagedPiece p; sh.next(rows, p);) {
     const int h = p.h / a.group;
     const float *q = a.q + ((long long)p.b * a.n_heads + p.h) * d;

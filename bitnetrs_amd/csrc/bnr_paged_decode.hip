@@ -54,7 +54,7 @@ constexpr int kBytes = F == kPagedF32 ? 4 : F == kPagedBf16 ? 2 : 1;
 // Waves of a SIMD that the registers are shared out for.  With three the join's
 // loads spill: one token over 4096 bf16 rows took 12.6 us.
 template <int F, int DP>
-constexpr int kWavesOf = DP == 256 && (F == kPagedF32 || F == kPagedBf16) ? 1 : 2;
+constexpr int kWavesOf = paged_waves(F, DP);
 
 // N dwords at p; NT: with the non-temporal hint.  V's loads take whole lines
 // and have it; K's take half of each line, the other half comes with the next
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
   const unsigned v_off = 4 * g * row_bytes + row * (U * B);
   const int first_len = paged_first_len(a);
   const auto rows = [&](int b) { return paged_len(a.lens[b], a.pool); };
-  PagedShare sh = paged_share(rows, a.batch, a.pool.n_kv, a.tile, a.wgs, a.join);
+  PagedShare sh = paged_share(rows, a.batch, a.pool.n_kv, a.tile, a.wgs);
 
   for (PagedPiece p; sh.next(rows, p);) {
     const int row1 = __builtin_amdgcn_readfirstlane(p.row1);

@@ -148,4 +148,46 @@ struct PagedShare {
   }
 };
 
+// ---------------------------------------------------------------------------
+// Joins.  The item on workgroups w0 .. w1 has a piece of each: w0's is its
+// last, in slot 2 w0 + 1, the others' their first, in slot 2 w.  A step of a
+// join takes `count` states from slots 2 (base + j * stride) (one higher for
+// w0's): all pieces at once, or kJoinGroup neighbours, whose joined state goes
+// to the first one's slot of a second array, and then those states.  A slot is
+// one piece's, so a group's ticket may go by its first slot; of the items that
+// a workgroup starts only the last can go on in the next, so an item's may go
+// by w0.
+// ---------------------------------------------------------------------------
+constexpr int kJoinGroup = 16;
+struct JoinStep {
+  unsigned base, stride;
+  int count;
+  bool last;  // the item's outputs come out, not a group's state
+  __host__ __device__ int slot(int j, unsigned w0) const {
+    const unsigned w = base + (unsigned)j * stride;
+    return (int)(2 * w + (w == w0 ? 1 : 0));
+  }
+  __host__ __device__ unsigned ticket(unsigned w0) const {
+    return last ? w0 : (unsigned)kPagedMaxWgs + (unsigned)slot(0, w0);
+  }
+};
+
+// The step of workgroup wg's piece.  A workgroup loads `at_once` states of an
+// output in one go, `rounds` times over for all outputs: past four goes the
+// pieces are grouped.  One token over 30000 bf16 rows of one kv head with 16
+// query heads 45.6 -> 16.6 us, over 85937 f32 rows of one with 12 of 80 57 -> 32;
+// 1 % more where nothing is grouped.
+__host__ __device__ inline JoinStep join_start(unsigned w0, unsigned w1, unsigned wg, int at_once, int rounds) {
+  const int n = (int)(w1 - w0) + 1;
+  if ((n + at_once - 1) / at_once * rounds <= 4 || n <= kJoinGroup) return JoinStep{w0, 1, n, true};
+  const unsigned base = wg - (wg - w0) % kJoinGroup;
+  const int left = (int)(w1 - base) + 1;
+  return JoinStep{base, 1, left < kJoinGroup ? left : kJoinGroup, false};
+}
+
+// The step of the groups' states.
+__host__ __device__ inline JoinStep join_groups(unsigned w0, unsigned w1) {
+  return JoinStep{w0, kJoinGroup, (int)(w1 - w0) / kJoinGroup + 1, true};
+}
+
 }  // namespace bnr

@@ -48,6 +48,31 @@ static PagedShare share_of(Rows rows, int batch, int items, unsigned tile, unsig
   return s;
 }
 
+// The steps that join an item's pieces: each piece is taken once, in order, by
+// the group that all its workgroups take it to be in; each group's state once.
+static void joins(unsigned w0, unsigned w1, int at_once, int turns, std::set<unsigned> &group_ticket) {
+  const auto piece = [&](unsigned w) { return (int)(2 * w + (w == w0 ? 1 : 0)); };
+  std::vector<int> groups;  // slots of their states
+  unsigned next = w0;
+  for (unsigned w = w0; w <= w1; ++w) {
+    const JoinStep c = join_start(w0, w1, w, at_once, turns);
+    CHECK(c.count >= 1 && c.base <= w && w < c.base + (unsigned)c.count && c.base + (unsigned)c.count <= w1 + 1);
+    CHECK(c.last ? c.base == w0 && c.count == (int)(w1 - w0) + 1 && c.ticket(w0) == w0
+                 : c.count <= kJoinGroup);
+    if (w != next) continue;  // the same group as the piece before
+    for (int j = 0; j < c.count; ++j) CHECK(c.slot(j, w0) == piece(w + (unsigned)j));
+    next = w + (unsigned)c.count;
+    if (c.last) return;
+    CHECK(c.ticket(w0) >= (unsigned)kPagedMaxWgs && c.ticket(w0) < (unsigned)kPagedTickets);
+    CHECK(group_ticket.insert(c.ticket(w0)).second);
+    groups.push_back(c.slot(0, w0));
+  }
+  CHECK(next == w1 + 1);
+  const JoinStep c = join_groups(w0, w1);
+  CHECK(c.last && c.count == (int)groups.size() && c.ticket(w0) == w0);
+  for (int j = 0; j < c.count; ++j) CHECK(c.slot(j, w0) == groups[(size_t)j]);
+}
+
 static long long shares(std::mt19937 &rng) {
   long long pieces = 0;
   for (int round = 0; round < 400; ++round) {
@@ -62,6 +87,8 @@ static long long shares(std::mt19937 &rng) {
     const unsigned wgs = 1 + rng() % (round % 2 ? 512u : std::max(1u, std::min(512u, room + 5)));
     unsigned line = 0;              // units given out so far
     std::set<unsigned> first;       // first workgroups of shared items
+    std::set<unsigned> group_ticket;  // of groups of pieces
+    const int at_once = 8 << rng() % 4, turns = 1 + (int)(rng() % 3);
     std::vector<std::vector<long long>> next((size_t)batch, std::vector<long long>((size_t)items, 0));
     // workgroups past the `wgs` that share the line have nothing
     for (unsigned wg = 0; wg < wgs + 20; ++wg) {
@@ -89,7 +116,10 @@ static long long shares(std::mt19937 &rng) {
           const unsigned slot = wg == w0 ? 2u : 1u;
           CHECK(!(unfinished & slot));
           unfinished |= slot;
-          if (wg == w0) CHECK(first.insert(w0).second);  // the ticket is this item's alone
+          if (wg == w0) {
+            CHECK(first.insert(w0).second);  // the ticket is this item's alone
+            joins(w0, w1, at_once, turns, group_ticket);
+          }
         }
       }
       CHECK(line == end);

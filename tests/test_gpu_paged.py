@@ -274,6 +274,21 @@ def test_decode_batches(backend, fmt, lens):
     check_decode(backend, pool, 20)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hq,hkv,d,lens", [(12, 1, 80, [30000]), (16, 1, 128, [17, 21000]), (16, 1, 256, [9000]),
+                                           (14, 2, 128, [12000, 3000]), (4, 1, 128, [40000]), (3, 1, 26, [9000])])
+def test_decode_many_pieces(backend, fmt, hq, hkv, d, lens):
+    """Items of many workgroups, joined in groups first, the last one not full;
+    the same bits again on the used workspace."""
+    say(f"decode many pieces {fmt} {hq}/{hkv}/{d} {lens}")
+    pool = Pool(rng_of("many", fmt, hq, d), fmt, lens, hkv, d, 16, spread=0.3)
+    kv = pool.device()
+    ws = backend.paged_workspace(kv, 2, hq)
+    first = check_decode(backend, pool, hq, kv=kv, workspace=ws)
+    assert (ws[:1536 * 256] == 0).all()
+    assert torch.equal(first, check_decode(backend, pool, hq, kv=kv, workspace=ws, times=3))
+
+
 @pytest.mark.parametrize("fmt,page", [("int8", 16), ("bf16", 48), ("f32", 64), ("fp8", 128)])
 def test_decode_long_pieces(backend, fmt, page):
     """Pieces of more than 4096 rows of one workgroup, with pages that are not
@@ -378,7 +393,7 @@ def test_decode_same_bits_and_workspace_left_ready(backend, fmt):
     kv, kv2 = pool.device(), small.device()
     ws = backend.paged_workspace(kv, 4, 20)
     first = check_decode(backend, pool, 20, kv=kv, workspace=ws)
-    assert (ws[:512 * 256] == 0).all()
+    assert (ws[:1536 * 256] == 0).all()
     check_decode(backend, small, 20, kv=kv2, workspace=ws)
     again = check_decode(backend, pool, 20, kv=kv, workspace=ws, times=4)
     assert torch.equal(first, again)
