@@ -748,7 +748,8 @@ constexpr int kPagedMaxWgs = 512;
 constexpr int paged_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // Waves of a SIMD by the registers that a form takes, and so workgroups of a
 // launch: wide rows of 16 or 32 bits leave room for one.  One token over 45908
-// bf16 rows of 14/2 heads of 256: 40.8 us with 512 workgroups, in two rounds.
+// bf16 rows of 14/2 heads of 256: 40.8 us with 512 workgroups, in two rounds,
+// 29.4 with 256.
 constexpr int paged_waves(int format, int d) {
   return paged_dim(d) == 256 && (format == kPagedF32 || format == kPagedBf16) ? 1 : 2;
 }
@@ -764,12 +765,13 @@ constexpr int kPagedGenericTile = 64;
 // rows.
 hipError_t launch_paged_decode(const PagedDecodeArgs &a, int format, hipStream_t s);
 // Rows of a unit there, for a table with room for `rows` rows of each of
-// `items` (sequence, kv head) pairs on `wgs` workgroups: 128, 32 for each wave.  f32 rows take
-// twice the loads of bf16 ones and their products four times as long, so that
-// two waves a workgroup on twice the workgroups are faster while no workgroup
-// gets two units.  One token over 512 f32 rows of 5 kv heads 10.0 -> 8.7 us, 4
+// `items` (sequence, kv head) pairs and at most `wgs` workgroups: 128, 32 for
+// each wave.  f32 rows take twice the loads of bf16 ones and their products four
+// times as long, so that two waves a workgroup on twice the workgroups are faster
+// while no workgroup gets two units.  One token over 512 f32 rows of 5 kv heads 10.0 -> 8.7 us, 4
 // over 500 10.4 -> 9.1; but 66 bf16 rows 5.6 -> 7.0 (a piece to join), 4096
-// bf16 rows 8.7 -> 12.0 (64 pieces), 9000 f32 rows 20.5 -> 22.5 (two units).
+// bf16 rows 8.7 -> 12.0 (64 pieces), 9000 f32 rows 20.5 -> 22.5 (two units);
+// 384 units of 64 rows of 256 on 256 workgroups 26.9, as 192 of 128 24.9.
 constexpr size_t paged_tile(int format, size_t rows, size_t items, size_t wgs) {
   return format == kPagedF32 && rows > 128 && (rows + 63) / 64 * items <= wgs ? 64 : 128;
 }

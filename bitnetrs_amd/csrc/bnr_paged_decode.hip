@@ -30,7 +30,7 @@
 // the loads alone take 97 % of the time of 64 int8 sequences of up to 32768
 // rows (233 us, 6.1 TB/s; a plain read of this card 7.1).  A short call is
 // latency: lengths, table and rows one after the other (3.5 us), a step, then
-// a store, a ticket and a load to join the pieces (3 us); 8.8 us over 4096
+// a store, a ticket and a load to join the pieces (3 us); 9.0 us over 4096
 // bf16 rows, 5.3 where nothing is joined.  Of the vector instructions of an
 // int8 step, 365 of a wave, half turn codes into bf16.
 #include "bnr_paged.h"

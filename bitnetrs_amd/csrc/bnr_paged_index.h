@@ -175,8 +175,10 @@ struct JoinStep {
 // The step of workgroup wg's piece.  A workgroup loads `at_once` states of an
 // output in one go, `rounds` times over for all outputs: past four goes the
 // pieces are grouped.  One token over 30000 bf16 rows of one kv head with 16
-// query heads 45.6 -> 16.6 us, over 85937 f32 rows of one with 12 of 80 57 -> 32;
-// 1 % more where nothing is grouped.
+// query heads: 45.6 us with every piece joined at once, 24.5 with shares kept
+// large so that pieces are few, 16.6 with groups; over 85937 f32 rows of one
+// with 12 of 80: 57.5 with large shares, 32.0 with groups.  Up to 2 % more where
+// nothing is grouped (15 int8 sequences 44.2 -> 45.1, 4096 bf16 rows 8.9 -> 9.0).
 __host__ __device__ inline JoinStep join_start(unsigned w0, unsigned w1, unsigned wg, int at_once, int rounds) {
   const int n = (int)(w1 - w0) + 1;
   if ((n + at_once - 1) / at_once * rounds <= 4 || n <= kJoinGroup) return JoinStep{w0, 1, n, true};
