@@ -88,10 +88,17 @@ __device__ __forceinline__ unsigned pack_hi(float a, float b) {
 }
 
 // Three bf16 parts of 8 floats: truncation leaves 8 bits a part, so the parts
-// sum to the value exactly.
+// sum to the value.  (Where the value is a product, the compiler may take the
+// first rest from it unrounded: a rest of the other sign is less than half of
+// the value's last place then.)  kFill: of a value of 2^-100 or more, a part with
+// no bits left or of the other sign is 2^-126 of the value's sign, at most
+// 2^-26 of the value and less than a sum's own rounding: an infinity of the
+// other operand meets no zero and no two signs, and the product is the infinity
+// that the value itself would give, not NaN.
 struct Parts {
   u32x4 p[3];
 };
+template <bool kFill>
 __device__ __forceinline__ Parts split8(const float (&x)[8]) {
   Parts s;
   float r[8];
@@ -105,6 +112,10 @@ __device__ __forceinline__ Parts split8(const float (&x)[8]) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         r[i] -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, r[i]) & 0xffff0000u);
+    if (kFill && k < 2)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(x[i] < 0.f ? r[i] < 0.f : r[i] > 0.f) && fabsf(x[i]) >= 0x1p-100f) r[i] = copysignf(0x1p-126f, x[i]);
   }
   return s;
 }
@@ -282,7 +293,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
       } else {
         const float4 lo = scale4(a.scale_log2, qx[i][0]), hi = scale4(a.scale_log2, qx[i][1]);
         const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        const Parts s = split8(x);
+        const Parts s = split8<F == kPagedBf16>(x);  // 8-bit rows hold no infinity
 #pragma unroll
         for (int k = 0; k < 3; ++k) s_q[(c * 3 + k) * 64 + lane] = s.p[k];
       }
@@ -391,7 +402,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
               o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[h][r][i]),
                                                           w[4 * h + r], o[i], 0, 0, 0);
       } else {
-        const Parts wp = split8(w);
+        const Parts wp = split8<false>(w);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           u32x4 c;  // dim i of the lane's 8 rows

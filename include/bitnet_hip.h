@@ -484,8 +484,12 @@ int bnr_paged_decode_workspace(bnr_ctx *ctx, const bnr_paged_kv *kv, size_t batc
 /* Attention of one new token of each sequence over rows 0..lens[s]-1 of its
  * own (which hold the new token's k and v already; q rotated): out[s][h] =
  * softmax(q_h . K[h/G] / sqrt(d)) V[h/G], q and out [batch x n_heads x d].  A
- * sequence without a row gives zeros.  A row with a non-finite value makes
- * the outputs that weigh it non-finite.  `workspace` (device memory,
+ * sequence without a row gives zeros.  Values that are not finite: one in V, in
+ * a row that is attended to, makes its column of the outputs non-finite; one in K
+ * makes the scores that its products with q make.  A NaN or +infinity as a
+ * score makes the outputs NaN; a row whose score is -infinity has no weight, and
+ * a query head with no other row gives zeros.  (An element of q below 2^-90 may
+ * count as zero beside an infinity, a NaN.)  `workspace` (device memory,
  * 16-byte aligned) must be zero-filled before its first use; each call leaves
  * it ready for the next.  Calls that share a workspace must be ordered, as on
  * one stream.  The same inputs give the same bits on every run. */
