@@ -90,11 +90,10 @@ __device__ __forceinline__ unsigned pack_hi(float a, float b) {
 // Three bf16 parts of 8 floats: truncation leaves 8 bits a part, so the parts
 // sum to the value.  (Where the value is a product, the compiler may take the
 // first rest from it unrounded: a rest of the other sign is less than half of
-// the value's last place then.)  kFill: of a value of 2^-100 or more, a part with
-// no bits left or of the other sign is 2^-126 of the value's sign, at most
-// 2^-26 of the value and less than a sum's own rounding: an infinity of the
-// other operand meets no zero and no two signs, and the product is the infinity
-// that the value itself would give, not NaN.
+// the value's last place then.)  kFill: no part is zero or of the other sign,
+// down to values of 2^-90: a rest is 2^-40 of the value at least, which no sum
+// notices.  An infinity of the other operand then makes the infinity in each
+// part's product that it makes with the value, where a zero would make NaN.
 struct Parts {
   u32x4 p[3];
 };
@@ -103,19 +102,20 @@ __device__ __forceinline__ Parts split8(const float (&x)[8]) {
   Parts s;
   float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = x[i];
+  for (int i = 0; i < 8; ++i) r[i] = kFill ? fabsf(x[i]) : x[i];
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s.p[k][i] = pack_hi(r[2 * i], r[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+      s.p[k][i] = pack_hi(r[2 * i], r[2 * i + 1]);
+      if (kFill) s.p[k][i] |= pack_hi(x[2 * i], x[2 * i + 1]) & 0x80008000u;
+    }
     if (k < 2)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
         r[i] -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, r[i]) & 0xffff0000u);
-    if (kFill && k < 2)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (!(x[i] < 0.f ? r[i] < 0.f : r[i] > 0.f) && fabsf(x[i]) >= 0x1p-100f) r[i] = copysignf(0x1p-126f, x[i]);
+        if (kFill) r[i] = fmaxf(r[i], fabsf(x[i]) * 0x1p-40f);
+      }
   }
   return s;
 }

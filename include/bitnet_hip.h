@@ -488,7 +488,7 @@ int bnr_paged_decode_workspace(bnr_ctx *ctx, const bnr_paged_kv *kv, size_t batc
  * a row that is attended to, makes its column of the outputs non-finite; one in K
  * makes the scores that its products with q make.  A NaN or +infinity as a
  * score makes the outputs NaN; a row whose score is -infinity has no weight, and
- * a query head with no other row gives zeros.  (An element of q below 2^-90 may
+ * a query head with no other row gives zeros.  (An element of q below 2^-80 may
  * count as zero beside an infinity, a NaN.)  `workspace` (device memory,
  * 16-byte aligned) must be zero-filled before its first use; each call leaves
  * it ready for the next.  Calls that share a workspace must be ordered, as on
