@@ -2756,9 +2756,14 @@ int check_paged_count(size_t n, const char *what) {
 // must be zero for the next one), then the pieces and the groups of them.
 constexpr size_t kPagedTicketBytes = (size_t)kPagedTickets * kCounterStride * sizeof(unsigned);
 
-size_t paged_workspace_bytes(size_t group, size_t head_dim) {
+// Pieces hold a kv head's query heads, at most kPagedMaxGroup, where the matrix
+// cores can take the pool, and one elsewhere.  More query heads go to the other
+// kernel, but the bytes stay: a workspace for n_heads also serves fewer.
+size_t paged_workspace_bytes(const bnr_paged_kv *kv, size_t n_heads) {
+  const size_t group = n_heads / kv->n_kv_heads;
+  const int heads = paged_matrix_pool(kv->head_dim, kv->page_size) ? (int)std::min<size_t>(group, kPagedMaxGroup) : 1;
   return kPagedTicketBytes +
-         (size_t)4 * kPagedMaxWgs * paged_part_floats((int)group, (int)head_dim) * sizeof(float);
+         (size_t)4 * kPagedMaxWgs * paged_part_floats(heads, (int)kv->head_dim) * sizeof(float);
 }
 
 int check_paged_heads(const bnr_paged_kv *kv, size_t batch, size_t n_heads) {
@@ -2878,7 +2883,7 @@ extern "C" int bnr_paged_decode_workspace(bnr_ctx *c, const bnr_paged_kv *kv, si
   int st = paged_pool(kv, nullptr, 1, p);
   if (!st) st = check_paged_heads(kv, batch, n_heads);
   if (st) return st;
-  *bytes = paged_workspace_bytes(n_heads / kv->n_kv_heads, kv->head_dim);
+  *bytes = paged_workspace_bytes(kv, n_heads);
   return set_ok();
 }
 
@@ -2896,7 +2901,7 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
   if (!q || !block_table || !lens || !out || !workspace)
     return err_backend("paged_decode_attention: NULL pointer");
   const size_t group = n_heads / kv->n_kv_heads;
-  const size_t need = paged_workspace_bytes(group, kv->head_dim);
+  const size_t need = paged_workspace_bytes(kv, n_heads);
   if (workspace_bytes < need)
     return err_shape(fmt("workspace of %zu bytes", need), fmt("%zu bytes", workspace_bytes));
   if (!aligned16(workspace))
@@ -2910,8 +2915,7 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
   a.n_heads = (int)n_heads;
   a.group = (int)group;
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)kv->head_dim));
-  const bool fast = kv->head_dim % 16 == 0 && kv->head_dim <= 256 && group <= 16 &&
-                    kv->page_size % 16 == 0 &&
+  const bool fast = paged_matrix_pool(kv->head_dim, kv->page_size) && group <= (size_t)kPagedMaxGroup &&
                     aligned16(q) && aligned16(out) && aligned16(kv->k) && aligned16(kv->v) &&
                     aligned16(a.pool.k_scales) && aligned16(a.pool.v_scales);
   const size_t items = batch * (fast ? kv->n_kv_heads : n_heads);

@@ -763,6 +763,10 @@ constexpr int kPagedGenericTile = 64;
 // On the matrix cores: 16-byte aligned pools, q and out, head_dim a multiple
 // of 16 up to 256, at most 16 query heads a kv head, pages of a multiple of 16
 // rows.
+constexpr int kPagedMaxGroup = 16;
+constexpr bool paged_matrix_pool(size_t head_dim, size_t page) {
+  return head_dim % 16 == 0 && head_dim <= 256 && page % 16 == 0;
+}
 hipError_t launch_paged_decode(const PagedDecodeArgs &a, int format, hipStream_t s);
 // Rows of a unit there, for a table with room for `rows` rows of each of
 // `items` (sequence, kv head) pairs and at most `wgs` workgroups: 128, 32 for

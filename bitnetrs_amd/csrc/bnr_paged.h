@@ -165,7 +165,6 @@ __device__ __forceinline__ void paged_empty(const PagedDecodeArgs &a, int first_
 // device's coherence point and back.  So the loads of N pieces are all in
 // flight before the first is used, and nothing else waits for memory.
 // ---------------------------------------------------------------------------
-constexpr int kJoinHeads = 16;  // heads of an item at most
 template <int W, int V>
 struct JoinShared {
   float o[W * 64][V], m[W * 64], l[W * 64];

@@ -170,7 +170,7 @@ __global__ __launch_bounds__(64 * kW, (kWavesOf<F, DP>)) void paged_decode_kerne
   // q * (4 group + 1) + g * group + row, which is free of bank conflicts both ways
   extern __shared__ f32x4 s_o[];
   __shared__ u32x4 s_q[QN * 64];
-  __shared__ float s_m[kW * kJoinHeads], s_l[kW * kJoinHeads];
+  __shared__ float s_m[kW * kPagedMaxGroup], s_l[kW * kPagedMaxGroup];
   __shared__ JoinShared<kW, 4> s_join;
   const int lane = threadIdx.x & 63, d = FULL ? DP : a.pool.d, G = a.group;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);

@@ -715,3 +715,18 @@ def test_rope_table_leaves_the_contexts_own(backend):
         torch.cuda.synchronize()
         assert (out - ref).abs().max() <= 1e-5 * ref.abs().max()
     del graph
+
+
+@pytest.mark.parametrize("hq,hkv,d,page", [(64, 1, 512, 16), (71, 1, 64, 16), (16, 1, 256, 16), (20, 1, 128, 8),
+                                           (12, 2, 130, 16), (5, 5, 48, 32)])
+def test_workspace_is_enough(backend, hq, hkv, d, page):
+    """Long sequences in many pieces: nothing is written behind the workspace's bytes."""
+    say(f"workspace {hq}/{hkv}/{d} page {page}")
+    pool = Pool(rng_of("enough", hq, d), "bf16", [7000, 1200], hkv, d, page, spread=0.3)
+    kv = pool.device()
+    n = backend.paged_workspace(kv, 2, hq).numel()
+    raw = torch.zeros(n + (1 << 20), dtype=torch.uint8, device="cuda")
+    raw[n:] = 0x5A
+    for _ in range(2):
+        check_decode(backend, pool, hq, kv=kv, workspace=raw[:n])
+    assert (raw[n:] == 0x5A).all() and (raw[:1536 * 256] == 0).all()

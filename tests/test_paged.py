@@ -248,3 +248,16 @@ def test_index_code_on_the_host():
         subprocess.run(["make", "-s", "-C", native, check], check=True)
     out = subprocess.run([check], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout + out.stderr
+
+
+def test_workspace_of_pieces_of_one_head():
+    """Shapes that only the kernel of one query head a piece can take ask for no more
+    than it uses; none of an accepted shape is out of reach."""
+    one = {d: workspace(desc(n_kv_heads=1, head_dim=d), n_heads=1)[1] for d in (26, 64, 130, 512)}
+    for kw in (dict(head_dim=512), dict(head_dim=130), dict(head_dim=26), dict(head_dim=64, page_size=8)):
+        for n_heads in (2, 16, 64, 65536):
+            st, n = workspace(desc(n_kv_heads=1, **kw), n_heads=n_heads)
+            assert st == 0 and n == one[kw["head_dim"]], (kw, n_heads, n)
+            assert decode(desc(n_kv_heads=1, **kw), n_heads=n_heads, bytes=n - 1) == _lib.BNR_INVALID_SHAPE
+    sizes = [workspace(desc(n_kv_heads=1, head_dim=256), n_heads=h)[1] for h in (1, 4, 16, 17, 64, 65536)]
+    assert sizes == sorted(sizes) and sizes[-1] <= 36 << 20  # one for many heads serves fewer
