@@ -2787,6 +2787,10 @@ extern "C" int bnr_dev_rope_table(bnr_ctx *c, size_t n_positions, size_t head_di
   if (!cos_out || !sin_out) return err_backend("rope_table: NULL pointer");
   DeviceGuard dg(c->device);
   hipStream_t s = (hipStream_t)stream;
+  // A captured copy would read its rows here after they are gone.
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing(s, &capture), "rope table");
+  if (capture != hipStreamCaptureStatusNone) return err_backend("rope_table: not under graph capture");
   // A block of rows at a time, and not through the context's own table, which
   // captured launches may read.
   constexpr size_t kRows = 4096;
@@ -2796,9 +2800,11 @@ extern "C" int bnr_dev_rope_table(bnr_ctx *c, size_t n_positions, size_t head_di
     for (size_t r = 0; r < n_positions; r += kRows) {
       const size_t n = std::min(kRows, n_positions - r), bytes = n * half * sizeof(float);
       rope_rows(r, n, head_dim, theta, hc.data(), hs.data());
-      HIP_TRY(hipMemcpyAsync(cos_out + r * half, hc.data(), bytes, hipMemcpyHostToDevice, s), "rope table copy");
-      HIP_TRY(hipMemcpyAsync(sin_out + r * half, hs.data(), bytes, hipMemcpyHostToDevice, s), "rope table copy");
-      HIP_TRY(hipStreamSynchronize(s), "rope table copy");
+      hipError_t e = hipMemcpyAsync(cos_out + r * half, hc.data(), bytes, hipMemcpyHostToDevice, s);
+      if (e == hipSuccess) e = hipMemcpyAsync(sin_out + r * half, hs.data(), bytes, hipMemcpyHostToDevice, s);
+      const hipError_t done = hipStreamSynchronize(s);  // of either, before the rows are written again or freed
+      HIP_TRY(e, "rope table copy");
+      HIP_TRY(done, "rope table copy");
     }
   } catch (const std::bad_alloc &) {
     return err_backend("rope_table: out of host memory");

@@ -442,7 +442,7 @@ typedef struct bnr_paged_kv {
 /* The rotation tables of bnr_rope_embed (the same values) for positions
  * 0..n_positions-1, into cos_out and sin_out [n_positions x head_dim/2] in
  * device memory: a caller of bnr_dev_paged_append keeps them.  Builds them on
- * the host and waits for the copy: not for use under graph capture.  The
+ * the host and waits for the copy: refused while `stream` is being captured.  The
  * context's own table stays as it is. */
 int bnr_dev_rope_table(bnr_ctx *ctx, size_t n_positions, size_t head_dim, float theta,
                        float *cos_out, float *sin_out, void *stream);

@@ -730,3 +730,23 @@ def test_workspace_is_enough(backend, hq, hkv, d, page):
     for _ in range(2):
         check_decode(backend, pool, hq, kv=kv, workspace=raw[:n])
     assert (raw[n:] == 0x5A).all() and (raw[:1536 * 256] == 0).all()
+
+
+def test_rope_table_is_refused_under_capture(backend):
+    """Its copies start in host memory that the call frees; the capture goes on."""
+    from bitnetrs_amd import BackendError
+
+    x = torch.zeros(8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(BackendError, match="capture"):
+            backend.rope_table(16, 64, THETA)
+        x += 1
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (x == 2 * (i + 1)).all()
+    cos, _ = backend.rope_table(16, 64, THETA)
+    assert (cos[0] == 1).all()
+    del graph
