@@ -347,7 +347,8 @@ class HipBackend:
 
     def rope_table(self, n_positions: int, head_dim: int, theta: float):
         """The rotation tables (cos, sin) [n_positions, head_dim/2] that rope_embed
-        uses, as tensors for dev_paged_append."""
+        uses, as tensors for dev_paged_append.  Waits for their copy; refused
+        under graph capture."""
         import torch
 
         cos, sin = (torch.empty(n_positions, head_dim // 2, device=f"cuda:{self.device_id}")

@@ -741,9 +741,13 @@ struct PagedDecodeArgs {
 };
 // Floats of a piece of `heads` query heads: outputs, then (max, sum) of each.
 constexpr int paged_part_floats(int heads, int d) { return (heads * (d + 2) + 3) / 4 * 4; }
-// Workgroups of a decode launch: two a CU.  A third, which the registers of
-// most forms allow, changed 64 int8 sequences of up to 32768 rows by less than
-// 1 % and cost one of 131072 e4m3 rows 8 % (each adds a piece to join).
+// Workgroups of a decode launch: two a CU, what the registers and LDS of most
+// forms leave room for.  A third, which the registers of most allow, changed 64
+// int8 sequences of up to 32768 rows by less than 1 % and cost one of 131072
+// e4m3 rows 8 % (each adds a piece to join).  For 13 to 16 query heads a kv head
+// over 8-bit rows of more than 128, LDS (85 to 98 KB a workgroup) leaves room
+// for one, so that the 512 run in two rounds: one token over 45908 int8 rows of
+// 256, 2 kv heads, takes 50.2 us with 32 query heads and 35.2 with 24.
 constexpr int kPagedMaxWgs = 512;
 constexpr int paged_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // Waves of a SIMD by the registers that a form takes, and so workgroups of a

@@ -204,7 +204,7 @@ struct JoinState {
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.f;
   }
-  // l is at least 1 wherever there is a row
+  // l is 0 only where no row has a weight, else near 1 or more
   __device__ __forceinline__ void write(float *out) const {
     const float r = l == 0.f ? 0.f : 1.0f / l;
     if constexpr (V == 4)

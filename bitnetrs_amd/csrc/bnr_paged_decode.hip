@@ -2,8 +2,9 @@
 // matrix cores.
 //
 // An item is one (sequence, kv head): its G <= 16 query heads share one read
-// of each row.  A wave takes 32 rows at a time and keeps everything in
-// registers: no operand passes through LDS.
+// of each row.  A wave takes 32 rows at a time; K, V, the scores and the weights
+// stay in its registers.  The query operands, the same for the workgroup's
+// waves, are read from LDS in each step.
 //
 //   S  = K q^T   A = 16 rows of K, B = the query heads as 16 columns
 //   O += V^T P   A = 16 dims of V, B = the weights of 32 rows
@@ -23,14 +24,17 @@
 // int8 codes are exact in bf16; q and the weights are cut into three bf16
 // parts of 8 bits each, which together hold all 24 bits of an fp32 value, and
 // every part has fp32's exponent range: the products are those of fp32, at a
-// third of the bf16 rate, which is far above what the rows' bytes need.  A
-// row's scale multiplies its score and its weight in fp32.
+// third of the bf16 rate, which is far above what the rows' bytes need.  Their
+// sum within an instruction keeps 2^-24 of its largest operand and is cut
+// there, not rounded to nearest (2 - 2^-69 beside a product of 4 came out as
+// 2 - 2^-22); outputs end up 3e-7 to 5e-7 of their norm from 64 bits.  A row's
+// scale multiplies its score and its weight in fp32.
 //
 // Bound by the rows' bytes once there are many: with the products taken out
-// the loads alone take 97 % of the time of 64 int8 sequences of up to 32768
-// rows (233 us, 6.1 TB/s; a plain read of this card 7.1).  A short call is
-// latency: lengths, table and rows one after the other (3.5 us), a step, then
-// a store, a ticket and a load to join the pieces (3 us); 9.0 us over 4096
+// the loads alone take 96 to 97 % of the time of 64 int8 sequences of up to
+// 32768 rows (231 to 238 us, 6.1 TB/s; a plain read of this card 7.1).  A short
+// call is latency: lengths, table and rows one after the other (3.5 us), a step,
+// then a store, a ticket and a load to join the pieces (3.5 us); 9.1 us over 4096
 // bf16 rows, 5.3 where nothing is joined.  Of the vector instructions of an
 // int8 step, 365 of a wave, half turn codes into bf16.
 #include "bnr_paged.h"

@@ -489,7 +489,9 @@ int bnr_paged_decode_workspace(bnr_ctx *ctx, const bnr_paged_kv *kv, size_t batc
  * makes the scores that its products with q make.  A NaN or +infinity as a
  * score makes the outputs NaN; a row whose score is -infinity has no weight, and
  * a query head with no other row gives zeros.  (An element of q below 2^-80 may
- * count as zero beside an infinity, a NaN.)  `workspace` (device memory,
+ * count as zero beside an infinity, a NaN.)  Sums are fp32 and divided at the end:
+ * V times the rows that weigh it, a score, and for FP8 and INT8 the sum of q times
+ * a row's codes without its scale, must lie within fp32's range.  `workspace` (device memory,
  * 16-byte aligned) must be zero-filled before its first use; each call leaves
  * it ready for the next.  Calls that share a workspace must be ordered, as on
  * one stream.  The same inputs give the same bits on every run. */
