@@ -496,7 +496,8 @@ class PagedKV:
     n_kv_heads, page_size, head_dim]`` and, for the 8-bit formats, one fp32
     scale a row (``k_scales``, ``v_scales`` ``[n_pages, n_kv_heads,
     page_size]``).  ``fmt``: "f32", "bf16", "fp8" (e4m3) or "int8".  Which page
-    holds which rows is the caller's block table."""
+    holds which rows is the caller's block table.  The tensors' contents are the
+    caller's to change, the tensors themselves stay."""
 
     FORMATS = {"f32": (_lib.BNR_KV_F32, "float32"), "bf16": (_lib.BNR_KV_BF16, "bfloat16"),
                "fp8": (_lib.BNR_KV_FP8, "float8_e4m3fn"), "int8": (_lib.BNR_KV_INT8, "int8")}
@@ -554,6 +555,14 @@ class PagedKV:
         self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda device: torch.cuda.current_stream(device).cuda_stream)
+        self._fixed = True
+
+    def __setattr__(self, name: str, value) -> None:
+        # the descriptor has the tensors' addresses and sizes: another tensor in
+        # their place would leave it with memory that is free again
+        if "_fixed" in self.__dict__:
+            raise AttributeError(f"a pool's {name} is fixed: make another one (from_tensors)")
+        object.__setattr__(self, name, value)
 
     def desc(self, device_id: int):
         """The pool as the library takes it."""

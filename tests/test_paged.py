@@ -261,3 +261,15 @@ def test_workspace_of_pieces_of_one_head():
             assert decode(desc(n_kv_heads=1, **kw), n_heads=n_heads, bytes=n - 1) == _lib.BNR_INVALID_SHAPE
     sizes = [workspace(desc(n_kv_heads=1, head_dim=256), n_heads=h)[1] for h in (1, 4, 16, 17, 64, 65536)]
     assert sizes == sorted(sizes) and sizes[-1] <= 36 << 20  # one for many heads serves fewer
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_scales", "v_scales", "n_pages", "n_kv_heads", "page_size", "head_dim", "fmt"])
+def test_paged_kv_stays_as_it_was_made(name):
+    """Calls take a pool by its descriptor, checks by its attributes: neither moves."""
+    kv = bitnetrs_amd.PagedKV(3, 16, 2, 64, "int8", device="cpu")
+    was = getattr(kv, name)
+    with pytest.raises(AttributeError, match=name):
+        setattr(kv, name, was.clone() if isinstance(was, torch.Tensor) else was)
+    assert getattr(kv, name) is was
+    kv.k.fill_(3)  # contents are the caller's
+    assert kv._desc.k == kv.k.data_ptr()
