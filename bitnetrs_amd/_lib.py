@@ -29,6 +29,7 @@ BNR_KV_F32 = 0
 BNR_KV_BF16 = 1
 BNR_KV_FP8 = 2
 BNR_KV_INT8 = 3
+BNR_KV_FP4 = 5
 
 BNR_GLUE_PLAIN = 0
 BNR_GLUE_RESIDUAL = 1

@@ -495,12 +495,15 @@ class PagedKV:
     """One layer's pool of a paged KV cache: codes ``k`` and ``v`` ``[n_pages,
     n_kv_heads, page_size, head_dim]`` and, for the 8-bit formats, one fp32
     scale a row (``k_scales``, ``v_scales`` ``[n_pages, n_kv_heads,
-    page_size]``).  ``fmt``: "f32", "bf16", "fp8" (e4m3) or "int8".  Which page
+    page_size]``).  ``fmt``: "f32", "bf16", "fp8" (e4m3), "int8" or "fp4" (e2m1:
+    uint8 codes, two in a byte along head_dim, and uint8 exponents ``[n_pages,
+    n_kv_heads, page_size, ceil(head_dim / 32)]`` as scales).  Which page
     holds which rows is the caller's block table.  The tensors' contents are the
     caller's to change, the tensors themselves stay."""
 
     FORMATS = {"f32": (_lib.BNR_KV_F32, "float32"), "bf16": (_lib.BNR_KV_BF16, "bfloat16"),
-               "fp8": (_lib.BNR_KV_FP8, "float8_e4m3fn"), "int8": (_lib.BNR_KV_INT8, "int8")}
+               "fp8": (_lib.BNR_KV_FP8, "float8_e4m3fn"), "int8": (_lib.BNR_KV_INT8, "int8"),
+               "fp4": (_lib.BNR_KV_FP4, "uint8")}
 
     def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
                  fmt: str = "bf16", device: str = "cuda"):
@@ -509,11 +512,16 @@ class PagedKV:
         if fmt not in self.FORMATS:
             raise InvalidConfig(f"unknown paged KV format {fmt!r}")
         dtype = getattr(torch, self.FORMATS[fmt][1])
-        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        if fmt == "fp4" and head_dim % 2:
+            raise InvalidConfig(f"paged KV head_dim must be even, got {head_dim}")
+        rows = (n_pages, n_kv_heads, page_size)
+        shape = (*rows, head_dim // 2 if fmt == "fp4" else head_dim)
         k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
         ks = vs = None
         if fmt in ("fp8", "int8"):
-            ks, vs = (torch.zeros(shape[:3], device=device) for _ in range(2))
+            ks, vs = (torch.zeros(rows, device=device) for _ in range(2))
+        elif fmt == "fp4":
+            ks, vs = (torch.zeros(*rows, -(-head_dim // 32), dtype=dtype, device=device) for _ in range(2))
         self._take(k, v, ks, vs)
 
     @classmethod
@@ -532,10 +540,13 @@ class PagedKV:
             raise InvalidShape("k and v [n_pages, n_kv_heads, page_size, head_dim]",
                                f"{list(k.shape)} and {list(v.shape)}")
         tensors = [k, v]
-        if fmt in ("fp8", "int8"):
+        scales, kind = k.shape[:3], "float32"
+        if fmt == "fp4":
+            scales, kind = (*scales, -(-k.shape[3] // 16)), "uint8"
+        if fmt in ("fp8", "int8", "fp4"):
             for s in (k_scales, v_scales):
-                if s is None or s.shape != k.shape[:3] or str(s.dtype) != "torch.float32":
-                    raise InvalidShape(f"float32 scales {list(k.shape[:3])}",
+                if s is None or s.shape != scales or str(s.dtype) != f"torch.{kind}":
+                    raise InvalidShape(f"{kind} scales {list(scales)}",
                                        "none" if s is None else f"{s.dtype} {list(s.shape)}")
             tensors += [k_scales, v_scales]
         elif k_scales is not None or v_scales is not None:
@@ -545,6 +556,8 @@ class PagedKV:
                 raise TypeError("a pool's tensors must be contiguous and on one device")
         self.fmt, self.k, self.v, self.k_scales, self.v_scales = fmt, k, v, k_scales, v_scales
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        if fmt == "fp4":
+            self.head_dim *= 2
         at = [t.data_ptr() for t in tensors] + [None] * (4 - len(tensors))
         self._desc = _lib.PagedKVDesc(*at, self.n_pages, self.page_size, self.n_kv_heads,
                                       self.head_dim, self.FORMATS[fmt][0])

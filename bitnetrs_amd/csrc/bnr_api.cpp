@@ -2698,7 +2698,7 @@ constexpr size_t kPagedMaxBatch = (size_t)1 << 20;  // sequences that a kernel a
 // Checks the pool and the table, and fills the kernels' view of them.
 int paged_pool(const bnr_paged_kv *kv, const int32_t *table, size_t table_stride, PagedPool &p) {
   if (!kv) return err_backend("paged: kv is NULL");
-  if (kv->format < BNR_KV_F32 || kv->format > BNR_KV_INT8)
+  if ((kv->format < BNR_KV_F32 || kv->format > BNR_KV_INT8) && kv->format != BNR_KV_FP4)
     return err_config(fmt("unknown paged KV format %d", kv->format));
   if (kv->n_kv_heads == 0) return err_config("n_kv_heads must be > 0");
   if (kv->head_dim == 0) return err_shape("head_dim > 0", "head_dim = 0");
@@ -2719,8 +2719,8 @@ int paged_pool(const bnr_paged_kv *kv, const int32_t *table, size_t table_stride
   if (table_stride == 0 || table_stride > kPagedMaxRows / kv->page_size)
     return err_shape(fmt("0 < table_stride * page_size <= %zu", kPagedMaxRows),
                      fmt("table_stride = %zu, page_size = %zu", table_stride, kv->page_size));
-  const bool scaled = kv->format == BNR_KV_FP8 || kv->format == BNR_KV_INT8;
-  if (!kv->k || !kv->v || (scaled && (!kv->k_scales || !kv->v_scales)))
+  const bool scaled = kv->format == BNR_KV_FP8 || kv->format == BNR_KV_INT8, fp4 = kv->format == BNR_KV_FP4;
+  if (!kv->k || !kv->v || ((scaled || fp4) && (!kv->k_scales || !kv->v_scales)))
     return err_backend("paged: NULL pool pointer");
   const uintptr_t unit = kv->format == BNR_KV_F32 ? 4 : kv->format == BNR_KV_BF16 ? 2 : 1;
   if (((uintptr_t)kv->k | (uintptr_t)kv->v) % unit != 0)
@@ -2731,6 +2731,8 @@ int paged_pool(const bnr_paged_kv *kv, const int32_t *table, size_t table_stride
   p.v = kv->v;
   p.k_scales = scaled ? kv->k_scales : nullptr;
   p.v_scales = scaled ? kv->v_scales : nullptr;
+  p.k_exps = fp4 ? (unsigned char *)kv->k_scales : nullptr;
+  p.v_exps = fp4 ? (unsigned char *)kv->v_scales : nullptr;
   p.table = table;
   p.table_stride = (long long)table_stride;
   p.n_pages = (int)kv->n_pages;
@@ -2923,7 +2925,8 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)kv->head_dim));
   const bool fast = paged_matrix_pool(kv->head_dim, kv->page_size) && group <= (size_t)kPagedMaxGroup &&
                     aligned16(q) && aligned16(out) && aligned16(kv->k) && aligned16(kv->v) &&
-                    aligned16(a.pool.k_scales) && aligned16(a.pool.v_scales);
+                    aligned16(a.pool.k_scales) && aligned16(a.pool.v_scales) && aligned16(a.pool.k_exps) &&
+                    aligned16(a.pool.v_exps);
   const size_t items = batch * (fast ? kv->n_kv_heads : n_heads);
   const size_t rows = table_stride * kv->page_size;
   const size_t most = fast ? kPagedMaxWgs / 2 * paged_waves(kv->format, (int)kv->head_dim) : kPagedMaxWgs;

@@ -682,12 +682,13 @@ hipError_t launch_residual(float *h, const float *delta, long long n, hipStream_
 
 // ---------------------------------------------------------------------------
 // Paged KV cache (bnr_paged.hip).  One pool holds the rows of many sequences:
-// codes [n_pages][n_kv][page][d] in one of four formats, scales [n_pages]
-// [n_kv][page] for the 8-bit ones.  table[seq * table_stride + i] names the
+// codes [n_pages][n_kv][page][d] in one of five formats, scales [n_pages]
+// [n_kv][page] for the 8-bit ones, exponents [n_pages][n_kv][page][groups] for
+// the 4-bit one, two codes of which share a byte.  table[seq * table_stride + i] names the
 // page of rows i * page .. of a sequence; an entry outside 0 .. n_pages - 1 is
 // a page that is not there.
 // ---------------------------------------------------------------------------
-constexpr int kPagedF32 = 0, kPagedBf16 = 1, kPagedFp8 = 2, kPagedInt8 = 3;
+constexpr int kPagedF32 = 0, kPagedBf16 = 1, kPagedFp8 = 2, kPagedInt8 = 3, kPagedFp4 = 5;
 constexpr int kPagedMaxDim = 512;
 // The least row maximum a scale is made from: 448 / 2^-100 and 2^-100 / 448
 // are both normal floats, so a row of zeros needs no case of its own.
@@ -699,7 +700,11 @@ struct PagedPool {
   const int *table;
   long long table_stride;
   int n_pages, page, n_kv, d;
+  unsigned char *k_exps, *v_exps;  // FP4
 };
+// Elements of an FP4 row that share an exponent, and such groups of a row.
+constexpr int kPagedGroup4 = 32;
+__host__ __device__ constexpr int paged_groups4(int d) { return (d + kPagedGroup4 - 1) / kPagedGroup4; }
 
 struct PagedAppendArgs {
   PagedPool pool;
@@ -772,6 +777,7 @@ constexpr bool paged_matrix_pool(size_t head_dim, size_t page) {
   return head_dim % 16 == 0 && head_dim <= 256 && page % 16 == 0;
 }
 hipError_t launch_paged_decode(const PagedDecodeArgs &a, int format, hipStream_t s);
+hipError_t launch_paged_decode_fp4(const PagedDecodeArgs &a, hipStream_t s);
 // Rows of a unit there, for a table with room for `rows` rows of each of
 // `items` (sequence, kv head) pairs and at most `wgs` workgroups: 128, 32 for
 // each wave.  f32 rows take twice the loads of bf16 ones and their products four

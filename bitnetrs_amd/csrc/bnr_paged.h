@@ -74,6 +74,61 @@ __device__ __forceinline__ float load_code(const void *codes, long long i) {
   return __builtin_amdgcn_cvt_f32_fp8(static_cast<const unsigned char *>(codes)[i], 0);
 }
 
+// ---------------------------------------------------------------------------
+// FP4: the codes of 32 neighbouring elements of a row (the last group of a row
+// may have fewer) are e2m1, 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign, times one
+// power of two, kept as its exponent + 127 in a byte.  With m = max(max|x|,
+// 2^-100) of the group the power is the one that leaves 3.5 <= m / 2^e < 7, at
+// most 2^125: one that leaves 4 <= m / 2^e < 8 cuts values between 7 and 8 by up
+// to 2, this one leaves every error at or under half a step and 1 at the top (6
+// to 7).  x / 2^e is exact, so a code is one rounding, to nearest, ties to the
+// even code.  A group with an infinity or a NaN gets the exponent 255, which
+// reads back as NaN, and codes 0.
+// ---------------------------------------------------------------------------
+constexpr unsigned kPagedNan4 = 255, kPagedTop4 = 252;
+
+__device__ __forceinline__ unsigned exponent4(unsigned largest) {
+  const unsigned tiny = __builtin_bit_cast(unsigned, kPagedTiny);
+  if (largest >= 0x7f800000u) return kPagedNan4;
+  const unsigned m = largest > tiny ? largest : tiny;
+  // a mantissa of 1.75 and more carries into the exponent
+  const unsigned e = ((m + 0x200000u) >> 23) - 2;
+  return e < kPagedTop4 ? e : kPagedTop4;
+}
+// The power as the conversions take it: NaN for 255.
+__device__ __forceinline__ float power4(unsigned e) { return __builtin_bit_cast(float, e << 23); }
+
+// Eight elements as codes, the first in the lowest bits.
+__device__ __forceinline__ unsigned codes4(float4 lo, float4 hi, unsigned e) {
+  if (e == kPagedNan4) return 0u;
+  const float p = power4(e);
+  unsigned w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, lo.x, lo.y, p, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, lo.z, lo.w, p, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, hi.x, hi.y, p, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, hi.z, hi.w, p, 3);
+}
+
+// The two elements of byte I of w, as bf16, which holds all of them exactly.
+template <int I>
+__device__ __forceinline__ unsigned pair4(unsigned w, float power) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, power, I));
+}
+__device__ __forceinline__ float low16(unsigned w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float high16(unsigned w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+
+// Element x of row `at` of a pool, before a row's scale.
+template <int F>
+__device__ __forceinline__ float load_element(const void *codes, const unsigned char *exps, long long at, int d,
+                                              int x) {
+  if constexpr (F == kPagedFp4) {
+    const unsigned w = static_cast<const unsigned char *>(codes)[at * (d / 2) + x / 2];
+    const unsigned p = pair4<0>(w, power4(exps[at * paged_groups4(d) + x / kPagedGroup4]));
+    return x & 1 ? high16(p) : low16(p);
+  } else {
+    return load_code<F>(codes, at * d + x);
+  }
+}
+
 // Inclusive sums over the wave's lanes.
 __device__ __forceinline__ unsigned wave_scan(unsigned v) {
 #define BNR_SCAN(CTRL, ROWS) \

@@ -34,8 +34,33 @@ __device__ __forceinline__ unsigned row_largest(unsigned v) {
   return v;
 }
 
+// What a wave wrote to LDS is there for its other lanes: LDS works in order, so
+// only the compiler has to keep the order.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Eight neighbouring elements (n of them in the row) as codes, and their
+// group's exponent: the lane's neighbours have the group's others.
+__device__ __forceinline__ void store_group4(const AppendRow &r, bool in, int x, int n, float4 lo, float4 hi) {
+  unsigned largest = max(max(max(magnitude(lo.x), magnitude(lo.y)), max(magnitude(lo.z), magnitude(lo.w))),
+                         max(max(magnitude(hi.x), magnitude(hi.y)), max(magnitude(hi.z), magnitude(hi.w))));
+  largest = row_largest<kPagedGroup4 / 8>(largest);
+  const unsigned e = exponent4(largest), w = codes4(lo, hi, e);
+  if (!in || n <= 0) return;
+  if (x % kPagedGroup4 == 0) r.exps[x / kPagedGroup4] = (unsigned char)e;
+  unsigned char *to = static_cast<unsigned char *>(r.codes) + (r.at + x) / 2;
+  if (n >= 8 && reinterpret_cast<uintptr_t>(to) % 4 == 0) {
+    *reinterpret_cast<unsigned *>(to) = w;
+  } else {
+    for (int i = 0; 2 * i < n && i < 4; ++i) to[i] = (unsigned char)(w >> (8 * i));
+  }
+}
+
 template <int F>
 __global__ __launch_bounds__(64 * kWaves) void paged_append_kernel(PagedAppendArgs a) {
+  __shared__ float s_row[F == kPagedFp4 ? kWaves : 1][F == kPagedFp4 ? kPagedMaxDim : 1];
   const int lane = threadIdx.x & 63, half = a.pool.d / 2, per = append_rows(a);
   for (long long n = (long long)blockIdx.x * kWaves + (threadIdx.x >> 6); n < a.n_tokens * per;
        n += (long long)gridDim.x * kWaves) {
@@ -62,6 +87,27 @@ __global__ __launch_bounds__(64 * kWaves) void paged_append_kernel(PagedAppendAr
         largest = max(largest, max(magnitude(lo[k]), magnitude(hi[k])));
       }
     }
+    if constexpr (F == kPagedFp4) {
+      if (!r.out) {
+        // eight neighbours a lane, of which a group of four has one exponent
+        float *row = s_row[threadIdx.x >> 6];
+        wave_order();  // the row before this one has been read
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          const int i = lane + 64 * k;
+          if (i >= half) continue;
+          row[i] = lo[k];
+          row[half + i] = hi[k];
+        }
+        wave_order();
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 8 * lane + i < a.pool.d ? row[8 * lane + i] : 0.f;
+        store_group4(r, true, 8 * lane, a.pool.d - 8 * lane, make_float4(x[0], x[1], x[2], x[3]),
+                     make_float4(x[4], x[5], x[6], x[7]));
+        continue;
+      }
+    }
     float inv = 1.f;
     if (kPagedScaled<F> && !r.out) {
       const RowScale s = row_scale<F>(row_largest<64>(largest));
@@ -75,7 +121,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_append_kernel(PagedAppendAr
       if (r.out) {
         r.out[i] = lo[k];
         r.out[half + i] = hi[k];
-      } else {
+      } else if constexpr (F != kPagedFp4) {
         store_code<F>(r.codes, r.at + i, lo[k], inv);
         store_code<F>(r.codes, r.at + half + i, hi[k], inv);
       }
@@ -115,6 +161,7 @@ __device__ __forceinline__ unsigned largest4(float4 x) {
 template <int F, int L>
 __global__ __launch_bounds__(64 * kWaves) void paged_append_vec_kernel(PagedAppendArgs a) {
   constexpr int kRows = 64 * kWaves / L;
+  __shared__ float4 s_row[F == kPagedFp4 ? kRows : 1][F == kPagedFp4 ? 2 * L : 1];
   const int x = 4 * (threadIdx.x % L), half = a.pool.d / 2, per = append_rows(a);
   const unsigned long long total = (unsigned long long)a.n_tokens * per;
   for (unsigned long long n0 = (unsigned long long)blockIdx.x * kRows; n0 < total;
@@ -145,11 +192,26 @@ __global__ __launch_bounds__(64 * kWaves) void paged_append_vec_kernel(PagedAppe
       inv = s.inv;
       if (in && !r.out && x == 0) *r.scale = s.scale;
     }
+    if constexpr (F == kPagedFp4) {
+      // the row as eight neighbours a lane; a row's lanes are of one wave
+      float4 *row = s_row[threadIdx.x / L];
+      wave_order();  // the rows before these have been read
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (x < half) {
+        row[x / 4] = in ? lo : zero;
+        row[(half + x) / 4] = in ? hi : zero;
+      }
+      wave_order();
+      const bool there = 2 * x < a.pool.d;
+      const float4 l8 = there ? row[x / 2] : zero, h8 = there ? row[x / 2 + 1] : zero;
+      // every lane takes part: those past a row's end bring zeros
+      store_group4(r, in && !r.out, 2 * x, a.pool.d - 2 * x, l8, h8);
+    }
     if (!in) continue;
     if (r.out) {
       st4(r.out + x, lo);
       st4(r.out + half + x, hi);
-    } else {
+    } else if constexpr (F != kPagedFp4) {
       store_codes4<F>(r.codes, r.at + x, lo, inv);
       store_codes4<F>(r.codes, r.at + half + x, hi, inv);
     }
@@ -181,8 +243,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_read_kernel(PagedReadArgs a
       vs = a.pool.v_scales[at];
     }
     for (int x = lane; x < d; x += 64) {
-      ko[x] = at < 0 ? 0.f : load_code<F>(a.pool.k, at * d + x) * ks;
-      vo[x] = at < 0 ? 0.f : load_code<F>(a.pool.v, at * d + x) * vs;
+      ko[x] = at < 0 ? 0.f : load_element<F>(a.pool.k, a.pool.k_exps, at, d, x) * ks;
+      vo[x] = at < 0 ? 0.f : load_element<F>(a.pool.v, a.pool.v_exps, at, d, x) * vs;
     }
   }
 }
@@ -204,11 +266,15 @@ constexpr int kReadPasses = 4;  // 2: 111 us, 8: 116 us, of 107 us then
 template <int L>
 constexpr int kReadRows = kReadPasses * 64 * kWaves / L;
 
-// Four codes as fp32, before the scale.
+// Four codes as fp32, before the scale; `power`: FP4's.
 template <int F>
-__device__ __forceinline__ float4 load_codes4(const void *codes, long long at) {
+__device__ __forceinline__ float4 load_codes4(const void *codes, long long at, float power) {
   if constexpr (F == kPagedF32) {
     return ld4(static_cast<const float *>(codes) + at);
+  } else if constexpr (F == kPagedFp4) {
+    const unsigned w = *reinterpret_cast<const unsigned short *>(static_cast<const unsigned char *>(codes) + at / 2);
+    const unsigned p = pair4<0>(w, power), q = pair4<1>(w, power);
+    return make_float4(low16(p), high16(p), low16(q), high16(q));
   } else if constexpr (F == kPagedBf16) {
     const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const unsigned short *>(codes) + at);
     return make_float4(__builtin_bit_cast(float, w.x << 16), __builtin_bit_cast(float, w.x & 0xffff0000u),
@@ -250,8 +316,14 @@ __global__ __launch_bounds__(64 * kWaves) void paged_read_vec_kernel(PagedReadAr
 #pragma unroll
       for (int n = 0; n < kReadPasses; ++n) {
         const long long from = at[n] < 0 ? 0 : at[n];
-        k[n] = load_codes4<F>(a.pool.k, from * d + x);
-        v[n] = load_codes4<F>(a.pool.v, from * d + x);
+        float kp = 1.f, vp = 1.f;
+        if constexpr (F == kPagedFp4) {
+          const long long group = from * paged_groups4(d) + x / kPagedGroup4;
+          kp = power4(a.pool.k_exps[group]);
+          vp = power4(a.pool.v_exps[group]);
+        }
+        k[n] = load_codes4<F>(a.pool.k, from * d + x, kp);
+        v[n] = load_codes4<F>(a.pool.v, from * d + x, vp);
         ks[n] = vs[n] = 1.f;
         if (kPagedScaled<F>) {
           ks[n] = a.pool.k_scales[from];
@@ -303,7 +375,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
       float x = 0.f;
 #pragma unroll
       for (int j = 0; j < kElems; ++j)
-        if (lane + 64 * j < d) x = fmaf(qr[j], load_code<F>(a.pool.k, at * d + lane + 64 * j), x);
+        if (lane + 64 * j < d)
+          x = fmaf(qr[j], load_element<F>(a.pool.k, a.pool.k_exps, at, d, lane + 64 * j), x);
       x = wave_sum(x) * a.scale_log2;
       float vs = 1.f;
       if (kPagedScaled<F>) {
@@ -317,7 +390,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
 #pragma unroll
       for (int j = 0; j < kElems; ++j)
         if (lane + 64 * j < d)
-          o[j] = fmaf(o[j], keep, w * (load_code<F>(a.pool.v, at * d + lane + 64 * j) * vs));
+          o[j] = fmaf(o[j], keep, w * (load_element<F>(a.pool.v, a.pool.v_exps, at, d, lane + 64 * j) * vs));
     }
     __syncthreads();  // the piece before this one has been read
 #pragma unroll
@@ -343,6 +416,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_generic_kernel(Paged
     case kPagedBf16: CALL(kPagedBf16); break;          \
     case kPagedFp8: CALL(kPagedFp8); break;            \
     case kPagedInt8: CALL(kPagedInt8); break;          \
+    case kPagedFp4: CALL(kPagedFp4); break;            \
     default: return hipErrorInvalidValue;              \
   }
 

@@ -37,17 +37,12 @@
 // then a store, a ticket and a load to join the pieces (3.5 us); 9.1 us over 4096
 // bf16 rows, 5.3 where nothing is joined.  Of the vector instructions of an
 // int8 step, 365 of a wave, half turn codes into bf16.
-#include "bnr_paged.h"
+#include "bnr_paged_mfma.h"
 
 #include <type_traits>
 
 namespace bnr {
 namespace {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kW = 4;  // waves of a workgroup
 constexpr int kStep = 32;  // rows of a wave's step
@@ -59,75 +54,6 @@ constexpr int kBytes = F == kPagedF32 ? 4 : F == kPagedBf16 ? 2 : 1;
 // loads spill: one token over 4096 bf16 rows took 12.6 us.
 template <int F, int DP>
 constexpr int kWavesOf = paged_waves(F, DP);
-
-// N dwords at p; NT: with the non-temporal hint.  V's loads take whole lines
-// and have it; K's take half of each line, the other half comes with the next
-// load and is not to be dropped before.  32 sequences of 128 to 4096 bf16 rows:
-// 38.4 us; 41.2 with the hint on both, 45.0 on neither.
-template <bool NT, int N>
-__device__ __forceinline__ void load_bytes(const char *p, unsigned (&r)[N]) {
-  const auto load = [](const auto *q) { return NT ? __builtin_nontemporal_load(q) : *q; };
-  if constexpr (N >= 4) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const u32x4 v = load(reinterpret_cast<const u32x4 *>(p + 4 * i));
-      r[i] = v.x;
-      r[i + 1] = v.y;
-      r[i + 2] = v.z;
-      r[i + 3] = v.w;
-    }
-  } else if constexpr (N == 2) {
-    const u32x2 v = load(reinterpret_cast<const u32x2 *>(p));
-    r[0] = v.x;
-    r[1] = v.y;
-  } else {
-    r[0] = load(reinterpret_cast<const unsigned *>(p));
-  }
-}
-
-// The upper halves of two floats: a's below b's.
-__device__ __forceinline__ unsigned pack_hi(float a, float b) {
-  return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a),
-                               0x07060302u);
-}
-
-// Three bf16 parts of 8 floats: truncation leaves 8 bits a part, so the parts
-// sum to the value.  (Where the value is a product, the compiler may take the
-// first rest from it unrounded: a rest of the other sign is less than half of
-// the value's last place then.)  kFill: no part is zero or of the other sign,
-// down to values of 2^-90: a rest is 2^-40 of the value at least, which no sum
-// notices.  An infinity of the other operand then makes the infinity in each
-// part's product that it makes with the value, where a zero would make NaN.
-struct Parts {
-  u32x4 p[3];
-};
-template <bool kFill>
-__device__ __forceinline__ Parts split8(const float (&x)[8]) {
-  Parts s;
-  float r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = kFill ? fabsf(x[i]) : x[i];
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s.p[k][i] = pack_hi(r[2 * i], r[2 * i + 1]);
-      if (kFill) s.p[k][i] |= pack_hi(x[2 * i], x[2 * i + 1]) & 0x80008000u;
-    }
-    if (k < 2)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        r[i] -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, r[i]) & 0xffff0000u);
-        if (kFill) r[i] = fmaxf(r[i], fabsf(x[i]) * 0x1p-40f);
-      }
-  }
-  return s;
-}
-
-__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 
 // Code i (0..3) of a dword of 8-bit codes, as a float.
 template <int F, int I>
@@ -509,6 +435,7 @@ hipError_t launch_paged_decode(const PagedDecodeArgs &a, int format, hipStream_t
     case kPagedBf16: return launch_format<kPagedBf16>(a, s);
     case kPagedFp8: return launch_format<kPagedFp8>(a, s);
     case kPagedInt8: return launch_format<kPagedInt8>(a, s);
+    case kPagedFp4: return launch_paged_decode_fp4(a, s);
     default: return hipErrorInvalidValue;
   }
 }

@@ -41,6 +41,7 @@ struct AppendRow {
   void *codes;          // k and v rows: the pool, the row's first element in it,
   long long at;
   float *scale;         // and where its scale goes
+  unsigned char *exps;  // or its groups' exponents
 };
 __host__ __device__ inline const float *append_in(const PagedAppendArgs &a, long long i, int j) {
   const int nq = a.q ? a.n_heads : 0, kv = a.pool.n_kv;
@@ -76,6 +77,8 @@ __host__ __device__ inline bool append_row(const PagedAppendArgs &a, long long i
   r.at = at * p.d;
   float *sc = is_v ? p.v_scales : p.k_scales;
   r.scale = sc ? sc + at : nullptr;
+  unsigned char *ex = is_v ? p.v_exps : p.k_exps;
+  r.exps = ex ? ex + at * paged_groups4(p.d) : nullptr;
   return true;
 }
 

@@ -425,15 +425,21 @@ int bnr_kv_dev_prefill(bnr_ctx *ctx, bnr_kv_cache *cache, size_t layer, float *q
  *   BF16  x rounded to nearest even
  *   FP8   e4m3(x * (448 / m)), scale m / 448     m = max(max|x|, 2^-100) of
  *   INT8  round(x * (127 / m)), scale m / 127    the row, ties to even
+ *   FP4   e2m1(x / 2^e), elements 2i and 2i+1 in the low and the high four bits
+ *         of byte i; e of each 32 neighbouring elements of the row (the last ones
+ *         may be fewer), with 3.5 <= m / 2^e < 7, m = max(max|x|, 2^-100) of them,
+ *         e at most 125, kept as the byte e + 127; 6 for what lies above it
  * A row of FP8 or INT8 that holds an infinity or a NaN gets the scale NaN and
- * reads back as NaN. */
+ * reads back as NaN; 32 such elements of FP4 the byte 255, and read back as NaN. */
 #define BNR_KV_F32 0
 #define BNR_KV_BF16 1
 #define BNR_KV_FP8 2
 #define BNR_KV_INT8 3
+#define BNR_KV_FP4 5
 typedef struct bnr_paged_kv {
-  void *k, *v;                /* [n_pages][n_kv_heads][page_size][head_dim] */
-  float *k_scales, *v_scales; /* [n_pages][n_kv_heads][page_size]; FP8 and INT8 only */
+  void *k, *v;                /* [n_pages][n_kv_heads][page_size][head_dim]; FP4: head_dim / 2 bytes a row */
+  float *k_scales, *v_scales; /* [n_pages][n_kv_heads][page_size]; FP8 and INT8 only.
+                                 FP4: uint8_t [n_pages][n_kv_heads][page_size][ceil(head_dim / 32)] */
   size_t n_pages, page_size, n_kv_heads;
   size_t head_dim; /* even, at most 512 */
   int format;      /* BNR_KV_* */
@@ -469,7 +475,7 @@ int bnr_dev_paged_append(bnr_ctx *ctx, const bnr_paged_kv *kv, const float *q, c
 /* Read rows back as fp32 in the contiguous layout of the other entry points:
  * rows starts[s] .. lens[s]-1 of sequence s (starts NULL: from row 0), at most
  * cap of them, go to k_out and v_out [batch x n_kv_heads x cap x d] from row 0
- * on; FP8 and INT8 rows as code * scale.  Rows behind them are left as they
+ * on; FP8, INT8 and FP4 rows as code * scale.  Rows behind them are left as they
  * were; a sequence with a negative start is left out. */
 int bnr_dev_paged_read(bnr_ctx *ctx, const bnr_paged_kv *kv, const int32_t *block_table,
                        size_t batch, size_t table_stride, const int32_t *starts,
