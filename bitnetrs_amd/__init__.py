@@ -12,7 +12,8 @@ from .stack import AttentionStack
 from .backend import (BNR_MIRROR_FULL, BNR_MIRROR_INCREMENTAL, BackendError, BitNetError,
                       DeviceKVCache, HipBackend, InvalidConfig, InvalidShape, NativeKVCache,
                       PagedKV, QuantizationError, UnsupportedDevice)
+from .rope import Rope
 
-__all__ = ["HipBackend", "DeviceKVCache", "NativeKVCache", "PagedKV", "AttentionStack", "BitNetError", "InvalidShape",
+__all__ = ["HipBackend", "DeviceKVCache", "NativeKVCache", "PagedKV", "Rope", "AttentionStack", "BitNetError", "InvalidShape",
            "InvalidConfig", "BackendError", "UnsupportedDevice", "QuantizationError",
            "BNR_MIRROR_FULL", "BNR_MIRROR_INCREMENTAL", "build", "load", "LIB_PATH"]

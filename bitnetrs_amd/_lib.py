@@ -31,6 +31,13 @@ BNR_KV_FP8 = 2
 BNR_KV_INT8 = 3
 BNR_KV_FP4 = 5
 
+BNR_ROPE_HALF = 0
+BNR_ROPE_INTERLEAVED = 1
+
+BNR_TYPE_F32 = 0
+BNR_TYPE_BF16 = 1
+BNR_TYPE_F16 = 2
+
 BNR_GLUE_PLAIN = 0
 BNR_GLUE_RESIDUAL = 1
 BNR_GLUE_SQRELU = 2
@@ -117,6 +124,22 @@ class PagedKVDesc(ctypes.Structure):
 
 _pkv = _c.POINTER(PagedKVDesc)
 
+
+class RopeDesc(ctypes.Structure):
+    """bnr_rope"""
+
+    _fields_ = [("rates", _vp), ("n_pairs", _sz), ("layout", _c.c_int), ("magnitude", _c.c_float)]
+
+
+class HeadsDesc(ctypes.Structure):
+    """bnr_heads"""
+
+    _fields_ = [("in_", _vp), ("out", _vp), ("n_heads", _sz), ("in_token", _sz), ("in_head", _sz),
+                ("out_token", _sz), ("out_head", _sz)]
+
+
+_heads = _c.POINTER(HeadsDesc)
+
 # name -> (restype, argtypes); one entry per function in include/bitnet_hip.h
 SIGNATURES = {
     "bnr_last_error": (_c.c_char_p, []),
@@ -193,6 +216,18 @@ SIGNATURES = {
     "bnr_paged_decode_workspace": (_c.c_int, [_vp, _pkv, _sz, _sz, _c.POINTER(_sz)]),
     "bnr_dev_paged_decode_attention": (_c.c_int, [_vp, _pkv, _vp, _sz, _vp, _sz, _sz, _vp, _vp,
                                                   _vp, _sz, _vp]),
+    "bnr_dev_paged_extend": (_c.c_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp,
+                                        _vp, _sz, _vp, _vp, _vp, _vp]),
+    "bnr_dev_paged_release": (_c.c_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp,
+                                         _vp, _vp]),
+    "bnr_dev_paged_copy": (_c.c_int, [_vp, _pkv, _vp, _sz, _sz, _vp, _vp, _vp, _vp]),
+    "bnr_beam_workspace": (_c.c_int, [_vp, _sz, _sz, _sz, _sz, _c.POINTER(_sz)]),
+    "bnr_dev_beam_select": (_c.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _c.c_int32, _vp,
+                                       _vp, _vp, _vp, _vp, _sz, _vp]),
+    "bnr_dev_beam_reorder": (_c.c_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
+    "bnr_dev_rope": (_c.c_int, [_vp, _c.POINTER(RopeDesc), _c.c_int, _sz, _sz, _vp, _heads, _heads,
+                                _vp]),
+    "bnr_dev_rope_scaled_table": (_c.c_int, [_vp, _c.POINTER(RopeDesc), _sz, _sz, _vp, _vp, _vp]),
 }
 
 _lib = None

@@ -68,6 +68,14 @@ def _on(t, name: str, dtype, device: int, shape=None):
     return t.data_ptr()
 
 
+def _raw_stream(device: int):
+    """The current stream of a device, as a number."""
+    import torch
+
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(device) if get else torch.cuda.current_stream(device).cuda_stream
+
+
 def _check_sizes(*operands) -> None:
     """Raise for the first of the (tensor, name, dimensions) that has others: what
     a call says whose operands' sizes did not unpack."""
@@ -441,6 +449,196 @@ class HipBackend:
             _on(block_table, "block_table", i32, dev), batch, stride, _on(lens, "lens", i32, dev, (batch,)),
             _on(out, "out", kv.f32, dev, qs), _on(workspace, "workspace", kv.u8, dev), n,
             self._paged_stream(kv, stream)))
+
+    # page tables -----------------------------------------------------------------
+    def dev_paged_extend(self, block_table, lens, new, free_pages, free_count, page_size, seqs, positions,
+                         offsets, lens_out, count_out, slots=None, stream=None) -> None:
+        """Pages for new[s] more tokens of each sequence of block_table [n_seqs,
+        pages], from the stack free_pages[0 .. free_count[0] - 1], its end first; the
+        table gets their entries.  seqs and positions [n_tokens] (and slots, int64)
+        say where each new token goes, as dev_paged_append takes them, -1 in places
+        that no token has; offsets [n_seqs + 1] which tokens are a sequence's;
+        lens_out and count_out [1] are lens and free_count afterwards.  All int32.
+        What does not fit gets nothing: see bnr_dev_paged_extend."""
+        dev = self.device_id
+        import torch
+
+        i32 = torch.int32
+        try:
+            (n, stride), (cap,), (n_tokens,) = block_table.shape, free_pages.shape, seqs.shape
+        except (AttributeError, ValueError):
+            _check_sizes((block_table, "block_table", 2), (free_pages, "free_pages", 1), (seqs, "seqs", 1))
+            raise
+        _lib.check(self._L.bnr_dev_paged_extend(
+            self._h, _on(block_table, "block_table", i32, dev), n, stride, page_size,
+            _on(lens, "lens", i32, dev, (n,)), _on(new, "new", i32, dev, (n,)),
+            _on(free_pages, "free_pages", i32, dev), cap, _on(free_count, "free_count", i32, dev, (1,)),
+            _on(seqs, "seqs", i32, dev), _on(positions, "positions", i32, dev, (n_tokens,)),
+            None if slots is None else _on(slots, "slots", torch.int64, dev, (n_tokens,)), n_tokens,
+            _on(offsets, "offsets", i32, dev, (n + 1,)), _on(lens_out, "lens_out", i32, dev, (n,)),
+            _on(count_out, "count_out", i32, dev, (1,)),
+            _raw_stream(dev) if stream is None else _stream(stream)))
+
+    def dev_paged_release(self, block_table, lens, which, free_pages, free_count, page_size, lens_out,
+                          count_out, keep=None, stream=None) -> None:
+        """The pages of the sequences with which[s] != 0 (uint8) back onto the stack;
+        with `keep` [n_seqs], those behind a sequence's first keep[s]."""
+        dev = self.device_id
+        import torch
+
+        i32 = torch.int32
+        try:
+            (n, stride), (cap,) = block_table.shape, free_pages.shape
+        except (AttributeError, ValueError):
+            _check_sizes((block_table, "block_table", 2), (free_pages, "free_pages", 1))
+            raise
+        _lib.check(self._L.bnr_dev_paged_release(
+            self._h, _on(block_table, "block_table", i32, dev), n, stride, page_size,
+            _on(lens, "lens", i32, dev, (n,)), _on(which, "which", torch.uint8, dev, (n,)),
+            None if keep is None else _on(keep, "keep", i32, dev, (n,)),
+            _on(free_pages, "free_pages", i32, dev), cap, _on(free_count, "free_count", i32, dev, (1,)),
+            _on(lens_out, "lens_out", i32, dev, (n,)), _on(count_out, "count_out", i32, dev, (1,)),
+            _raw_stream(dev) if stream is None else _stream(stream)))
+
+    def dev_paged_copy(self, kv: "PagedKV", block_table, src, lens, starts=None, stream=None) -> None:
+        """Rows starts[s] (None: 0) .. lens[s]-1 of sequence src[s] to those of
+        sequence s, where src[s] is another sequence of block_table [n_seqs, pages];
+        rows in pages that both have are left out.  No sequence is both copied to
+        and from."""
+        dev, i32 = self.device_id, kv.i32
+        try:
+            n, stride = block_table.shape
+        except (AttributeError, ValueError):
+            _check_sizes((block_table, "block_table", 2))
+            raise
+        _lib.check(self._L.bnr_dev_paged_copy(
+            self._h, kv.desc(dev), _on(block_table, "block_table", i32, dev), n, stride,
+            _on(src, "src", i32, dev, (n,)), None if starts is None else _on(starts, "starts", i32, dev, (n,)),
+            _on(lens, "lens", i32, dev, (n,)), self._paged_stream(kv, stream)))
+
+    # beam search -------------------------------------------------------------------
+    def beam_workspace(self, batch: int, beams: int, vocab: int, k: int):
+        """A workspace for dev_beam_select of up to that many requests."""
+        import torch
+
+        n = ctypes.c_size_t()
+        _lib.check(self._L.bnr_beam_workspace(self._h, batch, beams, vocab, k, ctypes.byref(n)))
+        return torch.empty(n.value, dtype=torch.uint8, device=f"cuda:{self.device_id}")
+
+    def dev_beam_select(self, logits, scores, tokens, parents, scores_out, workspace, done=None, eos=-1,
+                        done_out=None, stream=None) -> None:
+        """Of each request's beams the k best continuations, best first: logits
+        [batch, beams, vocab] (rows may lie further apart), scores [batch, beams],
+        tokens and parents (int32) and scores_out [batch, k].  done (uint8): beams
+        that have ended, with their one continuation eos; done_out [batch, k] is
+        theirs afterwards.  `workspace` from beam_workspace; calls that share one
+        must be ordered."""
+        dev = self.device_id
+        import torch
+
+        f32, i32, u8 = torch.float32, torch.int32, torch.uint8
+        try:
+            (batch, beams, vocab), (_, k), (n,) = logits.shape, tokens.shape, workspace.shape
+            far, row, one = logits.stride()
+        except (AttributeError, ValueError):
+            _check_sizes((logits, "logits", 3), (tokens, "tokens", 2), (workspace, "workspace", 1))
+            raise
+        if beams == 1:
+            row = far
+        if batch * beams == 1:
+            row = vocab
+        if (logits.dtype is not f32 or logits.get_device() != dev or (one != 1 and vocab > 1)
+                or (batch > 1 and far != beams * row)):
+            raise TypeError(f"logits must be a {f32} tensor on cuda:{dev} with rows of equal distance")
+        out = (batch, k)
+        _lib.check(self._L.bnr_dev_beam_select(
+            self._h, logits.data_ptr(), max(row, vocab) if batch == 0 else row, batch, beams, vocab, k,
+            _on(scores, "scores", f32, dev, (batch, beams)),
+            None if done is None else _on(done, "done", u8, dev, (batch, beams)), eos,
+            _on(tokens, "tokens", i32, dev, out), _on(parents, "parents", i32, dev, out),
+            _on(scores_out, "scores_out", f32, dev, out),
+            None if done_out is None else _on(done_out, "done_out", u8, dev, out),
+            _on(workspace, "workspace", u8, dev), n, _raw_stream(dev) if stream is None else _stream(stream)))
+
+    def dev_beam_reorder(self, block_table, parents, table_out, src, stream=None) -> None:
+        """The block tables [batch * beams, pages] after a selection of parents
+        [batch, beams], into table_out, and in src [batch * beams] the sequences that
+        dev_paged_copy has to copy from (-1: none)."""
+        dev = self.device_id
+        import torch
+
+        i32 = torch.int32
+        try:
+            (rows, stride), (batch, beams) = block_table.shape, parents.shape
+        except (AttributeError, ValueError):
+            _check_sizes((block_table, "block_table", 2), (parents, "parents", 2))
+            raise
+        if rows != batch * beams:
+            raise InvalidShape(f"block_table of {batch} * {beams} rows", f"{rows}")
+        _lib.check(self._L.bnr_dev_beam_reorder(
+            self._h, _on(block_table, "block_table", i32, dev), batch, beams, stride,
+            _on(parents, "parents", i32, dev), _on(table_out, "table_out", i32, dev, (rows, stride)),
+            _on(src, "src", i32, dev, (rows,)), _raw_stream(dev) if stream is None else _stream(stream)))
+
+    # rotary embeddings ---------------------------------------------------------------
+    def dev_rope(self, rope, q, k, positions, q_out=None, k_out=None, stream=None) -> None:
+        """Rotate q [n, n_heads, d] and k [n, n_kv_heads, d] (either may be None) by
+        `rope` (a Rope) at positions [n] (int32), into q_out and k_out (None: in
+        place).  float32, bfloat16 or float16; token and head strides are free, so
+        slices of a fused projection's output are taken as they are.  A token with a
+        negative position is left out."""
+        dev = self.device_id
+        import torch
+
+        types = {torch.float32: _lib.BNR_TYPE_F32, torch.bfloat16: _lib.BNR_TYPE_BF16,
+                 torch.float16: _lib.BNR_TYPE_F16}
+        first = k if q is None else q
+        try:
+            (n,), (_, _, d) = positions.shape, first.shape
+        except (AttributeError, ValueError):
+            _check_sizes((positions, "positions", 1), (first, "q" if first is q else "k", 3))
+            raise
+        kind = first.dtype
+        if kind not in types:
+            raise TypeError(f"q and k must be float32, bfloat16 or float16, not {kind}")
+        heads = []
+        for x, out, name in ((q, q_out, "q"), (k, k_out, "k")):
+            if x is None:
+                if out is not None:
+                    raise TypeError(f"{name}_out without {name}")
+                heads.append(None)
+                continue
+            if out is None:
+                out = x
+            for t, what in ((x, name), (out, name + "_out")):
+                try:
+                    fits = t.dtype is kind and t.get_device() == dev
+                except AttributeError:
+                    fits = False
+                if not fits:
+                    raise TypeError(f"{what} must be a {kind} tensor on cuda:{dev}")
+                if t.dim() != 3 or t.shape[0] != n or t.shape[2] != d or t.shape != x.shape:
+                    raise InvalidShape(f"{what} [{n}, heads, {d}]", f"{list(t.shape)}")
+                if t.stride(2) != 1 and d > 1:
+                    raise TypeError(f"the elements of a head of {what} must lie side by side")
+            (it, ih, _), (ot, oh, _) = x.stride(), out.stride()
+            heads.append(_lib.HeadsDesc(x.data_ptr(), out.data_ptr(), x.shape[1], it, ih, ot, oh))
+        _lib.check(self._L.bnr_dev_rope(
+            self._h, rope._ref, types[kind], n, d, _on(positions, "positions", torch.int32, dev), heads[0],
+            heads[1], _raw_stream(dev) if stream is None else _stream(stream)))
+
+    def rope_scaled_table(self, rope, n_positions: int, first: int = 0, out=None, stream=None):
+        """The rotation's tables (cos, sin) [n_positions, rope.dim / 2] of positions
+        first .. first + n_positions - 1, as dev_paged_append takes them (half layout,
+        whole heads); built on the GPU, into `out` (a pair of such tensors) if given."""
+        import torch
+
+        shape, dev = (n_positions, rope.dim // 2), self.device_id
+        cos, sin = out or (torch.empty(shape, device=f"cuda:{dev}") for _ in range(2))
+        _lib.check(self._L.bnr_dev_rope_scaled_table(
+            self._h, rope._ref, first, n_positions, _on(cos, "cos", torch.float32, dev, shape),
+            _on(sin, "sin", torch.float32, dev, shape), _raw_stream(dev) if stream is None else _stream(stream)))
+        return cos, sin
 
     def dev_synchronize(self, stream=None) -> None:
         _lib.check(self._L.bnr_dev_synchronize(self._h, _stream(stream)))

@@ -2942,3 +2942,408 @@ extern "C" int bnr_dev_paged_decode_attention(bnr_ctx *c, const bnr_paged_kv *kv
           "paged decode launch");
   return set_ok();
 }
+
+// ---------------------------------------------------------------------------
+// Page tables
+// ---------------------------------------------------------------------------
+namespace {
+
+// Whether n bytes at a and m bytes at b share one (NULL: nothing).
+bool overlap(const void *a, size_t n, const void *b, size_t m) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && n && m && x < y + m && y < x + n;
+}
+
+struct Span {
+  const void *at;
+  size_t bytes;
+  const char *name;
+};
+
+// Refuses outputs that overlap each other or an input.
+int check_apart(std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+  for (const Span *o = outs.begin(); o != outs.end(); ++o) {
+    for (const Span *p = o + 1; p != outs.end(); ++p)
+      if (overlap(o->at, o->bytes, p->at, p->bytes))
+        return err_shape(fmt("%s and %s apart", o->name, p->name), "memory that both have");
+    for (const Span &i : ins)
+      if (overlap(o->at, o->bytes, i.at, i.bytes))
+        return err_shape(fmt("%s and %s apart", o->name, i.name), "memory that both have");
+  }
+  return BNR_OK;
+}
+
+int check_pages_table(size_t n_seqs, size_t table_stride, size_t page_size, size_t free_cap) {
+  if (n_seqs > (size_t)kPagesMaxSeqs)
+    return err_shape(fmt("n_seqs <= %d", kPagesMaxSeqs), fmt("n_seqs = %zu", n_seqs));
+  if (page_size == 0 || page_size > kPagedMaxRows)
+    return err_shape(fmt("0 < page_size <= %zu", kPagedMaxRows), fmt("page_size = %zu", page_size));
+  if (table_stride == 0 || table_stride > kPagedMaxRows / page_size)
+    return err_shape(fmt("0 < table_stride * page_size <= %zu", kPagedMaxRows),
+                     fmt("table_stride = %zu, page_size = %zu", table_stride, page_size));
+  return check_paged_count(free_cap, "free_cap");
+}
+
+}  // namespace
+
+extern "C" int bnr_dev_paged_extend(bnr_ctx *c, int32_t *block_table, size_t n_seqs,
+                                    size_t table_stride, size_t page_size, const int32_t *lens,
+                                    const int32_t *new_tokens, const int32_t *free_pages,
+                                    size_t free_cap, const int32_t *free_count, int32_t *seqs,
+                                    int32_t *positions, int64_t *slots, size_t n_tokens,
+                                    int32_t *offsets, int32_t *lens_out, int32_t *free_count_out,
+                                    void *stream) {
+  if (!c) return err_backend("context is NULL");
+  int st = check_pages_table(n_seqs, table_stride, page_size, free_cap);
+  if (!st) st = check_paged_count(n_tokens, "n_tokens");
+  if (st) return st;
+  if ((n_seqs && (!block_table || !lens || !new_tokens || !lens_out)) || (n_tokens && (!seqs || !positions)) ||
+      (free_cap && !free_pages) || !free_count || !offsets || !free_count_out)
+    return err_backend("paged_extend: NULL pointer");
+  const size_t w = sizeof(int32_t), table = n_seqs * table_stride * w;
+  st = check_apart({{seqs, n_tokens * w, "seqs"},
+                    {positions, n_tokens * w, "positions"},
+                    {slots, n_tokens * sizeof(int64_t), "slots"},
+                    {offsets, (n_seqs + 1) * w, "offsets"},
+                    {lens_out, n_seqs * w, "lens_out"},
+                    {free_count_out, w, "free_count_out"},
+                    {block_table, table, "block_table"}},
+                   {{lens, n_seqs * w, "lens"},
+                    {new_tokens, n_seqs * w, "new_tokens"},
+                    {free_pages, free_cap * w, "free_pages"},
+                    {free_count, w, "free_count"}});
+  if (st) return st;
+  ExtendArgs a{};
+  a.table = block_table;
+  a.lens = lens;
+  a.fresh = new_tokens;
+  a.free_pages = free_pages;
+  a.free_count = free_count;
+  a.seqs = seqs;
+  a.positions = positions;
+  a.offsets = offsets;
+  a.lens_out = lens_out;
+  a.count_out = free_count_out;
+  a.slots = (long long *)slots;
+  a.table_stride = (long long)table_stride;
+  a.n_tokens = (long long)n_tokens;
+  a.n_seqs = (int)n_seqs;
+  a.page = (int)page_size;
+  a.free_cap = (int)free_cap;
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_paged_extend(a, (hipStream_t)stream), "paged extend launch");
+  return set_ok();
+}
+
+extern "C" int bnr_dev_paged_release(bnr_ctx *c, int32_t *block_table, size_t n_seqs,
+                                     size_t table_stride, size_t page_size, const int32_t *lens,
+                                     const uint8_t *which, const int32_t *keep,
+                                     int32_t *free_pages, size_t free_cap,
+                                     const int32_t *free_count, int32_t *lens_out,
+                                     int32_t *free_count_out, void *stream) {
+  if (!c) return err_backend("context is NULL");
+  int st = check_pages_table(n_seqs, table_stride, page_size, free_cap);
+  if (st) return st;
+  if ((n_seqs && (!block_table || !lens || !which || !lens_out)) || (free_cap && !free_pages) ||
+      !free_count || !free_count_out)
+    return err_backend("paged_release: NULL pointer");
+  const size_t w = sizeof(int32_t);
+  st = check_apart({{lens_out, n_seqs * w, "lens_out"},
+                    {free_count_out, w, "free_count_out"},
+                    {block_table, n_seqs * table_stride * w, "block_table"},
+                    {free_pages, free_cap * w, "free_pages"}},
+                   {{lens, n_seqs * w, "lens"},
+                    {which, n_seqs, "which"},
+                    {keep, n_seqs * w, "keep"},
+                    {free_count, w, "free_count"}});
+  if (st) return st;
+  ReleaseArgs a{};
+  a.table = block_table;
+  a.lens = lens;
+  a.keep = keep;
+  a.free_count = free_count;
+  a.which = which;
+  a.free_pages = free_pages;
+  a.lens_out = lens_out;
+  a.count_out = free_count_out;
+  a.table_stride = (long long)table_stride;
+  a.n_seqs = (int)n_seqs;
+  a.page = (int)page_size;
+  a.free_cap = (int)free_cap;
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_paged_release(a, (hipStream_t)stream), "paged release launch");
+  return set_ok();
+}
+
+extern "C" int bnr_dev_paged_copy(bnr_ctx *c, const bnr_paged_kv *kv, const int32_t *block_table,
+                                  size_t n_seqs, size_t table_stride, const int32_t *src,
+                                  const int32_t *starts, const int32_t *lens, void *stream) {
+  if (!c) return err_backend("context is NULL");
+  PagedCopyArgs a{};
+  int st = paged_pool(kv, block_table, table_stride, a.pool);
+  if (!st) st = check_paged_batch(n_seqs, kv->n_kv_heads);
+  if (st) return st;
+  if (n_seqs == 0) return set_ok();
+  if (!block_table || !src || !lens) return err_backend("paged_copy: NULL pointer");
+  a.src = src;
+  a.starts = starts;
+  a.lens = lens;
+  a.n_seqs = (int)n_seqs;
+  const size_t d = kv->head_dim;
+  switch (kv->format) {
+    case BNR_KV_F32: a.row_bytes = (int)(4 * d); break;
+    case BNR_KV_BF16: a.row_bytes = (int)(2 * d); break;
+    case BNR_KV_FP4: a.row_bytes = (int)(d / 2); break;
+    default: a.row_bytes = (int)d;
+  }
+  a.scale_bytes = kv->format == BNR_KV_FP4 ? paged_groups4((int)d) : a.pool.k_scales ? (int)sizeof(float) : 0;
+  const uintptr_t bits = (uintptr_t)kv->k | (uintptr_t)kv->v | (uintptr_t)a.row_bytes;
+  const int unit = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_paged_copy(a, unit, (hipStream_t)stream), "paged copy launch");
+  return set_ok();
+}
+
+// ---------------------------------------------------------------------------
+// Beam search
+// ---------------------------------------------------------------------------
+namespace {
+
+constexpr size_t kBeamMaxVocab = (size_t)1 << 30;
+constexpr size_t kBeamMaxRows = (size_t)1 << 20;  // times the parts of a row: under 2^31 workgroups
+
+int check_beams(size_t batch, size_t beams, size_t vocab, size_t k) {
+  if (beams == 0 || beams > (size_t)kMaxBeams)
+    return err_config(fmt("beams must be 1 to %d, got %zu", kMaxBeams, beams));
+  if (vocab == 0 || vocab > kBeamMaxVocab)
+    return err_shape(fmt("0 < vocab <= %zu", kBeamMaxVocab), fmt("vocab = %zu", vocab));
+  if (k == 0 || k > (size_t)kMaxBeams || k > vocab)
+    return err_config(fmt("continuations must be 1 to %zu, got %zu", std::min<size_t>(kMaxBeams, vocab), k));
+  if (batch > kBeamMaxRows / beams)
+    return err_shape(fmt("batch * beams <= %zu", kBeamMaxRows), fmt("batch = %zu, beams = %zu", batch, beams));
+  return BNR_OK;
+}
+
+// Of each part: maximum, sum, the k best and their indexes.
+size_t beam_bytes(size_t batch, size_t beams, size_t vocab, size_t k) {
+  const size_t rows = batch * beams, parts = rows * beam_chunks((long long)rows, (long long)vocab, (int)k);
+  return (parts * (sizeof(double) + sizeof(float) + k * (sizeof(float) + sizeof(int))) + 15) / 16 * 16;
+}
+
+}  // namespace
+
+extern "C" int bnr_beam_workspace(bnr_ctx *c, size_t batch, size_t beams, size_t vocab, size_t k,
+                                  size_t *bytes) {
+  if (!c) return err_backend("context is NULL");
+  if (!bytes) return err_backend("beam_workspace: NULL pointer");
+  const int st = check_beams(batch, beams, vocab, k);
+  if (st) return st;
+  *bytes = batch ? beam_bytes(batch, beams, vocab, k) : 0;
+  return set_ok();
+}
+
+extern "C" int bnr_dev_beam_select(bnr_ctx *c, const float *logits, size_t row_stride, size_t batch,
+                                   size_t beams, size_t vocab, size_t k, const float *scores,
+                                   const uint8_t *done, int32_t eos, int32_t *tokens,
+                                   int32_t *parents, float *scores_out, uint8_t *done_out,
+                                   void *workspace, size_t workspace_bytes, void *stream) {
+  if (!c) return err_backend("context is NULL");
+  int st = check_beams(batch, beams, vocab, k);
+  if (st) return st;
+  if (row_stride < vocab || row_stride > ((size_t)1 << 40))
+    return err_shape(fmt("vocab (%zu) <= row_stride <= 2^40", vocab), fmt("row_stride = %zu", row_stride));
+  if (eos < (done ? 0 : -1) || (eos >= 0 && (size_t)eos >= vocab))
+    return err_config(fmt("eos must be a token%s, got %d", done ? "" : " or -1", eos));
+  if (batch == 0) return set_ok();
+  if (!logits || !scores || !tokens || !parents || !scores_out || !workspace)
+    return err_backend("beam_select: NULL pointer");
+  const size_t need = beam_bytes(batch, beams, vocab, k);
+  if (workspace_bytes < need)
+    return err_shape(fmt("workspace of %zu bytes", need), fmt("%zu bytes", workspace_bytes));
+  if (!aligned16(workspace)) return err_shape("16-byte aligned workspace", "an unaligned pointer");
+  const size_t rows = batch * beams, w = sizeof(int32_t);
+  st = check_apart({{tokens, batch * k * w, "tokens"},
+                    {parents, batch * k * w, "parents"},
+                    {scores_out, batch * k * w, "scores_out"},
+                    {done_out, batch * k, "done_out"},
+                    {workspace, need, "workspace"}},
+                   {{logits, ((rows - 1) * row_stride + vocab) * sizeof(float), "logits"},
+                    {scores, rows * w, "scores"},
+                    {done, rows, "done"}});
+  if (st) return st;
+  BeamArgs a{};
+  a.logits = logits;
+  a.scores = scores;
+  a.done = done;
+  a.tokens = tokens;
+  a.parents = parents;
+  a.scores_out = scores_out;
+  a.done_out = done_out;
+  a.stride = (long long)row_stride;
+  a.batch = (int)batch;
+  a.beams = (int)beams;
+  a.vocab = (int)vocab;
+  a.k = (int)k;
+  a.eos = eos;
+  a.chunks = beam_chunks((long long)rows, (long long)vocab, (int)k);
+  a.chunk = (int)(((vocab + a.chunks - 1) / a.chunks + 3) / 4 * 4);
+  const size_t parts = rows * a.chunks;
+  a.part_sum = (double *)workspace;
+  a.part_max = (float *)(a.part_sum + parts);
+  a.part_val = a.part_max + parts;
+  a.part_idx = (int *)(a.part_val + parts * k);
+  DeviceGuard dg(c->device);
+  const bool vec = aligned16(logits) && row_stride % 4 == 0;
+  HIP_TRY(launch_beam_select(a, vec, (hipStream_t)stream), "beam select launch");
+  return set_ok();
+}
+
+extern "C" int bnr_dev_beam_reorder(bnr_ctx *c, const int32_t *block_table, size_t batch,
+                                    size_t beams, size_t table_stride, const int32_t *parents,
+                                    int32_t *table_out, int32_t *src, void *stream) {
+  if (!c) return err_backend("context is NULL");
+  if (beams == 0 || beams > (size_t)kMaxBeams)
+    return err_config(fmt("beams must be 1 to %d, got %zu", kMaxBeams, beams));
+  if (batch > kBeamMaxRows / beams)
+    return err_shape(fmt("batch * beams <= %zu", kBeamMaxRows), fmt("batch = %zu, beams = %zu", batch, beams));
+  if (table_stride == 0 || table_stride > kPagedMaxRows)
+    return err_shape(fmt("0 < table_stride <= %zu", kPagedMaxRows), fmt("table_stride = %zu", table_stride));
+  if (batch == 0) return set_ok();
+  if (!block_table || !parents || !table_out || !src) return err_backend("beam_reorder: NULL pointer");
+  const size_t rows = batch * beams, w = sizeof(int32_t), table = rows * table_stride * w;
+  const int st = check_apart({{table_out, table, "table_out"}, {src, rows * w, "src"}},
+                             {{block_table, table, "block_table"}, {parents, rows * w, "parents"}});
+  if (st) return st;
+  BeamTableArgs a{};
+  a.table = block_table;
+  a.parents = parents;
+  a.table_out = table_out;
+  a.src = src;
+  a.table_stride = (long long)table_stride;
+  a.batch = (int)batch;
+  a.beams = (int)beams;
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_beam_reorder(a, (hipStream_t)stream), "beam reorder launch");
+  return set_ok();
+}
+
+// ---------------------------------------------------------------------------
+// Rotary embeddings of other forms
+// ---------------------------------------------------------------------------
+namespace {
+
+// The rates as turns a position.
+int rope_turns(const bnr_rope *r, double *turns) {
+  if (!r) return err_backend("rope: NULL rotation");
+  if (r->n_pairs == 0 || r->n_pairs > (size_t)kRopeMaxPairs)
+    return err_config(fmt("a rotation has 1 to %d pairs, got %zu", kRopeMaxPairs, r->n_pairs));
+  if (r->layout != BNR_ROPE_HALF && r->layout != BNR_ROPE_INTERLEAVED)
+    return err_config(fmt("unknown rotary layout %d", r->layout));
+  if (!std::isfinite(r->magnitude)) return err_config("a rotation's magnitude must be finite");
+  if (!r->rates) return err_backend("rope: NULL rates");
+  for (size_t i = 0; i < r->n_pairs; ++i) {
+    // under 2^10 turns a position: a position's are exact to 2^-12 of a turn at the worst
+    if (!(std::fabs(r->rates[i]) <= 4096.0)) return err_config(fmt("rate %zu is not a number up to 4096", i));
+    turns[i] = r->rates[i] / 6.283185307179586476925;
+  }
+  return BNR_OK;
+}
+
+constexpr size_t kRopeMaxStride = (size_t)1 << 40;
+
+// One operand; `extent`: elements from the first to behind the last.
+int rope_heads(const bnr_heads *h, const char *name, size_t n_tokens, size_t d, size_t size, RopeHeads &r) {
+  r = RopeHeads{};
+  if (!h || h->n_heads == 0) return BNR_OK;
+  if (h->n_heads > ((size_t)1 << 24) / d)
+    return err_config(fmt("%s: heads * head_dim must be at most 2^24, got %zu * %zu", name, h->n_heads, d));
+  for (size_t s : {h->in_token, h->in_head, h->out_token, h->out_head})
+    if (s > kRopeMaxStride) return err_shape(fmt("%s: strides up to 2^40", name), fmt("%zu", s));
+  if (n_tokens == 0) return BNR_OK;
+  if (!h->in || !h->out) return err_backend("rope: NULL pointer");
+  if (((uintptr_t)h->in | (uintptr_t)h->out) % size != 0)
+    return err_shape(fmt("%s: pointers aligned to an element", name), "an unaligned pointer");
+  const size_t n = n_tokens - 1, m = h->n_heads - 1;
+  // heads within tokens, or tokens within heads
+  const bool rows = h->out_head >= d || m == 0, cols = h->out_token >= d || n == 0;
+  if (!((rows && (n == 0 || h->out_token >= m * h->out_head + d)) ||
+        (cols && (m == 0 || h->out_head >= n * h->out_token + d))))
+    return err_shape(fmt("%s: output rows of %zu apart", name, d),
+                     fmt("strides %zu and %zu", h->out_token, h->out_head));
+  const size_t in = n * h->in_token + m * h->in_head + d, out = n * h->out_token + m * h->out_head + d;
+  const bool itself = h->in == h->out && (n == 0 || h->in_token == h->out_token) &&
+                      (m == 0 || h->in_head == h->out_head);
+  if (!itself && overlap(h->in, in * size, h->out, out * size))
+    return err_shape(fmt("%s: output in place, or apart from the input", name), "memory that both have");
+  r.in = h->in;
+  r.out = h->out;
+  r.heads = (int)h->n_heads;
+  r.in_token = (long long)h->in_token;
+  r.in_head = (long long)h->in_head;
+  r.out_token = (long long)h->out_token;
+  r.out_head = (long long)h->out_head;
+  return BNR_OK;
+}
+
+// Whether every row starts at a 16-byte boundary.
+bool rope_aligned(const RopeHeads &r, size_t size) {
+  const uintptr_t bits = ((uintptr_t)r.in_token | (uintptr_t)r.in_head | (uintptr_t)r.out_token |
+                          (uintptr_t)r.out_head) * size;
+  return r.heads == 0 || (aligned16(r.in) && aligned16(r.out) && bits % 16 == 0);
+}
+
+}  // namespace
+
+extern "C" int bnr_dev_rope(bnr_ctx *c, const bnr_rope *rope, int type, size_t n_tokens,
+                            size_t head_dim, const int32_t *positions, const bnr_heads *q,
+                            const bnr_heads *k, void *stream) {
+  if (!c) return err_backend("context is NULL");
+  RopeArgs a{};
+  int st = rope_turns(rope, a.turns);
+  if (st) return st;
+  if (type != BNR_TYPE_F32 && type != BNR_TYPE_BF16 && type != BNR_TYPE_F16)
+    return err_config(fmt("unknown type %d", type));
+  if (head_dim < 2 * rope->n_pairs || head_dim > 65536)
+    return err_shape(fmt("%zu <= head_dim <= 65536", 2 * rope->n_pairs), fmt("head_dim = %zu", head_dim));
+  st = check_paged_count(n_tokens, "n_tokens");
+  const size_t size = type == BNR_TYPE_F32 ? 4 : 2;
+  if (!st) st = rope_heads(q, "q", n_tokens, head_dim, size, a.q);
+  if (!st) st = rope_heads(k, "k", n_tokens, head_dim, size, a.k);
+  if (st) return st;
+  if (n_tokens == 0 || a.q.heads + a.k.heads == 0) return set_ok();
+  if (!positions) return err_backend("rope: NULL positions");
+  a.positions = positions;
+  a.n_tokens = (long long)n_tokens;
+  a.d = (int)head_dim;
+  a.pairs = (int)rope->n_pairs;
+  a.magnitude = rope->magnitude;
+  const size_t unit = 16 / size;
+  const bool vec = rope->n_pairs % unit == 0 && head_dim % (2 * unit) == 0 && rope_aligned(a.q, size) &&
+                   rope_aligned(a.k, size);
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_rope(a, type, rope->layout == BNR_ROPE_HALF, vec, (hipStream_t)stream), "rope launch");
+  return set_ok();
+}
+
+extern "C" int bnr_dev_rope_scaled_table(bnr_ctx *c, const bnr_rope *rope, size_t first,
+                                         size_t n_positions, float *cos_out, float *sin_out,
+                                         void *stream) {
+  if (!c) return err_backend("context is NULL");
+  RopeTableArgs a{};
+  const int st = rope_turns(rope, a.turns);
+  if (st) return st;
+  if (n_positions > kPagedMaxRows || first >= kPagedMaxCount)
+    return err_shape(fmt("first < %zu and n_positions <= %zu", kPagedMaxCount, kPagedMaxRows),
+                     fmt("first = %zu, n_positions = %zu", first, n_positions));
+  if (n_positions == 0) return set_ok();
+  if (!cos_out || !sin_out) return err_backend("rope_scaled_table: NULL pointer");
+  a.cos_out = cos_out;
+  a.sin_out = sin_out;
+  a.first = (long long)first;
+  a.n_positions = (long long)n_positions;
+  a.pairs = (int)rope->n_pairs;
+  a.magnitude = rope->magnitude;
+  DeviceGuard dg(c->device);
+  HIP_TRY(launch_rope_table(a, (hipStream_t)stream), "rope table launch");
+  return set_ok();
+}

@@ -790,4 +790,106 @@ constexpr size_t paged_tile(int format, size_t rows, size_t items, size_t wgs) {
   return format == kPagedF32 && rows > 128 && (rows + 63) / 64 * items <= wgs ? 64 : 128;
 }
 
+// ---------------------------------------------------------------------------
+// Rotary embeddings (bnr_rope.hip).
+// ---------------------------------------------------------------------------
+constexpr int kRopeF32 = 0, kRopeBf16 = 1, kRopeF16 = 2;
+constexpr int kRopeMaxPairs = 256;
+// One operand's heads; strides in elements.
+struct RopeHeads {
+  const void *in;
+  void *out;
+  int heads;  // 0: none
+  long long in_token, in_head, out_token, out_head;
+};
+struct RopeArgs {
+  RopeHeads q, k;
+  const int *positions;  // [n_tokens]
+  long long n_tokens;
+  int d, pairs, tokens;  // tokens: of a workgroup, set by the launch
+  float magnitude;
+  double turns[kRopeMaxPairs];  // of a pair, a position
+};
+// vec: rows of 16-byte units, 2 * pairs and d multiples of two of them.
+hipError_t launch_rope(RopeArgs a, int type, bool half, bool vec, hipStream_t s);
+
+struct RopeTableArgs {
+  float *cos_out, *sin_out;  // [n_positions][pairs]
+  long long first, n_positions;
+  int pairs;
+  float magnitude;
+  double turns[kRopeMaxPairs];
+};
+hipError_t launch_rope_table(const RopeTableArgs &a, hipStream_t s);
+
+// ---------------------------------------------------------------------------
+// Page tables (bnr_pages.hip).
+// ---------------------------------------------------------------------------
+constexpr int kPagesMaxSeqs = 4096;  // whose prefix sums a workgroup holds in LDS
+struct ExtendArgs {
+  int *table;  // [n_seqs][table_stride]
+  const int *lens, *fresh, *free_pages, *free_count;
+  int *seqs, *positions, *offsets, *lens_out, *count_out;
+  long long *slots;  // or null
+  long long table_stride, n_tokens;
+  int n_seqs, page, free_cap;
+};
+hipError_t launch_paged_extend(const ExtendArgs &a, hipStream_t s);
+
+struct ReleaseArgs {
+  int *table;
+  const int *lens, *keep, *free_count;  // keep: or null
+  const unsigned char *which;
+  int *free_pages, *lens_out, *count_out;
+  long long table_stride;
+  int n_seqs, page, free_cap;
+};
+hipError_t launch_paged_release(const ReleaseArgs &a, hipStream_t s);
+
+struct BeamTableArgs {
+  const int *table, *parents;
+  int *table_out, *src;
+  long long table_stride;
+  int batch, beams;
+};
+hipError_t launch_beam_reorder(const BeamTableArgs &a, hipStream_t s);
+
+struct PagedCopyArgs {
+  PagedPool pool;
+  const int *src, *starts, *lens;  // starts: or null
+  int n_seqs, row_bytes, scale_bytes;  // of a row's codes and scales
+  int wgs, tile;  // set by the launch
+};
+// unit: bytes of a load, 16, 8, 4, 2 or 1, that divide the rows and the pool's address.
+hipError_t launch_paged_copy(PagedCopyArgs a, int unit, hipStream_t s);
+
+// ---------------------------------------------------------------------------
+// Beam search (bnr_beam.hip).
+// ---------------------------------------------------------------------------
+constexpr int kMaxBeams = 32;      // beams of a request, and continuations
+constexpr int kBeamChunks = 64;    // parts of a row at most: a wave joins their lists
+constexpr int kBeamTile = 4096;    // logits that a workgroup holds in registers
+struct BeamArgs {
+  const float *logits;  // [batch * beams][stride]
+  const float *scores;
+  const unsigned char *done;  // or null
+  int *tokens, *parents;
+  float *scores_out;
+  unsigned char *done_out;  // or null
+  // of each (row, chunk): its maximum and sum, and its k best with their indexes
+  float *part_max, *part_val;
+  double *part_sum;
+  int *part_idx;
+  long long stride;
+  int batch, beams, vocab, k, eos, chunks, chunk;
+};
+// The parts of a row, and their logits (a multiple of 4).
+constexpr int beam_chunks(long long rows, long long vocab, int k) {
+  const long long most = 1024 / k < kBeamChunks ? 1024 / k : kBeamChunks;
+  long long n = (1024 + rows - 1) / rows, room = (vocab + 1023) / 1024;
+  n = n < most ? n : most;
+  return (int)(n < room ? n : room);
+}
+hipError_t launch_beam_select(const BeamArgs &a, bool vec, hipStream_t s);
+
 }  // namespace bnr

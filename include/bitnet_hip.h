@@ -506,6 +506,140 @@ int bnr_dev_paged_decode_attention(bnr_ctx *ctx, const bnr_paged_kv *kv, const f
                                    size_t table_stride, const int32_t *lens, float *out,
                                    void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- Page tables -----------------------------------------------------------
+ * The paged cache's bookkeeping on the device, so that a captured step serves
+ * requests of any length: a stack of free pages, block tables and the arrays
+ * that bnr_dev_paged_append takes.  All integers are the caller's device memory;
+ * at most 4096 sequences a call.  Outputs may not overlap inputs, but for the
+ * block table and the stack, which are changed in place. */
+
+/* Pages and places for new tokens.  Sequence s has lens[s] rows and gets
+ * new_tokens[s] more (values below 0 count as 0): the table entries behind its
+ * ceil(lens / page_size) ones are filled from the stack, free_pages[*free_count
+ * - 1] first, sequence by sequence.  Tokens are numbered sequence by sequence:
+ * token offsets[s] + j is row lens[s] + j of sequence s; seqs, positions and slots
+ * (page * page_size + row in it; may be NULL) say so for each of n_tokens
+ * places, -1 in those that no token has, which bnr_dev_paged_append leaves out.
+ * lens_out[s] = lens[s] + what it got, *free_count_out the pages that are left.
+ * A sequence whose table row has no room gets nothing.  The first sequence for
+ * which the free pages or the n_tokens places do not suffice gets nothing, nor
+ * do those behind it; offsets [n_seqs + 1] tells.  free_cap: entries of
+ * free_pages; a *free_count outside 0..free_cap counts as the nearest.  Pages
+ * are taken from the stack and tables as they are, unchecked: a table's entry
+ * below 0 makes its slots -1. */
+int bnr_dev_paged_extend(bnr_ctx *ctx, int32_t *block_table, size_t n_seqs, size_t table_stride,
+                         size_t page_size, const int32_t *lens, const int32_t *new_tokens,
+                         const int32_t *free_pages, size_t free_cap, const int32_t *free_count,
+                         int32_t *seqs, int32_t *positions, int64_t *slots, size_t n_tokens,
+                         int32_t *offsets, int32_t *lens_out, int32_t *free_count_out,
+                         void *stream);
+
+/* Gives pages back: of each sequence with which[s] != 0 the table entries
+ * keep[s] .. ceil(lens[s] / page_size) - 1 (keep NULL: from 0) go onto the stack
+ * in order and become -1, and lens_out[s] is the rows of those it keeps, min(lens,
+ * keep * page_size); other sequences stay as they are.  `keep` is for pages
+ * that other sequences share.  Entries go onto the stack as they are, unchecked.
+ * A stack of free_cap entries that is too small takes the sequences in order up
+ * to the first that does not fit; that one and those behind it stay. */
+int bnr_dev_paged_release(bnr_ctx *ctx, int32_t *block_table, size_t n_seqs, size_t table_stride,
+                          size_t page_size, const int32_t *lens, const uint8_t *which,
+                          const int32_t *keep, int32_t *free_pages, size_t free_cap,
+                          const int32_t *free_count, int32_t *lens_out, int32_t *free_count_out,
+                          void *stream);
+
+/* Copies rows between sequences of one pool: rows starts[s] .. lens[s]-1 (starts
+ * NULL: from 0) of sequence src[s] to the same rows of sequence s, codes and
+ * scales as they are.  A sequence whose src is outside 0..n_seqs-1 or itself is
+ * left out, and so are rows that both have in one page or that either has no
+ * page for.  A sequence that is copied to may not be copied from in the same
+ * call. */
+int bnr_dev_paged_copy(bnr_ctx *ctx, const bnr_paged_kv *kv, const int32_t *block_table,
+                       size_t n_seqs, size_t table_stride, const int32_t *src,
+                       const int32_t *starts, const int32_t *lens, void *stream);
+
+/* ---- Beam search -----------------------------------------------------------
+ * At most 32 beams a request and 32 continuations. */
+
+/* Bytes of workspace that bnr_dev_beam_select needs; it serves every shape that
+ * needs no more, and holds nothing between calls. */
+int bnr_beam_workspace(bnr_ctx *ctx, size_t batch, size_t beams, size_t vocab, size_t k,
+                       size_t *bytes);
+
+/* Of each request's beams the k best continuations.  logits [batch x beams]
+ * rows of vocab floats, row_stride apart; scores [batch x beams].  A
+ * continuation's score is scores[b] + logit[b][t] - log sum_t exp(logit[b][t]).
+ * Each beam's k largest logits (of equal ones the lowest t) go in: of these
+ * beams * k, the k of highest score in 64 bits go out, the highest first; of
+ * equal ones that of the lowest beam, then of the larger logit, then of the
+ * lowest t: tokens, parents (the beam in its request) and scores_out [batch x
+ * k].  done [batch x beams] (may be NULL): a beam with done != 0 has one
+ * continuation, eos, at its own score; all its others count as -infinity (in
+ * order of t).  done_out [batch x k] (may be NULL): the parent was done, or the
+ * token is eos.  eos: 0..vocab-1, or -1 for none where done is NULL.  A beam
+ * whose score is not finite (done or not), whose logits hold a NaN or +infinity
+ * or are all -infinity has no continuation: its scores are -infinity, its tokens
+ * 0, 1, ...
+ * 1 <= k <= vocab.  `workspace`: device memory, 16-byte aligned; calls that
+ * share one must be ordered.  The same inputs give the same bits on every run. */
+int bnr_dev_beam_select(bnr_ctx *ctx, const float *logits, size_t row_stride, size_t batch,
+                        size_t beams, size_t vocab, size_t k, const float *scores,
+                        const uint8_t *done, int32_t eos, int32_t *tokens, int32_t *parents,
+                        float *scores_out, uint8_t *done_out, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/* The block tables after a selection: sequence b * beams + j goes on from beam
+ * parents[b][j] of its request (a value outside 0..beams-1 counts as j).  Of the
+ * beams with one parent the first gets the parent's table row and src -1; the
+ * others, in order, those of the beams that nothing goes on from, and in src the
+ * sequence whose rows they need: bnr_dev_paged_copy(table_out, src) makes the
+ * caches follow, layer by layer.  The beams of a request have the same length, and
+ * each a page for every row.  table_out [batch * beams x table_stride], src [batch
+ * * beams]; table_out may not overlap block_table. */
+int bnr_dev_beam_reorder(bnr_ctx *ctx, const int32_t *block_table, size_t batch, size_t beams,
+                         size_t table_stride, const int32_t *parents, int32_t *table_out,
+                         int32_t *src, void *stream);
+
+/* ---- Rotary embeddings of other forms ---------------------------------------
+ * Beside bnr_dev_rope_append's half-split rotation of whole heads by theta. */
+#define BNR_ROPE_HALF 0        /* pairs (i, i + n_pairs) */
+#define BNR_ROPE_INTERLEAVED 1 /* pairs (2i, 2i + 1)     */
+typedef struct bnr_rope {
+  const double *rates; /* HOST memory, read during the call: radians a position, of each pair */
+  size_t n_pairs;      /* 1..256: the first 2 * n_pairs elements of a head are rotated */
+  int layout;          /* BNR_ROPE_* */
+  float magnitude;     /* multiplies the rotated values; 1 for a plain rotation */
+} bnr_rope;
+
+/* Types of bnr_dev_rope's operands. */
+#define BNR_TYPE_F32 0
+#define BNR_TYPE_BF16 1
+#define BNR_TYPE_F16 2
+/* Heads of n_tokens tokens: element e of head h of token i lies at in[i *
+ * in_token + h * in_head + e] (strides in elements, so a slice of a fused
+ * projection's output is an operand as it is). */
+typedef struct bnr_heads {
+  const void *in;
+  void *out; /* `in` itself with its strides, or memory that does not overlap its range */
+  size_t n_heads;
+  size_t in_token, in_head, out_token, out_head;
+} bnr_heads;
+
+/* q and k (NULL: none) [n_tokens x heads x head_dim] rotated at positions
+ * (device memory), in fp32 and rounded once to their type; elements from 2 *
+ * n_pairs on are copied.  The angle position * rate is formed in fp64.  A token
+ * with a negative position is left out: its outputs are not written.  Rows of
+ * an output may not overlap. */
+int bnr_dev_rope(bnr_ctx *ctx, const bnr_rope *rope, int type, size_t n_tokens, size_t head_dim,
+                 const int32_t *positions, const bnr_heads *q, const bnr_heads *k, void *stream);
+
+/* The rotation's cos and sin (times magnitude) of positions first .. first +
+ * n_positions - 1, into cos_out and sin_out [n_positions x n_pairs] in device
+ * memory, as bnr_dev_paged_append takes them (half-split pairs, n_pairs =
+ * head_dim / 2; the same rotation as bnr_dev_rope's, to the bit in F32).  Built
+ * on the device: may be captured. */
+int bnr_dev_rope_scaled_table(bnr_ctx *ctx, const bnr_rope *rope, size_t first,
+                              size_t n_positions, float *cos_out, float *sin_out, void *stream);
+
 /* ---- Measurement ---------------------------------------------------------
  * A plain streaming read of two device ranges (a_bytes at a, b_bytes at b;
  * 16-byte aligned, multiples of 16), ordered on `stream`: no counterpart in
