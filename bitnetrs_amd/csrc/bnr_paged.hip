@@ -196,14 +196,16 @@ __global__ __launch_bounds__(64 * kWaves) void paged_append_vec_kernel(PagedAppe
       // the row as eight neighbours a lane; a row's lanes are of one wave
       float4 *row = s_row[threadIdx.x / L];
       wave_order();  // the rows before these have been read
-      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
       if (x < half) {
-        row[x / 4] = in ? lo : zero;
-        row[(half + x) / 4] = in ? hi : zero;
+        row[x / 4] = lo;
+        row[(half + x) / 4] = hi;
       }
       wave_order();
-      const bool there = 2 * x < a.pool.d;
-      const float4 l8 = there ? row[x / 2] : zero, h8 = there ? row[x / 2 + 1] : zero;
+      float4 l8 = make_float4(0.f, 0.f, 0.f, 0.f), h8 = l8;
+      if (2 * x < a.pool.d) {
+        l8 = row[x / 2];
+        h8 = row[x / 2 + 1];
+      }
       // every lane takes part: those past a row's end bring zeros
       store_group4(r, in && !r.out, 2 * x, a.pool.d - 2 * x, l8, h8);
     }

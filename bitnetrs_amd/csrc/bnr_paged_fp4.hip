@@ -25,10 +25,25 @@ namespace {
 
 constexpr int kW = 4;      // waves of a workgroup
 constexpr int kStep = 32;  // rows of a wave's step
+constexpr int kOcc = 2;
 
-// DP: head dim, rounded up to 64, 128 or 256; FULL: head dim is DP.
-template <int DP, bool FULL>
-__global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecodeArgs a) {
+// Sums over the lanes of a DPP row that hold one head's parts, four lanes apart.
+__device__ __forceinline__ float sum_parts(float v) {
+  v += dpp<0x128>(v);  // row_ror:8
+  return v + dpp<0x124>(v);  // row_ror:4
+}
+
+// The power whose exponent is byte (turn - 9) / 8 of w: the conversion reads the
+// exponent's bits of its scale only (checked for all codes and exponents with
+// every other bit set), so the other bytes may stay.
+__device__ __forceinline__ float power_at(unsigned w, unsigned turn) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_alignbit(w, w, turn));
+}
+
+// DP: head dim, rounded up to 64, 128 or 256; FULL: head dim is DP; PACK: at most
+// four heads, the three parts of q and of the weights in columns 4 part + head.
+template <int DP, bool FULL, bool PACK>
+__global__ __launch_bounds__(64 * kW, kOcc) void paged_decode_fp4_kernel(PagedDecodeArgs a) {
   constexpr int E = DP / 16;               // dims of a lane and V row
   constexpr int KL = DP > 128 ? 2 : 1;     // loads of a lane and K tile
   constexpr int KD = DP / 32 / KL;         // dwords of each: 2 (8 bytes) or 4 (16)
@@ -36,17 +51,28 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
   constexpr int QL = DP / 32;              // products of a tile's scores
   // outputs of the waves, as in the other formats' kernel
   extern __shared__ f32x4 s_o[];
-  __shared__ u32x4 s_q[QL * 3 * 64];
+  constexpr int QP = PACK ? 1 : 3;         // operands of a product's q and weights
+  __shared__ u32x4 s_q[QL * QP * 64];
   __shared__ float s_m[kW * kPagedMaxGroup], s_l[kW * kPagedMaxGroup];
   __shared__ JoinShared<kW, 4> s_join;
   const int lane = threadIdx.x & 63, d = FULL ? DP : a.pool.d, G = a.group;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int row = lane & 15, g = lane >> 4;
+  const int head = PACK ? row & 3 : row, part = PACK ? row >> 2 : 0;
+  // V's exponents: of 128 dims the four of a row are a dword, and those of a lane's
+  // four rows 16 bytes; else a byte each.  How far they turn to the exponent's place.
+  constexpr bool kRowExps = FULL && DP == 128;
+  const unsigned v_turn = 9 + (kRowExps ? 8 * (row * E / kPagedGroup4) : 0);
+  // what a weight loses before its part is cut
+  const unsigned cut1 = part >= 1 ? 0xffff0000u : 0u, cut2 = part >= 2 ? 0xffff0000u : 0u;
   const int page = a.pool.page, page_shift = page & (page - 1) ? -1 : __builtin_ctz(page);
   const int groups = paged_groups4(d);
   const unsigned row_bytes = (unsigned)d / 2;
   // the lane's dims of K: KD * 8 of them from KD * 8 * (4 j + g) on, load by load
   const auto k_dim = [&](int j) { return KD * 8 * (4 * j + g); };
+  const auto k_in = [&](int j, int i) { return FULL || k_dim(j) + 8 * i < d; };  // dword i's
+  // the lane's first dim of V; behind the head's end the first ones again, whose outputs go nowhere
+  const int v_dim = FULL || row * E < d ? row * E : 0;
   const int first_len = paged_first_len(a);
   const auto rows = [&](int b) { return paged_len(a.lens[b], a.pool); };
   PagedShare sh = paged_share(rows, a.batch, a.pool.n_kv, a.tile, a.wgs);
@@ -77,9 +103,9 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
 #pragma unroll
     for (int i = 0; i < QC; ++i) {
       const int c = wave + i * kW;
-      const float *q = a.q + ((long long)bs * a.n_heads + (long long)hk * G + row) * d;
+      const float *q = a.q + ((long long)bs * a.n_heads + (long long)hk * G + head) * d;
       const int e0 = k_dim(c / KD) + 8 * (c % KD);
-      const bool in = c < QL && row < G && (FULL || e0 < d);
+      const bool in = c < QL && head < G && (FULL || e0 < d);
 #pragma unroll
       for (int k = 0; k < 2; ++k) qx[i][k] = in ? ld4(q + e0 + 4 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -103,23 +129,23 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
         const unsigned char *exps = a.pool.k_exps + at * groups;
 #pragma unroll
         for (int j = 0; j < KL; ++j) {
-          const unsigned off = row * row_bytes + k_dim(j) / 2;
           unsigned w[KD];
           if constexpr (FULL) {
-            load_bytes<true>(src + off, w);
+            load_bytes<true>(src + row * row_bytes + k_dim(j) / 2, w);
           } else {
-            // a head dim that is a multiple of 16 ends between two halves of 16 bytes
+            // a head dim that is a multiple of 16 ends between two halves of 16 bytes;
+            // those behind it read the row's start (a branch would part the loads)
 #pragma unroll
             for (int i = 0; i < KD; i += 2) {
-              unsigned x[2] = {0u, 0u};
-              if (k_dim(j) + 8 * i < d) load_bytes<true>(src + off + 4 * i, x);
+              unsigned x[2];
+              load_bytes<true>(src + row * row_bytes + (k_in(j, i) ? k_dim(j) / 2 + 4 * i : 0), x);
               w[i] = x[0];
               w[i + 1] = x[1];
             }
           }
 #pragma unroll
           for (int i = 0; i < KD; ++i) kr[h][j * KD + i] = w[i];
-          ke[h][j] = FULL || k_dim(j) < d ? exps[row * groups + k_dim(j) / kPagedGroup4] : 0u;
+          ke[h][j] = exps[row * groups + (k_in(j, 0) ? k_dim(j) / kPagedGroup4 : 0)];
         }
       }
     };
@@ -129,19 +155,19 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
         const long long at = tile_row(pg[h], in[h]);
         const char *src = static_cast<const char *>(a.pool.v) + at * row_bytes;
         const unsigned char *exps = a.pool.v_exps + at * groups;
+        if constexpr (kRowExps) {
+          const u32x4 e = *reinterpret_cast<const u32x4 *>(exps + 16 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ve[h][r] = e[r];
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const char *from = src + (4 * g + r) * row_bytes + row * (E / 2);
-#pragma unroll
-          for (int i = 0; i < VD; ++i) vr[h][r][i] = 0u;
-          ve[h][r] = 0u;
-          if (FULL || row * E < d) {
-            if constexpr (E == 4)
-              vr[h][r][0] = *reinterpret_cast<const unsigned short *>(from);
-            else
-              load_bytes<true>(from, vr[h][r]);
-            ve[h][r] = exps[(4 * g + r) * groups + row * E / kPagedGroup4];
-          }
+          const char *from = src + (4 * g + r) * row_bytes + v_dim / 2;
+          if constexpr (E == 4)
+            vr[h][r][0] = *reinterpret_cast<const unsigned short *>(from);
+          else
+            load_bytes<true>(from, vr[h][r]);
+          if constexpr (!kRowExps) ve[h][r] = exps[(4 * g + r) * groups + v_dim / kPagedGroup4];
         }
       }
     };
@@ -170,8 +196,16 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
       const float4 lo = scale4(a.scale_log2, qx[i][0]), hi = scale4(a.scale_log2, qx[i][1]);
       const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
       const Parts s = split8<true>(x);  // exponents of 253 and 254 make infinities
+      if constexpr (PACK) {
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (part == 0) x = s.p[0];
+        if (part == 1) x = s.p[1];
+        if (part == 2) x = s.p[2];
+        s_q[c * 64 + lane] = x;
+      } else {
 #pragma unroll
-      for (int k = 0; k < 3; ++k) s_q[(c * 3 + k) * 64 + lane] = s.p[k];
+        for (int k = 0; k < 3; ++k) s_q[(c * 3 + k) * 64 + lane] = s.p[k];
+      }
     }
     const unsigned w0 = sh.wg_of(p.item0), w1 = sh.wg_of(p.item1 - 1);
     __syncthreads();  // the operands
@@ -181,36 +215,37 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
     const auto one_step = [&](auto more) {
       constexpr bool kMore = decltype(more)::value;
       const int tn = t + kW * kStep;
-      // Scores: lane has head `row`, rows 4 g + r of both tiles.
+      // Scores: lane has one head, rows 4 g + r of both tiles.
       f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
       int ql = lane;
       asm volatile("" : "+v"(ql));
-      u32x4 qc[3], qn[3];
+      u32x4 qc[QP], qn[QP];
 #pragma unroll
-      for (int k = 0; k < 3; ++k) qn[k] = s_q[k * 64 + ql];
+      for (int k = 0; k < QP; ++k) qn[k] = s_q[k * 64 + ql];
 #pragma unroll
       for (int c = 0; c < QL; ++c) {
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
+        for (int k = 0; k < QP; ++k) {
           qc[k] = qn[k];
-          if (c + 1 < QL) qn[k] = s_q[((c + 1) * 3 + k) * 64 + ql];
+          if (c + 1 < QL) qn[k] = s_q[((c + 1) * QP + k) * 64 + ql];
         }
         __builtin_amdgcn_sched_barrier(0);
         u32x4 w[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const unsigned x = kr[h][c];
-          const float e = power4(ke[h][c / KD]);
+          // q is zero behind the head's end; so are these, whatever the row's start holds
+          const float e = power4(k_in(c / KD, c % KD) ? ke[h][c / KD] : 0u);
           w[h] = u32x4{pair4<0>(x, e), pair4<1>(x, e), pair4<2>(x, e), pair4<3>(x, e)};
         }
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
+        for (int k = 0; k < QP; ++k)
 #pragma unroll
           for (int h = 0; h < 2; ++h) s[h] = mfma_bf16(w[h], qc[k], s[h]);
       }
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3];
+      for (int i = 0; i < 8; ++i) x[i] = PACK ? sum_parts(s[i >> 2][i & 3]) : s[i >> 2][i & 3];
       const bool all = pg[0] >= 0 && pg[1] >= 0 && t + kStep <= row1;
       if (!all)
 #pragma unroll
@@ -252,7 +287,18 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
               for (int i = 0; i < VD; ++i) vr[h][r][i] = 0u;
             }
 
-      const Parts wp = split8<false>(w);
+      Parts wp;
+      if constexpr (PACK) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          w[i] -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, w[i]) & cut1);
+          w[i] -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, w[i]) & cut2);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) wp.p[0][i] = pack_hi(w[2 * i], w[2 * i + 1]);
+      } else {
+        wp = split8<false>(w);
+      }
       // four dims of the lane's 8 rows at a time, as pairs of dims of a row first
 #pragma unroll
       for (int q = 0; q < E / 4; ++q) {
@@ -260,7 +306,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const unsigned x = vr[i >> 2][i & 3][q / 2];
-          const float e = power4(ve[i >> 2][i & 3]);
+          const float e = power_at(ve[i >> 2][i & 3], v_turn);
           two[i][0] = q % 2 ? pair4<2>(x, e) : pair4<0>(x, e);
           two[i][1] = q % 2 ? pair4<3>(x, e) : pair4<1>(x, e);
         }
@@ -272,7 +318,7 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
             c[k] = __builtin_amdgcn_perm(two[2 * k + 1][i / 2], two[2 * k][i / 2],
                                          i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-          for (int k = 0; k < 3; ++k) o[4 * q + i] = mfma_bf16(c, wp.p[k], o[4 * q + i]);
+          for (int k = 0; k < QP; ++k) o[4 * q + i] = mfma_bf16(c, wp.p[k], o[4 * q + i]);
         }
       }
       if constexpr (kMore) {
@@ -297,6 +343,13 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
 
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    if constexpr (PACK) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)  // lanes 0..3 of a row: the parts of their heads
+          o[i][r] = (o[i][r] + dpp<0x104>(o[i][r])) + dpp<0x108>(o[i][r]);
+    }
     if (row < G) {
       if (g == 0) {
         s_m[wave * G + row] = m;
@@ -321,6 +374,14 @@ __global__ __launch_bounds__(64 * kW, 2) void paged_decode_fp4_kernel(PagedDecod
   paged_empty(a, first_len);
 }
 
+template <bool PACK>
+auto kernel_of(int d) {
+  const int dp = paged_dim(d);
+  return dp == 64    ? (d == 64 ? paged_decode_fp4_kernel<64, true, PACK> : paged_decode_fp4_kernel<64, false, PACK>)
+         : dp == 128 ? (d == 128 ? paged_decode_fp4_kernel<128, true, PACK> : paged_decode_fp4_kernel<128, false, PACK>)
+                     : (d == 256 ? paged_decode_fp4_kernel<256, true, PACK> : paged_decode_fp4_kernel<256, false, PACK>);
+}
+
 }  // namespace
 
 hipError_t launch_paged_decode_fp4(const PagedDecodeArgs &a, hipStream_t s) {
@@ -329,9 +390,7 @@ hipError_t launch_paged_decode_fp4(const PagedDecodeArgs &a, hipStream_t s) {
   const dim3 grid((unsigned)a.wgs), block(64 * kW);
   // what a workgroup gets unasked is 64 KB, of which up to 32 are static
   constexpr size_t kUnasked = 32 * 1024;
-  const auto kernel = dp == 64    ? (d == 64 ? paged_decode_fp4_kernel<64, true> : paged_decode_fp4_kernel<64, false>)
-                      : dp == 128 ? (d == 128 ? paged_decode_fp4_kernel<128, true> : paged_decode_fp4_kernel<128, false>)
-                                  : (d == 256 ? paged_decode_fp4_kernel<256, true> : paged_decode_fp4_kernel<256, false>);
+  const auto kernel = a.group <= 4 ? kernel_of<true>(d) : kernel_of<false>(d);
   if (lds > kUnasked) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
