@@ -3124,10 +3124,10 @@ int check_beams(size_t batch, size_t beams, size_t vocab, size_t k) {
   return BNR_OK;
 }
 
-// Of each part: maximum, sum, the k best and their indexes.
+// Of each part: maximum, sum and the k best.
 size_t beam_bytes(size_t batch, size_t beams, size_t vocab, size_t k) {
   const size_t rows = batch * beams, parts = rows * beam_chunks((long long)rows, (long long)vocab, (int)k);
-  return (parts * (sizeof(double) + sizeof(float) + k * (sizeof(float) + sizeof(int))) + 15) / 16 * 16;
+  return (parts * (sizeof(double) + sizeof(float) + k * sizeof(unsigned long long)) + 15) / 16 * 16;
 }
 
 }  // namespace
@@ -3189,9 +3189,8 @@ extern "C" int bnr_dev_beam_select(bnr_ctx *c, const float *logits, size_t row_s
   a.chunk = (int)(((vocab + a.chunks - 1) / a.chunks + 3) / 4 * 4);
   const size_t parts = rows * a.chunks;
   a.part_sum = (double *)workspace;
-  a.part_max = (float *)(a.part_sum + parts);
-  a.part_val = a.part_max + parts;
-  a.part_idx = (int *)(a.part_val + parts * k);
+  a.part_key = (unsigned long long *)(a.part_sum + parts);
+  a.part_max = (float *)(a.part_key + parts * k);
   DeviceGuard dg(c->device);
   const bool vec = aligned16(logits) && row_stride % 4 == 0;
   HIP_TRY(launch_beam_select(a, vec, (hipStream_t)stream), "beam select launch");

@@ -4,7 +4,7 @@
 //   score(b, t) = scores[b] + logit[b, t] - lse[b],   lse = log sum_t exp(logit)
 //
 // Within a beam the order is that of the logits, so one pass over them finds
-// the sum and the k best: a workgroup holds 4096 logits in registers, and what
+// the sum and the k best: a workgroup holds its first logits in registers, and what
 // is under the k-th largest of a wave's 64 lane maxima (at least k logits are
 // no smaller) is not among the k best.  The few that are left are ranked by
 // counting.  A second launch joins the parts of each row and then the beams.
@@ -16,13 +16,18 @@
 // Bound by the logits' bytes, read once.
 #include "bnr_device.h"
 
+#include <algorithm>
+
 namespace bnr {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kHeld = kBeamTile / kThreads;  // logits of a thread
+constexpr int kJoinWaves = 16;
+constexpr int kJoinEntries = 4096;           // of the lists that LDS has room for
 constexpr int kCap = 512;                    // candidates of a tile that LDS has room for
-constexpr int kNone = 0x7fffffff;
+constexpr float kLargest = 3.402823466e38f;  // of fp32
+
+typedef unsigned long long u64;
 
 __device__ __forceinline__ float above(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -33,22 +38,24 @@ __device__ __forceinline__ float exp_from(float x, float m) {
   return fast_exp2(fmaf(d, 1.925963033500e-8f, d * 1.442695021629f));
 }
 
-// Order of a beam's continuations: the larger logit, then the lower index.
-__device__ __forceinline__ bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// A beam's continuations as whole numbers in their order, the larger logit first,
+// then the lower index; 0 is none (a NaN does not come here; -0 counts as 0).
+__device__ __forceinline__ unsigned ordered(float v) {
+  const unsigned b = __builtin_bit_cast(unsigned, v + 0.0f);
+  return b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ u64 key_of(float v, int i) { return (u64)ordered(v) << 32 | ~(unsigned)i; }
+__device__ __forceinline__ float logit_of(u64 key) {
+  const unsigned b = (unsigned)(key >> 32);
+  return __builtin_bit_cast(float, b ^ ((int)b < 0 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ int index_of(u64 key) { return (int)~(unsigned)key; }
 
-struct Best {
-  float v;
-  int i;
-};
-__device__ __forceinline__ Best wave_best(Best x) {
+__device__ __forceinline__ u64 wave_best(u64 x) {
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) {
-    const float v = __shfl_xor(x.v, k);
-    const int i = __shfl_xor(x.i, k);
-    if (better(v, i, x.v, x.i)) {
-      x.v = v;
-      x.i = i;
-    }
+    const u64 y = __shfl_xor(x, k);
+    x = y > x ? y : x;
   }
   return x;
 }
@@ -59,29 +66,67 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-// A workgroup's part of a row.
-template <bool VEC>
+// A workgroup's part of a row, H logits of a thread at a time, the next ones on
+// their way meanwhile.
+template <bool VEC, int H>
 __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
-  __shared__ float s_v[kCap], s_top[kWaves];
-  __shared__ int s_i[kCap], s_n;
+  constexpr int kTile = H * kThreads;
+  __shared__ __attribute__((aligned(16))) u64 s_key[kCap];
+  __shared__ float s_top[kWaves];
+  __shared__ int s_n;
   __shared__ double s_sum[kWaves];
-  __shared__ Best s_best[kWaves];
+  __shared__ u64 s_best[kWaves];
   const int row = blockIdx.x / (unsigned)a.chunks, part = blockIdx.x - row * a.chunks;
   if (a.done && a.done[row]) return;  // the joins know it
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x, k = a.k;
   const float *x = a.logits + row * a.stride;
   const int v0 = part * a.chunk, v1 = min(v0 + a.chunk, a.vocab);
-  float m = -INFINITY, sum = 0.f;
-  int have = 0;  // entries of the list so far: s_v[0..have), the best first
+  float m = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
+  int have = 0;  // candidates so far: s_key[0..have)
+  // What a candidate must reach.  Masked tokens (-infinity) are none: the join
+  // knows which of them fill up.
+  float least = -kLargest;
+  if (tid == 0) s_n = 0;
+  __syncthreads();
+  // The k best of n candidates to the front, in order: a candidate's place is how many are better.
+  const auto rank = [&](int n) {
+    constexpr int kRun = 8;  // keys that are compared at a time, from LDS 16 bytes a load
+    __syncthreads();
+    if (tid < kRun && n + tid < kCap) s_key[n + tid] = 0;  // up to a whole run
+    __syncthreads();
+    int place[kCap / kThreads];
+    u64 mine[kCap / kThreads];
+#pragma unroll
+    for (int c = 0; c < kCap / kThreads; ++c) {
+      const int e = tid + c * kThreads;
+      place[c] = k;
+      if (e >= n) continue;
+      mine[c] = s_key[e];
+      int p = 0;
+      for (int j = 0; j < n; j += kRun) {
+        u64 other[kRun];
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) other[i] = s_key[j + i];
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) p += other[i] > mine[c];
+      }
+      place[c] = p;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kCap / kThreads; ++c)
+      if (place[c] < k) s_key[place[c]] = mine[c];
+    __syncthreads();
+    return n < k ? n : k;
+  };
 
   // Element n of the thread's logits of the tile at t0.
   const auto index = [&](int t0, int n) {
     return VEC ? t0 + 4 * (tid + kThreads * (n / 4)) + n % 4 : t0 + tid + kThreads * n;
   };
-  for (int t0 = v0; t0 < v1; t0 += kBeamTile) {
-    float h[kHeld];
+  const auto load = [&](int t0, float (&h)[H]) {
 #pragma unroll
-    for (int n = 0; n < kHeld; n += VEC ? 4 : 1) {
+    for (int n = 0; n < H; n += VEC ? 4 : 1) {
       const int i = index(t0, n);
       if constexpr (VEC) {  // a part ends at a multiple of 4 or at the row's end
         float4 w = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -97,107 +142,89 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
         h[n] = i < v1 ? x[i] : -INFINITY;
       }
     }
+  };
+  float h[H], next[H];
+  if (v0 < v1) load(v0, next);
+  for (int t0 = v0; t0 < v1; t0 += kTile) {
+#pragma unroll
+    for (int n = 0; n < H; ++n) h[n] = next[n];
+    if (t0 + kTile < v1) load(t0 + kTile, next);
     float top = h[0];
 #pragma unroll
-    for (int n = 1; n < kHeld; ++n) top = fmaxf(top, h[n]);
+    for (int n = 1; n < H; ++n) top = fmaxf(top, h[n]);
     if (!(top > -INFINITY)) top = -INFINITY;  // all NaN
     // places past the end hold -infinity: they add nothing
-    const float mn = fmaxf(m, top), mu = above(mn);
-    sum *= exp_from(above(m) == m ? m : mu, mu);
+    const float mn = fmaxf(m, top), mu = above(mn), keep = exp_from(above(m) == m ? m : mu, mu);
 #pragma unroll
-    for (int n = 0; n < kHeld; ++n) sum += exp_from(h[n], mu);
+    for (int n = 0; n < 4; ++n) sum[n] *= keep;
+#pragma unroll
+    for (int n = 0; n < H; ++n) sum[n % 4] += exp_from(h[n], mu);
     m = mn;
 
-    // What a candidate must reach: the k-th largest lane maximum of some wave, or the list's last entry.
-    float least = -INFINITY;
-    if (have < k) {
-      float v = top;
+    // The k-th largest lane maximum of some wave, of the first tile that has as many finite ones.
+    if (least == -kLargest) {
+      float v = top, kth = -INFINITY;
       for (int r = 0; r < k; ++r) {
-        least = wave_max(v);
-        const int first = __builtin_ctzll(__ballot(v == least));
+        kth = wave_max(v);
+        const int first = __builtin_ctzll(__ballot(v == kth));
         if (lane == first) v = -INFINITY;
       }
-      __syncthreads();  // the list is complete; s_top has been read
-      if (lane == 0) s_top[wave] = least;
-      if (tid == 0) s_n = have;
+      __syncthreads();  // s_top has been read
+      if (lane == 0) s_top[wave] = kth;
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) least = fmaxf(least, s_top[w]);
-    } else {
-      const float last = s_v[k - 1];
-      // later logits have higher indexes: an equal one stays behind
-      if (!__syncthreads_or(top > last)) continue;
-      least = last;
-      if (tid == 0) s_n = have;
-      __syncthreads();
     }
-    const bool full = have == k;
+    int mine = 0;
 #pragma unroll
-    for (int n = 0; n < kHeld; ++n) {
-      const int i = index(t0, n);
-      if (i < v1 && (full ? h[n] > least : h[n] >= least)) {
-        const int at = atomicAdd(&s_n, 1);
-        if (at < kCap) {
-          s_v[at] = h[n];
-          s_i[at] = i;
+    for (int n = 0; n < H; ++n) mine += h[n] >= least;
+    if (mine) {
+      int at = atomicAdd(&s_n, mine);
+#pragma unroll
+      for (int n = 0; n < H; ++n)
+        if (h[n] >= least) {
+          if (at < kCap) s_key[at] = key_of(h[n], index(t0, n));
+          ++at;
         }
-      }
     }
     __syncthreads();
     const int n_cand = s_n;
-    if (n_cand <= kCap) {
-      // a candidate's place is how many are better
-      int place[kCap / kThreads];
-      Best mine[kCap / kThreads];
-#pragma unroll
-      for (int c = 0; c < kCap / kThreads; ++c) {
-        const int e = tid + c * kThreads;
-        place[c] = k;
-        if (e >= n_cand) continue;
-        mine[c] = Best{s_v[e], s_i[e]};
-        int p = 0;
-        for (int j = 0; j < n_cand; ++j) p += better(s_v[j], s_i[j], mine[c].v, mine[c].i);
-        place[c] = p;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < kCap / kThreads; ++c)
-        if (place[c] < k) {
-          s_v[place[c]] = mine[c].v;
-          s_i[place[c]] = mine[c].i;
-        }
-      have = n_cand < k ? n_cand : k;
-    } else {
-      // Too many equal ones: the best that is left, k times.  The old list is
-      // held by the first threads.
-      const Best old = tid < have ? Best{s_v[tid], s_i[tid]} : Best{-INFINITY, kNone};
-      Best last = {INFINITY, -1};
-      have = k;  // there are more than k candidates
+    __syncthreads();  // before another candidate
+    if (n_cand > kCap) {
+      // Too many (equal ones, say): the best that is left, k times.  Those of the
+      // tiles before, no more than threads, are each held by one.
+      const u64 old = tid < have ? s_key[tid] : 0;
+      u64 last = ~0ull;
       for (int r = 0; r < k; ++r) {
-        Best b = {-INFINITY, kNone};
-        if (better(last.v, last.i, old.v, old.i) && better(old.v, old.i, b.v, b.i)) b = old;
+        u64 best = old < last ? old : 0;
 #pragma unroll
-        for (int n = 0; n < kHeld; ++n) {
-          const int i = index(t0, n);
-          if (i < v1 && better(last.v, last.i, h[n], i) && better(h[n], i, b.v, b.i)) b = Best{h[n], i};
+        for (int n = 0; n < H; ++n) {
+          const u64 key = h[n] >= least ? key_of(h[n], index(t0, n)) : 0;
+          best = key < last && key > best ? key : best;
         }
-        b = wave_best(b);
-        __syncthreads();  // s_best and, the first time, the old list have been read
-        if (lane == 0) s_best[wave] = b;
+        best = wave_best(best);
+        __syncthreads();  // s_best and, the first time, the old ones have been read
+        if (lane == 0) s_best[wave] = best;
         __syncthreads();
-        b = s_best[0];
+        last = s_best[0];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w)
-          if (better(s_best[w].v, s_best[w].i, b.v, b.i)) b = s_best[w];
-        last = b;
-        if (tid == 0) {
-          s_v[r] = b.v;
-          s_i[r] = b.i;
-        }
+        for (int w = 1; w < kWaves; ++w) last = s_best[w] > last ? s_best[w] : last;
+        if (tid == 0) s_key[r] = last;
       }
+      have = k;  // there were more than k
+    } else {
+      have = n_cand;
+      if (have > kThreads) have = rank(have);
     }
-    __syncthreads();  // the list
+    if (have != n_cand) {
+      // the k best so far: later logits have higher indexes, so only the next larger float
+      // is a candidate (above the largest, infinity: such a row has no continuation)
+      if (tid == 0) s_n = have;
+      __syncthreads();
+      least = logit_of((s_key[k - 1] | 0xffffffffull) + 1);
+    }
   }
+  have = rank(have);
 
   // the part's maximum and sum
   const float wm = wave_max(m);
@@ -206,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
   float top = s_top[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_top[w]);
-  const double ws = wave_sum64((double)sum * (double)exp_from(above(m) == m ? m : above(top), above(top)));
+  const double ws = wave_sum64((((double)sum[0] + sum[1]) + ((double)sum[2] + sum[3])) * (double)exp_from(above(m) == m ? m : above(top), above(top)));
   if (lane == 0) s_sum[wave] = ws;
   __syncthreads();
   const long long at = (long long)row * a.chunks + part;
@@ -214,27 +241,44 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
     a.part_max[at] = top;
     a.part_sum[at] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
   }
-  if (tid < k) {
-    a.part_val[at * k + tid] = tid < have ? s_v[tid] : -INFINITY;
-    a.part_idx[at * k + tid] = tid < have ? s_i[tid] : kNone;
-  }
+  if (tid < k) a.part_key[at * k + tid] = tid < have ? s_key[tid] : 0;
+}
+
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+#define BNR_MAX(CTRL) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false))
+  BNR_MAX(0xB1);   // quad_perm [1,0,3,2]
+  BNR_MAX(0x4E);   // quad_perm [2,3,0,1]
+  BNR_MAX(0x141);  // row_half_mirror
+  BNR_MAX(0x140);  // row_mirror
+#undef BNR_MAX
+  const auto of = [&](int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); };
+  return max(max(of(0), of(16)), max(of(32), of(48)));
+}
+
+// A double as a whole number of the same order (no NaN comes here; -0 is not made).
+__device__ __forceinline__ u64 ordered(double v) {
+  const long long b = __builtin_bit_cast(long long, v);
+  return (u64)b ^ (u64)(b < 0 ? -1ll : (long long)(1ull << 63));
 }
 
 // Joins the parts of each beam's row, a wave for each, and then the request's
-// beams: lane c has part (beam) c's list and the best of them that is not taken.
-__global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
+// beams: lane c has part (beam) c's list and its best that is not taken.  The
+// largest of the wave's comes from one reduction; of equal ones the lowest
+// lane's has the lowest index.
+__global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a) {
   __shared__ double s_y[kMaxBeams * kMaxBeams];
   __shared__ int s_t[kMaxBeams * kMaxBeams];
-  extern __shared__ Best s_list[];  // [kWaves][chunks * k]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = a.k;
+  extern __shared__ u64 s_list[];  // [waves][chunks * k]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, k = a.k;
   const long long b = blockIdx.x;
-  Best *list = s_list + wave * a.chunks * k;
-  for (int beam = wave; beam < a.beams; beam += kWaves) {
+  u64 *list = s_list + wave * a.chunks * k;
+  for (int beam = wave; beam < a.beams; beam += waves) {
     const long long row = b * a.beams + beam;
-    const double base = (double)a.scores[row];
+    const double base = (double)a.scores[row] + 0.0;  // no -0
     double *y = s_y + beam * k;
     int *t = s_t + beam * k;
-    if (a.done && a.done[row] && fabs(base) < INFINITY) {
+    const bool ended = a.done && a.done[row];  // its parts have not been made
+    if (ended && fabs(base) < INFINITY) {
       // an ended beam goes on with the end's token alone
       if (lane < k) {
         y[lane] = lane == 0 ? base : -INFINITY;
@@ -242,12 +286,11 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
       }
       continue;
     }
-    const bool ended = a.done && a.done[row];  // its parts have not been made
     const long long at = row * a.chunks;
     const int parts = ended ? 0 : a.chunks;
     const float m = lane < parts ? a.part_max[at + lane] : -INFINITY;
     const double s = lane < parts ? a.part_sum[at + lane] : 0.0;
-    for (int e = lane; e < parts * k; e += 64) list[e] = Best{a.part_val[at * k + e], a.part_idx[at * k + e]};
+    for (int e = lane; e < parts * k; e += 64) list[e] = a.part_key[at * k + e];
     const float top = wave_max(m);
     const double sum = wave_sum64(s == 0.0 ? 0.0 : s * exp((double)m - (double)top));
     const double lse = (double)top + log(sum);
@@ -262,62 +305,87 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(BeamArgs a) {
       continue;
     }
     int head = 0;
-    Best mine = lane < parts ? list[lane * k] : Best{-INFINITY, kNone};
-    for (int r = 0; r < k; ++r) {
-      const Best w = wave_best(mine);
-      if (lane == 0) {
-        y[r] = base + ((double)w.v - lse);
-        t[r] = w.i;
-      }
-      if (mine.i == w.i && lane < parts) {  // indexes of a row are all different
+    u64 mine = lane < parts ? list[lane * k] : 0;
+    int r = 0;
+    for (; r < k; ++r) {
+      const unsigned v = wave_umax((unsigned)(mine >> 32));
+      if (v == 0) break;
+      const int first = __builtin_ctzll(__ballot((unsigned)(mine >> 32) == v));
+      if (lane == first) {
+        y[r] = base + ((double)logit_of(mine) - lse);
+        t[r] = index_of(mine);
         ++head;
-        mine = head < k ? list[lane * k + head] : Best{-INFINITY, kNone};
+        mine = head < k ? list[lane * k + head] : 0;
+      }
+    }
+    if (r < k) {
+      // All other tokens are masked: the lowest of them, of the first 64 (r < k <= 32
+      // are taken, and k <= vocab).
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      bool there = lane < a.vocab;
+      for (int i = 0; i < r; ++i) there = there && t[i] != lane;
+      const u64 masked = __ballot(there);
+      const int place = r + __builtin_popcountll(masked & ((1ull << lane) - 1));
+      __builtin_amdgcn_wave_barrier();
+      if (there && place < k) {
+        y[place] = -INFINITY;
+        t[place] = lane;
       }
     }
   }
   __syncthreads();
   if (wave != 0) return;
-  int head = 0;
-  const bool in = lane < a.beams;
-  double y = in ? s_y[lane * k] : -INFINITY;
+  // Lane b has beam b's list; where none is left, 0, which is less than -infinity's number.
+  int head = 0, token = 0;
+  double y = 0.0;
+  u64 key = 0;
+  const auto take = [&] {
+    const bool there = lane < a.beams && head < k;
+    y = there ? s_y[lane * k + head] : 0.0;
+    token = there ? s_t[lane * k + head] : 0;
+    key = there ? ordered(y) : 0;
+  };
+  take();
   for (int r = 0; r < k; ++r) {
-    // the largest score, of equal ones the first beam's; one without an entry left is behind all
-    double best = y;
-    int who = in && head < k ? lane : 64 + lane;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const double v = __shfl_xor(best, o);
-      const int w = __shfl_xor(who, o);
-      const bool there = w < 64, here = who < 64;
-      if (there && (!here || v > best || (v == best && w < who))) {
-        best = v;
-        who = w;
-      }
-    }
-    if (lane == who) {
+    const unsigned hi = wave_umax((unsigned)(key >> 32));
+    const unsigned lo = wave_umax((unsigned)(key >> 32) == hi ? (unsigned)key : 0u);
+    const int first = __builtin_ctzll(__ballot(key == ((u64)hi << 32 | lo)));
+    if (lane == first) {
       const long long to = b * k + r;
-      const int token = s_t[lane * k + head];
       a.tokens[to] = token;
       a.parents[to] = lane;
       a.scores_out[to] = (float)y;
       if (a.done_out) a.done_out[to] = (a.done && a.done[b * a.beams + lane]) || token == a.eos;
       ++head;
-      if (head < k) y = s_y[lane * k + head];
+      take();
     }
   }
+}
+
+template <bool VEC>
+void launch_rows(const BeamArgs &a, hipStream_t s) {
+  const unsigned grid = (unsigned)a.batch * (unsigned)a.beams * (unsigned)a.chunks;
+  // registers for a part's logits, or for 16 of a thread at a time
+  if (a.chunk <= 4 * kThreads)
+    beam_rows_kernel<VEC, 4><<<grid, kThreads, 0, s>>>(a);
+  else if (a.chunk <= 8 * kThreads)
+    beam_rows_kernel<VEC, 8><<<grid, kThreads, 0, s>>>(a);
+  else
+    beam_rows_kernel<VEC, 16><<<grid, kThreads, 0, s>>>(a);
 }
 
 }  // namespace
 
 hipError_t launch_beam_select(const BeamArgs &a, bool vec, hipStream_t s) {
-  const unsigned grid = (unsigned)a.batch * (unsigned)a.beams * (unsigned)a.chunks;
   if (vec)
-    beam_rows_kernel<true><<<grid, kThreads, 0, s>>>(a);
+    launch_rows<true>(a, s);
   else
-    beam_rows_kernel<false><<<grid, kThreads, 0, s>>>(a);
+    launch_rows<false>(a, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  beam_join_kernel<<<(unsigned)a.batch, kThreads, (size_t)kWaves * a.chunks * a.k * sizeof(Best), s>>>(a);
+  const int most = std::min(kJoinWaves, kJoinEntries / (a.chunks * a.k)), waves = std::min(a.beams, most);
+  beam_join_kernel<<<(unsigned)a.batch, 64 * waves, (size_t)waves * a.chunks * a.k * sizeof(u64), s>>>(a);
   return hipGetLastError();
 }
 

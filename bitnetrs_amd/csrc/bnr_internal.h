@@ -868,7 +868,6 @@ hipError_t launch_paged_copy(PagedCopyArgs a, int unit, hipStream_t s);
 // ---------------------------------------------------------------------------
 constexpr int kMaxBeams = 32;      // beams of a request, and continuations
 constexpr int kBeamChunks = 64;    // parts of a row at most: a wave joins their lists
-constexpr int kBeamTile = 4096;    // logits that a workgroup holds in registers
 struct BeamArgs {
   const float *logits;  // [batch * beams][stride]
   const float *scores;
@@ -876,10 +875,10 @@ struct BeamArgs {
   int *tokens, *parents;
   float *scores_out;
   unsigned char *done_out;  // or null
-  // of each (row, chunk): its maximum and sum, and its k best with their indexes
-  float *part_max, *part_val;
+  // of each (row, chunk): its maximum and sum, and its k best
+  float *part_max;
   double *part_sum;
-  int *part_idx;
+  unsigned long long *part_key;
   long long stride;
   int batch, beams, vocab, k, eos, chunks, chunk;
 };
