@@ -24,7 +24,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kJoinWaves = 16;
 constexpr int kJoinEntries = 4096;           // of the lists that LDS has room for
-constexpr int kCap = 512;                    // candidates of a tile that LDS has room for
+constexpr int kCap = 128;                    // candidates of a wave that LDS has room for
 constexpr float kLargest = 3.402823466e38f;  // of fp32
 
 typedef unsigned long long u64;
@@ -60,65 +60,72 @@ __device__ __forceinline__ u64 wave_best(u64 x) {
   return x;
 }
 
+// What a wave wrote to LDS is there for its other lanes: LDS works in order, so
+// only the compiler has to keep the order.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ int lanes_below(u64 mask) {
+  return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const u64 b = __builtin_bit_cast(u64, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, 0xF, 0xF, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (u64)hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp64<0xB1>(v);   // quad_perm [1,0,3,2]
+  v += dpp64<0x4E>(v);   // quad_perm [2,3,0,1]
+  v += dpp64<0x141>(v);  // row_half_mirror
+  v += dpp64<0x140>(v);  // row_mirror
+  const auto of = [&](int lane) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    return __builtin_bit_cast(double, (u64)(unsigned)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 |
+                                          (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, lane));
+  };
+  return (of(0) + of(16)) + (of(32) + of(48));
+}
+
+// How many of the n keys in LDS are larger than this one: eight at a time, 16
+// bytes a load; behind them are zeros up to a multiple of eight.
+__device__ __forceinline__ int larger(const u64 *keys, int n, u64 key) {
+  int p = 0;
+  for (int j = 0; j < n; j += 8) {
+    u64 other[8];
 #pragma unroll
-  for (int k = 1; k < 64; k *= 2) v += __shfl_xor(v, k);
-  return v;
+    for (int i = 0; i < 8; ++i) other[i] = keys[j + i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p += other[i] > key;
+  }
+  return p;
 }
 
 // A workgroup's part of a row, H logits of a thread at a time, the next ones on
-// their way meanwhile.
+// their way meanwhile.  After the first logits, whose threads' maxima give the
+// threshold, the waves work by themselves until the end.
 template <bool VEC, int H>
 __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
   constexpr int kTile = H * kThreads;
-  __shared__ __attribute__((aligned(16))) u64 s_key[kCap];
-  __shared__ float s_top[kWaves];
-  __shared__ int s_n;
+  __shared__ __attribute__((aligned(16))) u64 s_cand[kWaves][kCap + 8];
+  __shared__ float s_best[kWaves], s_top[kWaves];
+  __shared__ int s_have[kWaves];
   __shared__ double s_sum[kWaves];
-  __shared__ u64 s_best[kWaves];
   const int row = blockIdx.x / (unsigned)a.chunks, part = blockIdx.x - row * a.chunks;
-  if (a.done && a.done[row]) return;  // the joins know it
+  const bool ended = a.done && a.done[row];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x, k = a.k;
   const float *x = a.logits + row * a.stride;
   const int v0 = part * a.chunk, v1 = min(v0 + a.chunk, a.vocab);
   float m = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
-  int have = 0;  // candidates so far: s_key[0..have)
-  // What a candidate must reach.  Masked tokens (-infinity) are none: the join
+  u64 *cand = s_cand[wave];
+  int have = 0;  // candidates so far, the same in all lanes
+  // What a candidate must reach: at least k of the workgroup's do.  Masked tokens (-infinity) are none: the join
   // knows which of them fill up.
   float least = -kLargest;
-  if (tid == 0) s_n = 0;
-  __syncthreads();
-  // The k best of n candidates to the front, in order: a candidate's place is how many are better.
-  const auto rank = [&](int n) {
-    constexpr int kRun = 8;  // keys that are compared at a time, from LDS 16 bytes a load
-    __syncthreads();
-    if (tid < kRun && n + tid < kCap) s_key[n + tid] = 0;  // up to a whole run
-    __syncthreads();
-    int place[kCap / kThreads];
-    u64 mine[kCap / kThreads];
-#pragma unroll
-    for (int c = 0; c < kCap / kThreads; ++c) {
-      const int e = tid + c * kThreads;
-      place[c] = k;
-      if (e >= n) continue;
-      mine[c] = s_key[e];
-      int p = 0;
-      for (int j = 0; j < n; j += kRun) {
-        u64 other[kRun];
-#pragma unroll
-        for (int i = 0; i < kRun; ++i) other[i] = s_key[j + i];
-#pragma unroll
-        for (int i = 0; i < kRun; ++i) p += other[i] > mine[c];
-      }
-      place[c] = p;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < kCap / kThreads; ++c)
-      if (place[c] < k) s_key[place[c]] = mine[c];
-    __syncthreads();
-    return n < k ? n : k;
-  };
 
   // Element n of the thread's logits of the tile at t0.
   const auto index = [&](int t0, int n) {
@@ -145,6 +152,7 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
   };
   float h[H], next[H];
   if (v0 < v1) load(v0, next);
+  if (ended) return;  // the join knows it (asked before the loads, that it be here with them)
   for (int t0 = v0; t0 < v1; t0 += kTile) {
 #pragma unroll
     for (int n = 0; n < H; ++n) h[n] = next[n];
@@ -161,39 +169,50 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
     for (int n = 0; n < H; ++n) sum[n % 4] += exp_from(h[n], mu);
     m = mn;
 
-    // The k-th largest lane maximum of some wave, of the first tile that has as many finite ones.
-    if (least == -kLargest) {
-      float v = top, kth = -INFINITY;
-      for (int r = 0; r < k; ++r) {
-        kth = wave_max(v);
-        const int first = __builtin_ctzll(__ballot(v == kth));
+    // The first tile's threshold: of each wave's lane maxima the n-th largest, n
+    // a quarter of k or more, and of these the least.  (The k-th of all 256 leaves
+    // half as many candidates and costs four times the rounds.)
+    if (t0 == v0) {
+      float v = top, nth = -INFINITY;
+      for (int r = 0; r < k; r += kWaves) {
+        nth = wave_max(v);
+        const int first = __builtin_ctzll(__ballot(v == nth));
         if (lane == first) v = -INFINITY;
       }
-      __syncthreads();  // s_top has been read
-      if (lane == 0) s_top[wave] = kth;
+      if (lane == 0) s_best[wave] = nth;
       __syncthreads();
+      nth = s_best[0];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) least = fmaxf(least, s_top[w]);
+      for (int w = 1; w < kWaves; ++w) nth = fminf(nth, s_best[w]);
+      least = fmaxf(least, nth);
     }
-    int mine = 0;
+    if (!__any(top >= least)) continue;
+    const int before = have;
 #pragma unroll
-    for (int n = 0; n < H; ++n) mine += h[n] >= least;
-    if (mine) {
-      int at = atomicAdd(&s_n, mine);
-#pragma unroll
-      for (int n = 0; n < H; ++n)
-        if (h[n] >= least) {
-          if (at < kCap) s_key[at] = key_of(h[n], index(t0, n));
-          ++at;
-        }
+    for (int n = 0; n < H; ++n) {
+      const u64 in = __ballot(h[n] >= least);
+      if (in == 0) continue;
+      const int at = have + lanes_below(in);
+      if (h[n] >= least && at < kCap) cand[at] = key_of(h[n], index(t0, n));
+      have += __builtin_popcountll(in);
     }
-    __syncthreads();
-    const int n_cand = s_n;
-    __syncthreads();  // before another candidate
-    if (n_cand > kCap) {
+    if (have <= 64) continue;
+    if (have <= kCap) {
+      if (lane < 8) cand[have + lane] = 0;
+      wave_order();
+      const u64 mine[2] = {cand[lane], 64 + lane < have ? cand[64 + lane] : 0};
+      const int place[2] = {larger(cand, have, mine[0]), larger(cand, have, mine[1])};
+      wave_order();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (place[i] < k && mine[i]) cand[place[i]] = mine[i];
+      have = k;
+    } else {
       // Too many (equal ones, say): the best that is left, k times.  Those of the
-      // tiles before, no more than threads, are each held by one.
-      const u64 old = tid < have ? s_key[tid] : 0;
+      // tiles before, 64 at most, are held by a lane each.
+      wave_order();
+      const u64 old = lane < before ? cand[lane] : 0;
+      wave_order();
       u64 last = ~0ull;
       for (int r = 0; r < k; ++r) {
         u64 best = old < last ? old : 0;
@@ -202,46 +221,48 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
           const u64 key = h[n] >= least ? key_of(h[n], index(t0, n)) : 0;
           best = key < last && key > best ? key : best;
         }
-        best = wave_best(best);
-        __syncthreads();  // s_best and, the first time, the old ones have been read
-        if (lane == 0) s_best[wave] = best;
-        __syncthreads();
-        last = s_best[0];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) last = s_best[w] > last ? s_best[w] : last;
-        if (tid == 0) s_key[r] = last;
+        last = wave_best(best);
+        if (lane == 0) cand[r] = last;
       }
       have = k;  // there were more than k
-    } else {
-      have = n_cand;
-      if (have > kThreads) have = rank(have);
     }
-    if (have != n_cand) {
-      // the k best so far: later logits have higher indexes, so only the next larger float
-      // is a candidate (above the largest, infinity: such a row has no continuation)
-      if (tid == 0) s_n = have;
-      __syncthreads();
-      least = logit_of((s_key[k - 1] | 0xffffffffull) + 1);
-    }
+    // the k best so far: later logits have higher indexes, so only the next larger float
+    // is a candidate (above the largest, infinity: such a row has no continuation)
+    wave_order();
+    least = logit_of((cand[k - 1] | 0xffffffffull) + 1);
   }
-  have = rank(have);
-
-  // the part's maximum and sum
+  // The part's k best: a candidate's place is how many of all waves' are larger.
   const float wm = wave_max(m);
-  if (lane == 0) s_top[wave] = wm;
+  const double ws = wave_sum64((((double)sum[0] + sum[1]) + ((double)sum[2] + sum[3])) *
+                               (double)exp_from(above(m) == m ? m : above(wm), above(wm)));
+  if (lane < 8) cand[have + lane] = 0;
+  if (lane == 0) {
+    s_top[wave] = wm;
+    s_sum[wave] = ws;
+    s_have[wave] = have;
+  }
   __syncthreads();
+  const long long at = (long long)row * a.chunks + part;
+  const u64 mine = lane < have ? cand[lane] : 0;
+  int place = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const int n = s_have[w];
+    place += larger(s_cand[w], n, mine);
+    all += n;
+  }
+  if (mine && place < k) a.part_key[at * k + place] = mine;
+  if (tid >= all && tid < k) a.part_key[at * k + tid] = 0;
+  if (tid != 0) return;
   float top = s_top[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_top[w]);
-  const double ws = wave_sum64((((double)sum[0] + sum[1]) + ((double)sum[2] + sum[3])) * (double)exp_from(above(m) == m ? m : above(top), above(top)));
-  if (lane == 0) s_sum[wave] = ws;
-  __syncthreads();
-  const long long at = (long long)row * a.chunks + part;
-  if (tid == 0) {
-    a.part_max[at] = top;
-    a.part_sum[at] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-  }
-  if (tid < k) a.part_key[at * k + tid] = tid < have ? s_key[tid] : 0;
+  double total = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    total += s_sum[w] * (double)exp_from(above(s_top[w]) == s_top[w] ? s_top[w] : above(top), above(top));
+  a.part_max[at] = top;
+  a.part_sum[at] = total;
 }
 
 __device__ __forceinline__ unsigned wave_umax(unsigned v) {
@@ -294,8 +315,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a) 
     const float top = wave_max(m);
     const double sum = wave_sum64(s == 0.0 ? 0.0 : s * exp((double)m - (double)top));
     const double lse = (double)top + log(sum);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
     if (!(fabs(base) < INFINITY) || !(fabs(lse) < INFINITY)) {
       // no continuation of its own: the first tokens, behind all others
       if (lane < k) {
@@ -321,13 +341,12 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a) 
     if (r < k) {
       // All other tokens are masked: the lowest of them, of the first 64 (r < k <= 32
       // are taken, and k <= vocab).
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      wave_order();
       bool there = lane < a.vocab;
       for (int i = 0; i < r; ++i) there = there && t[i] != lane;
       const u64 masked = __ballot(there);
       const int place = r + __builtin_popcountll(masked & ((1ull << lane) - 1));
-      __builtin_amdgcn_wave_barrier();
+      wave_order();
       if (there && place < k) {
         y[place] = -INFINITY;
         t[place] = lane;
