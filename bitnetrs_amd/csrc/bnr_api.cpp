@@ -3030,6 +3030,7 @@ extern "C" int bnr_dev_paged_extend(bnr_ctx *c, int32_t *block_table, size_t n_s
   a.n_seqs = (int)n_seqs;
   a.page = (int)page_size;
   a.free_cap = (int)free_cap;
+  a.vec = aligned16(seqs) && aligned16(positions) && aligned16(slots);
   DeviceGuard dg(c->device);
   HIP_TRY(launch_paged_extend(a, (hipStream_t)stream), "paged extend launch");
   return set_ok();

@@ -806,7 +806,8 @@ struct RopeArgs {
   RopeHeads q, k;
   const int *positions;  // [n_tokens]
   long long n_tokens;
-  int d, pairs, tokens;  // tokens: of a workgroup, set by the launch
+  int d, pairs;
+  int tokens, lanes;  // of a workgroup, of a row; set by the launch
   float magnitude;
   double turns[kRopeMaxPairs];  // of a pair, a position
 };
@@ -833,6 +834,7 @@ struct ExtendArgs {
   long long *slots;  // or null
   long long table_stride, n_tokens;
   int n_seqs, page, free_cap;
+  bool vec;  // seqs, positions and slots 16-byte aligned
 };
 hipError_t launch_paged_extend(const ExtendArgs &a, hipStream_t s);
 

@@ -12,31 +12,15 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 
 typedef unsigned long long u64;
 
-// Inclusive sums of two values over a workgroup's threads.
-struct Two {
-  u64 a, b;
+// Rows of a page as a divisor; the shift where it is a power of two.
+struct PageSize {
+  int rows, shift;
+  __device__ __forceinline__ explicit PageSize(int page)
+      : rows(page), shift(page & (page - 1) ? -1 : __builtin_ctz((unsigned)page)) {}
+  __device__ __forceinline__ int of(int row) const { return shift >= 0 ? row >> shift : row / rows; }
+  // pages of n rows; n + rows <= 2^31
+  __device__ __forceinline__ int pages(int n) const { return of(n + rows - 1); }
 };
-__device__ __forceinline__ Two block_scan(Two v, Two *s_wave) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) {
-    const u64 a = __shfl_up(v.a, k), b = __shfl_up(v.b, k);
-    if (lane >= k) {
-      v.a += a;
-      v.b += b;
-    }
-  }
-  __syncthreads();  // the sums before these have been read
-  if (lane == 63) s_wave[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    v.a += s_wave[w].a;
-    v.b += s_wave[w].b;
-  }
-  return v;
-}
-
-__device__ __forceinline__ int pages_of(long long rows, int page) { return (int)((rows + page - 1) / page); }
 
 // The sequence whose part of the line off[0..n] has place x: off[s] <= x < off[s + 1].
 __device__ __forceinline__ int part_of(const int *off, int n, int x) {
@@ -51,105 +35,155 @@ __device__ __forceinline__ int part_of(const int *off, int n, int x) {
   return lo;
 }
 
+// Sums that stay at 2^32 - 1: more than any limit.
+__device__ __forceinline__ unsigned sat(unsigned a, unsigned b) { return __builtin_elementwise_add_sat(a, b); }
+
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ unsigned scan_sat(unsigned v) {
+#define BNR_SCAN(CTRL, ROWS) v = sat(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false))
+  BNR_SCAN(0x111, 0xF);  // row_shr:1, 2, 4, 8: sums within each row of 16 lanes
+  BNR_SCAN(0x112, 0xF);
+  BNR_SCAN(0x114, 0xF);
+  BNR_SCAN(0x118, 0xF);
+  BNR_SCAN(0x142, 0xA);  // row_bcast:15 into rows 1 and 3
+  BNR_SCAN(0x143, 0xC);  // row_bcast:31 into rows 2 and 3
+#undef BNR_SCAN
+  return v;
+}
+
 // Every workgroup adds up the whole batch for itself, so that one launch does
 // it all and nothing is kept between launches: two loads a sequence, from L2.
-// want(s): the sequence's two amounts; keep(s, first, taken): what precedes it on
-// the two lines, and whether it has its place.  In order, up to the first
-// sequence that goes past a limit: it and those behind it get nothing.
+// want(s, a, b): the sequence's two amounts.  Leaves in line_a and line_b
+// [n_seqs + 1] (LDS) what each sequence's parts of the two lines start at.  In order,
+// up to the first sequence that goes past a limit: it and those behind it get nothing.
 struct Shares {
-  Two wave[kWaves];
-  Two stop;
-  int stopped;
+  unsigned wave[kWaves][2], stop[2];
 };
-template <class Want, class Keep>
-__device__ __forceinline__ Two share_out(int n_seqs, u64 limit_a, u64 limit_b, Shares &sh, Want want, Keep keep) {
-  const int tid = threadIdx.x;
-  Two base = {0, 0};
-  if (tid == 0) sh.stopped = 0;
-  for (int s0 = 0; s0 < n_seqs; s0 += kThreads) {
-    const int s = s0 + tid;
-    Two v = {0, 0};
-    if (s < n_seqs) v = want(s);
-    const Two own = v;
-    v = block_scan(v, sh.wave);
-    v.a += base.a;
-    v.b += base.b;
-    const Two first = {v.a - own.a, v.b - own.b};
-    const bool fits = v.a <= limit_a && v.b <= limit_b;
-    if (!fits && first.a <= limit_a && first.b <= limit_b && !sh.stopped) {
-      // the first that does not fit (sums only grow); there is one such thread
-      sh.stop = first;
-      sh.stopped = 1;
-    }
-    __syncthreads();
-    const bool stopped = sh.stopped;
-    if (s < n_seqs) keep(s, fits ? first : sh.stop, fits);
-    if (stopped) {
-      base = sh.stop;
-      for (int r = s0 + kThreads + tid; r < n_seqs; r += kThreads) {
-        want(r);
-        keep(r, base, false);
-      }
-      break;
-    }
-    if (tid == kThreads - 1) sh.wave[0] = v;
-    __syncthreads();
-    base = sh.wave[0];
+template <class Want>
+__device__ __forceinline__ void share_out(int n_seqs, unsigned limit_a, unsigned limit_b, Shares &sh, int *line_a,
+                                          int *line_b, Want want) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // a run of sequences a thread
+  const int per = (n_seqs + kThreads - 1) / kThreads, s0 = tid * per, s1 = s0 + per < n_seqs ? s0 + per : n_seqs;
+  unsigned sum[2] = {0, 0};
+  for (int s = s0; s < s1; ++s) {
+    unsigned a, b;
+    want(s, a, b);
+    line_a[s] = (int)a;
+    line_b[s] = (int)b;
+    sum[0] = sat(sum[0], a);
+    sum[1] = sat(sum[1], b);
+  }
+  const unsigned in[2] = {scan_sat(sum[0]), scan_sat(sum[1])};
+  if (lane == 63) {
+    sh.wave[wave][0] = in[0];
+    sh.wave[wave][1] = in[1];
   }
   __syncthreads();
-  return base;
+  unsigned at[2], all[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    at[i] = (unsigned)__builtin_amdgcn_update_dpp(0, (int)in[i], 0x138, 0xF, 0xF, false);  // wave_shr:1
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) at[i] = sat(at[i], sh.wave[w][i]);
+      all[i] = sat(all[i], sh.wave[w][i]);
+    }
+  }
+  const bool whole = all[0] <= limit_a && all[1] <= limit_b;
+  for (int s = s0; s < s1; ++s) {
+    const unsigned to[2] = {sat(at[0], (unsigned)line_a[s]), sat(at[1], (unsigned)line_b[s])};
+    // the first that does not fit (sums only grow): there is one
+    if ((to[0] > limit_a || to[1] > limit_b) && at[0] <= limit_a && at[1] <= limit_b) {
+      sh.stop[0] = at[0];
+      sh.stop[1] = at[1];
+    }
+    line_a[s] = (int)at[0];
+    line_b[s] = (int)at[1];
+    at[0] = to[0];
+    at[1] = to[1];
+  }
+  __syncthreads();
+  const unsigned end[2] = {whole ? all[0] : sh.stop[0], whole ? all[1] : sh.stop[1]};
+  if (!whole)
+    for (int s = s0; s < s1; ++s)
+      if ((unsigned)line_a[s] > end[0] || (unsigned)line_b[s] > end[1]) {
+        line_a[s] = (int)end[0];
+        line_b[s] = (int)end[1];
+      }
+  if (tid == 0) {
+    line_a[n_seqs] = (int)end[0];
+    line_b[n_seqs] = (int)end[1];
+  }
+  __syncthreads();
 }
 
 // ---------------------------------------------------------------------------
-// Extend.  16 bytes written for each token; a decode step's is latency: lengths
-// and counts, sums, then a page and its entry.
+// Extend.  16 bytes written for each token, N tokens a thread: four where that
+// leaves workgroups enough (790949 tokens of 300 sequences: 8.5 us, 11 with one),
+// one for a decode step, which is latency: lengths and counts, sums, then a page
+// and its entry (64 sequences: 4.6 us, 5.3 with four).
 // ---------------------------------------------------------------------------
+typedef int int4v __attribute__((ext_vector_type(4)));
+typedef long long ll2v __attribute__((ext_vector_type(2)));
+
+template <int N>
 __global__ __launch_bounds__(kThreads) void paged_extend_kernel(ExtendArgs a) {
-  __shared__ int s_tok[kPagesMaxSeqs + 1], s_page[kPagesMaxSeqs + 1], s_len[kPagesMaxSeqs];
+  extern __shared__ int s_line[];  // [3][n_seqs + 1]: places of pages, of tokens; lengths
   __shared__ Shares sh;
-  const long long room = a.table_stride * a.page;
+  int *s_page = s_line, *s_tok = s_line + a.n_seqs + 1, *s_len = s_tok + a.n_seqs + 1;
+  const PageSize ps(a.page);
+  const int room = (int)(a.table_stride * a.page);
   int free = *a.free_count;
   free = free < 0 ? 0 : free > a.free_cap ? a.free_cap : free;
-  const auto want = [&](int s) {
-    const long long len = max(a.lens[s], 0);
-    long long n = max(a.fresh[s], 0);
-    if (len + n > room) n = 0;
-    s_len[s] = (int)len;
-    return Two{n == 0 ? 0 : (u64)(pages_of(len + n, a.page) - pages_of(len, a.page)), (u64)n};
-  };
-  const auto keep = [&](int s, Two first, bool) {
-    s_page[s] = (int)first.a;
-    s_tok[s] = (int)first.b;
-  };
-  const Two all = share_out(a.n_seqs, (u64)free, (u64)a.n_tokens, sh, want, keep);
-  const int pages = (int)all.a, tokens = (int)all.b, tid = threadIdx.x;
-  if (tid == 0) {
-    s_page[a.n_seqs] = pages;
-    s_tok[a.n_seqs] = tokens;
-  }
-  __syncthreads();
+  share_out(a.n_seqs, (unsigned)free, (unsigned)a.n_tokens, sh, s_page, s_tok, [&](int s, unsigned &p, unsigned &n) {
+    const int len = max(a.lens[s], 0), more = max(a.fresh[s], 0);
+    s_len[s] = len;
+    n = len <= room && more <= room - len ? (unsigned)more : 0u;
+    p = n ? (unsigned)(ps.pages(len + (int)n) - ps.pages(len)) : 0u;
+  });
+  const int pages = s_page[a.n_seqs], tokens = s_tok[a.n_seqs], tid = threadIdx.x;
   const long long first = (long long)blockIdx.x * kThreads + tid, step = (long long)gridDim.x * kThreads;
   for (long long e = first; e < pages; e += step) {
     const int s = part_of(s_page, a.n_seqs, (int)e);
-    a.table[s * a.table_stride + pages_of(s_len[s], a.page) + ((int)e - s_page[s])] = a.free_pages[free - 1 - e];
+    a.table[s * a.table_stride + ps.pages(s_len[s]) + ((int)e - s_page[s])] = a.free_pages[free - 1 - e];
   }
-  for (long long i = first; i < a.n_tokens; i += step) {
-    int seq = -1, at = -1;
-    long long slot = -1;
-    if (i < tokens) {
-      seq = part_of(s_tok, a.n_seqs, (int)i);
-      const int len = s_len[seq];
-      at = len + ((int)i - s_tok[seq]);
+  for (long long i0 = N * first; i0 < a.n_tokens; i0 += N * step) {
+    int seq[N], at[N];
+    long long slot[N];
+    int s = i0 < tokens ? part_of(s_tok, a.n_seqs, (int)i0) : 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const long long i = i0 + j;
+      seq[j] = at[j] = -1;
+      slot[j] = -1;
+      if (i >= tokens) continue;
+      while (s_tok[s + 1] <= (int)i) ++s;  // ends: i < tokens
+      const int len = s_len[s], t = len + ((int)i - s_tok[s]);
+      seq[j] = s;
+      at[j] = t;
       if (a.slots) {
-        const int p = at / a.page, have = pages_of(len, a.page);
-        const int page = p < have ? a.table[seq * a.table_stride + p]
-                                  : a.free_pages[free - 1 - (s_page[seq] + p - have)];
-        slot = page < 0 ? -1 : (long long)page * a.page + at % a.page;
+        const int p = ps.of(t), have = ps.pages(len);
+        const int page = p < have ? a.table[s * a.table_stride + p] : a.free_pages[free - 1 - (s_page[s] + p - have)];
+        slot[j] = page < 0 ? -1 : (long long)page * a.page + (t - p * a.page);
       }
     }
-    a.seqs[i] = seq;
-    a.positions[i] = at;
-    if (a.slots) a.slots[i] = slot;
+    if constexpr (N == 4)
+      if (a.vec && i0 + 4 <= a.n_tokens) {
+        *reinterpret_cast<int4v *>(a.seqs + i0) = int4v{seq[0], seq[1], seq[2], seq[3]};
+        *reinterpret_cast<int4v *>(a.positions + i0) = int4v{at[0], at[1], at[2], at[3]};
+        if (a.slots) {
+          *reinterpret_cast<ll2v *>(a.slots + i0) = ll2v{slot[0], slot[1]};
+          *reinterpret_cast<ll2v *>(a.slots + i0 + 2) = ll2v{slot[2], slot[3]};
+        }
+        continue;
+      }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i0 + j < a.n_tokens) {
+        a.seqs[i0 + j] = seq[j];
+        a.positions[i0 + j] = at[j];
+        if (a.slots) a.slots[i0 + j] = slot[j];
+      }
   }
   for (long long s = first; s < a.n_seqs; s += step) {
     a.lens_out[s] = s_len[s] + (s_tok[s + 1] - s_tok[s]);
@@ -165,25 +199,22 @@ __global__ __launch_bounds__(kThreads) void paged_extend_kernel(ExtendArgs a) {
 // Release: the marked sequences' pages behind those to keep, back on the stack.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kThreads) void paged_release_kernel(ReleaseArgs a) {
-  __shared__ int s_page[kPagesMaxSeqs + 1];
+  extern __shared__ int s_line[];  // [2][n_seqs + 1]: places of pages; nothing
   __shared__ Shares sh;
-  const long long room = a.table_stride * a.page;
+  int *s_page = s_line;
+  const PageSize ps(a.page);
+  const int room = (int)(a.table_stride * a.page);
   int free = *a.free_count;
   free = free < 0 ? 0 : free > a.free_cap ? a.free_cap : free;
   const auto kept = [&](int s) { return a.keep ? max(a.keep[s], 0) : 0; };
-  const auto length = [&](int s) {
-    const long long len = max(a.lens[s], 0);
-    return len < room ? len : room;
-  };
-  const auto want = [&](int s) {
-    const int n = a.which[s] ? pages_of(length(s), a.page) - kept(s) : 0;
-    return Two{n > 0 ? (u64)n : 0, 0};
-  };
-  const auto keep = [&](int s, Two first, bool) { s_page[s] = (int)first.a; };
-  const Two all = share_out(a.n_seqs, (u64)(a.free_cap - free), 0, sh, want, keep);
-  const int pages = (int)all.a, tid = threadIdx.x;
-  if (tid == 0) s_page[a.n_seqs] = pages;
-  __syncthreads();
+  const auto pages_of = [&](int s) { return ps.pages(min(max(a.lens[s], 0), room)); };
+  share_out(a.n_seqs, (unsigned)(a.free_cap - free), 0u, sh, s_page, s_line + a.n_seqs + 1,
+            [&](int s, unsigned &p, unsigned &none) {
+              const int n = a.which[s] ? pages_of(s) - kept(s) : 0;
+              p = n > 0 ? (unsigned)n : 0u;
+              none = 0;
+            });
+  const int pages = s_page[a.n_seqs], tid = threadIdx.x;
   const long long first = (long long)blockIdx.x * kThreads + tid, step = (long long)gridDim.x * kThreads;
   for (long long e = first; e < pages; e += step) {
     const int s = part_of(s_page, a.n_seqs, (int)e);
@@ -194,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void paged_release_kernel(ReleaseArgs a) 
   for (long long s = first; s < a.n_seqs; s += step) {
     const long long len = max(a.lens[s], 0), most = (long long)kept((int)s) * a.page;
     // all of its pages went (none where it does not fit), or it had none to give
-    const bool gone = a.which[s] && (s_page[s + 1] > s_page[s] || pages_of(length((int)s), a.page) <= kept((int)s));
+    const bool gone = a.which[s] && (s_page[s + 1] > s_page[s] || pages_of((int)s) <= kept((int)s));
     a.lens_out[s] = (int)(gone && most < len ? most : len);
   }
   if (first == 0) *a.count_out = free + pages;
@@ -294,18 +325,23 @@ __global__ __launch_bounds__(kThreads) void paged_copy_kernel(PagedCopyArgs a) {
 
 }  // namespace
 
-static unsigned grid_for(long long n) {
-  return (unsigned)std::max<long long>(1, std::min<long long>((n + 2 * kThreads - 1) / (2 * kThreads), 2048));
+// Workgroups for n items, each of which adds up all sequences first.
+static unsigned grid_for(long long n, long long per) {
+  return (unsigned)std::max<long long>(1, std::min<long long>((n + per - 1) / per, 1024));
 }
 
 hipError_t launch_paged_extend(const ExtendArgs &a, hipStream_t s) {
-  paged_extend_kernel<<<grid_for(a.n_tokens), kThreads, 0, s>>>(a);
+  const size_t lds = 3 * (a.n_seqs + 1) * sizeof(int);
+  if (a.n_tokens >= 256 * kThreads)
+    paged_extend_kernel<4><<<grid_for(a.n_tokens, 4 * kThreads), kThreads, lds, s>>>(a);
+  else
+    paged_extend_kernel<1><<<grid_for(a.n_tokens, kThreads), kThreads, lds, s>>>(a);
   return hipGetLastError();
 }
 
 hipError_t launch_paged_release(const ReleaseArgs &a, hipStream_t s) {
   const long long pages = std::min<long long>(a.n_seqs * a.table_stride, a.free_cap);
-  paged_release_kernel<<<grid_for(pages), kThreads, 0, s>>>(a);
+  paged_release_kernel<<<grid_for(pages, kThreads), kThreads, 2 * (a.n_seqs + 1) * sizeof(int), s>>>(a);
   return hipGetLastError();
 }
 

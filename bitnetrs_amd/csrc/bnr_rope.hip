@@ -82,45 +82,49 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
     s_cs[i] = rope_angle((double)p * a.turns[i % pairs], a.magnitude);
   }
   __syncthreads();
-  // a head's steps: those of its pairs, then those of the elements behind them
+  // A row's (a head's) steps: those of its pairs, then those of the elements behind
+  // them; `lanes` threads (a power of two) share a row.
   const int rot = (pairs + U - 1) / U, steps = rot + (a.d - 2 * pairs + 2 * U - 1) / (2 * U);
-  const int heads = a.q.heads + a.k.heads, per = heads * steps;
-  for (int n = tid; n < here * per; n += kThreads) {
-    const int t = n / per, m = n - t * per, h = m / steps, u = m - h * steps;
+  const int heads = a.q.heads + a.k.heads, rows = here * heads;
+  const int u0 = tid & (a.lanes - 1), per = kThreads / a.lanes;
+  for (int r = tid / a.lanes; r < rows; r += per) {
+    const int t = r / heads, h = r - t * heads;
     if (s_pos[t] < 0) continue;  // left out
     const bool is_k = h >= a.q.heads;
     const RopeHeads &x = is_k ? a.k : a.q;
     const int head = is_k ? h - a.q.heads : h;
     const T *in = static_cast<const T *>(x.in) + (token0 + t) * x.in_token + head * x.in_head;
     T *out = static_cast<T *>(x.out) + (token0 + t) * x.out_token + head * x.out_head;
-    if (u >= rot) {
-      if (in == out) continue;
-      const int e = 2 * pairs + (u - rot) * 2 * U;
-      if constexpr (U == 1) {
-        out[e] = in[e];
-        if (e + 1 < a.d) out[e + 1] = in[e + 1];
-      } else {
-        const auto lo = load_some<T, U>(in + e), hi = load_some<T, U>(in + e + U);
-        store_some(out + e, lo);
-        store_some(out + e + U, hi);
+    for (int u = u0; u < steps; u += a.lanes) {
+      if (u >= rot) {
+        if (in == out) continue;
+        const int e = 2 * pairs + (u - rot) * 2 * U;
+        if constexpr (U == 1) {
+          out[e] = in[e];
+          if (e + 1 < a.d) out[e + 1] = in[e + 1];
+        } else {
+          const auto lo = load_some<T, U>(in + e), hi = load_some<T, U>(in + e + U);
+          store_some(out + e, lo);
+          store_some(out + e + U, hi);
+        }
+        continue;
       }
-      continue;
-    }
-    const int i = u * U, e0 = HALF ? i : 2 * i, e1 = HALF ? i + pairs : 2 * i + U;
-    Some<T, U> lo = load_some<T, U>(in + e0), hi = load_some<T, U>(in + e1);
+      const int i = u * U, e0 = HALF ? i : 2 * i, e1 = HALF ? i + pairs : 2 * i + U;
+      Some<T, U> lo = load_some<T, U>(in + e0), hi = load_some<T, U>(in + e1);
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const float2 cs = s_cs[t * pairs + i + j];
-      // pairs: the runs' elements j, or neighbours of the two runs taken as one
-      T &p = HALF || U == 1 ? lo.x[j] : 2 * j < U ? lo.x[(2 * j) % U] : hi.x[(2 * j) % U];
-      T &q = HALF || U == 1 ? hi.x[j] : 2 * j < U ? lo.x[(2 * j + 1) % U] : hi.x[(2 * j + 1) % U];
-      float y, z;
-      rot_pair((float)p, (float)q, cs.x, cs.y, y, z);
-      p = (T)y;
-      q = (T)z;
+      for (int j = 0; j < U; ++j) {
+        const float2 cs = s_cs[t * pairs + i + j];
+        // pairs: the runs' elements j, or neighbours of the two runs taken as one
+        T &p = HALF || U == 1 ? lo.x[j] : 2 * j < U ? lo.x[(2 * j) % U] : hi.x[(2 * j) % U];
+        T &q = HALF || U == 1 ? hi.x[j] : 2 * j < U ? lo.x[(2 * j + 1) % U] : hi.x[(2 * j + 1) % U];
+        float y, z;
+        rot_pair((float)p, (float)q, cs.x, cs.y, y, z);
+        p = (T)y;
+        q = (T)z;
+      }
+      store_some(out + e0, lo);
+      store_some(out + e1, hi);
     }
-    store_some(out + e0, lo);
-    store_some(out + e1, hi);
   }
 }
 
@@ -161,6 +165,10 @@ hipError_t launch_rope(RopeArgs a, int type, bool half, bool vec, hipStream_t s)
   a.tokens = 1;
   if (a.n_tokens >= 2048 && a.pairs <= kThreads / 2) a.tokens = kThreads / a.pairs;
   if (a.tokens > 32) a.tokens = 32;
+  const int unit = vec ? 16 / (type == kRopeF32 ? 4 : 2) : 1;
+  const int steps = (a.pairs + unit - 1) / unit + (a.d - 2 * a.pairs + 2 * unit - 1) / (2 * unit);
+  a.lanes = 1;
+  while (a.lanes < steps && a.lanes < kThreads) a.lanes *= 2;
   switch (type) {
     case kRopeF32: launch_type<float>(a, half, vec, s); break;
     case kRopeBf16: launch_type<__bf16>(a, half, vec, s); break;
