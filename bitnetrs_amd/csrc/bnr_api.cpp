@@ -3317,9 +3317,8 @@ extern "C" int bnr_dev_rope(bnr_ctx *c, const bnr_rope *rope, int type, size_t n
   a.d = (int)head_dim;
   a.pairs = (int)rope->n_pairs;
   a.magnitude = rope->magnitude;
-  const size_t unit = 16 / size;
-  const bool vec = rope->n_pairs % unit == 0 && head_dim % (2 * unit) == 0 && rope_aligned(a.q, size) &&
-                   rope_aligned(a.k, size);
+  const size_t unit = 16 / size, run = rope->layout == BNR_ROPE_HALF ? rope->n_pairs : 2 * rope->n_pairs;
+  const bool vec = run % unit == 0 && head_dim % unit == 0 && rope_aligned(a.q, size) && rope_aligned(a.k, size);
   DeviceGuard dg(c->device);
   HIP_TRY(launch_rope(a, type, rope->layout == BNR_ROPE_HALF, vec, (hipStream_t)stream), "rope launch");
   return set_ok();

@@ -811,7 +811,7 @@ struct RopeArgs {
   float magnitude;
   double turns[kRopeMaxPairs];  // of a pair, a position
 };
-// vec: rows of 16-byte units, 2 * pairs and d multiples of two of them.
+// vec: rows, their pairs' runs and d in 16-byte units.
 hipError_t launch_rope(RopeArgs a, int type, bool half, bool vec, hipStream_t s);
 
 struct RopeTableArgs {

@@ -32,8 +32,11 @@ __device__ __forceinline__ float2 rope_angle(double turns, float m) {
 }
 
 template <class T>
-__device__ __forceinline__ float widen(T x) {
-  return (float)x;
+__device__ __forceinline__ void rotate(T &p, T &q, float2 cs) {
+  float y, z;
+  rot_pair((float)p, (float)q, cs.x, cs.y, y, z);
+  p = (T)y;
+  q = (T)z;
 }
 
 // N elements (16 bytes at most) at p.
@@ -67,8 +70,12 @@ __device__ __forceinline__ void store_some(T *p, const Some<T, N> &r) {
   }
 }
 
-// U: pairs of a thread's step, whose elements are two runs of U; 1 where
-// alignment or sizes leave no more.
+// U: elements of 16 bytes, or 1 where alignment or sizes leave no more.  A step of
+// a thread is U pairs of two runs (half), U / 2 pairs of one run (interleaved; one
+// pair where U is 1), or U elements that are copied: neighbouring threads' steps
+// are neighbours, so a wave's loads and stores are whole lines.  16384 tokens of
+// 32/8 bf16 heads of 128, 32 of them rotated in pairs of neighbours: KEEPUS; with 32
+// bytes a thread, 80 us, with non-temporal stores 103.
 template <class T, int U, bool HALF>
 __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
   __shared__ float2 s_cs[kThreads > kRopeMaxPairs ? kThreads : kRopeMaxPairs];
@@ -84,46 +91,52 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
   __syncthreads();
   // A row's (a head's) steps: those of its pairs, then those of the elements behind
   // them; `lanes` threads (a power of two) share a row.
-  const int rot = (pairs + U - 1) / U, steps = rot + (a.d - 2 * pairs + 2 * U - 1) / (2 * U);
-  const int heads = a.q.heads + a.k.heads, rows = here * heads;
-  const int u0 = tid & (a.lanes - 1), per = kThreads / a.lanes;
-  for (int r = tid / a.lanes; r < rows; r += per) {
-    const int t = r / heads, h = r - t * heads;
-    if (s_pos[t] < 0) continue;  // left out
-    const bool is_k = h >= a.q.heads;
-    const RopeHeads &x = is_k ? a.k : a.q;
-    const int head = is_k ? h - a.q.heads : h;
-    const T *in = static_cast<const T *>(x.in) + (token0 + t) * x.in_token + head * x.in_head;
-    T *out = static_cast<T *>(x.out) + (token0 + t) * x.out_token + head * x.out_head;
-    for (int u = u0; u < steps; u += a.lanes) {
-      if (u >= rot) {
-        if (in == out) continue;
-        const int e = 2 * pairs + (u - rot) * 2 * U;
-        if constexpr (U == 1) {
-          out[e] = in[e];
-          if (e + 1 < a.d) out[e + 1] = in[e + 1];
-        } else {
-          const auto lo = load_some<T, U>(in + e), hi = load_some<T, U>(in + e + U);
-          store_some(out + e, lo);
-          store_some(out + e + U, hi);
-        }
-        continue;
-      }
-      const int i = u * U, e0 = HALF ? i : 2 * i, e1 = HALF ? i + pairs : 2 * i + U;
-      Some<T, U> lo = load_some<T, U>(in + e0), hi = load_some<T, U>(in + e1);
+  constexpr int W = HALF || U > 1 ? U : 2;  // elements of a run
+  const int rot = HALF ? pairs / U : 2 * pairs / W, steps = rot + (a.d - 2 * pairs) / U;
+  const int heads = a.q.heads + a.k.heads, rows = here * heads, per = kThreads / a.lanes;
+  constexpr int N = U > 1 ? 2 : 1;  // rows of a thread on their way at a time
+  for (int u = tid & (a.lanes - 1); u < steps; u += a.lanes) {
+    const bool turn = u < rot;
+    const int e = turn ? u * W : 2 * pairs + (u - rot) * U, e2 = HALF && turn ? e + pairs : e;
+    for (int r0 = tid / a.lanes; r0 < rows; r0 += N * per) {
+      Some<T, W> x[N], x2[N];
+      T *out[N];
+      int at[N];
+      bool there[N];
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const float2 cs = s_cs[t * pairs + i + j];
-        // pairs: the runs' elements j, or neighbours of the two runs taken as one
-        T &p = HALF || U == 1 ? lo.x[j] : 2 * j < U ? lo.x[(2 * j) % U] : hi.x[(2 * j) % U];
-        T &q = HALF || U == 1 ? hi.x[j] : 2 * j < U ? lo.x[(2 * j + 1) % U] : hi.x[(2 * j + 1) % U];
-        float y, z;
-        rot_pair((float)p, (float)q, cs.x, cs.y, y, z);
-        p = (T)y;
-        q = (T)z;
+      for (int n = 0; n < N; ++n) {
+        // past the last row: the first again, not written (a branch would part the loads)
+        const int r = r0 + n * per < rows ? r0 + n * per : r0, t = r / heads, h = r - t * heads;
+        const bool is_k = h >= a.q.heads;
+        const RopeHeads &o = is_k ? a.k : a.q;
+        const int head = is_k ? h - a.q.heads : h;
+        const T *in = static_cast<const T *>(o.in) + (token0 + t) * o.in_token + head * o.in_head;
+        out[n] = static_cast<T *>(o.out) + (token0 + t) * o.out_token + head * o.out_head;
+        at[n] = t;
+        there[n] = r0 + n * per < rows && s_pos[t] >= 0 && (turn || in != out[n]);
+        if (W == U || turn) x[n] = load_some<T, W>(in + e);
+        else x[n].x[0] = in[e];
+        if (HALF) x2[n] = load_some<T, W>(in + e2);
       }
-      store_some(out + e0, lo);
-      store_some(out + e1, hi);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (!there[n]) continue;
+        if (turn) {
+          const float2 *cs = s_cs + at[n] * pairs + (HALF ? u * U : u * (W / 2));
+#pragma unroll
+          for (int j = 0; j < (HALF ? U : W / 2); ++j) {
+            if constexpr (HALF)
+              rotate(x[n].x[j], x2[n].x[j], cs[j]);
+            else
+              rotate(x[n].x[2 * j], x[n].x[2 * j + 1], cs[j]);
+          }
+          if (HALF) store_some(out[n] + e2, x2[n]);
+        }
+        if (W == U || turn)
+          store_some(out[n] + e, x[n]);
+        else
+          out[n][e] = x[n].x[0];
+      }
     }
   }
 }
@@ -160,13 +173,13 @@ void launch_type(const RopeArgs &a, bool half, bool vec, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_rope(RopeArgs a, int type, bool half, bool vec, hipStream_t s) {
-  // tokens of a workgroup: as many as its threads make the angles of, where
-  // there are workgroups enough
+  // tokens of a workgroup: as many as its threads make the angles of, at most
+  // four, where there are workgroups enough
   a.tokens = 1;
   if (a.n_tokens >= 2048 && a.pairs <= kThreads / 2) a.tokens = kThreads / a.pairs;
-  if (a.tokens > 32) a.tokens = 32;
+  if (a.tokens > 4) a.tokens = 4;
   const int unit = vec ? 16 / (type == kRopeF32 ? 4 : 2) : 1;
-  const int steps = (a.pairs + unit - 1) / unit + (a.d - 2 * a.pairs + 2 * unit - 1) / (2 * unit);
+  const int steps = (half ? a.pairs / unit : unit > 1 ? 2 * a.pairs / unit : a.pairs) + (a.d - 2 * a.pairs) / unit;
   a.lanes = 1;
   while (a.lanes < steps && a.lanes < kThreads) a.lanes *= 2;
   switch (type) {
