@@ -138,8 +138,6 @@ class HeadsDesc(ctypes.Structure):
                 ("out_token", _sz), ("out_head", _sz)]
 
 
-_heads = _c.POINTER(HeadsDesc)
-
 # name -> (restype, argtypes); one entry per function in include/bitnet_hip.h
 SIGNATURES = {
     "bnr_last_error": (_c.c_char_p, []),
@@ -225,8 +223,8 @@ SIGNATURES = {
     "bnr_dev_beam_select": (_c.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _c.c_int32, _vp,
                                        _vp, _vp, _vp, _vp, _sz, _vp]),
     "bnr_dev_beam_reorder": (_c.c_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
-    "bnr_dev_rope": (_c.c_int, [_vp, _c.POINTER(RopeDesc), _c.c_int, _sz, _sz, _vp, _heads, _heads,
-                                _vp]),
+    # bnr_heads as packed bytes: making a structure takes longer than the rotation of a token
+    "bnr_dev_rope": (_c.c_int, [_vp, _c.POINTER(RopeDesc), _c.c_int, _sz, _sz, _vp, _vp, _vp, _vp]),
     "bnr_dev_rope_scaled_table": (_c.c_int, [_vp, _c.POINTER(RopeDesc), _sz, _sz, _vp, _vp, _vp]),
 }
 

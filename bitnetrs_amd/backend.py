@@ -14,6 +14,8 @@ library sees raw pointers and the current HIP stream.
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 
 import numpy as np
 
@@ -68,12 +70,23 @@ def _on(t, name: str, dtype, device: int, shape=None):
     return t.data_ptr()
 
 
-def _raw_stream(device: int):
-    """The current stream of a device, as a number."""
-    import torch
+class _Torch:
+    """What the calls of a decode step need of torch, looked up once (at the first
+    call: the package loads without it)."""
 
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(device) if get else torch.cuda.current_stream(device).cuda_stream
+    def __init__(self):
+        import torch
+
+        self.f32, self.i32, self.i64, self.u8 = torch.float32, torch.int32, torch.int64, torch.uint8
+        self.rope = {torch.float32: _lib.BNR_TYPE_F32, torch.bfloat16: _lib.BNR_TYPE_BF16,
+                     torch.float16: _lib.BNR_TYPE_F16}
+        # the current stream of a device, as a number
+        self.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+_torch = functools.lru_cache(None)(_Torch)
+_pack_heads = struct.Struct("PP5N").pack  # bnr_heads
 
 
 def _check_sizes(*operands) -> None:
@@ -460,10 +473,8 @@ class HipBackend:
         that no token has; offsets [n_seqs + 1] which tokens are a sequence's;
         lens_out and count_out [1] are lens and free_count afterwards.  All int32.
         What does not fit gets nothing: see bnr_dev_paged_extend."""
-        dev = self.device_id
-        import torch
-
-        i32 = torch.int32
+        dev, torch = self.device_id, _torch()
+        i32 = torch.i32
         try:
             (n, stride), (cap,), (n_tokens,) = block_table.shape, free_pages.shape, seqs.shape
         except (AttributeError, ValueError):
@@ -474,19 +485,17 @@ class HipBackend:
             _on(lens, "lens", i32, dev, (n,)), _on(new, "new", i32, dev, (n,)),
             _on(free_pages, "free_pages", i32, dev), cap, _on(free_count, "free_count", i32, dev, (1,)),
             _on(seqs, "seqs", i32, dev), _on(positions, "positions", i32, dev, (n_tokens,)),
-            None if slots is None else _on(slots, "slots", torch.int64, dev, (n_tokens,)), n_tokens,
+            None if slots is None else _on(slots, "slots", torch.i64, dev, (n_tokens,)), n_tokens,
             _on(offsets, "offsets", i32, dev, (n + 1,)), _on(lens_out, "lens_out", i32, dev, (n,)),
             _on(count_out, "count_out", i32, dev, (1,)),
-            _raw_stream(dev) if stream is None else _stream(stream)))
+            torch.stream(dev) if stream is None else _stream(stream)))
 
     def dev_paged_release(self, block_table, lens, which, free_pages, free_count, page_size, lens_out,
                           count_out, keep=None, stream=None) -> None:
         """The pages of the sequences with which[s] != 0 (uint8) back onto the stack;
         with `keep` [n_seqs], those behind a sequence's first keep[s]."""
-        dev = self.device_id
-        import torch
-
-        i32 = torch.int32
+        dev, torch = self.device_id, _torch()
+        i32 = torch.i32
         try:
             (n, stride), (cap,) = block_table.shape, free_pages.shape
         except (AttributeError, ValueError):
@@ -494,11 +503,11 @@ class HipBackend:
             raise
         _lib.check(self._L.bnr_dev_paged_release(
             self._h, _on(block_table, "block_table", i32, dev), n, stride, page_size,
-            _on(lens, "lens", i32, dev, (n,)), _on(which, "which", torch.uint8, dev, (n,)),
+            _on(lens, "lens", i32, dev, (n,)), _on(which, "which", torch.u8, dev, (n,)),
             None if keep is None else _on(keep, "keep", i32, dev, (n,)),
             _on(free_pages, "free_pages", i32, dev), cap, _on(free_count, "free_count", i32, dev, (1,)),
             _on(lens_out, "lens_out", i32, dev, (n,)), _on(count_out, "count_out", i32, dev, (1,)),
-            _raw_stream(dev) if stream is None else _stream(stream)))
+            torch.stream(dev) if stream is None else _stream(stream)))
 
     def dev_paged_copy(self, kv: "PagedKV", block_table, src, lens, starts=None, stream=None) -> None:
         """Rows starts[s] (None: 0) .. lens[s]-1 of sequence src[s] to those of
@@ -533,10 +542,8 @@ class HipBackend:
         that have ended, with their one continuation eos; done_out [batch, k] is
         theirs afterwards.  `workspace` from beam_workspace; calls that share one
         must be ordered."""
-        dev = self.device_id
-        import torch
-
-        f32, i32, u8 = torch.float32, torch.int32, torch.uint8
+        dev, torch = self.device_id, _torch()
+        f32, i32, u8 = torch.f32, torch.i32, torch.u8
         try:
             (batch, beams, vocab), (_, k), (n,) = logits.shape, tokens.shape, workspace.shape
             far, row, one = logits.stride()
@@ -558,16 +565,14 @@ class HipBackend:
             _on(tokens, "tokens", i32, dev, out), _on(parents, "parents", i32, dev, out),
             _on(scores_out, "scores_out", f32, dev, out),
             None if done_out is None else _on(done_out, "done_out", u8, dev, out),
-            _on(workspace, "workspace", u8, dev), n, _raw_stream(dev) if stream is None else _stream(stream)))
+            _on(workspace, "workspace", u8, dev), n, torch.stream(dev) if stream is None else _stream(stream)))
 
     def dev_beam_reorder(self, block_table, parents, table_out, src, stream=None) -> None:
         """The block tables [batch * beams, pages] after a selection of parents
         [batch, beams], into table_out, and in src [batch * beams] the sequences that
         dev_paged_copy has to copy from (-1: none)."""
-        dev = self.device_id
-        import torch
-
-        i32 = torch.int32
+        dev, torch = self.device_id, _torch()
+        i32 = torch.i32
         try:
             (rows, stride), (batch, beams) = block_table.shape, parents.shape
         except (AttributeError, ValueError):
@@ -578,7 +583,7 @@ class HipBackend:
         _lib.check(self._L.bnr_dev_beam_reorder(
             self._h, _on(block_table, "block_table", i32, dev), batch, beams, stride,
             _on(parents, "parents", i32, dev), _on(table_out, "table_out", i32, dev, (rows, stride)),
-            _on(src, "src", i32, dev, (rows,)), _raw_stream(dev) if stream is None else _stream(stream)))
+            _on(src, "src", i32, dev, (rows,)), torch.stream(dev) if stream is None else _stream(stream)))
 
     # rotary embeddings ---------------------------------------------------------------
     def dev_rope(self, rope, q, k, positions, q_out=None, k_out=None, stream=None) -> None:
@@ -587,45 +592,55 @@ class HipBackend:
         place).  float32, bfloat16 or float16; token and head strides are free, so
         slices of a fused projection's output are taken as they are.  A token with a
         negative position is left out."""
-        dev = self.device_id
-        import torch
-
-        types = {torch.float32: _lib.BNR_TYPE_F32, torch.bfloat16: _lib.BNR_TYPE_BF16,
-                 torch.float16: _lib.BNR_TYPE_F16}
+        dev, torch = self.device_id, _torch()
         first = k if q is None else q
         try:
             (n,), (_, _, d) = positions.shape, first.shape
-        except (AttributeError, ValueError):
-            _check_sizes((positions, "positions", 1), (first, "q" if first is q else "k", 3))
+            kind = first.dtype
+            heads = [self._rope_heads(x, out, kind, n, d) for x, out in ((q, q_out), (k, k_out))]
+            type_ = torch.rope[kind]
+        except (AttributeError, KeyError, TypeError, ValueError):
+            self._rope_refuse(positions, q, k, q_out, k_out, torch.rope)
             raise
-        kind = first.dtype
+        if heads[0] is False or heads[1] is False:
+            self._rope_refuse(positions, q, k, q_out, k_out, torch.rope)
+        _lib.check(self._L.bnr_dev_rope(
+            self._h, rope._ref, type_, n, d, _on(positions, "positions", torch.i32, dev), heads[0], heads[1],
+            torch.stream(dev) if stream is None else _stream(stream)))
+
+    def _rope_heads(self, x, out, kind, n, d):
+        """One operand of dev_rope as bnr_heads; False where something about it is wrong."""
+        if x is None:
+            return False if out is not None else None
+        if out is None:
+            out = x
+        dev, shape, (it, ih, ie), (ot, oh, oe) = self.device_id, x.shape, x.stride(), out.stride()
+        if not (x.dtype is kind and out.dtype is kind and x.get_device() == dev and out.get_device() == dev
+                and shape[0] == n and shape[2] == d and out.shape == shape and (d == 1 or ie == oe == 1)):
+            return False
+        return _pack_heads(x.data_ptr(), out.data_ptr(), shape[1], it, ih, ot, oh)
+
+    def _rope_refuse(self, positions, q, k, q_out, k_out, types) -> None:
+        """Says what is wrong about the operands of dev_rope."""
+        operands = [(x, out, name) for x, out, name in ((q, q_out, "q"), (k, k_out, "k"))]
+        first = next((o for o in operands if o[0] is not None), operands[0])
+        _check_sizes((positions, "positions", 1), (first[0], first[2], 3))
+        n, d, kind = positions.shape[0], first[0].shape[2], first[0].dtype
         if kind not in types:
             raise TypeError(f"q and k must be float32, bfloat16 or float16, not {kind}")
-        heads = []
-        for x, out, name in ((q, q_out, "q"), (k, k_out, "k")):
+        for x, out, name in operands:
             if x is None:
                 if out is not None:
                     raise TypeError(f"{name}_out without {name}")
-                heads.append(None)
                 continue
-            if out is None:
-                out = x
-            for t, what in ((x, name), (out, name + "_out")):
-                try:
-                    fits = t.dtype is kind and t.get_device() == dev
-                except AttributeError:
-                    fits = False
-                if not fits:
-                    raise TypeError(f"{what} must be a {kind} tensor on cuda:{dev}")
-                if t.dim() != 3 or t.shape[0] != n or t.shape[2] != d or t.shape != x.shape:
+            for t, what in ((x, name), (x if out is None else out, name + "_out")):
+                _check_sizes((t, what, 3))
+                if t.dtype != kind or t.get_device() != self.device_id:
+                    raise TypeError(f"{what} must be a {kind} tensor on cuda:{self.device_id}")
+                if t.shape[0] != n or t.shape[2] != d or t.shape != x.shape:
                     raise InvalidShape(f"{what} [{n}, heads, {d}]", f"{list(t.shape)}")
                 if t.stride(2) != 1 and d > 1:
                     raise TypeError(f"the elements of a head of {what} must lie side by side")
-            (it, ih, _), (ot, oh, _) = x.stride(), out.stride()
-            heads.append(_lib.HeadsDesc(x.data_ptr(), out.data_ptr(), x.shape[1], it, ih, ot, oh))
-        _lib.check(self._L.bnr_dev_rope(
-            self._h, rope._ref, types[kind], n, d, _on(positions, "positions", torch.int32, dev), heads[0],
-            heads[1], _raw_stream(dev) if stream is None else _stream(stream)))
 
     def rope_scaled_table(self, rope, n_positions: int, first: int = 0, out=None, stream=None):
         """The rotation's tables (cos, sin) [n_positions, rope.dim / 2] of positions
@@ -637,7 +652,8 @@ class HipBackend:
         cos, sin = out or (torch.empty(shape, device=f"cuda:{dev}") for _ in range(2))
         _lib.check(self._L.bnr_dev_rope_scaled_table(
             self._h, rope._ref, first, n_positions, _on(cos, "cos", torch.float32, dev, shape),
-            _on(sin, "sin", torch.float32, dev, shape), _raw_stream(dev) if stream is None else _stream(stream)))
+            _on(sin, "sin", torch.float32, dev, shape),
+            _torch().stream(dev) if stream is None else _stream(stream)))
         return cos, sin
 
     def dev_synchronize(self, stream=None) -> None:

@@ -64,7 +64,7 @@ def rotation(rates=RATES, n=32, layout=0, magnitude=1.0):
 
 
 def heads(i=1, o=None, n=4, it=256, ih=64, ot=256, oh=64):
-    return HeadsDesc(at(i), at(i) if o is None else o, n, it, ih, ot, oh)
+    return bytes(HeadsDesc(at(i), at(i) if o is None else o, n, it, ih, ot, oh))
 
 
 def rope(ctx=CTX, r=None, **kw):
@@ -147,8 +147,8 @@ REFUSED = [
     (rope, dict(k=heads(3, o=at(3) + 4)), SHAPE, "in place"),
     (rope, dict(k=heads(3, it=512)), SHAPE, "in place"),
     (rope, dict(q=heads(1, it=1 << 41, ot=1 << 41)), SHAPE, "strides"),
-    (rope, dict(q=HeadsDesc(None, at(1), 4, 256, 64, 256, 64)), BACKEND, "NULL"),
-    (rope, dict(q=HeadsDesc(at(1) + 2, at(1) + 2, 4, 256, 64, 256, 64)), SHAPE, "aligned"),
+    (rope, dict(q=bytes(HeadsDesc(None, at(1), 4, 256, 64, 256, 64))), BACKEND, "NULL"),
+    (rope, dict(q=bytes(HeadsDesc(at(1) + 2, at(1) + 2, 4, 256, 64, 256, 64))), SHAPE, "aligned"),
     (table, dict(r=rotation(n=0)), CONFIG, "pairs"),
     (table, dict(n=(1 << 30) + 1), SHAPE, "n_positions"),
     (table, dict(first=1 << 31), SHAPE, "first"),
@@ -174,6 +174,13 @@ def test_null_context(call):
 ])
 def test_nothing_to_do_is_no_error(call, nothing):
     assert call(**nothing) == _lib.BNR_OK
+
+
+def test_packed_heads_are_the_structure():
+    from bitnetrs_amd import backend
+
+    v = [at(1), at(2), 3, 4, 5, 6, (1 << 40) + 7]
+    assert backend._pack_heads(*v) == bytes(HeadsDesc(*v))
 
 
 def test_beam_workspace():
