@@ -860,7 +860,7 @@ struct PagedCopyArgs {
   PagedPool pool;
   const int *src, *starts, *lens;  // starts: or null
   int n_seqs, row_bytes, scale_bytes;  // of a row's codes and scales
-  int wgs, tile;  // set by the launch
+  int wgs, tile, lanes;  // lanes: of a row; set by the launch
 };
 // unit: bytes of a load, 16, 8, 4, 2 or 1, that divide the rows and the pool's address.
 hipError_t launch_paged_copy(PagedCopyArgs a, int unit, hipStream_t s);

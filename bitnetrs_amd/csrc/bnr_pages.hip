@@ -275,6 +275,7 @@ __global__ __launch_bounds__(kThreads) void beam_reorder_kernel(BeamTableArgs a)
 // lanes share a row.  Bound by the rows' bytes, read and written.
 // ---------------------------------------------------------------------------
 constexpr int kCopyWgs = 4096, kCopyRows = 64;
+constexpr int kCopyPasses = 4;  // rows of a thread on their way at a time
 
 template <int U>
 struct Unit;
@@ -297,27 +298,47 @@ __global__ __launch_bounds__(kThreads) void paged_copy_kernel(PagedCopyArgs a) {
     const int from = a.src[s], len = paged_len(a.lens[s], a.pool), first = start(s);
     return from < 0 || from >= a.n_seqs || from == s || first >= len ? 0 : len - first;
   };
-  const int units = a.row_bytes / U, per = 2 * units;
-  const char *pool[2] = {static_cast<const char *>(a.pool.k), static_cast<const char *>(a.pool.v)};
+  const int units = a.row_bytes / U, x0 = threadIdx.x & (a.lanes - 1), pass = kThreads / a.lanes;
+  const T *const k = static_cast<const T *>(a.pool.k), *const v = static_cast<const T *>(a.pool.v);
+  T *const ko = static_cast<T *>(a.pool.k), *const vo = static_cast<T *>(a.pool.v);
   PagedShare sh = paged_share(rows, a.n_seqs, a.pool.n_kv, a.tile, a.wgs);
   for (PagedPiece p; sh.next(rows, p);) {
-    const int first = start(p.b), src = a.src[p.b], n = p.row1 - p.row0;
-    for (int e = threadIdx.x; e < n * per; e += kThreads) {
-      const int r = e / per, x = e - r * per, t = first + p.row0 + r;
-      const long long from = paged_row(a.pool, src, p.h, t), to = paged_row(a.pool, p.b, p.h, t);
-      if (from < 0 || to < 0 || from == to) continue;
-      const int v = x >= units, at = x - v * units;
-      char *base = const_cast<char *>(pool[v]);
-      reinterpret_cast<T *>(base + to * a.row_bytes)[at] = reinterpret_cast<const T *>(base + from * a.row_bytes)[at];
+    const int first = start(p.b) + p.row0, src = a.src[p.b], n = p.row1 - p.row0;
+    for (int r0 = (int)threadIdx.x / a.lanes; r0 < n; r0 += kCopyPasses * pass) {
+      long long from[kCopyPasses], to[kCopyPasses];
+#pragma unroll
+      for (int i = 0; i < kCopyPasses; ++i) {
+        // past the last row: the first again, not written (a branch would part the loads)
+        const int r = r0 + i * pass < n ? r0 + i * pass : r0;
+        from[i] = paged_row(a.pool, src, p.h, first + r);
+        to[i] = paged_row(a.pool, p.b, p.h, first + r);
+        if (r0 + i * pass >= n || from[i] < 0 || from[i] == to[i]) to[i] = -1;
+        if (from[i] < 0) from[i] = 0;
+      }
+      for (int x = x0; x < units; x += a.lanes) {
+        T ks[kCopyPasses], vs[kCopyPasses];
+#pragma unroll
+        for (int i = 0; i < kCopyPasses; ++i) {
+          ks[i] = k[from[i] * units + x];
+          vs[i] = v[from[i] * units + x];
+        }
+#pragma unroll
+        for (int i = 0; i < kCopyPasses; ++i)
+          if (to[i] >= 0) {
+            ko[to[i] * units + x] = ks[i];
+            vo[to[i] * units + x] = vs[i];
+          }
+      }
     }
     if (a.scale_bytes == 0) continue;
     for (int e = threadIdx.x; e < n * 2 * a.scale_bytes; e += kThreads) {
-      const int r = e / (2 * a.scale_bytes), x = e - r * 2 * a.scale_bytes, t = first + p.row0 + r;
+      const int r = e / (2 * a.scale_bytes), x = e - r * 2 * a.scale_bytes, t = first + r;
       const long long from = paged_row(a.pool, src, p.h, t), to = paged_row(a.pool, p.b, p.h, t);
       if (from < 0 || to < 0 || from == to) continue;
-      const int v = x >= a.scale_bytes, at = x - v * a.scale_bytes;
-      unsigned char *sc = a.pool.k_exps ? (v ? a.pool.v_exps : a.pool.k_exps)
-                                        : reinterpret_cast<unsigned char *>(v ? a.pool.v_scales : a.pool.k_scales);
+      const int is_v = x >= a.scale_bytes, at = x - is_v * a.scale_bytes;
+      unsigned char *sc = a.pool.k_exps
+                              ? (is_v ? a.pool.v_exps : a.pool.k_exps)
+                              : reinterpret_cast<unsigned char *>(is_v ? a.pool.v_scales : a.pool.k_scales);
       sc[to * a.scale_bytes + at] = sc[from * a.scale_bytes + at];
     }
   }
@@ -355,6 +376,8 @@ hipError_t launch_paged_copy(PagedCopyArgs a, int unit, hipStream_t s) {
   a.tile = kCopyRows;
   while ((rows + a.tile - 1) / a.tile * items >= 1ll << 31) a.tile *= 2;
   a.wgs = (int)std::min<long long>(kCopyWgs, (rows + a.tile - 1) / a.tile * items);
+  a.lanes = 1;
+  while (a.lanes < a.row_bytes / unit && a.lanes < kThreads) a.lanes *= 2;
   switch (unit) {
     case 16: paged_copy_kernel<16><<<a.wgs, kThreads, 0, s>>>(a); break;
     case 8: paged_copy_kernel<8><<<a.wgs, kThreads, 0, s>>>(a); break;
