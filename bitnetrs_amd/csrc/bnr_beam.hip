@@ -295,10 +295,15 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a) 
   u64 *list = s_list + wave * a.chunks * k;
   for (int beam = wave; beam < a.beams; beam += waves) {
     const long long row = b * a.beams + beam;
-    const double base = (double)a.scores[row] + 0.0;  // no -0
     double *y = s_y + beam * k;
     int *t = s_t + beam * k;
-    const bool ended = a.done && a.done[row];  // its parts have not been made
+    // all that is read, at once (of an ended beam's parts, which have not been made, whatever is there)
+    const long long at = row * a.chunks;
+    const unsigned char ended = a.done ? a.done[row] : 0;
+    const double base = (double)a.scores[row] + 0.0;  // no -0
+    const float m = lane < a.chunks ? a.part_max[at + lane] : -INFINITY;
+    const double s = lane < a.chunks ? a.part_sum[at + lane] : 0.0;
+    for (int e = lane; e < a.chunks * k; e += 64) list[e] = a.part_key[at * k + e];
     if (ended && fabs(base) < INFINITY) {
       // an ended beam goes on with the end's token alone
       if (lane < k) {
@@ -307,16 +312,11 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a) 
       }
       continue;
     }
-    const long long at = row * a.chunks;
-    const int parts = ended ? 0 : a.chunks;
-    const float m = lane < parts ? a.part_max[at + lane] : -INFINITY;
-    const double s = lane < parts ? a.part_sum[at + lane] : 0.0;
-    for (int e = lane; e < parts * k; e += 64) list[e] = a.part_key[at * k + e];
     const float top = wave_max(m);
     const double sum = wave_sum64(s == 0.0 ? 0.0 : s * exp((double)m - (double)top));
     const double lse = (double)top + log(sum);
     wave_order();
-    if (!(fabs(base) < INFINITY) || !(fabs(lse) < INFINITY)) {
+    if (ended || !(fabs(base) < INFINITY) || !(fabs(lse) < INFINITY)) {
       // no continuation of its own: the first tokens, behind all others
       if (lane < k) {
         y[lane] = -INFINITY;
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a) 
       continue;
     }
     int head = 0;
-    u64 mine = lane < parts ? list[lane * k] : 0;
+    u64 mine = lane < a.chunks ? list[lane * k] : 0;
     int r = 0;
     for (; r < k; ++r) {
       const unsigned v = wave_umax((unsigned)(mine >> 32));
