@@ -282,104 +282,109 @@ __device__ __forceinline__ u64 ordered(double v) {
   return (u64)b ^ (u64)(b < 0 ? -1ll : (long long)(1ull << 63));
 }
 
-// Joins the parts of each beam's row, a wave for each, and then the request's
-// beams: lane c has part (beam) c's list and its best that is not taken.  The
-// largest of the wave's comes from one reduction; of equal ones the lowest
-// lane's has the lowest index.
-__global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a) {
-  __shared__ double s_y[kMaxBeams * kMaxBeams];
-  __shared__ int s_t[kMaxBeams * kMaxBeams];
-  extern __shared__ u64 s_list[];  // [waves][chunks * k]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, k = a.k;
+// Joins the parts of each beam's row, and then the request's beams.  Of a beam one
+// wave finds the k best, lane c having part c's list and its best that is not
+// taken (of equal logits the lowest lane's has the lowest index), while another
+// makes lse.  Then a thread has one continuation of one beam, whose place is how
+// many come before it: rounds of the wave for these too took 2 us more of 8.
+__global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a, int pairs) {
+  __shared__ __attribute__((aligned(16))) u64 s_key[kMaxBeams * kMaxBeams + 8];
+  __shared__ double s_base[kMaxBeams], s_lse[kMaxBeams];
+  __shared__ unsigned char s_done[kMaxBeams];
+  extern __shared__ u64 s_list[];  // [pairs][chunks * k]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = a.k;
   const long long b = blockIdx.x;
-  u64 *list = s_list + wave * a.chunks * k;
-  for (int beam = wave; beam < a.beams; beam += waves) {
-    const long long row = b * a.beams + beam;
-    double *y = s_y + beam * k;
-    int *t = s_t + beam * k;
-    // all that is read, at once (of an ended beam's parts, which have not been made, whatever is there)
-    const long long at = row * a.chunks;
-    const unsigned char ended = a.done ? a.done[row] : 0;
-    const double base = (double)a.scores[row] + 0.0;  // no -0
-    const float m = lane < a.chunks ? a.part_max[at + lane] : -INFINITY;
-    const double s = lane < a.chunks ? a.part_sum[at + lane] : 0.0;
-    for (int e = lane; e < a.chunks * k; e += 64) list[e] = a.part_key[at * k + e];
-    if (ended && fabs(base) < INFINITY) {
-      // an ended beam goes on with the end's token alone
-      if (lane < k) {
-        y[lane] = lane == 0 ? base : -INFINITY;
-        t[lane] = lane == 0 ? a.eos : lane - 1 + (lane - 1 >= a.eos);
-      }
-      continue;
-    }
-    const float top = wave_max(m);
-    const double sum = wave_sum64(s == 0.0 ? 0.0 : s * exp((double)m - (double)top));
-    const double lse = (double)top + log(sum);
-    wave_order();
-    if (ended || !(fabs(base) < INFINITY) || !(fabs(lse) < INFINITY)) {
-      // no continuation of its own: the first tokens, behind all others
-      if (lane < k) {
-        y[lane] = -INFINITY;
-        t[lane] = lane;
-      }
-      continue;
-    }
-    int head = 0;
-    u64 mine = lane < a.chunks ? list[lane * k] : 0;
-    int r = 0;
-    for (; r < k; ++r) {
-      const unsigned v = wave_umax((unsigned)(mine >> 32));
-      if (v == 0) break;
-      const int first = __builtin_ctzll(__ballot((unsigned)(mine >> 32) == v));
-      if (lane == first) {
-        y[r] = base + ((double)logit_of(mine) - lse);
-        t[r] = index_of(mine);
-        ++head;
-        mine = head < k ? list[lane * k + head] : 0;
-      }
-    }
-    if (r < k) {
-      // All other tokens are masked: the lowest of them, of the first 64 (r < k <= 32
-      // are taken, and k <= vocab).
+  if (wave < pairs) {
+    u64 *list = s_list + wave * a.chunks * k;
+    for (int beam = wave; beam < a.beams; beam += pairs) {
+      const long long at = (b * a.beams + beam) * a.chunks;  // (of an ended beam's parts, whatever is there)
+      wave_order();  // the list before this one has been read
+      for (int e = lane; e < a.chunks * k; e += 64) list[e] = a.part_key[at * k + e];
       wave_order();
-      bool there = lane < a.vocab;
-      for (int i = 0; i < r; ++i) there = there && t[i] != lane;
-      const u64 masked = __ballot(there);
-      const int place = r + __builtin_popcountll(masked & ((1ull << lane) - 1));
-      wave_order();
-      if (there && place < k) {
-        y[place] = -INFINITY;
-        t[place] = lane;
+      const u64 *next = list + lane * k, *const end = lane < a.chunks ? next + k : next;
+      u64 mine = next < end ? *next++ : 0;
+      for (int r = 0; r < k; ++r) {
+        const u64 then = next < end ? *next : 0;
+        const unsigned v = wave_umax((unsigned)(mine >> 32));
+        const int first = __builtin_ctzll(__ballot((unsigned)(mine >> 32) == v));
+        if (lane == first) {
+          s_key[beam * k + r] = mine;  // 0 where none is left
+          mine = then;
+          ++next;
+        }
       }
+    }
+  } else if (wave < 2 * pairs) {
+    for (int beam = wave - pairs; beam < a.beams; beam += pairs) {
+      const long long row = b * a.beams + beam, at = row * a.chunks;
+      const float m = lane < a.chunks ? a.part_max[at + lane] : -INFINITY;
+      const double s = lane < a.chunks ? a.part_sum[at + lane] : 0.0;
+      if (lane == 0) {
+        s_done[beam] = a.done ? a.done[row] : 0;
+        s_base[beam] = (double)a.scores[row] + 0.0;  // no -0
+      }
+      const float top = wave_max(m);
+      const double sum = wave_sum64(s == 0.0 ? 0.0 : s * exp((double)m - (double)top));
+      if (lane == 0) s_lse[beam] = (double)top + log(sum);
     }
   }
   __syncthreads();
-  if (wave != 0) return;
-  // Lane b has beam b's list; where none is left, 0, which is less than -infinity's number.
-  int head = 0, token = 0;
-  double y = 0.0;
+  // continuation e % k of beam e / k: its token, its score and that as a key
+  const int n = a.beams * k;
+  int token = 0;
+  double y = -INFINITY;
   u64 key = 0;
-  const auto take = [&] {
-    const bool there = lane < a.beams && head < k;
-    y = there ? s_y[lane * k + head] : 0.0;
-    token = there ? s_t[lane * k + head] : 0;
-    key = there ? ordered(y) : 0;
-  };
-  take();
-  for (int r = 0; r < k; ++r) {
-    const unsigned hi = wave_umax((unsigned)(key >> 32));
-    const unsigned lo = wave_umax((unsigned)(key >> 32) == hi ? (unsigned)key : 0u);
-    const int first = __builtin_ctzll(__ballot(key == ((u64)hi << 32 | lo)));
-    if (lane == first) {
-      const long long to = b * k + r;
-      a.tokens[to] = token;
-      a.parents[to] = lane;
-      a.scores_out[to] = (float)y;
-      if (a.done_out) a.done_out[to] = (a.done && a.done[b * a.beams + lane]) || token == a.eos;
-      ++head;
-      take();
+  const int e = threadIdx.x;
+  if (e < n) {
+    const int beam = e / k, r = e - beam * k;
+    const double base = s_base[beam], lse = s_lse[beam];
+    const bool ended = s_done[beam] != 0, fine = fabs(base) < INFINITY;
+    const u64 best = s_key[e];
+    if (ended && fine) {
+      // an ended beam goes on with the end's token alone
+      y = r == 0 ? base : -INFINITY;
+      token = r == 0 ? a.eos : r - 1 + (r - 1 >= a.eos);
+    } else if (ended || !fine || !(fabs(lse) < INFINITY)) {
+      // no continuation of its own: the first tokens, behind all others
+      token = r;
+    } else if (best) {
+      y = base + ((double)logit_of(best) - lse);
+      token = index_of(best);
+    } else {
+      // all other tokens are masked: the lowest of them, in order
+      int skip = r;
+      for (int i = 0; i < k; ++i) skip -= s_key[beam * k + i] != 0;
+      for (token = 0;; ++token) {  // ends: k <= vocab, and fewer than k are taken
+        bool taken = false;
+        for (int i = 0; i < k; ++i) {
+          const u64 other = s_key[beam * k + i];
+          taken = taken || (other != 0 && index_of(other) == token);
+        }
+        if (!taken && skip-- == 0) break;
+      }
     }
+    key = ordered(y);
   }
+  __syncthreads();  // the beams' lists have been read
+  if (e < n) s_key[e] = key;
+  if (e < 8) s_key[n + e] = 0;
+  __syncthreads();
+  if (e >= n) return;
+  // the larger score, of equal ones the lower beam's, then its larger logit's
+  int place = 0;
+  for (int j = 0; j < n; j += 8) {
+    u64 other[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) other[i] = s_key[j + i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) place += other[i] > key || (other[i] == key && j + i < e);
+  }
+  if (place >= k) return;
+  const long long to = b * k + place;
+  a.tokens[to] = token;
+  a.parents[to] = e / k;
+  a.scores_out[to] = (float)y;
+  if (a.done_out) a.done_out[to] = s_done[e / k] != 0 || token == a.eos;
 }
 
 template <bool VEC>
@@ -403,8 +408,10 @@ hipError_t launch_beam_select(const BeamArgs &a, bool vec, hipStream_t s) {
     launch_rows<false>(a, s);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int most = std::min(kJoinWaves, kJoinEntries / (a.chunks * a.k)), waves = std::min(a.beams, most);
-  beam_join_kernel<<<(unsigned)a.batch, 64 * waves, (size_t)waves * a.chunks * a.k * sizeof(u64), s>>>(a);
+  // two waves a beam, and a thread for each of its continuations
+  const int pairs = std::min({a.beams, kJoinWaves / 2, kJoinEntries / (a.chunks * a.k)});
+  const int waves = std::max(2 * pairs, (a.beams * a.k + 63) / 64);
+  beam_join_kernel<<<(unsigned)a.batch, 64 * waves, (size_t)pairs * a.chunks * a.k * sizeof(u64), s>>>(a, pairs);
   return hipGetLastError();
 }
 
