@@ -526,3 +526,162 @@ def test_search(backend, fmt, layout, captured):
             _, kr, vr = rows_of(history[r][j], range(len(history[r][j])))
             for o, w in zip(back, (kr, vr)):
                 assert same(o[r * K + j, :, :len(w)].cpu().numpy().transpose(1, 0, 2), w)
+
+
+# ---------------------------------------------------------------------------
+# long rows of many requests, streams, threads
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("V", [20001, 33000])
+def test_select_many_rows(backend, V):
+    """So many rows that a workgroup takes a whole one, in several turns: ties over
+    the turns' borders, floods of equal logits early and late, masks that leave
+    the first turn, all turns but the last, or a few tokens."""
+    B, K, k = 40, 26, 20
+    rng = np.random.default_rng(V)
+    logits = (2 * rng.standard_normal((B, K, V))).astype(np.float32)
+    logits[0] = 1.5
+    logits[1, :, :4096] = -np.inf
+    logits[2, :, : V - 30] = -np.inf
+    logits[3] = -np.inf
+    logits[3, :, [5, 4095, 4096, 4097, 8191, 8192, V - 1]] = 2.0
+    logits[4, :, 4000:4200] = 40.0
+    logits[5, :, -300:] = 40.0
+    logits[6, :, ::7] = 9.25
+    logits[7] = np.sort(logits[7], -1)
+    logits[8] = np.sort(logits[8], -1)[:, ::-1]
+    logits[9] = rng.integers(-3, 4, (K, V))
+    logits[10, :, 200:] = -np.inf
+    logits[10, :, :200] = 0.5
+    logits[11, 3, 9000], logits[11, 4, V - 1] = np.nan, np.inf
+    scores = (-3 * rng.random((B, K))).astype(np.float32)
+    scores[12] = -1.25
+    logits[12] = logits[12, 0]
+    check_select(backend, logits, scores, k)
+    done = (rng.random((B, K)) < 0.3).astype(np.uint8)
+    check_select(backend, logits, scores, k, done, 4096)
+
+
+def test_streams_of_their_own(backend):
+    """The calls on two streams at once, each with its own buffers, by the stream
+    that is current and by the argument: the results of one after the other."""
+    rng = np.random.default_rng(77)
+    V, K = 9001, 4
+    sides = []
+    for i in range(2):
+        s = {"logits": cuda((2 * rng.standard_normal((8, K, V))).astype(np.float32)), "scores": torch.zeros(8, K, device="cuda"),
+             "tokens": i32(np.zeros((8, K))), "parents": i32(np.zeros((8, K))), "out": torch.zeros(8, K, device="cuda"),
+             "ws": backend.beam_workspace(8, K, V, K), "kv": PagedKV(200, 16, 2, 64, "fp4"),
+             "table": cuda(rng.permutation(200)[:192].reshape(32, 6).astype(np.int32)), "lens": i32([90] * 32),
+             "to": torch.zeros(32, 6, dtype=torch.int32, device="cuda"), "src": i32([0] * 32),
+             "q": torch.randn(32, 6, 64, device="cuda"), "pos": i32(rng.integers(0, 1 << 20, 32)), "rot": torch.zeros(32, 6, 64, device="cuda")}
+        for t in (s["kv"].k, s["kv"].v):
+            t.random_(0, 256)
+        for t in (s["kv"].k_scales, s["kv"].v_scales):
+            t.random_(120, 130)
+        sides.append(s)
+    rope = Rope(64, 10000.0, "interleaved")
+
+    def run(s, stream=None):
+        backend.dev_beam_select(s["logits"], s["scores"], s["tokens"], s["parents"], s["out"], s["ws"], stream=stream)
+        backend.dev_beam_reorder(s["table"], s["parents"], s["to"], s["src"], stream=stream)
+        backend.dev_paged_copy(s["kv"], s["to"], s["src"], s["lens"], stream=stream)
+        backend.dev_rope(rope, s["q"], None, s["pos"], s["rot"], stream=stream)
+
+    keys = ("tokens", "parents", "out", "to", "src", "rot")
+    pools = [(s["kv"].k.clone(), s["kv"].v.clone()) for s in sides]
+    want = []
+    for s in sides:
+        run(s)
+        torch.cuda.synchronize()
+        want.append([s[k].clone() for k in keys] + [s["kv"].k.clone(), s["kv"].v.clone()])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for s, (k, v) in zip(sides, pools):
+            s["kv"].k.copy_(k)
+            s["kv"].v.copy_(v)
+            for n in keys:
+                s[n].zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            run(sides[0])
+        run(sides[1], streams[1])
+        torch.cuda.synchronize()
+        for s, w in zip(sides, want):
+            for got, exp in zip([s[k] for k in keys] + [s["kv"].k, s["kv"].v], w):
+                assert torch.equal(got, exp)
+
+
+def test_two_threads(backend):
+    """Two host threads make the calls side by side, on streams of their own."""
+    import threading
+
+    V, K, n = 3001, 3, 50
+    rope = Rope(32, 10000.0)
+    wrong = []
+
+    def work(seed):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                g = torch.Generator(device="cuda").manual_seed(seed)
+                x = torch.randn(2, K, V, device="cuda", generator=g)
+                q = torch.randn(n, 2, 48, device="cuda", generator=g)
+                p = torch.randint(0, 9999, (n,), device="cuda", dtype=torch.int32, generator=g)
+                ws, first = backend.beam_workspace(2, K, V, K), None
+                for _ in range(30):
+                    t, par = (torch.zeros(2, K, dtype=torch.int32, device="cuda") for _ in range(2))
+                    out, rot = torch.zeros(2, K, device="cuda"), torch.zeros_like(q)
+                    backend.dev_beam_select(x, torch.zeros(2, K, device="cuda"), t, par, out, ws)
+                    backend.dev_rope(rope, q, None, p, rot)
+                    got = [y.clone() for y in (t, par, out, rot)]
+                    stream.synchronize()
+                    if first is not None and not all(torch.equal(a, b) for a, b in zip(first, got)):
+                        wrong.append(seed)
+                    first = got
+        except Exception as e:  # noqa: BLE001 (reported by the test)
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not wrong and not any(t.is_alive() for t in threads)
+
+
+@pytest.mark.parametrize("n", [1, 64])
+def test_extend_and_release_captured(backend, n):
+    """One graph of an extend and a release, replayed on other counts."""
+    rng = np.random.default_rng(n)
+    page, width, free = 16, 8, 8 * n
+    t = Tables(rng, rng.integers(0, 60, n), width, page, free, cap=free + 8 * n)
+    table, lens, stack, count = cuda(t.table), cuda(t.lens), cuda(t.free), i32([free])
+    new, which = i32([1] * n), torch.zeros(n, dtype=torch.uint8, device="cuda")
+    seqs, pos, off = i32([0] * 40 * n), i32([0] * 40 * n), i32([0] * (n + 1))
+    l2, c2, l3, c3 = i32([0] * n), i32([0]), i32([0] * n), i32([0])
+
+    def both():
+        backend.dev_paged_extend(table, lens, new, stack, count, page, seqs, pos, off, l2, c2)
+        backend.dev_paged_release(table, l2, which, stack, c2, page, l3, c3)
+
+    g = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        both()
+    torch.cuda.current_stream().wait_stream(s)
+    with torch.cuda.graph(g):
+        both()
+    for i in range(4):
+        table.copy_(cuda(t.table))
+        stack.copy_(cuda(t.free))
+        more, gone = rng.integers(0, 40, n), (rng.random(n) < 0.5).astype(np.uint8)
+        new.copy_(i32(more))
+        which.copy_(cuda(gone))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        a = extend(t.table, t.lens, more, t.free, free, page, 40 * n)
+        b = release(a[0], a[1], gone, None, t.free, a[2], page)
+        for got, w in zip((seqs, pos, off, l2, table, l3, stack, c3), (a[3], a[4], a[6], a[1], b[0], b[1], b[2], [b[3]])):
+            assert np.array_equal(got.cpu().numpy(), w)
