@@ -876,7 +876,7 @@ extern "C" int bnr_last_error_parts(const char **first, const char **second) {
   return g_err.kind;
 }
 
-extern "C" uint32_t bnr_abi_version(void) { return (1u << 16) | 3u; }
+extern "C" uint32_t bnr_abi_version(void) { return (1u << 16) | 4u; }
 
 extern "C" int bnr_create(int device_id, bnr_ctx **out) {
   if (!out) return err_backend("bnr_create: out is NULL");

@@ -4,16 +4,19 @@
 //   score(b, t) = scores[b] + logit[b, t] - lse[b],   lse = log sum_t exp(logit)
 //
 // Within a beam the order is that of the logits, so one pass over them finds
-// the sum and the k best: a workgroup holds its first logits in registers, and what
-// is under the k-th largest of a wave's 64 lane maxima (at least k logits are
-// no smaller) is not among the k best.  The few that are left are ranked by
-// counting.  A second launch joins the parts of each row and then the beams.
+// the sum and the k best: of a workgroup's first logits, in registers, the threads'
+// maxima give a threshold that at least k of them reach, and the few that do are
+// ranked by counting at the end.  A second launch joins the parts of each row and
+// then the beams.
 //
 // Beams are compared by scores in 64 bits: lse is what the order of two beams'
 // continuations hangs on, so its exponentials carry the part of log2(e) that
 // fp32 leaves out and their sums are joined in 64 bits.
 //
-// Bound by the logits' bytes, read once.
+// Read once, the logits of 16 requests of 8 beams and 128256 tokens (61 MB) take 8.6
+// us at the rate of a plain read; the rows' launch takes 16.2, of which 12.0 are
+// left without search, candidates and exponentials (its start, the first load and
+// the stream), and the join 5.8.  Four beams: 4.8 and 4.3, all latency.
 #include "bnr_device.h"
 
 #include <algorithm>

@@ -16,6 +16,18 @@
 // The conversion multiplies with the group's power of two, and bf16 holds a
 // code times a power exactly: no scale is left for the scores or the weights,
 // and a NaN group (exponent 255) comes out as NaN.
+//
+// With at most four query heads a kv head the three parts of q and of the weights
+// are columns 4 part + head of one product instead of three products (64
+// sequences of up to 32768 rows, 20/5 heads of 128: 172 -> 150 us; a short call
+// pays 0.3 us for adding the columns at its end).  V's exponents come 16 bytes a
+// load there (150 -> 136).
+//
+// Bound by the rows' bytes where there are many: those 64 sequences take 136 us,
+// 5.4 TB/s, their loads alone 124.  262 vector instructions of a wave's step, 64 of
+// them conversions.  Loads two steps ahead (148), steps of 64 rows (141; short
+// shares lose more) and a third workgroup a CU (137) gained nothing.  A short call
+// is latency as in the other formats: 9.0 us over 4096 rows.
 #include "bnr_paged_mfma.h"
 
 #include <type_traits>

@@ -2,8 +2,9 @@
  * bitnet_hip.h -- C ABI of the MI355X (gfx950) GQA attention hot path of
  * bitnetrs: RoPE (half-split, any theta) on Q/K, KV-cache append into an
  * HBM-resident head-major cache, split-K decode attention and causal
- * flash prefill; the same over a paged cache that may hold its rows in 16 or
- * 8 bits; and the W2A8 ternary GEMV of the layer projections.
+ * flash prefill; the same over a paged cache that may hold its rows in 16, 8 or
+ * 4 bits, with the page tables, beam search and rotary forms that go with it; and
+ * the W2A8 ternary GEMV of the layer projections.
  *
  * Conventions
  *  - Every entry point returns an int status (BNR_OK == 0) and never aborts.
