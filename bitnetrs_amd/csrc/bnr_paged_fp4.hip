@@ -24,7 +24,7 @@
 // load there (150 -> 136).
 //
 // Bound by the rows' bytes where there are many: those 64 sequences take 136 us,
-// 5.4 TB/s, their loads alone 124.  262 vector instructions of a wave's step, 64 of
+// 5.4 TB/s, their loads alone 124.  254 vector instructions of a wave's step, 64 of
 // them conversions.  Loads two steps ahead (148), steps of 64 rows (141; short
 // shares lose more) and a third workgroup a CU (137) gained nothing.  A short call
 // is latency as in the other formats: 9.0 us over 4096 rows.
