@@ -19,15 +19,16 @@
 //
 // With at most four query heads a kv head the three parts of q and of the weights
 // are columns 4 part + head of one product instead of three products (64
-// sequences of up to 32768 rows, 20/5 heads of 128: 172 -> 150 us; a short call
-// pays 0.3 us for adding the columns at its end).  V's exponents come 16 bytes a
+// sequences of up to 32768 rows, 20/5 heads of 128: 172 -> 150 us; short calls, which
+// would pay 0.2 to 0.8 us for adding the columns at a piece's end, keep the
+// products).  V's exponents come 16 bytes a
 // load there (150 -> 136).
 //
 // Bound by the rows' bytes where there are many: those 64 sequences take 136 us,
 // 5.4 TB/s, their loads alone 124.  254 vector instructions of a wave's step, 64 of
 // them conversions.  Loads two steps ahead (148), steps of 64 rows (141; short
 // shares lose more) and a third workgroup a CU (137) gained nothing.  A short call
-// is latency as in the other formats: 9.0 us over 4096 rows.
+// is latency as in the other formats: 8.8 us over 4096 rows.
 #include "bnr_paged_mfma.h"
 
 #include <type_traits>
@@ -402,7 +403,14 @@ hipError_t launch_paged_decode_fp4(const PagedDecodeArgs &a, hipStream_t s) {
   const dim3 grid((unsigned)a.wgs), block(64 * kW);
   // what a workgroup gets unasked is 64 KB, of which up to 32 are static
   constexpr size_t kUnasked = 32 * 1024;
-  const auto kernel = a.group <= 4 ? kernel_of<true>(d) : kernel_of<false>(d);
+  // Columns instead of products pay once a wave has more than two steps or so; what
+  // they cost is the adding at a piece's end.  20/5 heads of 128: 4 sequences of 4096
+  // rows (640 units) 11.9 us, 11.1 with products, 8 of them (1280) 14.3 and 14.2, 32 of
+  // 128 to 4096 21.9 and 22.5; 16 of 2000 of 8/8 heads (2048) 14.3 and 15.0.
+  const long long rows = a.pool.table_stride * a.pool.page;
+  const long long units = (rows + a.tile - 1) / a.tile * a.batch * a.pool.n_kv;
+  const bool pack = a.group <= 4 && units > 2 * kPagedMaxWgs;
+  const auto kernel = pack ? kernel_of<true>(d) : kernel_of<false>(d);
   if (lds > kUnasked) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

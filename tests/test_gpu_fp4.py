@@ -126,6 +126,11 @@ def test_read(backend, hq, hkv, d, page):
             assert (o[s, :, b - a:] == 3).all()
 
 
+def room(n_seqs, hkv, page, wide):
+    """Pages of a table with room for more than 1024 units of 128 rows, from which on up to four heads share columns."""
+    return 150000 // (n_seqs * hkv * page) + 1 if wide else 0
+
+
 def run_decode(be, pool, hq, lens, seed=1, q=None, out=None):
     rng = np.random.default_rng(seed)
     q = rng.standard_normal((len(lens), hq, pool.d)).astype(np.float32) if q is None else q
@@ -170,16 +175,32 @@ def test_decode_batches(backend, lens):
     check_decode(pool, q, got, lens)
 
 
+@pytest.mark.parametrize("hq,hkv,d,page,n", [(20, 5, 128, 16, 3000), (8, 8, 64, 64, 1500), (3, 1, 256, 16, 9000),
+                                              (6, 3, 80, 32, 2500), (2, 1, 144, 16, 20000), (16, 2, 128, 16, 5000)])
+def test_decode_large_tables(backend, hq, hkv, d, page, n):
+    """Tables with room for many units, where up to four heads share columns:
+    ragged lengths, long, short and none, in the same table."""
+    say(f"decode fp4 {hq}/{hkv}/{d} up to {n} rows")
+    lens = [n, 0, 1, n - 1, 700, n // 2 + 5, 33, n] + [129] * 4
+    pool = Pool4(rng_of("large", hq, d, n), lens, hkv, d, page, width=max(-(-n // page), room(len(lens), hkv, page, True)))
+    q, got = run_decode(backend, pool, hq, lens)
+    check_decode(pool, q, got, lens)
+    assert (got[1] == 0).all()
+    few = [5, 0, 1, 0, 700, 3, 33, 2] + [129] * 4
+    check_decode(pool, *run_decode(backend, pool, hq, few, q=q), few)
+
+
 @pytest.mark.parametrize("hq,hkv,d,page,lens", [(12, 1, 80, 16, [30000]), (16, 1, 128, 64, [17, 21000]),
                                                 (16, 1, 256, 16, [9000]), (4, 1, 64, 128, [40001]),
                                                 (3, 1, 34, 7, [9000])])
-def test_decode_counts_every_row_once(backend, hq, hkv, d, page, lens):
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_counts_every_row_once(backend, hq, hkv, d, page, lens, wide):
     """No score differs, so an output is its column's sum over the number of rows.
     The sum is of small whole numbers and halves, exact in fp32; what is left is
     the waves' and pieces' factors (powers of two, exact here) and one division:
     a reciprocal's rounding and a product's, 2^-23 together."""
     rng = rng_of("count", hq, d, lens)
-    pool = Pool4(rng, lens, hkv, d, page)
+    pool = Pool4(rng, lens, hkv, d, page, width=max(-(-max(lens) // page), room(len(lens), hkv, page, wide)))
     pool.exps["v"][:] = rng.integers(127, 129, pool.exps["v"].shape)
     q, got = run_decode(backend, pool, hq, lens, q=np.zeros((len(lens), hq, d), np.float32))
     for s, n in enumerate(lens):
@@ -191,11 +212,12 @@ def test_decode_counts_every_row_once(backend, hq, hkv, d, page, lens):
 
 
 @pytest.mark.parametrize("d,page", [(128, 16), (128, 64), (80, 32), (10, 3)])
-def test_decode_missing_pages_and_lengths(backend, d, page):
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_missing_pages_and_lengths(backend, d, page, wide):
     """Pages that are not there are left out; lengths outside the table are cut;
     NaN codes behind a sequence's last row, and in pages of others, do not show."""
     lens = [10 * page, 4 * page + 1, 3 * page, 2]
-    pool = Pool4(rng_of("missing", d, page), lens, 2, d, page)
+    pool = Pool4(rng_of("missing", d, page), lens, 2, d, page, width=max(10, room(4, 2, page, wide)))
     n_pages = pool.codes["k"].shape[0]
     for n in "kv":
         used = np.zeros(pool.exps[n].shape[:3], bool)
@@ -210,15 +232,16 @@ def test_decode_missing_pages_and_lengths(backend, d, page):
     check_decode(pool, q, got, asked)
     assert (got[2] == 0).all()
     q, got = run_decode(backend, pool, 4, [1 << 30, -5, 0, 2])
-    check_decode(pool, q, got, [10 * page, 0, 0, 2])
+    check_decode(pool, q, got, [pool.table.shape[1] * page, 0, 0, 2])
 
 
 @pytest.mark.parametrize("d,page", [(128, 16), (64, 16), (256, 16), (80, 32), (26, 4)])
-def test_decode_non_finite_groups_show(backend, d, page):
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_non_finite_groups_show(backend, d, page, wide):
     """A NaN group in V makes its columns NaN, one in K the heads that read it; no
     other sequence, head or column."""
     lens = [200, 200, 200]
-    pool = Pool4(rng_of("nan", d), lens, 2, d, page)
+    pool = Pool4(rng_of("nan", d), lens, 2, d, page, width=max(-(-200 // page), room(3, 2, page, wide)))
     g = groups(d) - 1
     pool.exps["v"][pool.table[0, 77 // page], 1, 77 % page, g] = 255
     pool.exps["k"][pool.table[1, 150 // page], 0, 150 % page, 0] = 255
@@ -236,10 +259,11 @@ def test_decode_non_finite_groups_show(backend, d, page):
 
 
 @pytest.mark.parametrize("d,page", [(128, 16), (26, 4)])
-def test_decode_scores_of_any_size(backend, d, page):
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_scores_of_any_size(backend, d, page, wide):
     """Scores hundreds apart, and groups of very different powers."""
     lens = [700, 90]
-    pool = Pool4(rng_of("wide", d), lens, 2, d, page, spread=6.0)
+    pool = Pool4(rng_of("wide", d), lens, 2, d, page, width=max(-(-700 // page), room(2, 2, page, wide)), spread=6.0)
     q, got = run_decode(backend, pool, 4, lens)
     check_decode(pool, q, got, lens)
 

@@ -244,6 +244,16 @@ def test_select_padded_rows(backend, V, pad):
     check_select(backend, logits[:1, :1], np.zeros((1, 1), np.float32), 4, device=one)
 
 
+def test_select_rows_past_32_bits(backend):
+    """Rows further apart than 32 bits count elements."""
+    rng = np.random.default_rng(3)
+    V, far = 2000, (1 << 31) + 8
+    logits = (2 * rng.standard_normal((1, 3, V))).astype(np.float32)
+    wide = torch.empty(2 * far + V, device="cuda").as_strided((1, 3, V), (3 * far, far, 1))
+    wide.copy_(cuda(logits))
+    check_select(backend, logits, np.array([[-1, -0.5, -2]], np.float32), 3, device=wide)
+
+
 def test_select_same_bits_captured(backend):
     """Replayed on new logits; one workspace for two shapes, one after the other."""
     B, K, V = 4, 4, 30001

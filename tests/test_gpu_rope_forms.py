@@ -132,6 +132,20 @@ def test_tables_are_the_same_rotation(backend, dim):
     assert torch.equal(some[0], cos[8000:8100]) and torch.equal(some[1], sin[8000:8100])
 
 
+def test_tokens_past_32_bits(backend):
+    """Tokens further apart than 32 bits count elements, read and written."""
+    rope, far = Rope(64, 10000.0), (1 << 31) + 16
+    x = torch.randn(2, 3, 64, device="cuda", dtype=torch.float16)
+    big = torch.empty(far + 192, dtype=torch.float16, device="cuda").as_strided((2, 3, 64), (far, 64, 1))
+    big.copy_(x)
+    p, want, out = i32([7, 123456]), torch.empty_like(x), torch.empty_like(x)
+    backend.dev_rope(rope, x, None, p, want)
+    backend.dev_rope(rope, big, None, p, out)
+    assert torch.equal(out, want)
+    backend.dev_rope(rope, big, None, p)
+    assert torch.equal(big, want)
+
+
 def test_special_values(backend):
     """Infinities and NaN stay in their pairs; zeros stay zero."""
     rope = Rope(8, 100.0)
