@@ -146,6 +146,24 @@ def test_tokens_past_32_bits(backend):
     assert torch.equal(big, want)
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_more_tokens_than_a_launch_holds(backend, layout):
+    """2^26 workgroups' tokens and some: as calls over parts of them."""
+    rope, n = Rope(2, 10000.0, layout=layout), (5 << 24) + 5
+    x = torch.randn(1 << 20, 1, 2, device="cuda", dtype=torch.bfloat16).repeat(81, 1, 1)[:n].contiguous()
+    p = torch.arange(n, dtype=torch.int32, device="cuda")
+    p[::7] = -1
+    q, k = x.clone(), torch.zeros_like(x)
+    backend.dev_rope(rope, q, x, p, None, k)
+    for a in range(0, n, 1 << 22):
+        b = min(n, a + (1 << 22))
+        part = x[a:b].clone()
+        backend.dev_rope(rope, part, None, p[a:b])
+        assert torch.equal(q[a:b], part)
+        part[p[a:b] < 0] = 0
+        assert torch.equal(k[a:b], part)
+
+
 def test_special_values(backend):
     """Infinities and NaN stay in their pairs; zeros stay zero."""
     rope = Rope(8, 100.0)
