@@ -292,6 +292,17 @@ struct Unit<2> { typedef unsigned short type; };
 template <>
 struct Unit<1> { typedef unsigned char type; };
 
+// Whole lines go out with the non-temporal hint: 16 requests of 8 beams, 523 bf16 rows of 5 heads of 128 each,
+// 31.5 -> 26.7 us with the tables'; eight layers copied and then attended over, as a step does, 86.3 -> 80.0 a
+// layer; each layer's attention right behind its copy 74.3 -> 75.2.
+template <int U, class T>
+__device__ __forceinline__ void store_unit(T *p, T v) {
+  if constexpr (U == 16)
+    __builtin_nontemporal_store(v, p);
+  else
+    *p = v;
+}
+
 template <int U>
 __global__ __launch_bounds__(kThreads) void paged_copy_kernel(PagedCopyArgs a) {
   typedef typename Unit<U>::type T;
@@ -327,8 +338,8 @@ __global__ __launch_bounds__(kThreads) void paged_copy_kernel(PagedCopyArgs a) {
 #pragma unroll
         for (int i = 0; i < kCopyPasses; ++i)
           if (to[i] >= 0) {
-            ko[to[i] * units + x] = ks[i];
-            vo[to[i] * units + x] = vs[i];
+            store_unit<U>(ko + to[i] * units + x, ks[i]);
+            store_unit<U>(vo + to[i] * units + x, vs[i]);
           }
       }
     }
