@@ -3285,11 +3285,11 @@ int rope_heads(const bnr_heads *h, const char *name, size_t n_tokens, size_t d, 
   return BNR_OK;
 }
 
-// Whether every row starts at a 16-byte boundary.
-bool rope_aligned(const RopeHeads &r, size_t size) {
-  const uintptr_t bits = ((uintptr_t)r.in_token | (uintptr_t)r.in_head | (uintptr_t)r.out_token |
-                          (uintptr_t)r.out_head) * size;
-  return r.heads == 0 || (aligned16(r.in) && aligned16(r.out) && bits % 16 == 0);
+// Where the rows start: addresses and distances in bytes, or'ed.
+size_t rope_starts(const RopeHeads &r, size_t size) {
+  if (r.heads == 0) return 0;
+  return (uintptr_t)r.in | (uintptr_t)r.out |
+         ((size_t)r.in_token | (size_t)r.in_head | (size_t)r.out_token | (size_t)r.out_head) * size;
 }
 
 }  // namespace
@@ -3317,10 +3317,12 @@ extern "C" int bnr_dev_rope(bnr_ctx *c, const bnr_rope *rope, int type, size_t n
   a.d = (int)head_dim;
   a.pairs = (int)rope->n_pairs;
   a.magnitude = rope->magnitude;
-  const size_t unit = 16 / size, run = rope->layout == BNR_ROPE_HALF ? rope->n_pairs : 2 * rope->n_pairs;
-  const bool vec = run % unit == 0 && head_dim % unit == 0 && rope_aligned(a.q, size) && rope_aligned(a.k, size);
+  // rows, their runs of pairs and what lies behind them
+  const size_t run = rope->layout == BNR_ROPE_HALF ? rope->n_pairs : 2 * rope->n_pairs;
+  const size_t bits = run * size | head_dim * size | rope_starts(a.q, size) | rope_starts(a.k, size);
+  const int bytes = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : 0;
   DeviceGuard dg(c->device);
-  HIP_TRY(launch_rope(a, type, rope->layout == BNR_ROPE_HALF, vec, (hipStream_t)stream), "rope launch");
+  HIP_TRY(launch_rope(a, type, rope->layout == BNR_ROPE_HALF, bytes, (hipStream_t)stream), "rope launch");
   return set_ok();
 }
 

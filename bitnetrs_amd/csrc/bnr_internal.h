@@ -811,8 +811,8 @@ struct RopeArgs {
   float magnitude;
   double turns[kRopeMaxPairs];  // of a pair, a position
 };
-// vec: rows, their pairs' runs and d in 16-byte units.
-hipError_t launch_rope(RopeArgs a, int type, bool half, bool vec, hipStream_t s);
+// bytes: rows, their pairs' runs and d are whole units of 16 or 8 bytes; 0: neither.
+hipError_t launch_rope(RopeArgs a, int type, bool half, int bytes, hipStream_t s);
 
 struct RopeTableArgs {
   float *cos_out, *sin_out;  // [n_positions][pairs]

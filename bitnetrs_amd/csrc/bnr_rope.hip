@@ -39,43 +39,53 @@ __device__ __forceinline__ void rotate(T &p, T &q, float2 cs) {
   q = (T)z;
 }
 
-// N elements (16 bytes at most) at p.
+// N elements at p; WIDE: 8 or 16 aligned bytes in one access.
 template <class T, int N>
 struct Some {
   T x[N];
 };
-template <class T, int N>
+template <int BYTES>
+struct Words {
+  typedef unsigned type __attribute__((ext_vector_type(BYTES / 4)));
+};
+template <bool WIDE, class T, int N>
 __device__ __forceinline__ Some<T, N> load_some(const T *p) {
   Some<T, N> r;
-  if constexpr (sizeof(r) == 16) {
-    typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    const u4 w = *reinterpret_cast<const u4 *>(p);
-    __builtin_memcpy(&r, &w, 16);
+  if constexpr (WIDE) {
+    typedef typename Words<sizeof(r)>::type W;
+    const W w = *reinterpret_cast<const W *>(p);
+    __builtin_memcpy(&r, &w, sizeof(r));
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) r.x[i] = p[i];
   }
   return r;
 }
-template <class T, int N>
+template <bool WIDE, class T, int N>
 __device__ __forceinline__ void store_some(T *p, const Some<T, N> &r) {
-  if constexpr (sizeof(r) == 16) {
-    typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    u4 w;
-    __builtin_memcpy(&w, &r, 16);
-    *reinterpret_cast<u4 *>(p) = w;
+  if constexpr (WIDE) {
+    typedef typename Words<sizeof(r)>::type W;
+    W w;
+    __builtin_memcpy(&w, &r, sizeof(r));
+    if constexpr (sizeof(r) == 16)
+      __builtin_nontemporal_store(w, reinterpret_cast<W *>(p));
+    else
+      *reinterpret_cast<W *>(p) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = r.x[i];
   }
 }
 
-// U: elements of 16 bytes, or 1 where alignment or sizes leave no more.  A step of
+// U: elements of 16 bytes, of 8, or 1 where alignment or sizes leave no more.  A step of
 // a thread is U pairs of two runs (half), U / 2 pairs of one run (interleaved; one
 // pair where U is 1), or U elements that are copied: neighbouring threads' steps
 // are neighbours, so a wave's loads and stores are whole lines.  16384 tokens of
-// 32/8 bf16 heads of 128, 32 of them rotated in pairs of neighbours: 69 us, 95 % of a
-// copy's rate; with 32 bytes a thread 80, with non-temporal stores 103.
+// 32/8 bf16 heads of 128, 32 of them rotated in pairs of neighbours: 66 us, 5.1 TB/s,
+// as a copy; with 32 bytes a thread 80.  16 bytes go out with the non-temporal hint (69
+// without; with kernels that make q and read it 158 both; 64 tokens 3.7 both).  4096
+// tokens of 32/8 bf16 heads of 80, 40 of them rotated in halves, so that runs are units
+// of 8 bytes: 14 us, 44 with single elements.
 template <class T, int U, bool HALF>
 __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
   __shared__ float2 s_cs[kThreads > kRopeMaxPairs ? kThreads : kRopeMaxPairs];
@@ -114,9 +124,9 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
         out[n] = static_cast<T *>(o.out) + (token0 + t) * o.out_token + head * o.out_head;
         at[n] = t;
         there[n] = r0 + n * per < rows && s_pos[t] >= 0 && (turn || in != out[n]);
-        if (W == U || turn) x[n] = load_some<T, W>(in + e);
+        if (W == U || turn) x[n] = load_some<(U > 1), T, W>(in + e);
         else x[n].x[0] = in[e];
-        if (HALF) x2[n] = load_some<T, W>(in + e2);
+        if (HALF) x2[n] = load_some<(U > 1), T, W>(in + e2);
       }
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -130,10 +140,10 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
             else
               rotate(x[n].x[2 * j], x[n].x[2 * j + 1], cs[j]);
           }
-          if (HALF) store_some(out[n] + e2, x2[n]);
+          if (HALF) store_some<(U > 1)>(out[n] + e2, x2[n]);
         }
         if (W == U || turn)
-          store_some(out[n] + e, x[n]);
+          store_some<(U > 1)>(out[n] + e, x[n]);
         else
           out[n][e] = x[n].x[0];
       }
@@ -180,29 +190,31 @@ void launch_layout(RopeArgs &a, bool half, hipStream_t s) {
 }
 
 template <class T>
-void launch_type(RopeArgs &a, bool half, bool vec, hipStream_t s) {
-  if (vec)
+void launch_type(RopeArgs &a, bool half, int bytes, hipStream_t s) {
+  if (bytes == 16)
     launch_layout<T, 16 / sizeof(T)>(a, half, s);
+  else if (bytes == 8)
+    launch_layout<T, 8 / sizeof(T)>(a, half, s);
   else
     launch_layout<T, 1>(a, half, s);
 }
 
 }  // namespace
 
-hipError_t launch_rope(RopeArgs a, int type, bool half, bool vec, hipStream_t s) {
+hipError_t launch_rope(RopeArgs a, int type, bool half, int bytes, hipStream_t s) {
   // tokens of a workgroup: as many as its threads make the angles of, at most
   // four, where there are workgroups enough
   a.tokens = 1;
   if (a.n_tokens >= 2048 && a.pairs <= kThreads / 2) a.tokens = kThreads / a.pairs;
   if (a.tokens > 4) a.tokens = 4;
-  const int unit = vec ? 16 / (type == kRopeF32 ? 4 : 2) : 1;
+  const int unit = bytes ? bytes / (type == kRopeF32 ? 4 : 2) : 1;
   const int steps = (half ? a.pairs / unit : unit > 1 ? 2 * a.pairs / unit : a.pairs) + (a.d - 2 * a.pairs) / unit;
   a.lanes = 1;
   while (a.lanes < steps && a.lanes < kThreads) a.lanes *= 2;
   switch (type) {
-    case kRopeF32: launch_type<float>(a, half, vec, s); break;
-    case kRopeBf16: launch_type<__bf16>(a, half, vec, s); break;
-    case kRopeF16: launch_type<_Float16>(a, half, vec, s); break;
+    case kRopeF32: launch_type<float>(a, half, bytes, s); break;
+    case kRopeBf16: launch_type<__bf16>(a, half, bytes, s); break;
+    case kRopeF16: launch_type<_Float16>(a, half, bytes, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

@@ -43,7 +43,8 @@ def check(got, x, positions, rope, kind):
 
 
 SHAPES = [(20, 5, 128, 128), (32, 8, 128, 32), (14, 2, 80, 40), (4, 4, 64, 16), (2, 1, 256, 256), (3, 3, 96, 6), (1, 1, 2, 2),
-          (5, 1, 34, 34), (2, 2, 512, 512), (3, 1, 130, 128), (2, 1, 7, 6), (4, 2, 48, 24)]
+          (5, 1, 34, 34), (2, 2, 512, 512), (3, 1, 130, 128), (2, 1, 7, 6), (4, 2, 48, 24),
+          (2, 1, 14, 12)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -94,6 +95,29 @@ def test_rope_many_tokens(backend, n, dim):
     back = torch.zeros(3, n, 128, device="cuda").transpose(0, 1)
     backend.dev_rope(rope, None, q, i32(positions), None, back)
     assert torch.equal(back, out)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_alignments(backend, kind, layout):
+    """Rows that start at any element have the bits of aligned ones, and what lies
+    around them stays."""
+    rope, n = Rope(48, 10000.0, layout=layout), 9
+    p = i32(np.arange(n) * 77)
+    x = torch.randn(n, 3, 64, device="cuda").to(TYPES[kind])
+    want = torch.empty_like(x)
+    backend.dev_rope(rope, x, None, p, want)
+    for first, far in ((1, 64), (2, 64), (4, 64), (8, 64), (0, 65), (0, 66), (0, 68), (0, 72), (4, 68), (2, 72)):
+        whole = torch.full((n * 3 * far + 8,), 7.0, dtype=TYPES[kind], device="cuda")
+        rows = whole.as_strided((n, 3, 64), (3 * far, far, 1), first)
+        out = whole.clone().as_strided((n, 3, 64), (3 * far, far, 1), first)
+        rows.copy_(x)
+        backend.dev_rope(rope, rows, x, p, out, torch.empty_like(x))
+        assert torch.equal(out, want), (first, far)
+        backend.dev_rope(rope, rows, None, p)
+        assert torch.equal(rows, want), (first, far)
+        rows.fill_(7.0)
+        assert (whole == 7).all(), (first, far)
 
 
 def test_shared_rows_as_input(backend):
