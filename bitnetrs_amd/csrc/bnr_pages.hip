@@ -273,8 +273,9 @@ __global__ __launch_bounds__(kThreads) void beam_reorder_kernel(BeamTableArgs a)
 // Copy: rows starts[s] .. lens[s]-1 of sequence src[s] to sequence s, their codes
 // and scales as they are, in equal shares of all rows that are to be copied;
 // `lanes` threads share a row.  Bound by the rows' bytes, read and written: 126 MB in
-// 27.9 us, 4.5 TB/s (16 requests of 8 beams, 523 bf16 rows of 5 heads of 128 each;
-// shares of 32 rows 34, of 16 rows 48, two rows of a thread on their way 29).
+// 24.1 us, 5.2 TB/s (16 requests of 8 beams, 523 bf16 rows of 5 heads of 128 each;
+// 27.9 before stores had the non-temporal hint, then shares of 32 rows 34, of 16 rows
+// 48, two rows of a thread on their way 29).
 // ---------------------------------------------------------------------------
 constexpr int kCopyWgs = 4096, kCopyRows = 64;
 constexpr int kCopyPasses = 4;  // rows of a thread on their way at a time
