@@ -527,7 +527,8 @@ class HipBackend:
 
     # beam search -------------------------------------------------------------------
     def beam_workspace(self, batch: int, beams: int, vocab: int, k: int):
-        """A workspace for dev_beam_select of up to that many requests."""
+        """A workspace for dev_beam_select of up to that many requests, beams, tokens
+        and continuations."""
         import torch
 
         n = ctypes.c_size_t()

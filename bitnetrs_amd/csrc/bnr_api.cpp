@@ -3126,8 +3126,7 @@ int check_beams(size_t batch, size_t beams, size_t vocab, size_t k) {
 }
 
 // Of each part: maximum, sum and the k best.
-size_t beam_bytes(size_t batch, size_t beams, size_t vocab, size_t k) {
-  const size_t rows = batch * beams, parts = rows * beam_chunks((long long)rows, (long long)vocab, (int)k);
+size_t beam_bytes(size_t parts, size_t k) {
   return (parts * (sizeof(double) + sizeof(float) + k * sizeof(unsigned long long)) + 15) / 16 * 16;
 }
 
@@ -3139,7 +3138,7 @@ extern "C" int bnr_beam_workspace(bnr_ctx *c, size_t batch, size_t beams, size_t
   if (!bytes) return err_backend("beam_workspace: NULL pointer");
   const int st = check_beams(batch, beams, vocab, k);
   if (st) return st;
-  *bytes = batch ? beam_bytes(batch, beams, vocab, k) : 0;
+  *bytes = beam_bytes((size_t)beam_parts_most((long long)(batch * beams), (long long)vocab), k);
   return set_ok();
 }
 
@@ -3158,11 +3157,12 @@ extern "C" int bnr_dev_beam_select(bnr_ctx *c, const float *logits, size_t row_s
   if (batch == 0) return set_ok();
   if (!logits || !scores || !tokens || !parents || !scores_out || !workspace)
     return err_backend("beam_select: NULL pointer");
-  const size_t need = beam_bytes(batch, beams, vocab, k);
+  const size_t rows = batch * beams, w = sizeof(int32_t);
+  const int chunks = beam_chunks((long long)rows, (long long)vocab, (int)k);
+  const size_t parts = rows * chunks, need = beam_bytes(parts, k);
   if (workspace_bytes < need)
     return err_shape(fmt("workspace of %zu bytes", need), fmt("%zu bytes", workspace_bytes));
   if (!aligned16(workspace)) return err_shape("16-byte aligned workspace", "an unaligned pointer");
-  const size_t rows = batch * beams, w = sizeof(int32_t);
   st = check_apart({{tokens, batch * k * w, "tokens"},
                     {parents, batch * k * w, "parents"},
                     {scores_out, batch * k * w, "scores_out"},
@@ -3186,9 +3186,8 @@ extern "C" int bnr_dev_beam_select(bnr_ctx *c, const float *logits, size_t row_s
   a.vocab = (int)vocab;
   a.k = (int)k;
   a.eos = eos;
-  a.chunks = beam_chunks((long long)rows, (long long)vocab, (int)k);
-  a.chunk = (int)(((vocab + a.chunks - 1) / a.chunks + 3) / 4 * 4);
-  const size_t parts = rows * a.chunks;
+  a.chunks = chunks;
+  a.chunk = (int)(((vocab + chunks - 1) / chunks + 3) / 4 * 4);
   a.part_sum = (double *)workspace;
   a.part_key = (unsigned long long *)(a.part_sum + parts);
   a.part_max = (float *)(a.part_key + parts * k);

@@ -891,6 +891,12 @@ constexpr int beam_chunks(long long rows, long long vocab, int k) {
   n = n < most ? n : most;
   return (int)(n < room ? n : room);
 }
+// At least the parts of any call with no more rows, a vocabulary no larger and any k:
+// rows * ceil(1024 / rows), which goes up and down with the rows, is at most rows + 1023.
+constexpr long long beam_parts_most(long long rows, long long vocab) {
+  const long long room = (vocab + 1023) / 1024, chunks = room < kBeamChunks ? room : kBeamChunks;
+  return rows * chunks < rows + 1023 ? rows * chunks : rows + 1023;
+}
 hipError_t launch_beam_select(const BeamArgs &a, bool vec, hipStream_t s);
 
 }  // namespace bnr

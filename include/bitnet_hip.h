@@ -564,8 +564,8 @@ int bnr_dev_paged_copy(bnr_ctx *ctx, const bnr_paged_kv *kv, const int32_t *bloc
 /* ---- Beam search -----------------------------------------------------------
  * At most 32 beams a request and 32 continuations. */
 
-/* Bytes of workspace that bnr_dev_beam_select needs; it serves every shape that
- * needs no more, and holds nothing between calls. */
+/* Bytes of workspace for bnr_dev_beam_select: enough for every call with no more
+ * requests, beams, tokens and continuations.  It holds nothing between calls. */
 int bnr_beam_workspace(bnr_ctx *ctx, size_t batch, size_t beams, size_t vocab, size_t k,
                        size_t *bytes);
 

@@ -695,3 +695,20 @@ def test_extend_and_release_captured(backend, n):
         b = release(a[0], a[1], gone, None, t.free, a[2], page)
         for got, w in zip((seqs, pos, off, l2, table, l3, stack, c3), (a[3], a[4], a[6], a[1], b[0], b[1], b[2], [b[3]])):
             assert np.array_equal(got.cpu().numpy(), w)
+
+
+def test_workspace_of_the_largest_batch(backend):
+    """A workspace made once for 16 requests of 8 beams, as requests end: fewer rows
+    are cut into more parts."""
+    K, V = 8, 40000
+    ws = backend.beam_workspace(16, K, V, K)
+    rng = np.random.default_rng(15)
+    logits = (3 * rng.standard_normal((16, K, V))).astype(np.float32)
+    scores = (-4 * rng.random((16, K))).astype(np.float32)
+    for B, beams, k in ((16, K, K), (15, K, K), (14, K, K), (9, K, 5), (3, K, K), (1, K, K), (1, 1, 8), (16, 3, 3)):
+        say(f"select {B}x{beams} k {k} in the workspace of 16x8")
+        x, s = logits[:B, :beams], scores[:B, :beams]
+        tokens, parents, _, _, gap = select(x, s, k)
+        assert gap > 2.0 ** -16
+        got = run_select(backend, cuda(x), cuda(s), k, ws=ws)
+        assert np.array_equal(got[0], tokens) and np.array_equal(got[1], parents)

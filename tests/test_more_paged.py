@@ -2,6 +2,7 @@
 entry points refuse before they touch the device, and the rotations' rates."""
 import ctypes
 import math
+import re
 
 import numpy as np
 import pytest
@@ -248,3 +249,39 @@ def test_rope_is_fixed():
     kept = Rope.from_rates(own)
     own[:] = 7
     assert (kept.rates == 1).all()
+
+
+def beam_need(batch, beams, vocab, k):
+    """What a selection asks for, from its refusal of a workspace of no bytes."""
+    assert select(batch=batch, beams=beams, vocab=vocab, stride=vocab, k=k, bytes=0, eos=0) == SHAPE
+    return int(re.search(r"workspace of (\d+) bytes", error_from_parts()[1]).group(1))
+
+
+@pytest.mark.parametrize("vocab", [40, 2000, 32000, 128256])
+def test_beam_workspace_serves_smaller_calls(vocab):
+    """A workspace serves every call with no more requests, beams, tokens and
+    continuations: a server makes one for its largest."""
+    lib, n = _lib.load(), ctypes.c_size_t()
+
+    def room(batch, beams, vocab, k):
+        assert lib.bnr_beam_workspace(CTX, batch, beams, vocab, k, ctypes.byref(n)) == _lib.BNR_OK
+        return n.value
+
+    batches, ks = [1, 2, 3, 4, 7, 12, 15, 16, 31, 32, 128, 300], [1, 2, 5, 8, 15, 16, 17, 31, 32]
+    for beams in (1, 4, 8, 32):
+        for k in ks:
+            most = 0
+            for b in batches:
+                most = max(most, beam_need(b, beams, vocab, k))
+                assert room(b, beams, vocab, k) >= most, (b, beams, k)
+    for beams in (1, 8, 32):
+        for b in batches:
+            most = 0
+            for k in ks:
+                most = max(most, beam_need(b, beams, vocab, k))
+                assert room(b, beams, vocab, k) >= most, (b, beams, k)
+    for b in batches:
+        most = 0
+        for beams in range(1, 33):
+            most = max(most, beam_need(b, beams, vocab, 8), beam_need(b, beams, vocab // 2, 8))
+            assert room(b, beams, vocab, 8) >= most, (b, beams)
