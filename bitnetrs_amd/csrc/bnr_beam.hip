@@ -11,7 +11,8 @@
 //
 // Beams are compared by scores in 64 bits: lse is what the order of two beams'
 // continuations hangs on, so its exponentials carry the part of log2(e) that
-// fp32 leaves out and their sums are joined in 64 bits.
+// fp32 leaves out, and at most 16 of them are added in fp32 before they join a
+// sum in 64 bits: lse is within 2^-17 whatever the vocabulary.
 //
 // Read once, the logits of 16 requests of 8 beams and 128256 tokens (61 MB) take 8.6
 // us at the rate of a plain read; the rows' launch takes 16.2, of which 12.0 are
@@ -29,6 +30,9 @@ constexpr int kJoinWaves = 16;
 constexpr int kJoinEntries = 4096;           // of the lists that LDS has room for
 constexpr int kCap = 128;                    // candidates of a wave that LDS has room for
 constexpr float kLargest = 3.402823466e38f;  // of fp32
+// How far a logit may lie above what a thread's exponentials are taken from.  Each
+// factor that raises it costs a sum a place of exp2, so that it does not follow every logit.
+constexpr float kSlack = 2.f;
 
 typedef unsigned long long u64;
 
@@ -123,7 +127,8 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x, k = a.k;
   const float *x = a.logits + row * a.stride;
   const int v0 = part * a.chunk, v1 = min(v0 + a.chunk, a.vocab);
-  float m = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY;  // what exponentials are taken from
+  double sum = 0.0;
   u64 *cand = s_cand[wave];
   int have = 0;  // candidates so far, the same in all lanes
   // What a candidate must reach: at least k of the workgroup's do.  Masked tokens (-infinity) are none: the join
@@ -165,11 +170,12 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
     for (int n = 1; n < H; ++n) top = fmaxf(top, h[n]);
     if (!(top > -INFINITY)) top = -INFINITY;  // all NaN
     // places past the end hold -infinity: they add nothing
-    const float mn = fmaxf(m, top), mu = above(mn), keep = exp_from(above(m) == m ? m : mu, mu);
+    const bool rise = top > m + kSlack;
+    const float mn = rise ? top : m, mu = above(mn), keep = rise ? exp_from(m, mn) : 1.f;
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int n = 0; n < 4; ++n) sum[n] *= keep;
-#pragma unroll
-    for (int n = 0; n < H; ++n) sum[n % 4] += exp_from(h[n], mu);
+    for (int n = 0; n < H; ++n) add[n % 4] += exp_from(h[n], mu);
+    sum = fma(sum, (double)keep, (double)((add[0] + add[1]) + (add[2] + add[3])));
     m = mn;
 
     // The first tile's threshold: of each wave's lane maxima the n-th largest, n
@@ -236,8 +242,7 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(BeamArgs a) {
   }
   // The part's k best: a candidate's place is how many of all waves' are larger.
   const float wm = wave_max(m);
-  const double ws = wave_sum64((((double)sum[0] + sum[1]) + ((double)sum[2] + sum[3])) *
-                               (double)exp_from(above(m) == m ? m : above(wm), above(wm)));
+  const double ws = wave_sum64(sum * (double)exp_from(above(m) == m ? m : above(wm), above(wm)));
   if (lane < 8) cand[have + lane] = 0;
   if (lane == 0) {
     s_top[wave] = wm;

@@ -576,7 +576,8 @@ int bnr_beam_workspace(bnr_ctx *ctx, size_t batch, size_t beams, size_t vocab, s
  * beams * k, the k of highest score in 64 bits go out, the highest first; of
  * equal ones that of the lowest beam, then of the larger logit, then of the
  * lowest t: tokens, parents (the beam in its request) and scores_out [batch x
- * k].  done [batch x beams] (may be NULL): a beam with done != 0 has one
+ * k].  The logarithm is within 2^-17 for every vocabulary: two beams' continuations
+ * whose scores are closer than 2^-16 may come in either order.  done [batch x beams] (may be NULL): a beam with done != 0 has one
  * continuation, eos, at its own score; all its others count as -infinity (in
  * order of t).  done_out [batch x k] (may be NULL): the parent was done, or the
  * token is eos.  eos: 0..vocab-1, or -1 for none where done is NULL.  A beam

@@ -712,3 +712,67 @@ def test_workspace_of_the_largest_batch(backend):
         assert gap > 2.0 ** -16
         got = run_select(backend, cuda(x), cuda(s), k, ws=ws)
         assert np.array_equal(got[0], tokens) and np.array_equal(got[1], parents)
+
+
+# Any vocabulary: a part's sum is joined in 64 bits every 16 terms of a thread, whose
+# additions are five roundings (5 * 2^-24).  A term is a product of factors exp(d):
+# its own, from a reference that is at most 2 below the largest logit so far, and
+# one each time the reference rises by more than 2, or two threads, waves or parts
+# are joined.  The |d| of one term come to its distance from the largest logit and
+# at most 2 + 4, on the mean over the softmax ln V + 6 < 27 (V <= 2^30); each is off
+# by 3 |d| 2^-24 + 2^-23, and there are at most 27 / 2 + 3 of them: 81 + 33 + 5 = 119
+# times 2^-24, under 2^-17.
+LSE = 2.0 ** -17
+
+
+def flood(V, part):
+    """Of each `part` logits the first 1024 are 0, and all others so small that an
+    fp32 sum of 1 does not notice one of them: exp is just under 2^-24."""
+    x = torch.full((V // part, part), -24 * float(np.log(2)) - 1e-5, device="cuda")
+    x[:, :1024] = 0
+    return x.view(V)
+
+
+def lse64(x):
+    return float(torch.logsumexp(x.double(), -1))
+
+
+def test_select_sums_of_a_large_vocabulary(backend):
+    """2^25 logits in 64 parts: what half a million small ones add decides between
+    two beams."""
+    V = 1 << 25
+    logits = torch.full((1, 2, V), -float("inf"), device="cuda")
+    logits[0, 0] = flood(V, V // 64)
+    logits[0, 1, :1 << 16] = 0
+    want = -np.array([lse64(logits[0, 0]), np.log(65536.0)])
+    assert want[1] - want[0] > 2 * LSE
+    tokens, parents, got, _ = run_select(backend, logits, torch.zeros(1, 2, device="cuda"), 2)
+    assert parents.tolist() == [[1, 1]] and tokens.tolist() == [[0, 1]]
+    tokens, parents, got, _ = run_select(backend, logits, torch.tensor([[1.0, 0.0]], device="cuda"), 2)
+    assert parents.tolist() == [[0, 0]] and tokens.tolist() == [[0, 1]]
+    assert np.abs(got - (1 + want[0])).max() <= LSE + 12 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("V", [1 << 18, (1 << 18) - 1])
+def test_select_sums_of_whole_rows(backend, V):
+    """1024 rows and more: a row is one part, with 256 terms a thread's sum."""
+    x = flood(1 << 18, 1 << 18)[:V]
+    logits = x.expand(128, 8, V).contiguous()
+    scores = -torch.arange(8, device="cuda", dtype=torch.float32).expand(128, 8).contiguous()
+    tokens, parents, got, _ = run_select(backend, logits, scores, 4)
+    assert (parents == 0).all() and (tokens == np.arange(4)).all()
+    assert np.abs(got + lse64(x)).max() <= LSE + 8 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("step", [2.0 ** -20, 2.0 ** -16, 2.0 ** -13])
+@pytest.mark.parametrize("B,V", [(1, 1 << 22), (1024, 1 << 16)])
+def test_select_sums_of_rising_logits(backend, B, V, step):
+    """Each logit is larger than those before it, and the other way round."""
+    up = torch.arange(V, device="cuda", dtype=torch.float32) * step
+    for x in (up, up.flip(0)):
+        logits = x.expand(B, 1, V).contiguous()
+        tokens, _, got, _ = run_select(backend, logits, torch.zeros(B, 1, device="cuda"), 3)
+        best = torch.topk(x, 3)
+        assert (tokens == best.indices.cpu().numpy()).all()
+        want = best.values.double().cpu().numpy() - lse64(x)
+        assert (np.abs(got - want) <= LSE + np.abs(want) * 2.0 ** -24).all()
