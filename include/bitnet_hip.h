@@ -433,8 +433,8 @@ int bnr_kv_dev_prefill(bnr_ctx *ctx, bnr_kv_cache *cache, size_t layer, float *q
  * A row of FP8 or INT8 that holds an infinity or a NaN gets the scale NaN and
  * reads back as NaN; 32 such elements of FP4 the byte 255, and read back as NaN.
  * (Bytes 253 and 254 are not written.  They stand for 2^126 and 2^127, so that
- * codes of 4 and 2 and more are infinite: attention over such an element is NaN or
- * leaves its row out.) */
+ * codes of 4 and 2 and more are infinite: attention over such an element of K is NaN,
+ * or leaves its row out where the score is -infinity; of V its column is not finite.) */
 #define BNR_KV_F32 0
 #define BNR_KV_BF16 1
 #define BNR_KV_FP8 2

@@ -389,3 +389,47 @@ def test_offsets_past_32_bits(backend):
     backend.dev_paged_read(kv, table, i32([40]), *back)
     assert same(back[1][0].cpu().numpy().transpose(1, 0, 2), v)
     assert not kv.k[:-1].any()
+
+
+def plant_infinity(pool, n, s, t, h, x, sign, exp, page):
+    """Element x of a row as 6 * 2^(exp - 127), its group's others as zeros."""
+    at = (pool.table[s, t // page], h, t % page)
+    g = x // 32
+    pool.exps[n][at][g] = exp
+    pool.codes[n][at][16 * g: 16 * g + 16] = 0
+    pool.codes[n][at][x // 2] = (15 if sign < 0 else 7) << 4 * (x % 2)
+
+
+@pytest.mark.parametrize("hq", [4, 6, 8, 12])
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 16), (256, 16), (80, 32), (26, 4)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_infinite_elements(backend, hq, d, page, wide):
+    """Exponents 253 and 254 from elsewhere: a row of K whose score is -infinity is
+    left out and one of +infinity makes the head NaN, however wide the table is; in
+    V the columns show it, and nothing else."""
+    lens = [200, 300, 150]
+    pool = Pool4(rng_of("infinite", d), lens, 2, d, page, width=max(-(-300 // page), room(3, 2, page, wide)))
+    plant_infinity(pool, "k", 0, 60, 1, d - 1, 1, 253, page)
+    plant_infinity(pool, "k", 1, 299, 0, 3, -1, 254, page)
+    plant_infinity(pool, "v", 2, 77, 1, d // 2, -1, 254, page)
+    q, got = run_decode(backend, pool, hq, lens)
+    G = hq // 2
+    for s, row, h0, x, sign in ((0, 60, G, d - 1, 1), (1, 299, 0, 3, -1)):
+        k, v = pool.rows("k", s)[0], pool.rows("v", s)[0]
+        assert np.isinf(k[row]).sum() == 1
+        nan = np.zeros(hq, bool)
+        nan[h0:h0 + G] = q[s, h0:h0 + G, x] * sign > 0
+        assert np.array_equal(np.isnan(got[s]), np.repeat(nan[:, None], d, 1)), s
+        for h in np.nonzero(~nan)[0]:
+            rows = np.arange(lens[s]) != (row if h // G == h0 // G else -1)
+            want, mag, size = attention(q[s, h:h + 1], k[rows][:, [h // G]], v[rows][:, [h // G]])
+            bound = attention_bound(int(rows.sum()), d, mag, size)
+            assert (np.abs(got[s, h:h + 1] - want) <= bound).all(), (s, h)
+    shows = np.zeros((hq, d), bool)
+    shows[G:, d // 2] = True
+    assert np.array_equal(~np.isfinite(got[2]), shows)
+    v = pool.rows("v", 2)[0].copy()
+    v[77, 1, d // 2] = 0
+    want, mag, size = attention(q[2], pool.rows("k", 2)[0], v)
+    bound = np.broadcast_to(attention_bound(150, d, mag, size), want.shape)
+    assert (np.abs(got[2] - want) <= bound)[~shows].all()
