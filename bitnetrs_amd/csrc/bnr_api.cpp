@@ -3249,6 +3249,7 @@ int rope_turns(const bnr_rope *r, double *turns) {
 }
 
 constexpr size_t kRopeMaxStride = (size_t)1 << 40;
+constexpr size_t kRopeMaxExtent = (size_t)1 << 58;
 
 // One operand; `extent`: elements from the first to behind the last.
 int rope_heads(const bnr_heads *h, const char *name, size_t n_tokens, size_t d, size_t size, RopeHeads &r) {
@@ -3259,6 +3260,11 @@ int rope_heads(const bnr_heads *h, const char *name, size_t n_tokens, size_t d, 
   for (size_t s : {h->in_token, h->in_head, h->out_token, h->out_head})
     if (s > kRopeMaxStride) return err_shape(fmt("%s: strides up to 2^40", name), fmt("%zu", s));
   if (n_tokens == 0) return BNR_OK;
+  const size_t token = std::max(h->in_token, h->out_token), head = std::max(h->in_head, h->out_head);
+  if (n_tokens - 1 > kRopeMaxExtent / std::max<size_t>(token, 1) ||
+      h->n_heads - 1 > kRopeMaxExtent / std::max<size_t>(head, 1))
+    return err_shape(fmt("%s: rows within 2^58 elements", name),
+                     fmt("%zu tokens %zu apart, %zu heads %zu apart", n_tokens, token, h->n_heads, head));
   if (!h->in || !h->out) return err_backend("rope: NULL pointer");
   if (((uintptr_t)h->in | (uintptr_t)h->out) % size != 0)
     return err_shape(fmt("%s: pointers aligned to an element", name), "an unaligned pointer");
@@ -3282,6 +3288,44 @@ int rope_heads(const bnr_heads *h, const char *name, size_t n_tokens, size_t d, 
   r.out_token = (long long)h->out_token;
   r.out_head = (long long)h->out_head;
   return BNR_OK;
+}
+
+// One side of an operand, in bytes.
+struct RopeRows {
+  uintptr_t at;
+  long long token, head;
+  int heads;
+};
+RopeRows rope_rows(const RopeHeads &r, bool out, size_t size) {
+  return {(uintptr_t)(out ? r.out : r.in), (out ? r.out_token : r.in_token) * (long long)size,
+          (out ? r.out_head : r.in_head) * (long long)size, r.heads};
+}
+
+// Whether rows of a and rows of b share a byte (where their tokens are not equally far
+// apart, or there are thousands of heads, whether their ranges do).  Slices of a fused projection have
+// overlapping ranges, but not a token's heads: that is looked at before single heads.
+bool rope_rows_meet(const RopeRows &a, const RopeRows &b, long long n, long long d) {
+  const long long la = (a.heads - 1) * a.head + d, lb = (b.heads - 1) * b.head + d;
+  if (!overlap((const void *)a.at, (size_t)((n - 1) * a.token + la), (const void *)b.at,
+               (size_t)((n - 1) * b.token + lb)))
+    return false;
+  if (n > 1 && (a.token != b.token || a.token == 0)) return true;
+  // whether x + u * token lies between -below and above (both exclusive) for two tokens u apart
+  const auto reaches = [&](long long x, long long below, long long above) {
+    if (n == 1) return -below < x && x < above;
+    const long long y = -below - x, u = y / a.token - (y % a.token < 0) + 1;  // the least above -below
+    return u < n && x + std::max(u, 1 - n) * a.token < above;
+  };
+  const long long x = (long long)(b.at - a.at);
+  if (!reaches(x, lb, la)) return false;
+  // heads equally far apart: only the difference of their numbers counts
+  const bool same = a.heads == 1 || b.heads == 1 || a.head == b.head;
+  if (!same && (long long)a.heads * b.heads > 1 << 16) return true;
+  const long long head = a.heads == 1 ? b.head : a.head;
+  for (long long i = 0; i < (same ? 1 : a.heads); ++i)
+    for (long long j = same ? 1 - a.heads : 0; j < b.heads; ++j)
+      if (reaches(x + (same ? j * head : j * b.head - i * a.head), d, d)) return true;
+  return false;
 }
 
 // Where the rows start: addresses and distances in bytes, or'ed.
@@ -3310,7 +3354,16 @@ extern "C" int bnr_dev_rope(bnr_ctx *c, const bnr_rope *rope, int type, size_t n
   if (!st) st = rope_heads(k, "k", n_tokens, head_dim, size, a.k);
   if (st) return st;
   if (n_tokens == 0 || a.q.heads + a.k.heads == 0) return set_ok();
+  for (int i = 0; i < 3 && a.q.heads && a.k.heads; ++i)  // what one writes, against what the other writes or reads
+    if (rope_rows_meet(rope_rows(a.q, i != 2, size), rope_rows(a.k, i != 1, size), (long long)n_tokens,
+                       (long long)(head_dim * size)))
+      return err_shape("q and k apart", "memory that one writes and both have");
   if (!positions) return err_backend("rope: NULL positions");
+  for (const RopeHeads *h : {&a.q, &a.k})
+    if (h->heads && overlap(positions, n_tokens * sizeof(int32_t), h->out,
+                            (size_t)((long long)(n_tokens - 1) * h->out_token + (h->heads - 1) * h->out_head +
+                                     (long long)head_dim) * size))
+      return err_shape("outputs and positions apart", "memory that both have");
   a.positions = positions;
   a.n_tokens = (long long)n_tokens;
   a.d = (int)head_dim;

@@ -633,7 +633,8 @@ typedef struct bnr_heads {
  * (device memory), in fp32 and rounded once to their type; elements from 2 *
  * n_pairs on are copied.  The angle position * rate is formed in fp64.  A token
  * with a negative position is left out: its outputs are not written.  Rows of
- * an output may not overlap. */
+ * an output may not overlap, nor what one operand writes and the other's rows or the
+ * positions.  Two operands of one buffer have their tokens equally far apart. */
 int bnr_dev_rope(bnr_ctx *ctx, const bnr_rope *rope, int type, size_t n_tokens, size_t head_dim,
                  const int32_t *positions, const bnr_heads *q, const bnr_heads *k, void *stream);
 

@@ -249,3 +249,25 @@ def test_python_refusals(backend):
     ]:
         with pytest.raises(error):
             bad()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_operands_of_one_buffer(backend, layout):
+    """Slices of fused projections, whose ranges overlap but not their rows, as
+    calls on tensors of their own; one tensor as both operands is refused."""
+    rope, n, p = Rope(64, 10000.0, layout), 33, i32(np.arange(33) * 7)
+    for shape, q_of, k_of in (((n, 12, 64), lambda x: x[:, :8], lambda x: x[:, 8:10]),
+                              ((n, 4, 3, 64), lambda x: x[:, :, 0], lambda x: x[:, :, 1]),
+                              ((2, 3, n, 64), lambda x: x[0].transpose(0, 1), lambda x: x[1, :2].transpose(0, 1))):
+        x = torch.randn(shape, device="cuda", dtype=torch.bfloat16)
+        want = x.clone()
+        for of in (q_of, k_of):
+            part = of(x).contiguous()
+            backend.dev_rope(rope, part, None, p)
+            of(want).copy_(part)
+        backend.dev_rope(rope, q_of(x), k_of(x), p)
+        assert torch.equal(x, want)
+    q = x[0].transpose(0, 1)
+    for k, out in ((q, None), (q[:, 1:], None), (x[1].transpose(0, 1), q)):
+        with pytest.raises(InvalidShape):
+            backend.dev_rope(rope, q, k, p, None, out)

@@ -285,3 +285,79 @@ def test_beam_workspace_serves_smaller_calls(vocab):
         for beams in range(1, 33):
             most = max(most, beam_need(b, beams, vocab, 8), beam_need(b, beams, vocab // 2, 8))
             assert room(b, beams, vocab, 8) >= most, (b, beams)
+
+
+# ---------------------------------------------------------------------------
+# rotations whose operands meet
+# ---------------------------------------------------------------------------
+def place(base, n_heads, token, head, out=None, out_token=None, out_head=None):
+    """Heads at elements of one buffer (fp32); in place unless `out` is given."""
+    out, out_token, out_head = (base, token, head) if out is None else (out, out_token, out_head)
+    return bytes(HeadsDesc(BASE + 4 * base, BASE + 4 * out, n_heads, token, head, out_token, out_head))
+
+
+APART = [  # q, k of heads of 64
+    (dict(base=0, n_heads=4, token=384, head=64), dict(base=256, n_heads=1, token=384, head=64)),  # a fused projection
+    (dict(base=0, n_heads=4, token=512, head=128), dict(base=64, n_heads=4, token=512, head=128)),  # head by head
+    (dict(base=0, n_heads=2, token=768, head=192), dict(base=400, n_heads=3, token=768, head=80)),
+    (dict(base=0, n_heads=2, token=64, head=1024), dict(base=256, n_heads=2, token=64, head=1024)),  # tokens within heads
+]
+MEET = [
+    (dict(base=0, n_heads=4, token=256, head=64), dict(base=0, n_heads=4, token=256, head=64)),
+    (dict(base=0, n_heads=4, token=384, head=64), dict(base=255, n_heads=2, token=384, head=64)),
+    (dict(base=0, n_heads=4, token=384, head=64), dict(base=256, n_heads=3, token=384, head=64)),
+    (dict(base=0, n_heads=4, token=512, head=128), dict(base=60, n_heads=4, token=512, head=128)),
+    (dict(base=0, n_heads=4, token=256, head=64, out=4096, out_token=256, out_head=64),
+     dict(base=4100, n_heads=2, token=256, head=64, out=9000, out_token=128, out_head=64)),  # k reads what q writes
+    (dict(base=0, n_heads=1, token=128, head=64), dict(base=64, n_heads=1, token=256, head=64)),
+]
+
+
+@pytest.mark.parametrize("q,k", APART)
+def test_rope_operands_of_one_buffer(q, k):
+    """Accepted: the next refusal is the positions'."""
+    for a, b in ((q, k), (k, q)):
+        assert rope(q=place(**a), k=place(**b), positions=None) == BACKEND
+        assert "positions" in error_from_parts()[1]
+
+
+@pytest.mark.parametrize("q,k", MEET)
+def test_rope_operands_that_meet_are_refused(q, k):
+    for a, b in ((q, k), (k, q)):
+        assert rope(q=place(**a), k=place(**b)) == SHAPE
+        assert "apart" in error_from_parts()[1]
+
+
+def test_rope_operands_against_their_elements():
+    """Random places in one buffer: refused where an element that one operand
+    writes is the other's, and nowhere else (operands of equal token distance)."""
+    rng = np.random.default_rng(11)
+    n, d, seen = 3, 4, [0, 0]
+    r = rotation(n=2)
+    for _ in range(4000):
+        token = int(rng.integers(4, 40))
+        sides = []
+        for _ in range(2):
+            m, head = int(rng.integers(1, 4)), int(rng.integers(4, 40))
+            base, away = int(rng.integers(0, 60)), bool(rng.random() < 0.3)
+            args = dict(base=base, n_heads=m, token=token, head=head)
+            if away:
+                args.update(out=base + 400, out_token=token, out_head=head)
+            at = {base + i * token + h * head + e for i in range(n) for h in range(m) for e in range(d)}
+            sides.append((args, at, {x + 400 for x in at} if away else at))
+        if any(len(at) != n * d * a["n_heads"] for a, at, _ in sides):
+            continue
+        (a, ai, ao), (b, bi, bo) = sides
+        kind = rope(r=r, n=n, d=d, positions=None, q=place(**a), k=place(**b))
+        text = error_from_parts()[1]
+        if "output rows" in text:  # neither heads within tokens nor tokens within heads
+            continue
+        meet = bool(ao & bo or ao & bi or ai & bo)
+        assert (kind == SHAPE and "apart" in text) == meet and (kind == BACKEND) == (not meet), (a, b)
+        seen[meet] += 1
+    assert min(seen) > 50
+
+
+@pytest.mark.parametrize("bad", [dict(positions=at(1)), dict(positions=at(3) + 16)])
+def test_rope_positions_in_an_output(bad):
+    assert rope(**bad) == SHAPE and "positions" in error_from_parts()[1]
