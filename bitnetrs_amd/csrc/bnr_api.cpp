@@ -3390,6 +3390,8 @@ extern "C" int bnr_dev_rope_scaled_table(bnr_ctx *c, const bnr_rope *rope, size_
                      fmt("first = %zu, n_positions = %zu", first, n_positions));
   if (n_positions == 0) return set_ok();
   if (!cos_out || !sin_out) return err_backend("rope_scaled_table: NULL pointer");
+  const size_t table = n_positions * rope->n_pairs * sizeof(float);
+  if (overlap(cos_out, table, sin_out, table)) return err_shape("cos_out and sin_out apart", "memory that both have");
   a.cos_out = cos_out;
   a.sin_out = sin_out;
   a.first = (long long)first;

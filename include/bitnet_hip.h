@@ -641,8 +641,8 @@ int bnr_dev_rope(bnr_ctx *ctx, const bnr_rope *rope, int type, size_t n_tokens, 
 /* The rotation's cos and sin (times magnitude) of positions first .. first +
  * n_positions - 1, into cos_out and sin_out [n_positions x n_pairs] in device
  * memory, as bnr_dev_paged_append takes them (half-split pairs, n_pairs =
- * head_dim / 2; the same rotation as bnr_dev_rope's, to the bit in F32).  Built
- * on the device: may be captured. */
+ * head_dim / 2; the same rotation as bnr_dev_rope's, to the bit in F32).  The two
+ * may not overlap.  Built on the device: may be captured. */
 int bnr_dev_rope_scaled_table(bnr_ctx *ctx, const bnr_rope *rope, size_t first,
                               size_t n_positions, float *cos_out, float *sin_out, void *stream);
 

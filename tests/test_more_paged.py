@@ -361,3 +361,8 @@ def test_rope_operands_against_their_elements():
 @pytest.mark.parametrize("bad", [dict(positions=at(1)), dict(positions=at(3) + 16)])
 def test_rope_positions_in_an_output(bad):
     assert rope(**bad) == SHAPE and "positions" in error_from_parts()[1]
+
+
+@pytest.mark.parametrize("off", [0, 4, 4 * (8 * 32 - 1), -4])
+def test_rotation_tables_apart(off):
+    assert table(sin=at(0) + off) == SHAPE and "apart" in error_from_parts()[1]
