@@ -433,3 +433,24 @@ def test_decode_infinite_elements(backend, hq, d, page, wide):
     want, mag, size = attention(q[2], pool.rows("k", 2)[0], v)
     bound = np.broadcast_to(attention_bound(150, d, mag, size), want.shape)
     assert (np.abs(got[2] - want) <= bound)[~shows].all()
+
+
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 16), (256, 16), (80, 32), (26, 4)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_values_beside_non_finite_groups(backend, d, page, wide):
+    """The heads and columns that no NaN group reaches have their values."""
+    lens = [200, 200]
+    pool = Pool4(rng_of("beside", d), lens, 2, d, page, width=max(-(-200 // page), room(2, 2, page, wide)))
+    g = groups(d) - 1
+    pool.exps["v"][pool.table[0, 77 // page], 1, 77 % page, g] = 255
+    pool.exps["k"][pool.table[1, 150 // page], 0, 150 % page, 0] = 255
+    q, got = run_decode(backend, pool, 6, lens)
+    fine = np.ones((2, 6, d), bool)
+    fine[0, 3:, 32 * g:] = False
+    fine[1, :3] = False
+    assert np.array_equal(np.isfinite(got), fine)
+    for s in range(2):
+        k, v = (np.nan_to_num(pool.rows(n, s)[0], nan=0.0) for n in "kv")
+        want, mag, size = attention(q[s], k, v)
+        off = np.abs(got[s] - want)
+        assert (off <= attention_bound(200, d, mag, size))[fine[s]].all()

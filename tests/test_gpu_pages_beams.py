@@ -776,3 +776,42 @@ def test_select_sums_of_rising_logits(backend, B, V, step):
         assert (tokens == best.indices.cpu().numpy()).all()
         want = best.values.double().cpu().numpy() - lse64(x)
         assert (np.abs(got - want) <= LSE + np.abs(want) * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp8", "int8"])
+def test_copies_on_two_streams(backend, fmt):
+    """Copies of two pools on two streams at once: codes and scales byte by byte."""
+    rng = np.random.default_rng(5)
+    n, page, width, rows = 32, 16, 6, 90
+    sides = []
+    for i in range(2):
+        kv = PagedKV(n * width + 8, page, 2, 64, fmt)
+        table = rng.permutation(n * width + 8)[:n * width].reshape(n, width).astype(np.int32)
+        src = np.full(n, -1, np.int32)
+        src[1::2] = rng.integers(0, n // 2, n // 2) * 2  # odd sequences from even ones
+        tensors = [kv.k, kv.v, kv.k_scales, kv.v_scales]
+        for t in tensors:
+            t.view(torch.uint8).random_(0, 256)
+        first = [t.view(torch.uint8).cpu().numpy().copy() for t in tensors]
+        want = [x.copy() for x in first]
+        for s in range(1, n, 2):
+            for t in range(3, rows):
+                a, b = table[src[s], t // page], table[s, t // page]
+                for x, w in zip(first, want):
+                    # [pages, kv heads, page, bytes of a row] (a scale's four bytes as a row of their own)
+                    x, w = (y.reshape(n * width + 8, 2, page, -1) for y in (x, w))
+                    w[b, :, t % page] = x[a, :, t % page]
+        sides.append((kv, cuda(table), i32(src), tensors, first, want))
+    lens, starts = i32([rows] * n), i32([3] * n)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for _, _, _, tensors, first, _ in sides:
+            for t, x in zip(tensors, first):
+                t.view(torch.uint8).copy_(cuda(x))
+        torch.cuda.synchronize()
+        for (kv, table, src, *_), stream in zip(sides, streams):
+            backend.dev_paged_copy(kv, table, src, lens, starts, stream=stream)
+        torch.cuda.synchronize()
+        for _, _, _, tensors, _, want in sides:
+            for t, w in zip(tensors, want):
+                assert np.array_equal(t.view(torch.uint8).cpu().numpy(), w)
