@@ -815,3 +815,45 @@ def test_copies_on_two_streams(backend, fmt):
         for _, _, _, tensors, _, want in sides:
             for t, w in zip(tensors, want):
                 assert np.array_equal(t.view(torch.uint8).cpu().numpy(), w)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "bf16"])
+def test_steps_from_a_fused_projection(backend, fmt):
+    """A server's step on slices of one projection's output, as the integration
+    guide has it: the results of the same calls on tensors of their own."""
+    batch, hq, hkv, d, page, width = 3, 8, 2, 64, 16, 4
+    rope = Rope(d, 10000.0, scaling="parts", factor=8.0, original=4096, magnitude=1.2)
+    sides = []
+    for _ in range(2):
+        kv = PagedKV(batch * width, page, hkv, d, fmt)
+        sides.append([kv, i32(np.full((batch, width), -1)), i32(np.arange(batch * width)), i32([0, 20, 16]), i32([batch * width])])
+        table, free, lens, count = sides[-1][1:]
+        # pages of the rows that are there
+        for s, n in enumerate(lens.tolist()):
+            for p in range(pages_of(n, page)):
+                count -= 1
+                table[s, p] = free[count.item()]
+    new, seqs, positions, offsets = i32([1] * batch), i32([0] * batch), i32([0] * batch), i32([0] * (batch + 1))
+    ws = backend.paged_workspace(sides[0][0], batch, hq)
+    for _ in range(5):
+        qkv = torch.randn(batch, hq + 2 * hkv, d, device="cuda")
+        outs = []
+        for fused, side in ((True, sides[0]), (False, sides[1])):
+            kv, table, free, lens, count = side
+            lens2, count2 = torch.empty_like(lens), torch.empty_like(count)
+            backend.dev_paged_extend(table, lens, new, free, count, page, seqs, positions, offsets, lens2, count2)
+            q, k, v = qkv[:, :hq], qkv[:, hq:-hkv], qkv[:, -hkv:].contiguous()
+            if fused:
+                to = torch.empty(batch, hq, d, device="cuda"), torch.empty(batch, hkv, d, device="cuda")
+                backend.dev_rope(rope, q, k, positions, *to)
+                q, k = to
+            else:
+                q, k = q.contiguous(), k.contiguous()
+                backend.dev_rope(rope, q, k, positions)
+            backend.dev_paged_append(kv, None, k, v, None, positions, table, seqs=seqs)
+            out = torch.empty_like(q)
+            backend.dev_paged_decode_attention(kv, q, table, lens2, out, ws)
+            side[3:] = lens2, count2
+            outs.append(out)
+        assert torch.equal(*outs) and torch.isfinite(outs[0]).all()
+    assert torch.equal(sides[0][0].k.view(torch.uint8), sides[1][0].k.view(torch.uint8)) and sides[0][3].tolist() == [5, 25, 21]
