@@ -49,22 +49,25 @@ class Rope:
         if not math.isfinite(magnitude):
             raise InvalidConfig(f"magnitude must be finite, got {magnitude}")
         i = np.arange(dim // 2, dtype=np.float64)
-        base = float(theta)
-        if scaling == "ntk":
-            if dim == 2:
-                raise InvalidConfig("ntk scaling needs a rotary dim of more than 2")
-            base *= float(factor) ** (dim / (dim - 2))
-        rates = base ** (-2.0 * i / dim)
-        if scaling == "linear":
-            rates = rates / factor
-        elif scaling == "parts":
-            if original <= 0 or not alpha < beta:
-                raise InvalidConfig("parts scaling needs original > 0 and alpha < beta, got "
-                                    f"{original}, {alpha}, {beta}")
-            keep = np.clip((original * rates / (2 * math.pi) - alpha) / (beta - alpha), 0, 1)
-            rates = rates * (keep + (1 - keep) / factor)
-        elif scaling not in (None, "ntk"):
-            raise InvalidConfig(f"unknown rotary scaling {scaling!r}")
+        base = np.float64(theta)
+        with np.errstate(all="ignore"):  # what is no number is refused below
+            if scaling == "ntk":
+                if dim == 2:
+                    raise InvalidConfig("ntk scaling needs a rotary dim of more than 2")
+                base *= np.float64(factor) ** (dim / (dim - 2))
+            rates = base ** (-2.0 * i / dim)
+            if scaling == "linear":
+                rates = rates / factor
+            elif scaling == "parts":
+                if original <= 0 or not alpha < beta:
+                    raise InvalidConfig("parts scaling needs original > 0 and alpha < beta, got "
+                                        f"{original}, {alpha}, {beta}")
+                keep = np.clip((original * rates / (2 * math.pi) - alpha) / (beta - alpha), 0, 1)
+                rates = rates * (keep + (1 - keep) / factor)
+            elif scaling not in (None, "ntk"):
+                raise InvalidConfig(f"unknown rotary scaling {scaling!r}")
+        if not (np.isfinite(base) and np.isfinite(rates).all()):
+            raise InvalidConfig(f"theta {theta} with this scaling leaves rates that are no numbers")
         self._take(rates, layout, magnitude)
 
     @classmethod

@@ -366,3 +366,13 @@ def test_rope_positions_in_an_output(bad):
 @pytest.mark.parametrize("off", [0, 4, 4 * (8 * 32 - 1), -4])
 def test_rotation_tables_apart(off):
     assert table(sin=at(0) + off) == SHAPE and "apart" in error_from_parts()[1]
+
+
+@pytest.mark.filterwarnings("error")
+@pytest.mark.parametrize("bad", [
+    dict(scaling="ntk", factor=1e308), dict(scaling="ntk", factor=1e300, theta=1e200), dict(theta=1e-300, dim=512, scaling="linear", factor=1e-20),
+    dict(scaling="parts", factor=2.0, original=math.nan), dict(scaling="parts", factor=2.0, original=10, alpha=-math.inf),
+])
+def test_rates_that_are_no_numbers_are_refused(bad):
+    with pytest.raises(bitnetrs_amd.InvalidConfig):
+        Rope(**{**dict(dim=64, theta=1e4), **bad})
