@@ -206,20 +206,13 @@ __global__ __launch_bounds__(64 * kW, kOcc) void paged_decode_fp4_kernel(PagedDe
       const int c = wave + i * kW;
       if (c >= QL) break;
       // scores come out times log2(e) / sqrt(d): their weights are powers of two
-      const float4 lo = scale4(a.scale_log2, qx[i][0]), hi = scale4(a.scale_log2, qx[i][1]);
+      // (the fourth column is added to them too: 2^-40 of q there, for an infinity as in split8)
+      const float scale = PACK && part == 3 ? a.scale_log2 * 0x1p-40f : a.scale_log2;
+      const float4 lo = scale4(scale, qx[i][0]), hi = scale4(scale, qx[i][1]);
       const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
       const Parts s = split8<true>(x);  // exponents of 253 and 254 make infinities
       if constexpr (PACK) {
-        // the fourth column is added too: 2^-40 of q there, for an infinity as in split8
-        u32x4 y;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          y[k] = pack_hi(fabsf(x[2 * k]) * 0x1p-40f, fabsf(x[2 * k + 1]) * 0x1p-40f) |
-                 (pack_hi(x[2 * k], x[2 * k + 1]) & 0x80008000u);
-        if (part == 0) y = s.p[0];
-        if (part == 1) y = s.p[1];
-        if (part == 2) y = s.p[2];
-        s_q[c * 64 + lane] = y;
+        s_q[c * 64 + lane] = part == 1 ? s.p[1] : part == 2 ? s.p[2] : s.p[0];
       } else {
 #pragma unroll
         for (int k = 0; k < 3; ++k) s_q[(c * 3 + k) * 64 + lane] = s.p[k];
