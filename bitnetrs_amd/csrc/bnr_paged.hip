@@ -431,9 +431,12 @@ static unsigned row_grid(long long n) { return (unsigned)(n < kMaxRowGrid ? n : 
 template <int F, int L>
 static void append_vec(const PagedAppendArgs &a, hipStream_t s) {
   const long long rows = a.n_tokens * append_rows(a), per = 64 * kWaves / L;
-  // 4 MB of q and more go out with the non-temporal hint.  20/5 heads of 128 in 4 bits: 4096 tokens 26.6 ->
-  // 23.1 us, with the kernels that make the inputs and read q 67.9 -> 68.9; 16384 tokens 92.9 -> 83.5 and
-  // 238 -> 232; 64 tokens 3.7 both, with those kernels 11.2 -> 11.5.
+  // 4 MB of q and more go out with the non-temporal hint.  20/5 heads of 128: 2048 tokens in int8 13.1 -> 12.7
+  // us, with the kernels that make the inputs and read q 38.8 -> 37.8; 4096 25.6 -> 22.1 and 67.4 -> 68.7;
+  // 8192 46.9 -> 43.8 and 130.5 -> 132.0; 16384 87.8 -> 80.7 and 231.6 -> 223.4.  (40 to 80 MB of q the next
+  // kernel would have found in the 256 MB cache; in 4 bits those two are 68.3 -> 68.8 and 133.8 -> 133.0, in
+  // bf16 67.1 -> 67.6 and 130.1 both, and 16384 238.2 -> 231.5 and 235.8 -> 223.7.)  64 tokens, if they had
+  // it: 3.7 both, 11.2 -> 11.5.
   const bool stream = a.q && a.n_tokens * a.n_heads * a.pool.d >= 1 << 20;
   paged_append_vec_kernel<F, L><<<row_grid((rows + per - 1) / per), 64 * kWaves, 0, s>>>(a, stream);
 }

@@ -5,7 +5,7 @@
 //
 // for the pairs (a, b) = (i, i + dim/2) or (2i, 2i + 1); elements from dim on
 // are copied.  A position times a rate needs more places than fp32 has: the
-// angle is counted in turns in fp64, whole turns and the nearest eighths are
+// angle is counted in turns in fp64, whole turns and the nearest quarters are
 // taken off exactly, and what is left (at most an eighth of a turn) goes to
 // fp32's sine and cosine.
 //
@@ -83,7 +83,9 @@ __device__ __forceinline__ void store_some(T *p, const Some<T, N> &r) {
 // are neighbours, so a wave's loads and stores are whole lines.  16384 tokens of
 // 32/8 bf16 heads of 128, 32 of them rotated in pairs of neighbours: 66 us, 5.1 TB/s,
 // as a copy; with 32 bytes a thread 80.  16 bytes go out with the non-temporal hint (69
-// without; with kernels that make q and read it 158 both; 64 tokens 3.7 both).  4096
+// without; 512 f32 tokens of 32/8 heads of 128 6.2, 7.1 without; 64 3.7 both).  With
+// kernels that make q and read it the hint changes nothing: 64 tokens 11.2, 512 of f32
+// 19.5, 4096 of bf16 48.8, 16384 158 with it and without.  4096
 // tokens of 32/8 bf16 heads of 80, 40 of them rotated in halves, so that runs are units
 // of 8 bytes: 14 us, 44 with single elements.
 template <class T, int U, bool HALF>

@@ -11,7 +11,8 @@ theta^(-2i / dim), with the scaling:
   "parts"   by how often a pair turns over the trained context, n = original *
             rate / 2 pi: at alpha turns or fewer as "linear", at beta or more
             as it was, in between rate * (g + (1 - g) / factor) with
-            g = (n - alpha) / (beta - alpha)
+            g = (n - alpha) / (beta - alpha).  The ramp is over turns: for one
+            over the pairs' numbers, or with rounded ends, take from_rates
 
 `magnitude` multiplies the rotated values (cos and sin), for models that sharpen
 attention over long contexts with it.
